@@ -399,6 +399,55 @@ int lf_peer_sum(const uint64_t* bases, int32_t rank, int32_t world, float* z, in
                 int64_t capacity_floats, int64_t spin_limit, void* stream);
 
 /*
+ * Routing for mixture-of-experts layers (no counterpart in the reference, like the entry
+ * points below).  For each token, the top_k largest logits (ties to the lowest index; NaN and
+ * -infinity are never taken, +infinity counts as the largest finite value) and their weights
+ * scale * p or, with renormalize, scale * p / sum of the taken p, p = softmax(logits) in FP32:
+ *   weights, experts [T, k]: largest first; weight 0 and expert -1 where none was left;
+ *   offsets [E + 1], rows [T*k], positions [T, k]: the taken slots sorted by expert, ties by
+ *   slot.  Row r in [offsets[e], offsets[e+1]) belongs to expert e and token rows[r];
+ *   positions[t, j] is the slot's row or -1; rows beyond offsets[E] are -1.
+ * Sizes: 1 <= k <= 32, k <= E <= 1024, T*k < 2^31.  workspace: lf_route_experts_workspace_ints
+ * int32 values, not initialised.  One launch up to 32 tokens, else two.
+ */
+int64_t lf_route_experts_workspace_ints(int64_t num_tokens, int32_t num_experts);
+int lf_route_experts(int32_t dtype, const void* logits, int64_t logits_stride, int64_t num_tokens,
+                     int32_t num_experts, int32_t top_k, int32_t renormalize, float scale,
+                     float* weights, int32_t* experts, int32_t* offsets, int32_t* rows,
+                     int32_t* positions, int32_t* workspace, int64_t workspace_ints, void* stream);
+
+/*
+ * Gradient of lf_route_experts' weights: with d = sum_j w_j g_j / scale, w_i (g_i - d) for the
+ * taken experts and 0 (renormalize) or -scale p_i d for the others; a token with no expert
+ * gets zeros.  `weights` and `experts` are the forward's outputs, `grad_weights` [T, k] FP32.
+ */
+int lf_route_experts_backward(int32_t dtype, const void* logits, int64_t logits_stride,
+                              const float* weights, const int32_t* experts,
+                              const float* grad_weights, int64_t grad_stride, int64_t num_tokens,
+                              int32_t num_experts, int32_t top_k, int32_t renormalize, float scale,
+                              void* grad_logits, int64_t out_stride, void* stream);
+
+/*
+ * out[t] = sum_j weights[t, j] * y[positions[t, j]] in FP32, rounded once; positions outside
+ * [0, num_rows) add nothing and weights = NULL stands for ones.  dtype is that of y and out.
+ */
+int lf_combine_experts(int32_t dtype, const void* y, int64_t y_stride, int64_t num_rows,
+                       const float* weights, const int32_t* positions, int64_t num_tokens,
+                       int32_t top_k, int32_t width, void* out, int64_t out_stride, void* stream);
+
+/*
+ * Gradients of lf_combine_experts: grad_y[positions[t, j]] = weights[t, j] * grad[t] and (when
+ * not NULL) grad_weights[t, j] = <grad[t], y[positions[t, j]]>, 0 without a position.  The
+ * positions that are not -1 must be the rows 0 .. n-1, each once (as lf_route_experts leaves
+ * them); rows n .. num_rows-1 of grad_y become zero.
+ */
+int lf_combine_experts_backward(int32_t dtype, const void* grad, int64_t grad_stride,
+                                const void* y, int64_t y_stride, int64_t num_rows,
+                                const float* weights, const int32_t* positions,
+                                int64_t num_tokens, int32_t top_k, int32_t width, void* grad_y,
+                                int64_t grad_y_stride, float* grad_weights, void* stream);
+
+/*
  * Number of bounded device-side waits (mbarrier polls in the bulk-copy kernels)
  * that expired since the last reset; a non-zero count means a kernel gave up and
  * skipped work instead of hanging.  Synchronous; reset != 0 clears the counter.

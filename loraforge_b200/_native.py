@@ -85,6 +85,16 @@ SIGNATURES = {
         _i64, _i64, _i32, _i32, _i32, _i32, _i32, _p,
     ],
     "lf_fused_noalloc_reset": [_p],
+    "lf_route_experts": [
+        _i32, _p, _i64, _i64, _i32, _i32, _i32, _f32, _p, _p, _p, _p, _p, _p, _i64, _p,
+    ],
+    "lf_route_experts_backward": [
+        _i32, _p, _i64, _p, _p, _p, _i64, _i64, _i32, _i32, _i32, _f32, _p, _i64, _p,
+    ],
+    "lf_combine_experts": [_i32, _p, _i64, _i64, _p, _p, _i64, _i32, _i32, _p, _i64, _p],
+    "lf_combine_experts_backward": [
+        _i32, _p, _i64, _p, _i64, _i64, _p, _p, _i64, _i32, _i32, _p, _i64, _p, _p,
+    ],
 }
 
 _lock = threading.Lock()
@@ -95,7 +105,7 @@ def exported_symbols() -> tuple[str, ...]:
     """Every symbol the header declares (checked by the CPU test suite)."""
     return ("lf_version", "lf_last_error_string", "lf_fused_workspace_floats",
             "lf_sgmv_prefill_workspace_floats", "lf_lora_base_gemm_workspace_floats",
-            "lf_peer_buffer_bytes", "lf_peer_handle_bytes", *SIGNATURES)
+            "lf_peer_buffer_bytes", "lf_peer_handle_bytes", "lf_route_experts_workspace_ints", *SIGNATURES)
 
 
 def library() -> ctypes.CDLL:
@@ -127,6 +137,8 @@ def library() -> ctypes.CDLL:
             lib.lf_peer_buffer_bytes.argtypes = [_i64]
             lib.lf_peer_handle_bytes.restype = ctypes.c_int
             lib.lf_peer_handle_bytes.argtypes = []
+            lib.lf_route_experts_workspace_ints.restype = ctypes.c_int64
+            lib.lf_route_experts_workspace_ints.argtypes = [_i64, _i32]
             _lib = lib
     return _lib
 
@@ -161,6 +173,14 @@ def lora_base_gemm_workspace_floats(num_tokens: int, width: int, num_slices: int
     n = library().lf_lora_base_gemm_workspace_floats(num_tokens, width, num_slices, capacity)
     if n < 0:
         raise ValueError("invalid sizes for the base GEMM workspace")
+    return n
+
+
+def route_experts_workspace_ints(num_tokens: int, num_experts: int) -> int:
+    """int32 workspace size of lf_route_experts for these sizes."""
+    n = library().lf_route_experts_workspace_ints(num_tokens, num_experts)
+    if n < 0:
+        raise ValueError("invalid sizes for the routing workspace")
     return n
 
 

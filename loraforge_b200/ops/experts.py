@@ -1,0 +1,226 @@
+"""Mixture-of-experts operators over the sm_100a C ABI: routing and the sum over experts.
+
+A layer with E experts runs ``route_experts`` on its router's logits, multiplies the rows it
+gives by their experts' weights, and adds each token's rows up with ``combine_experts``.
+Every operator reads its tables on the device, so a layer can be captured in a CUDA graph;
+the LoRA operators take the same batch beside it (the rows of a token keep its adapter).
+Each forward has an explicit gradient (``*_backward``).  The reference has no counterpart.
+"""
+
+from __future__ import annotations
+
+from typing import NamedTuple
+
+from loraforge_b200 import _native
+from loraforge_b200.ops._contract import INT32_LIMIT, first_failure, output_is_distinct
+
+MAX_EXPERTS = 1024
+MAX_TOP_K = 32
+
+
+class ExpertRouting(NamedTuple):
+    """Tables of a routed batch: T tokens, k slots each, R = T*k rows sorted by expert."""
+
+    weights: object  # FP32 [T, k], largest first; 0 where no expert was left
+    experts: object  # int32 [T, k]; -1 where no expert was left
+    offsets: object  # int32 [E + 1]: rows [offsets[e], offsets[e+1]) are expert e's
+    rows: object  # int32 [R]: token of each row; -1 beyond offsets[E]
+    positions: object  # int32 [T, k]: row of each slot or -1
+
+
+def cuda_tensor(value, name: str, ndim: int, dtypes, device=None) -> None:
+    """A CUDA tensor of rank `ndim` and one of `dtypes`, int32-indexable, on `device` if given."""
+    import torch
+
+    if not isinstance(value, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if value.ndim != ndim or value.dtype not in dtypes:
+        raise ValueError(f"{name} must be {ndim}D with dtype {' or '.join(str(d) for d in dtypes)}")
+    if max(value.shape, default=0) >= INT32_LIMIT:
+        raise ValueError(f"{name} dimensions must fit signed int32 indexing")
+    if value.device.type != "cuda" or (device is not None and value.device != device):
+        raise ValueError(f"{name} must be on the same CUDA GPU")
+
+
+def row_matrix(value, name: str, dtypes, device=None) -> None:
+    """A 2-D `cuda_tensor` of rows that do not overlap, with unit column stride."""
+    cuda_tensor(value, name, 2, dtypes, device)
+    if value.shape[0] > 1 and value.stride(0) < value.shape[1] or (value.shape[1] > 1 and value.stride(1) != 1):
+        raise ValueError(f"{name} must have unit column stride and rows that do not overlap")
+
+
+def row_stride(t) -> int:
+    """Row stride of a `row_matrix` (a one-row tensor's own stride says nothing)."""
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+def packed_table(value, name: str, shape, device, dtype) -> None:
+    """A contiguous table of exactly `shape`."""
+    cuda_tensor(value, name, len(shape), (dtype,), device)
+    if tuple(value.shape) != tuple(shape) or not value.is_contiguous():
+        raise ValueError(f"{name} must be contiguous with shape {tuple(shape)}")
+
+
+def _floats():
+    import torch
+
+    return (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _scale(value) -> float:
+    scale = float(value)
+    if not 0.0 < scale <= 3.4028234663852886e38:
+        raise ValueError("scale must be positive and finite")
+    return scale
+
+
+def route_experts(logits, top_k: int, *, renormalize: bool = True, scale: float = 1.0,
+                  out: ExpertRouting | None = None) -> ExpertRouting:
+    """The ``top_k`` experts of each token, their weights, and the rows sorted by expert.
+
+    ``logits`` [T, E] (FP32 / FP16 / BF16, unit column stride).  The experts are those of the
+    largest logits, ties to the lowest index; NaN and -inf are never taken (a masked expert;
+    a padding token is a row of -inf and gets no rows), +inf counts as the largest finite
+    value.  With p = softmax(logits) in FP32 the weights are ``scale * p``, divided by the
+    taken experts' sum when ``renormalize``.  ``out``: tables of an earlier call with the
+    same sizes to write into (fixed addresses for CUDA graphs).
+    """
+    import torch
+
+    row_matrix(logits, "logits", _floats())
+    T, E = logits.shape
+    if type(top_k) is not int or not 1 <= top_k <= min(E, MAX_TOP_K):
+        raise ValueError(f"top_k must be in 1..min(experts, {MAX_TOP_K})")
+    first_failure((
+        (E > MAX_EXPERTS, f"at most {MAX_EXPERTS} experts"),
+        (T * top_k >= INT32_LIMIT, "tokens * top_k must fit signed int32 indexing"),
+        (type(renormalize) is not bool, "renormalize must be a bool"),
+    ))
+    scale = _scale(scale)
+    device = logits.device
+    if out is None:
+        out = ExpertRouting(
+            torch.empty((T, top_k), dtype=torch.float32, device=device),
+            torch.empty((T, top_k), dtype=torch.int32, device=device),
+            torch.empty(E + 1, dtype=torch.int32, device=device),
+            torch.empty(T * top_k, dtype=torch.int32, device=device),
+            torch.empty((T, top_k), dtype=torch.int32, device=device),
+        )
+    else:
+        for name, shape, dtype in (("weights", (T, top_k), torch.float32), ("experts", (T, top_k), torch.int32),
+                                   ("offsets", (E + 1,), torch.int32), ("rows", (T * top_k,), torch.int32),
+                                   ("positions", (T, top_k), torch.int32)):
+            packed_table(getattr(out, name), f"out.{name}", shape, device, dtype)
+            output_is_distinct(getattr(out, name), (logits,))
+    workspace = torch.empty(_native.route_experts_workspace_ints(T, E), dtype=torch.int32, device=device)
+    with torch.cuda.device(device):
+        _native.call(
+            "lf_route_experts", _native.dtype_code(logits.dtype), logits.data_ptr(), row_stride(logits), T, E, top_k,
+            int(renormalize), scale, out.weights.data_ptr(), out.experts.data_ptr(), out.offsets.data_ptr(),
+            out.rows.data_ptr(), out.positions.data_ptr(), workspace.data_ptr(), workspace.numel(),
+            _native.stream_of(device),
+        )
+    return out
+
+
+def route_experts_backward(logits, routing: ExpertRouting, grad_weights, *, renormalize: bool = True,
+                           scale: float = 1.0):
+    """Gradient of ``route_experts``' weights with respect to the logits, in their dtype.
+
+    ``logits``, ``renormalize`` and ``scale`` as in the forward call, ``routing`` its result,
+    ``grad_weights`` FP32 [T, k].  Experts count as fixed; a token without experts gets zeros.
+    """
+    import torch
+
+    row_matrix(logits, "logits", _floats())
+    T, E = logits.shape
+    if not isinstance(routing, ExpertRouting):
+        raise TypeError("routing must be the ExpertRouting of the forward call")
+    device = logits.device
+    cuda_tensor(routing.weights, "routing.weights", 2, (torch.float32,), device)
+    k = routing.weights.shape[1]
+    packed_table(routing.weights, "routing.weights", (T, k), device, torch.float32)
+    packed_table(routing.experts, "routing.experts", (T, k), device, torch.int32)
+    row_matrix(grad_weights, "grad_weights", (torch.float32,), device)
+    first_failure((
+        (tuple(grad_weights.shape) != (T, k), "grad_weights must have the weights' shape"),
+        (not 1 <= k <= min(E, MAX_TOP_K) or E > MAX_EXPERTS, "routing does not fit the logits"),
+        (type(renormalize) is not bool, "renormalize must be a bool"),
+    ))
+    scale = _scale(scale)
+    grad = torch.empty((T, E), dtype=logits.dtype, device=device)
+    with torch.cuda.device(device):
+        _native.call(
+            "lf_route_experts_backward", _native.dtype_code(logits.dtype), logits.data_ptr(), row_stride(logits),
+            routing.weights.data_ptr(), routing.experts.data_ptr(), grad_weights.data_ptr(), row_stride(grad_weights),
+            T, E, k, int(renormalize), scale, grad.data_ptr(), E, _native.stream_of(device),
+        )
+    return grad
+
+
+def _combine_tables(positions, weights, device):
+    import torch
+
+    cuda_tensor(positions, "positions", 2, (torch.int32,), device)
+    T, k = positions.shape
+    packed_table(positions, "positions", (T, k), device, torch.int32)
+    if weights is not None:
+        packed_table(weights, "weights", (T, k), device, torch.float32)
+    if not 1 <= k <= MAX_TOP_K or T * k >= INT32_LIMIT:
+        raise ValueError(f"positions must have 1..{MAX_TOP_K} columns and fit signed int32 indexing")
+    return T, k
+
+
+def combine_experts(y, weights, positions, *, out=None):
+    """``out[t] = sum_j weights[t, j] * y[positions[t, j]]``, summed in FP32, in y's dtype.
+
+    ``y`` [R, N] are the experts' rows, ``weights`` FP32 [T, k] (None: ones, the gradient of
+    a gather), ``positions`` int32 [T, k]; a position outside [0, R) adds nothing, so a token
+    without experts gets zeros.
+    """
+    import torch
+
+    row_matrix(y, "y", _floats())
+    T, k = _combine_tables(positions, weights, y.device)
+    if y.shape[1] < 1:
+        raise ValueError("y must have at least one column")
+    if out is None:
+        out = torch.empty((T, y.shape[1]), dtype=y.dtype, device=y.device)
+    else:
+        row_matrix(out, "out", (y.dtype,), y.device)
+        if tuple(out.shape) != (T, y.shape[1]):
+            raise ValueError("out must be [tokens, width]")
+        output_is_distinct(out, (y, positions) if weights is None else (y, positions, weights))
+    with torch.cuda.device(y.device):
+        _native.call(
+            "lf_combine_experts", _native.dtype_code(y.dtype), y.data_ptr(), row_stride(y), y.shape[0],
+            None if weights is None else weights.data_ptr(), positions.data_ptr(), T, k, y.shape[1], out.data_ptr(),
+            row_stride(out), _native.stream_of(y.device),
+        )
+    return out
+
+
+def combine_experts_backward(grad, y, weights, positions):
+    """Gradients of ``combine_experts``: (grad_y [R, N] in y's dtype, grad_weights FP32 [T, k]).
+
+    The positions that are not -1 must be the rows 0 .. n-1, each once, as ``route_experts``
+    gives them; the rows behind them get zeros.  ``weights=None`` stands for ones and gives
+    None for their gradient.
+    """
+    import torch
+
+    row_matrix(y, "y", _floats())
+    T, k = _combine_tables(positions, weights, y.device)
+    row_matrix(grad, "grad", (y.dtype,), y.device)
+    if tuple(grad.shape) != (T, y.shape[1]) or y.shape[1] < 1:
+        raise ValueError("grad must be [tokens, width]")
+    grad_y = torch.empty(tuple(y.shape), dtype=y.dtype, device=y.device)
+    grad_weights = None if weights is None else torch.empty((T, k), dtype=torch.float32, device=y.device)
+    with torch.cuda.device(y.device):
+        _native.call(
+            "lf_combine_experts_backward", _native.dtype_code(y.dtype), grad.data_ptr(), row_stride(grad),
+            y.data_ptr(), row_stride(y), y.shape[0], None if weights is None else weights.data_ptr(),
+            positions.data_ptr(), T, k, y.shape[1], grad_y.data_ptr(), y.shape[1],
+            None if weights is None else grad_weights.data_ptr(), _native.stream_of(y.device),
+        )
+    return grad_y, grad_weights
