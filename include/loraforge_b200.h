@@ -448,6 +448,48 @@ int lf_combine_experts_backward(int32_t dtype, const void* grad, int64_t grad_st
                                 int64_t grad_y_stride, float* grad_weights, void* stream);
 
 /*
+ * Matrix products grouped by expert, BF16 or FP16 operands, FP32 sums, one rounding.  Rows
+ * offsets[e] <= r < offsets[e+1] (the tables of lf_route_experts; bounds are kept ascending and
+ * within [0, num_rows)) belong to expert e; groups may be empty.  W [E, out_width, width] with
+ * unit inner stride; i(r) = rows[r], or r when rows = NULL (then x has num_rows rows).
+ *   lf_expert_linear              y[r, n]     = sum_k W[e, n, k] x[i(r), k]
+ *   lf_expert_linear_input_grad   dx[r, k]    = sum_n W[e, n, k] dy[r, n]
+ *   lf_expert_linear_weight_grad  dW[e, n, k] = sum_{r of e} dy[r, n] x[i(r), k]
+ * y and dx have the operands' type and zeros in the rows of no group; dW (contiguous; zeros
+ * for an empty group) theirs or FP32 (out_dtype).  An i(r) outside [0, x_rows) reads a zero row.
+ * dx is by row: lf_combine_experts with weights = NULL adds it up by token.
+ * Widths are multiples of 8; x, dy and W 16-byte aligned with strides that are multiples of 8.
+ * One launch each, no workspace.
+ */
+int lf_expert_linear(int32_t dtype, const void* x, int64_t x_stride, int64_t x_rows,
+                     const int32_t* rows, const void* w, int64_t w_expert_stride,
+                     int64_t w_row_stride, const int32_t* offsets, int32_t num_experts,
+                     int64_t num_rows, int64_t out_width, int64_t width, void* y,
+                     int64_t y_stride, void* stream);
+int lf_expert_linear_input_grad(int32_t dtype, const void* dy, int64_t dy_stride, const void* w,
+                                int64_t w_expert_stride, int64_t w_row_stride,
+                                const int32_t* offsets, int32_t num_experts, int64_t num_rows,
+                                int64_t out_width, int64_t width, void* dx, int64_t dx_stride,
+                                void* stream);
+int lf_expert_linear_weight_grad(int32_t dtype, const void* dy, int64_t dy_stride, const void* x,
+                                 int64_t x_stride, int64_t x_rows, const int32_t* rows,
+                                 const int32_t* offsets, int32_t num_experts, int64_t num_rows,
+                                 int64_t out_width, int64_t width, int32_t out_dtype, void* dw,
+                                 void* stream);
+
+/*
+ * MXFP4: blocks of 32 values along a row share 2^e, e = floor(log2 max|x|) - 2 (>= -127), held
+ * as the byte e + 127; codes are E2M1 of x / 2^e, nearest even, saturating, two a byte, the
+ * even-indexed one in the low nibble.  A block with an infinity or NaN: scale 255, codes 0.
+ * width is a multiple of 32; codes [rows, width/2] (16-byte aligned) and scales
+ * [rows, width/32] are contiguous, and so is the dequantised output.
+ */
+int lf_mxfp4_quantize(int32_t dtype, const void* x, int64_t x_stride, int64_t rows,
+                      int64_t width, uint8_t* codes, uint8_t* scales, void* stream);
+int lf_mxfp4_dequantize(int32_t dtype, const uint8_t* codes, const uint8_t* scales, int64_t rows,
+                        int64_t width, void* out, void* stream);
+
+/*
  * Number of bounded device-side waits (mbarrier polls in the bulk-copy kernels)
  * that expired since the last reset; a non-zero count means a kernel gave up and
  * skipped work instead of hanging.  Synchronous; reset != 0 clears the counter.

@@ -95,6 +95,17 @@ SIGNATURES = {
     "lf_combine_experts_backward": [
         _i32, _p, _i64, _p, _i64, _i64, _p, _p, _i64, _i32, _i32, _p, _i64, _p, _p,
     ],
+    "lf_expert_linear": [
+        _i32, _p, _i64, _i64, _p, _p, _i64, _i64, _p, _i32, _i64, _i64, _i64, _p, _i64, _p,
+    ],
+    "lf_expert_linear_input_grad": [
+        _i32, _p, _i64, _p, _i64, _i64, _p, _i32, _i64, _i64, _i64, _p, _i64, _p,
+    ],
+    "lf_expert_linear_weight_grad": [
+        _i32, _p, _i64, _p, _i64, _i64, _p, _p, _i32, _i64, _i64, _i64, _i32, _p, _p,
+    ],
+    "lf_mxfp4_quantize": [_i32, _p, _i64, _i64, _i64, _p, _p, _p],
+    "lf_mxfp4_dequantize": [_i32, _p, _p, _i64, _i64, _p, _p],
 }
 
 _lock = threading.Lock()

@@ -1,0 +1,303 @@
+// Pieces shared by the expert products (16-bit and MXFP4): CTA pairs and clusters on tcgen05,
+// gathered TMA rows, and the tile list over ragged groups of rows.
+#pragma once
+
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <mutex>
+#include <string>
+
+#include "launch.cuh"
+#include "tcgen05.cuh"
+#include "tma.cuh"
+
+namespace lfb {
+namespace grouped {
+
+using namespace tc;
+
+constexpr int kMaxExperts = 1024;
+constexpr int kThreads = 192;  // warp 0 loads, warp 1 MMA, warps 2-5 epilogue (TMEM lane quarter = warp & 3)
+
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// ------------------------------------------------------------------ clusters
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The shared::cluster address of `p` in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t mapa(const void* p, uint32_t rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ float lds_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ bool try_wait_cluster(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+      " selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(done)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+// wait_or_abort for barriers on which other CTAs of the cluster arrive.
+__device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  if (*abort) return false;
+  if (try_wait_cluster(bar, parity)) return true;
+  const uint64_t start = global_timer_ns();
+  while (!try_wait_cluster(bar, parity)) {
+    if (global_timer_ns() - start > kWaitLimitNs) {
+      atomicAdd(&g_lf_wait_timeouts, 1u);
+      *abort = 1;
+      return false;
+    }
+  }
+  return true;
+}
+
+// ------------------------------------------------------------------ tcgen05 on one CTA or a pair
+template <int kCtas>
+__device__ __forceinline__ void alloc_tmem(uint32_t* slot, uint32_t columns) {
+  if constexpr (kCtas == 1) {
+    tc_alloc(slot, columns);
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(columns)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+}
+template <int kCtas>
+__device__ __forceinline__ void free_tmem(uint32_t addr, uint32_t columns) {
+  if constexpr (kCtas == 1) {
+    tc_dealloc(addr, columns);
+  } else {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(columns) : "memory");
+  }
+}
+// D (+)= A . B^T, 16-bit operands (both of one type), FP32 sums.
+template <int kCtas>
+__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  if constexpr (kCtas == 1) {
+    tc_mma(d, a, b, idesc, accumulate);
+  } else {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+  }
+}
+// Arrive on `bar`, in both CTAs of a pair, when this thread's MMAs so far are complete.
+template <int kCtas>
+__device__ __forceinline__ void commit(uint64_t* bar) {
+  if constexpr (kCtas == 1) {
+    tc_commit(bar);
+  } else {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            smem_u32(bar)),
+        "h"(uint16_t(3))
+        : "memory");
+  }
+}
+
+// ------------------------------------------------------------------ TMA; `bar` may be the pair's first CTA's
+template <int kCtas>
+__device__ __forceinline__ void load_2d(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
+  if constexpr (kCtas == 1) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
+        "[%4];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar)
+        : "memory");
+  } else {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, "
+        "{%2, %3}], [%4];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar)
+        : "memory");
+  }
+}
+template <int kCtas>
+__device__ __forceinline__ void load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
+  if constexpr (kCtas == 1) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
+        "[%5];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+        : "memory");
+  } else {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, "
+        "{%2, %3, %4}], [%5];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+        : "memory");
+  }
+}
+// Four rows of one box width, from columns c0 on; a row index past the tensor reads zeros.
+template <int kCtas>
+__device__ __forceinline__ void gather4(uint32_t dst, const CUtensorMap* map, int c0, const int (&r)[4], uint32_t bar) {
+  if constexpr (kCtas == 1) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+        "%3, %4, %5, %6}], [%7];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(bar)
+        : "memory");
+  } else {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes.cta_group::2 [%0], "
+        "[%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(bar)
+        : "memory");
+  }
+}
+
+// ------------------------------------------------------------------ tiles of ragged groups
+__host__ __device__ constexpr int ceil_div(int a, int b) { return (a + b - 1) / b; }
+__host__ __device__ constexpr int round_up(int a, int b) { return (a + b - 1) / b * b; }
+
+// Inclusive scan over the CTA's threads of `v` under `op`, going on from `*carry`, which ends
+// as the scan's last value.  `part`: one int a warp.  Two barriers.
+template <typename Op>
+__device__ __forceinline__ int scan_threads(int v, int* carry, int* part, Op&& op) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, v, d);
+    if (lane >= d) v = op(v, up);
+  }
+  if (lane == 31) part[warp] = v;
+  __syncthreads();
+  int before = *carry, all = *carry;
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) before = op(before, part[w]);
+    all = op(all, part[w]);
+  }
+  __syncthreads();
+  *carry = all;
+  return op(before, v);
+}
+
+// Fills bounds[0..E] with the groups' row bounds, ascending and in [0, R] whatever `offsets`
+// holds, and starts[0..E] with the first tile of each group, `tiles_of(rows)` tiles a group.
+// All threads of the CTA; ends with a barrier.
+template <typename F>
+__device__ void list_tiles(const int32_t* offsets, int E, int R, int* bounds, int* starts, int* part, F&& tiles_of) {
+  const int tid = threadIdx.x;
+  int largest = 0, total = 0;
+  for (int e0 = 0; e0 <= E; e0 += kThreads) {
+    const int e = e0 + tid;
+    const int v = scan_threads(e <= E ? min(max(offsets[e], 0), R) : 0, &largest, part,
+                               [](int a, int b) { return max(a, b); });
+    if (e <= E) bounds[e] = v;
+  }
+  __syncthreads();
+  for (int e0 = 0; e0 < E; e0 += kThreads) {
+    const int e = e0 + tid;
+    const int n = e < E ? tiles_of(bounds[e + 1] - bounds[e]) : 0;
+    const int v = scan_threads(n, &total, part, [](int a, int b) { return a + b; });
+    if (e < E) starts[e] = v - n;
+  }
+  if (tid == 0) starts[E] = total;
+  __syncthreads();
+}
+
+// The group of tile t: the last e with starts[e] <= t (empty groups share their successor's start).
+__device__ __forceinline__ int group_of(const int* starts, int E, int t) {
+  int lo = 0, hi = E - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (starts[mid] <= t) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+// Order of a group's tiles (m feature tiles x n row tiles): bands of up to eight row tiles,
+// inside a band row tiles fastest, so that the CTAs of a wave share both operands in L2.
+constexpr int kBand = 8;
+__device__ __forceinline__ void place_tile(int q, int mt, int nt, int* m, int* n) {
+  const int band = q / (kBand * mt), width = min(kBand, nt - band * kBand);
+  const int w = q - band * kBand * mt;
+  *m = w / width;
+  *n = band * kBand + w % width;
+}
+
+// ------------------------------------------------------------------ host
+inline PFN_cuTensorMapEncodeTiled_v12000 map_encoder() {
+  static std::mutex mutex;
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  std::lock_guard<std::mutex> lock(mutex);
+  if (!fn) {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult status;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &status) == cudaSuccess &&
+        status == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
+  }
+  return fn;
+}
+
+// A map of `ndim` dimensions (innermost first, strides in bytes from the second on) with
+// 128-byte swizzle; false when the driver refuses it.
+inline bool encode_map(CUtensorMap* map, CUtensorMapDataType type, int ndim, const void* base, const cuuint64_t* dims,
+                       const cuuint64_t* strides, const cuuint32_t* box) {
+  const PFN_cuTensorMapEncodeTiled_v12000 encode = map_encoder();
+  const cuuint32_t ones[3] = {1, 1, 1};
+  return encode && encode(map, type, ndim, const_cast<void*>(base), dims, strides, box, ones,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+inline int sm_count(int* sms) {
+  static int known[64] = {};
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return check_launch("cudaGetDevice");
+  int& have = known[device & 63];
+  if (!have && cudaDeviceGetAttribute(&have, cudaDevAttrMultiProcessorCount, device) != cudaSuccess)
+    return check_launch("cudaDeviceGetAttribute");
+  *sms = have;
+  return LF_OK;
+}
+
+template <typename P>
+int launch_clusters(void (*kernel)(P), int grid, int cluster, int smem, void* stream, const char* what, const P& p) {
+  cudaLaunchConfig_t config = {};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  config.attrs = attr;
+  config.numAttrs = 2;
+  config.gridDim = dim3(grid);
+  config.blockDim = dim3(kThreads);
+  config.dynamicSmemBytes = smem;
+  config.stream = static_cast<cudaStream_t>(stream);
+  const cudaError_t err = cudaLaunchKernelEx(&config, kernel, p);
+  if (err != cudaSuccess) {
+    last_error() = std::string(what) + ": " + cudaGetErrorString(err);
+    return LF_E_CUDA;
+  }
+  return LF_OK;
+}
+
+}  // namespace grouped
+}  // namespace lfb

@@ -1,0 +1,599 @@
+// Matrix products grouped by expert, 16-bit operands, on tcgen05 + TMEM.  Rows r of group e
+// (offsets[e] <= r < offsets[e+1]) belong to expert e:
+//
+//   forward   y[r, n]     = sum_k W[e, n, k] x[i(r), k]          i(r) = rows[r], or r
+//   input     dx[r, k]    = sum_n W[e, n, k] dy[r, n]
+//   weight    dW[e, n, k] = sum_{r of e} dy[r, n] x[i(r), k]
+//
+// One kernel for the three: D[feature, column] with 128 output features on the TMEM lanes (256
+// in a CTA pair) and up to kNT columns, rows of the group (forward, input) or the N features of
+// dy (weight).  Rows on the MMA's N side cost in steps of 16, so a ragged group pays at most 15
+// rows of padding, and a lane's neighbours are neighbours in the output row: a warp stores 32
+// adjacent features of one row at a time.
+//
+//   mode      A (lanes)                     B (columns)                 contraction
+//   forward   W[e], K-major                 x rows, K-major, gathered   K
+//   input     W[e], MN-major (k on lanes)   dy rows, K-major            N
+//   weight    x rows, MN-major, gathered    dy rows, MN-major           the group's rows
+//
+// Nothing is transposed or gathered in memory: MN-major operands are read as they lie through
+// the shared-memory descriptor, and x's rows by token come with gather4 loads.  Steps past K, N
+// or a group's last row read zeros (out of bounds for the tensor map, or a row index that is),
+// so a neighbouring group's infinities never reach a sum.
+//
+// Per CTA: warp 0 loads 64-deep stages into a ring, warp 1 issues the MMAs and owns the TMEM
+// (two accumulators, so a tile's stores overlap the next tile's MMAs), warps 2-5 store.  The
+// grid is persistent and computes its tile list from `offsets` on the device.
+//
+//   wide    CTA pairs (cta_group::2), 256 x 256 tiles: each CTA loads half of both operands.
+//   narrow  one CTA, 128 features x up to 64 rows, for groups of few rows, where the weights'
+//           bytes are the cost; the contraction can be split over a cluster of CTAs, whose
+//           partial sums are added in rank order through distributed shared memory.
+//
+// Every wait is bounded (tma.cuh): an expiry stops every role at its next wait.
+#include "grouped.cuh"
+#include "sgmv.cuh"
+
+namespace lfb {
+namespace {
+
+using namespace grouped;
+
+enum Mode { kForward = 0, kInput = 1, kWeight = 2 };
+
+constexpr int kStep = 64;             // contraction per stage: 128 bytes
+constexpr int kABytes = 128 * 128;    // 128 features x 128 bytes (K-major), or two 64-feature boxes of 64 steps
+constexpr int kMaxSplit = 8;
+
+struct GParams {
+  const int32_t* offsets;  // [E + 1]
+  const int32_t* rows;     // [R] or null
+  void* out;
+  int64_t out_stride;
+  int E, R, x_rows;
+  int M, C;  // output features, contraction (forward K, input N; weight: the groups' rows)
+  int N;     // weight: columns of D (dy's features)
+  int out_type, elem_bf16, split;
+  CUtensorMap a_map;     // forward: W boxes 64 k x 128 n; input: 64 k x 64 n; weight: x boxes 64 k x 64 rows
+  CUtensorMap a_gather;  // weight: single x rows of 64 k
+  CUtensorMap b_map;     // forward / input: 64 wide x 64 rows; weight: dy boxes 64 n x 64 rows
+  CUtensorMap b_small;   // forward / input: 64 wide x 8 rows
+  CUtensorMap b_gather;  // forward: single x rows; weight: single dy rows
+};
+
+template <int kCtas, int kNT>
+struct Shape {
+  static constexpr int kBRows = kNT / kCtas;  // a CTA's share of the columns
+  static constexpr int kStageBytes = kABytes + kBRows * 128;
+  static constexpr int kPartBytes = kCtas == 1 ? kNT * 128 * 4 : 0;
+  static constexpr int kStages = 6;
+  static constexpr int kColumns = 2 * kNT;  // TMEM
+};
+
+// Descriptor of an MN-major tile: boxes of 64 elements (128 bytes, swizzled) x kStep rows,
+// the boxes 8 KiB apart, groups of 8 rows 1024 bytes apart.  16 steps are 2048 bytes.
+__device__ __forceinline__ uint64_t mn_desc(uint32_t saddr) {
+  return uint64_t((saddr & 0x3FFFFu) >> 4) | (uint64_t((kStep * 128) >> 4) << 16) | (uint64_t(1024 >> 4) << 32) |
+         (uint64_t(1) << 46) | (uint64_t(2) << 61);
+}
+
+__device__ __forceinline__ uint32_t instruction(int bf16, int a_mn, int b_mn, int m, int n) {
+  return (1u << 4) | (uint32_t(bf16) << 7) | (uint32_t(bf16) << 10) | (uint32_t(a_mn) << 15) | (uint32_t(b_mn) << 16) |
+         (uint32_t(n >> 3) << 17) | (uint32_t(m >> 4) << 24);
+}
+
+struct Tile {
+  int e, m0, n0, nt, valid, steps;  // n0: first row (forward, input) or feature of dy; valid columns
+  int lo, hi;                       // the group's rows
+};
+
+template <int kMode, int kCtas, int kNT>
+__device__ __forceinline__ Tile tile_of(const GParams& p, const int* bounds, const int* starts, int t) {
+  Tile x;
+  x.e = group_of(starts, p.E, t);
+  x.lo = bounds[x.e];
+  x.hi = bounds[x.e + 1];
+  const int mt = ceil_div(p.M, 128 * kCtas);
+  const int columns = kMode == kWeight ? p.N : x.hi - x.lo;
+  const int nt = ceil_div(columns, kNT);
+  int m, n;
+  place_tile(t - starts[x.e], mt, nt, &m, &n);
+  x.m0 = m * 128 * kCtas;
+  if (kMode == kWeight) {
+    x.n0 = n * kNT;
+    x.valid = min(kNT, p.N - x.n0);
+    x.nt = round_up(x.valid, kNT / 2);  // whole 64-feature boxes in each CTA
+    x.steps = ceil_div(x.hi - x.lo, kStep);
+  } else {
+    const int each = round_up(ceil_div(columns, nt), 16);  // the group's rows in even tiles
+    x.n0 = x.lo + n * each;
+    x.valid = min(each, x.hi - x.n0);
+    x.nt = round_up(x.valid, 16);
+    x.steps = ceil_div(p.C, kStep);
+  }
+  return x;
+}
+
+template <typename O>
+__device__ __forceinline__ void store_out(void* out, int64_t at, float v) {
+  static_cast<typename O::storage*>(out)[at] = O::from_float(v);
+}
+__device__ __forceinline__ void store_typed(const GParams& p, int64_t at, float v) {
+  if (p.out_type == LF_BF16) store_out<bf16_t>(p.out, at, v);
+  else if (p.out_type == LF_F16) store_out<f16_t>(p.out, at, v);
+  else store_out<f32_t>(p.out, at, v);
+}
+
+template <int kMode, int kCtas, int kNT>
+__global__ void __launch_bounds__(kThreads, 1) grouped_kernel(const __grid_constant__ GParams p) {
+  using S = Shape<kCtas, kNT>;
+  constexpr int kStages = S::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = align1024(smem_raw);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  uint8_t* ring = smem;
+  float* part = reinterpret_cast<float*>(ring + kStages * S::kStageBytes);  // narrow: [kNT][128]
+  uint64_t* full = reinterpret_cast<uint64_t*>(ring + kStages * S::kStageBytes + S::kPartBytes);
+  uint64_t* empty = full + kStages;
+  uint64_t* acc_full = empty + kStages;
+  uint64_t* acc_empty = acc_full + 2;
+  uint64_t* part_full = acc_empty + 2;
+  uint64_t* part_empty = part_full + 1;
+  uint64_t* fin = part_empty + 1;
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(fin + 1);
+  volatile int* abort = reinterpret_cast<volatile int*>(tslot + 1);
+  int* scan = reinterpret_cast<int*>(tslot + 2);  // one int a warp
+  int* bounds = scan + 6;                         // [E + 1]
+  int* starts = bounds + p.E + 1;                 // [E + 1]
+
+  // Pair: rank 0 issues the MMAs of both CTAs.  Split: the cluster's CTAs share the contraction.
+  const int cluster = kCtas == 2 ? 2 : p.split;
+  const int rank = cluster > 1 ? int(cluster_rank()) : 0;
+  if (tid == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_empty[i], 4 * kCtas);
+    }
+    mbar_init(part_full, 4 * cluster);
+    mbar_init(part_empty, 4 * cluster);
+    mbar_init(fin, 1);
+    fence_mbar_init();
+    *abort = 0;
+  }
+  if (warp == 1) alloc_tmem<kCtas>(tslot, S::kColumns);
+  pdl_wait();
+  const int mtiles = ceil_div(p.M, 128 * kCtas);
+  list_tiles(p.offsets, p.E, p.R, bounds, starts, scan, [&](int rows) {
+    return mtiles * ceil_div(kMode == kWeight ? p.N : rows, kNT);
+  });
+  tc_fence_before();
+  __syncthreads();
+  if (cluster > 1) cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = *tslot;
+  const int tiles = starts[p.E];
+  const int first = int(blockIdx.x) / cluster, stride = int(gridDim.x) / cluster;
+
+  if (kMode != kWeight) {  // rows of no group
+    const int64_t bytes = int64_t(p.M) * (p.out_type == LF_F32 ? 4 : 2);
+    const int64_t pitch = p.out_stride * (p.out_type == LF_F32 ? 4 : 2);
+    for (int64_t r = bounds[p.E] + int64_t(blockIdx.x); r < p.R; r += gridDim.x) {
+      uint8_t* row = static_cast<uint8_t*>(p.out) + r * pitch;
+      if (((reinterpret_cast<uintptr_t>(row) | uintptr_t(bytes)) & 15) == 0) {
+        for (int64_t i = tid * 16; i < bytes; i += kThreads * 16)
+          *reinterpret_cast<uint4*>(row + i) = make_uint4(0, 0, 0, 0);
+      } else {
+        for (int64_t i = tid * 2; i < bytes; i += kThreads * 2) *reinterpret_cast<uint16_t*>(row + i) = 0;
+      }
+    }
+  }
+
+  // The steps of a tile that this CTA takes.
+  auto my_steps = [&](const Tile& x, int* ks0, int* ks1) {
+    if (kCtas == 1 && cluster > 1) {
+      const int each = ceil_div(x.steps, cluster);
+      *ks0 = min(x.steps, rank * each);
+      *ks1 = min(x.steps, *ks0 + each);
+    } else {
+      *ks0 = 0;
+      *ks1 = x.steps;
+    }
+  };
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ loads
+    int it = 0;
+    for (int t = first; t < tiles; t += stride) {
+      const Tile x = tile_of<kMode, kCtas, kNT>(p, bounds, starts, t);
+      const int m_cta = x.m0 + (kCtas == 2 ? rank * 128 : 0);
+      const int share = x.nt / kCtas;  // columns this CTA loads
+      const int n_cta = x.n0 + (kCtas == 2 ? rank * share : 0);
+      int ks0, ks1;
+      my_steps(x, &ks0, &ks1);
+      // Forward: this lane's four rows of the tile (fixed over the steps).
+      int row4[4];
+      if (kMode == kForward && p.rows) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = n_cta + 4 * lane + i;
+          const int src = 4 * lane + i < share && r < x.hi ? p.rows[r] : -1;
+          row4[i] = src >= 0 && src < p.x_rows ? src : p.x_rows;
+        }
+      }
+      // Weight: this lane's four rows of each step, one step ahead (lanes 0-15 the first box, 16-31 the second).
+      auto step_rows = [&](int ks, int (&r4)[4], int (&d4)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = x.lo + ks * kStep + 4 * (lane & 15) + i;
+          const bool in = r < x.hi;
+          const int src = in ? (p.rows ? p.rows[r] : r) : -1;
+          r4[i] = src >= 0 && src < p.x_rows ? src : p.x_rows;
+          d4[i] = in ? r : p.R;
+        }
+      };
+      int x4[4], d4[4], x4n[4], d4n[4];
+      if (kMode == kWeight && ks0 < ks1) step_rows(ks0, x4n, d4n);
+      const uint32_t bytes = kCtas * (kABytes + uint32_t(share) * 128u);
+      bool ok = true;
+      for (int ks = ks0; ks < ks1; ++ks, ++it) {
+        const int st = it % kStages;
+        if (kMode == kWeight) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x4[i] = x4n[i], d4[i] = d4n[i];
+          if (ks + 1 < ks1) step_rows(ks + 1, x4n, d4n);
+        }
+        ok = __all_sync(0xffffffffu, wait_or_abort(&empty[st], (uint32_t(it / kStages) & 1u) ^ 1u, abort));
+        if (!ok) break;
+        const uint32_t a = smem_u32(ring + st * S::kStageBytes), b = a + kABytes;
+        const uint32_t bar = kCtas == 2 ? mapa(&full[st], 0) : smem_u32(&full[st]);
+        if (lane == 0 && rank * (kCtas - 1) == 0) mbar_arrive_expect_tx(&full[st], bytes);
+        __syncwarp();
+        const int c = ks * kStep;
+        if (kMode == kWeight) {
+          const int box = lane >> 4;
+          const bool tail = x.lo + c + kStep > x.hi;
+          if (p.rows || tail) {
+            gather4<kCtas>(a + box * 8192 + (lane & 15) * 512, &p.a_gather, m_cta + 64 * box, x4, bar);
+          } else if (lane < 2) {
+            load_2d<kCtas>(a + lane * 8192, &p.a_map, m_cta + 64 * lane, x.lo + c, bar);
+          }
+          if (box * 64 < share) {
+            if (tail) {
+              gather4<kCtas>(b + box * 8192 + (lane & 15) * 512, &p.b_gather, n_cta + 64 * box, d4, bar);
+            } else if ((lane & 15) == 2) {
+              load_2d<kCtas>(b + box * 8192, &p.b_map, n_cta + 64 * box, x.lo + c, bar);
+            }
+          }
+        } else {
+          if (kMode == kForward) {
+            if (lane == 0) load_3d<kCtas>(a, &p.a_map, c, m_cta, x.e, bar);
+          } else if (lane < 2) {
+            load_3d<kCtas>(a + lane * 8192, &p.a_map, m_cta + 64 * lane, c, x.e, bar);
+          }
+          if (kMode == kForward && p.rows) {
+            if (4 * lane < share) gather4<kCtas>(b + lane * 512, &p.b_gather, c, row4, bar);
+          } else {
+            const int big = share / 64;  // boxes of 64 rows, then of 8
+            const int i = lane - 2;
+            if (i >= 0 && i < big) {
+              load_2d<kCtas>(b + i * 8192, &p.b_map, c, n_cta + 64 * i, bar);
+            } else if (i >= big && i - big < (share - big * 64) / 8) {
+              const int r = big * 64 + (i - big) * 8;
+              load_2d<kCtas>(b + r * 128, &p.b_small, c, n_cta + r, bar);
+            }
+          }
+        }
+      }
+      if (!ok) break;
+    }
+    // A pair's CTA stays until the commits that arrive here from the other CTA have.
+    if (kCtas == 2)
+      for (int j = max(0, it - kStages); j < it; ++j) wait_or_abort(&empty[j % kStages], uint32_t(j / kStages) & 1u, abort);
+    // No load may still be landing when the CTA exits (only an expired wait leaves any).
+    if (*abort && lane == 0 && rank * (kCtas - 1) == 0)
+      for (int j = max(0, it - kStages); j < it; ++j) mbar_wait(&full[j % kStages], uint32_t(j / kStages) & 1u);
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA thread
+    if (lane == 0 && rank * (kCtas - 1) == 0) {
+      int it = 0, count = 0;
+      for (int t = first; t < tiles; t += stride) {
+        const Tile x = tile_of<kMode, kCtas, kNT>(p, bounds, starts, t);
+        int ks0, ks1;
+        my_steps(x, &ks0, &ks1);
+        if (ks0 >= ks1) continue;
+        const int ab = count & 1;
+        if (!wait_cluster(&acc_empty[ab], (uint32_t(count >> 1) & 1u) ^ 1u, abort)) break;
+        ++count;
+        tc_fence_after();
+        const uint32_t d = tmem + uint32_t(ab * kNT);
+        const uint32_t idesc = instruction(p.elem_bf16, kMode != kForward, kMode == kWeight, 128 * kCtas, x.nt);
+        bool ok = true;
+        for (int ks = ks0; ks < ks1; ++ks, ++it) {
+          const int st = it % kStages;
+          ok = wait_or_abort(&full[st], uint32_t(it / kStages) & 1u, abort);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t sa = smem_u32(ring + st * S::kStageBytes);
+          const uint64_t ad = kMode == kForward ? sw128_desc(sa) : mn_desc(sa);
+          const uint64_t bd = kMode == kWeight ? mn_desc(sa + kABytes) : sw128_desc(sa + kABytes);
+          constexpr int kAStep = kMode == kForward ? 2 : 128, kBStep = kMode == kWeight ? 128 : 2;
+#pragma unroll
+          for (int k = 0; k < kStep / 16; ++k)
+            mma_f16<kCtas>(d, ad + kAStep * k, bd + kBStep * k, idesc, (ks > ks0 || k > 0) ? 1u : 0u);
+          commit<kCtas>(&empty[st]);
+        }
+        if (!ok) break;
+        commit<kCtas>(&acc_full[ab]);
+      }
+      if (*abort) {  // every MMA has retired before the TMEM columns are released
+        commit<kCtas>(fin);
+        mbar_wait(fin, 0);
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ stores
+    const int quarter = warp & 3;
+    const uint32_t lanes = uint32_t(quarter * 32) << 16;
+    int count = 0, parts = 0;
+    for (int t = first; t < tiles; t += stride) {
+      const Tile x = tile_of<kMode, kCtas, kNT>(p, bounds, starts, t);
+      int ks0, ks1;
+      my_steps(x, &ks0, &ks1);
+      const bool live = ks1 > ks0;
+      const int ab = count & 1;
+      if (live) {
+        if (!__all_sync(0xffffffffu, wait_or_abort(&acc_full[ab], uint32_t(count >> 1) & 1u, abort))) break;
+        ++count;
+        tc_fence_after();
+      }
+      const uint32_t d = tmem + lanes + uint32_t(ab * kNT);
+      const int f = x.m0 + (kCtas == 2 ? rank * 128 : 0) + quarter * 32 + lane;
+      const int64_t row0 = kMode == kWeight ? int64_t(x.e) * p.N + x.n0 : x.n0;
+      auto release = [&]() {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (kCtas == 2) arrive_cluster(mapa(&acc_empty[ab], 0));
+          else mbar_arrive(&acc_empty[ab]);
+        }
+      };
+      if (kCtas == 1 && cluster > 1) {
+        // Partial sums to this CTA's buffer, then every CTA adds a share of the columns in rank order.
+        if (!__all_sync(0xffffffffu, wait_cluster(part_empty, (uint32_t(parts) & 1u) ^ 1u, abort))) break;
+        for (int c0 = 0; c0 < x.nt; c0 += 16) {
+          uint32_t r[16];
+          if (live) tc_ld16(d + uint32_t(c0), r);
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            part[(c0 + j) * 128 + quarter * 32 + lane] = live ? __uint_as_float(r[j]) : 0.f;
+        }
+        if (live) release();
+        __syncwarp();
+        if (lane < cluster) arrive_cluster(mapa(part_full, lane));
+        if (!__all_sync(0xffffffffu, wait_cluster(part_full, uint32_t(parts) & 1u, abort))) break;
+        ++parts;
+        const uint32_t own = smem_u32(part) + uint32_t(quarter * 32 + lane) * 4u;
+        uint32_t peer[kMaxSplit];
+#pragma unroll
+        for (int q = 0; q < kMaxSplit; ++q)
+          if (q < cluster) asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer[q]) : "r"(own), "r"(q));
+        for (int c = rank; c < x.valid; c += cluster) {
+          float v[kMaxSplit], sum = 0.f;
+#pragma unroll
+          for (int q = 0; q < kMaxSplit; ++q)
+            if (q < cluster) v[q] = lds_cluster(peer[q] + uint32_t(c) * 512u);
+#pragma unroll
+          for (int q = 0; q < kMaxSplit; ++q)
+            if (q < cluster) sum += v[q];
+          if (f < p.M) store_typed(p, (row0 + c) * p.out_stride + f, sum);
+        }
+        __syncwarp();
+        if (lane < cluster) arrive_cluster(mapa(part_empty, lane));
+      } else {
+        for (int c0 = 0; c0 < x.nt; c0 += 16) {
+          uint32_t r[16];
+          if (live) tc_ld16(d + uint32_t(c0), r);
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (f < p.M && c0 + j < x.valid)
+              store_typed(p, (row0 + c0 + j) * p.out_stride + f, live ? __uint_as_float(r[j]) : 0.f);
+        }
+        if (live) release();
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (cluster > 1) cluster_sync();
+  if (warp == 1) {
+    tc_fence_after();
+    free_tmem<kCtas>(tmem, S::kColumns);
+  }
+}
+
+template <int kMode, int kCtas, int kNT>
+int launch_grouped(const GParams& p, int64_t tiles, void* stream, const char* what) {
+  using S = Shape<kCtas, kNT>;
+  int sms = 0;
+  if (int rc = sm_count(&sms)) return rc;
+  const int cluster = kCtas == 2 ? 2 : p.split;
+  int64_t grid = int64_t(sms / cluster) * cluster;
+  if (tiles * cluster < grid) grid = tiles * cluster;
+  const int smem = 1024 + S::kStages * S::kStageBytes + S::kPartBytes + 256 + int(sizeof(int)) * (8 + 2 * (p.E + 1));
+  static int flags[64] = {};
+  if (int rc = ensure_smem(grouped_kernel<kMode, kCtas, kNT>, smem, flags)) return rc;
+  return launch_clusters(grouped_kernel<kMode, kCtas, kNT>, int(grid), cluster, smem, stream, what, p);
+}
+
+// Waves of clusters times a CTA's share of a tile, for a split of S: the least wins, smaller S on a tie.
+int choose_split(int64_t tiles, int steps) {
+  int sms = 148, best = 1;
+  sm_count(&sms);
+  double least = 1e30;
+  for (int s = 1; s <= kMaxSplit; s *= 2) {
+    if (s > 1 && steps < 4 * s) break;
+    const int64_t clusters = sms / s;
+    const double cost = double((tiles + clusters - 1) / clusters) / s;
+    if (cost < 0.95 * least) {
+      least = cost;
+      best = s;
+    }
+  }
+  return best;
+}
+
+constexpr int kWideRows = 256, kNarrowRows = 64;
+
+int check_sizes(const char* what, int dtype, int E, int64_t R, int64_t N, int64_t K) {
+  const int64_t limit = int64_t(1) << 31;
+  if (dtype != LF_BF16 && dtype != LF_F16)
+    return fail(LF_E_INVALID, (std::string(what) + ": operands must be BF16 or FP16").c_str());
+  if (E < 1 || E > kMaxExperts || R < 0 || R >= limit - 256 || N < 1 || K < 1 || N % 8 || K % 8 || N >= limit - 256 ||
+      K >= limit - 256)
+    return fail(LF_E_INVALID,
+                (std::string(what) + ": needs 1..1024 experts, widths that are multiples of 8, and rows that fit int32").c_str());
+  // Tiles are counted in int32, also those of narrow tiles.
+  const int64_t m = (N > K ? N : K) / 128 + 1;
+  if ((R / kNarrowRows + E + 1) * m >= limit || (N / kWideRows + 1) * (K / 256 + 1) * int64_t(E) >= limit)
+    return fail(LF_E_INVALID, (std::string(what) + ": too many tiles").c_str());
+  return LF_OK;
+}
+
+bool good_rows(const void* p, int64_t stride, int64_t width) {
+  return p && aligned16(p) && stride % 8 == 0 && stride >= width;
+}
+
+bool encode_rows(CUtensorMap* map, CUtensorMapDataType type, const void* p, int64_t width, int64_t rows,
+                 int64_t stride, int box_rows) {
+  const cuuint64_t dims[2] = {cuuint64_t(width), cuuint64_t(rows)};
+  const cuuint64_t strides[1] = {cuuint64_t(stride) * 2};
+  const cuuint32_t box[2] = {64, cuuint32_t(box_rows)};
+  return encode_map(map, type, 2, p, dims, strides, box);
+}
+
+bool encode_weights(CUtensorMap* map, CUtensorMapDataType type, const void* w, int64_t K, int64_t N, int64_t E,
+                    int64_t row_stride, int64_t expert_stride, int box_rows) {
+  const cuuint64_t dims[3] = {cuuint64_t(K), cuuint64_t(N), cuuint64_t(E)};
+  const cuuint64_t strides[2] = {cuuint64_t(row_stride) * 2, cuuint64_t(expert_stride) * 2};
+  const cuuint32_t box[3] = {64, cuuint32_t(box_rows), 1};
+  return encode_map(map, type, 3, w, dims, strides, box);
+}
+
+CUtensorMapDataType map_type(int dtype) {
+  return dtype == LF_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+}
+
+// Groups of up to 64 rows on average take the narrow tiles.
+template <int kMode>
+int launch_rows(GParams& p, void* stream, const char* what) {
+  const int64_t groups = p.E < p.R ? p.E : p.R;
+  if (p.R <= kNarrowRows * groups) {
+    const int64_t mt = ceil_div(p.M, 128);
+    const int64_t tiles = mt * (groups + p.R / kNarrowRows);  // at most
+    p.split = choose_split(mt * groups, ceil_div(p.C, kStep));
+    return launch_grouped<kMode, 1, kNarrowRows>(p, tiles, stream, what);
+  }
+  p.split = 1;
+  const int64_t tiles = int64_t(ceil_div(p.M, 256)) * (groups + p.R / kWideRows);
+  return launch_grouped<kMode, 2, kWideRows>(p, tiles, stream, what);
+}
+
+}  // namespace
+
+int grouped_wait_timeouts(unsigned int* value, int reset) {
+  if (cudaMemcpyFromSymbol(value, g_lf_wait_timeouts, sizeof(*value)) != cudaSuccess)
+    return check_launch("device_wait_timeouts (expert products)");
+  if (reset && *value) {
+    const unsigned int zero = 0;
+    if (cudaMemcpyToSymbol(g_lf_wait_timeouts, &zero, sizeof(zero)) != cudaSuccess)
+      return check_launch("device_wait_timeouts (expert products)");
+  }
+  return LF_OK;
+}
+
+}  // namespace lfb
+
+using namespace lfb;
+
+extern "C" int lf_expert_linear(int32_t dtype, const void* x, int64_t x_stride, int64_t x_rows, const int32_t* rows,
+                                const void* w, int64_t w_expert_stride, int64_t w_row_stride, const int32_t* offsets,
+                                int32_t num_experts, int64_t num_rows, int64_t out_width, int64_t width, void* y,
+                                int64_t y_stride, void* stream) {
+  const char* what = "expert_linear";
+  if (int rc = check_sizes(what, dtype, num_experts, num_rows, out_width, width)) return rc;
+  if (num_rows == 0) return LF_OK;
+  if (!offsets || !y || y_stride < out_width || !good_rows(w, w_row_stride, width) || w_expert_stride % 8 ||
+      w_expert_stride < (out_width - 1) * w_row_stride + width)
+    return fail(LF_E_INVALID, "expert_linear: W must be 16-byte aligned with strides that are multiples of 8, y's rows must not overlap");
+  if (x_rows < 1 || x_rows >= (int64_t(1) << 31) - 1 || (!rows && x_rows < num_rows) || !good_rows(x, x_stride, width))
+    return fail(LF_E_INVALID, "expert_linear: x must have rows, 16-byte aligned, with a stride that is a multiple of 8");
+  GParams p{};
+  p.offsets = offsets, p.rows = rows, p.out = y, p.out_stride = y_stride;
+  p.E = num_experts, p.R = int(num_rows), p.x_rows = int(x_rows);
+  p.M = int(out_width), p.C = int(width), p.out_type = dtype, p.elem_bf16 = dtype == LF_BF16;
+  const CUtensorMapDataType type = map_type(dtype);
+  if (!encode_weights(&p.a_map, type, w, width, out_width, num_experts, w_row_stride, w_expert_stride, 128) ||
+      !encode_rows(&p.b_map, type, x, width, x_rows, x_stride, 64) ||
+      !encode_rows(&p.b_small, type, x, width, x_rows, x_stride, 8) ||
+      !encode_rows(&p.b_gather, type, x, width, x_rows, x_stride, 1))
+    return fail(LF_E_CUDA, "expert_linear: cuTensorMapEncodeTiled failed");
+  return launch_rows<kForward>(p, stream, what);
+}
+
+extern "C" int lf_expert_linear_input_grad(int32_t dtype, const void* dy, int64_t dy_stride, const void* w,
+                                           int64_t w_expert_stride, int64_t w_row_stride, const int32_t* offsets,
+                                           int32_t num_experts, int64_t num_rows, int64_t out_width, int64_t width,
+                                           void* dx, int64_t dx_stride, void* stream) {
+  const char* what = "expert_linear_input_grad";
+  if (int rc = check_sizes(what, dtype, num_experts, num_rows, out_width, width)) return rc;
+  if (num_rows == 0) return LF_OK;
+  if (!offsets || !dx || dx_stride < width || !good_rows(w, w_row_stride, width) || w_expert_stride % 8 ||
+      w_expert_stride < (out_width - 1) * w_row_stride + width || !good_rows(dy, dy_stride, out_width))
+    return fail(LF_E_INVALID, "expert_linear_input_grad: W and dy must be 16-byte aligned with strides that are multiples of 8, dx's rows must not overlap");
+  GParams p{};
+  p.offsets = offsets, p.out = dx, p.out_stride = dx_stride;
+  p.E = num_experts, p.R = int(num_rows), p.x_rows = int(num_rows);
+  p.M = int(width), p.C = int(out_width), p.out_type = dtype, p.elem_bf16 = dtype == LF_BF16;
+  const CUtensorMapDataType type = map_type(dtype);
+  if (!encode_weights(&p.a_map, type, w, width, out_width, num_experts, w_row_stride, w_expert_stride, 64) ||
+      !encode_rows(&p.b_map, type, dy, out_width, num_rows, dy_stride, 64) ||
+      !encode_rows(&p.b_small, type, dy, out_width, num_rows, dy_stride, 8))
+    return fail(LF_E_CUDA, "expert_linear_input_grad: cuTensorMapEncodeTiled failed");
+  return launch_rows<kInput>(p, stream, what);
+}
+
+extern "C" int lf_expert_linear_weight_grad(int32_t dtype, const void* dy, int64_t dy_stride, const void* x,
+                                            int64_t x_stride, int64_t x_rows, const int32_t* rows,
+                                            const int32_t* offsets, int32_t num_experts, int64_t num_rows,
+                                            int64_t out_width, int64_t width, int32_t out_dtype, void* dw,
+                                            void* stream) {
+  const char* what = "expert_linear_weight_grad";
+  if (int rc = check_sizes(what, dtype, num_experts, num_rows, out_width, width)) return rc;
+  if (out_dtype != dtype && out_dtype != LF_F32)
+    return fail(LF_E_INVALID, "expert_linear_weight_grad: dW is of the operands' type or FP32");
+  if (!dw) return fail(LF_E_INVALID, "expert_linear_weight_grad: null buffer");
+  if (num_rows == 0) {
+    const size_t bytes = size_t(num_experts) * out_width * width * (out_dtype == LF_F32 ? 4 : 2);
+    if (cudaMemsetAsync(dw, 0, bytes, static_cast<cudaStream_t>(stream)) != cudaSuccess) return check_launch(what);
+    return LF_OK;
+  }
+  if (!offsets || x_rows < 1 || x_rows >= (int64_t(1) << 31) - 1 || (!rows && x_rows < num_rows) ||
+      !good_rows(x, x_stride, width) || !good_rows(dy, dy_stride, out_width))
+    return fail(LF_E_INVALID, "expert_linear_weight_grad: x and dy must have rows, 16-byte aligned, with strides that are multiples of 8");
+  GParams p{};
+  p.offsets = offsets, p.rows = rows, p.out = dw, p.out_stride = width;
+  p.E = num_experts, p.R = int(num_rows), p.x_rows = int(x_rows);
+  p.M = int(width), p.N = int(out_width), p.out_type = out_dtype, p.elem_bf16 = dtype == LF_BF16, p.split = 1;
+  const CUtensorMapDataType type = map_type(dtype);
+  if (!encode_rows(&p.a_map, type, x, width, x_rows, x_stride, 64) ||
+      !encode_rows(&p.a_gather, type, x, width, x_rows, x_stride, 1) ||
+      !encode_rows(&p.b_map, type, dy, out_width, num_rows, dy_stride, 64) ||
+      !encode_rows(&p.b_gather, type, dy, out_width, num_rows, dy_stride, 1))
+    return fail(LF_E_CUDA, "expert_linear_weight_grad: cuTensorMapEncodeTiled failed");
+  const int64_t tiles = int64_t(ceil_div(p.M, 256)) * ceil_div(p.N, kWideRows) * num_experts;
+  return launch_grouped<kWeight, 2, kWideRows>(p, tiles, stream, what);
+}

@@ -1736,7 +1736,9 @@ extern "C" int lf_device_wait_timeouts(int32_t* count, int32_t reset) {
     return check_launch("device_wait_timeouts");
   unsigned int prefill = 0;
   if (int rc = prefill_wait_timeouts(&prefill, reset)) return rc;
-  if (count) *count = int32_t(value + prefill);
+  unsigned int grouped = 0;
+  if (int rc = grouped_wait_timeouts(&grouped, reset)) return rc;
+  if (count) *count = int32_t(value + prefill + grouped);
   if (reset) {
     const unsigned int zero = 0;
     if (cudaMemcpyToSymbol(g_lf_wait_timeouts, &zero, sizeof(zero)) != cudaSuccess)

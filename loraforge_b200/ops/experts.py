@@ -1,7 +1,8 @@
-"""Mixture-of-experts operators over the sm_100a C ABI: routing and the sum over experts.
+"""Mixture-of-experts operators over the sm_100a C ABI: routing, the experts' products, their sum.
 
 A layer with E experts runs ``route_experts`` on its router's logits, multiplies the rows it
-gives by their experts' weights, and adds each token's rows up with ``combine_experts``.
+gives by their experts' weights (``expert_linear``, which reads the tokens' rows through the
+tables), and adds each token's rows up with ``combine_experts``.
 Every operator reads its tables on the device, so a layer can be captured in a CUDA graph;
 the LoRA operators take the same batch beside it (the rows of a token keep its adapter).
 Each forward has an explicit gradient (``*_backward``).  The reference has no counterpart.
@@ -224,3 +225,115 @@ def combine_experts_backward(grad, y, weights, positions):
             None if weights is None else grad_weights.data_ptr(), _native.stream_of(y.device),
         )
     return grad_y, grad_weights
+
+
+def _halves():
+    import torch
+
+    return (torch.float16, torch.bfloat16)
+
+
+def _operand(value, name: str, dtypes, device=None) -> None:
+    """A row matrix that TMA can read: aligned, its row stride a multiple of 8."""
+    row_matrix(value, name, dtypes, device)
+    if value.shape[1] < 8 or value.shape[1] % 8 or (value.shape[0] > 1 and value.stride(0) % 8) or value.data_ptr() % 16:
+        raise ValueError(f"{name} must be 16-byte aligned with a width and row stride that are multiples of 8")
+
+
+def _expert_weight(weight, dtype, device) -> None:
+    cuda_tensor(weight, "weight", 3, (dtype,), device)
+    E, N, K = weight.shape
+    if not 1 <= E <= MAX_EXPERTS or N < 8 or N % 8 or K < 8 or K % 8:
+        raise ValueError(f"weight must be [experts, out, in] with 1..{MAX_EXPERTS} experts and widths that are multiples of 8")
+    if (weight.stride(2) != 1 or weight.stride(1) % 8 or weight.stride(1) < K or weight.data_ptr() % 16
+            or (E > 1 and (weight.stride(0) % 8 or weight.stride(0) < (N - 1) * weight.stride(1) + K))):
+        raise ValueError("weight must be 16-byte aligned with unit inner stride and outer strides that are multiples of 8")
+
+
+def expert_stride(weight) -> int:
+    """Stride between experts (a single expert's own stride says nothing)."""
+    return weight.stride(0) if weight.shape[0] > 1 else weight.shape[1] * weight.stride(1)
+
+
+def group_tables(offsets, rows, num_experts: int, x_rows: int, device) -> int:
+    """Checks ``offsets`` [E + 1] and ``rows`` [R] (or None); the number of rows R."""
+    import torch
+
+    packed_table(offsets, "offsets", (num_experts + 1,), device, torch.int32)
+    if rows is None:
+        return x_rows
+    cuda_tensor(rows, "rows", 1, (torch.int32,), device)
+    packed_table(rows, "rows", (rows.numel(),), device, torch.int32)
+    if rows.numel() and not x_rows:
+        raise ValueError("x must have at least one row")
+    return rows.numel()
+
+
+def expert_linear(x, weight, offsets, *, rows=None, out=None):
+    """``y[r] = weight[e] @ x[rows[r]]`` for the rows ``offsets[e] <= r < offsets[e+1]`` of expert e.
+
+    ``x`` [T, K] and ``weight`` [E, N, K] are BF16 or FP16 (both the same; widths multiples of
+    8); ``offsets`` int32 [E + 1] and ``rows`` int32 [R] are ``route_experts``' tables.  Without
+    ``rows``, x's own rows are the sorted ones.  Sums are FP32, rounded once; rows of no group
+    are zeros.  Returns y [R, N] (``out`` when given).
+    """
+    import torch
+
+    _operand(x, "x", _halves())
+    _expert_weight(weight, x.dtype, x.device)
+    E, N, K = weight.shape
+    if x.shape[1] != K:
+        raise ValueError("x's width must be the weight's")
+    R = group_tables(offsets, rows, E, x.shape[0], x.device)
+    if out is None:
+        out = torch.empty((R, N), dtype=x.dtype, device=x.device)
+    else:
+        row_matrix(out, "out", (x.dtype,), x.device)
+        if tuple(out.shape) != (R, N):
+            raise ValueError("out must be [rows, out features]")
+        output_is_distinct(out, (x, weight, offsets) if rows is None else (x, weight, offsets, rows))
+    with torch.cuda.device(x.device):
+        _native.call(
+            "lf_expert_linear", _native.dtype_code(x.dtype), x.data_ptr(), row_stride(x), x.shape[0],
+            None if rows is None else rows.data_ptr(), weight.data_ptr(), expert_stride(weight), weight.stride(1),
+            offsets.data_ptr(), E, R, N, K, out.data_ptr(), row_stride(out), _native.stream_of(x.device),
+        )
+    return out
+
+
+def expert_linear_backward(grad, x, weight, offsets, *, rows=None, weight_grad_dtype=None):
+    """Gradients of ``expert_linear``: (grad_x [R, K], grad_weight [E, N, K]).
+
+    ``grad`` [R, N] is the gradient of y.  ``grad_x`` is by row; ``combine_experts(grad_x,
+    None, positions)`` adds it up by token.  ``weight_grad_dtype`` is the operands' type
+    (default) or FP32.  Experts without rows get zeros.
+    """
+    import torch
+
+    _operand(x, "x", _halves())
+    _expert_weight(weight, x.dtype, x.device)
+    _operand(grad, "grad", (x.dtype,), x.device)
+    E, N, K = weight.shape
+    if x.shape[1] != K:
+        raise ValueError("x's width must be the weight's")
+    R = group_tables(offsets, rows, E, x.shape[0], x.device)
+    if tuple(grad.shape) != (R, N):
+        raise ValueError("grad must be [rows, out features]")
+    weight_grad_dtype = x.dtype if weight_grad_dtype is None else weight_grad_dtype
+    if weight_grad_dtype not in (x.dtype, torch.float32):
+        raise ValueError("weight_grad_dtype must be the operands' type or float32")
+    grad_x = torch.empty((R, K), dtype=x.dtype, device=x.device)
+    grad_weight = torch.empty((E, N, K), dtype=weight_grad_dtype, device=x.device)
+    dtype = _native.dtype_code(x.dtype)
+    with torch.cuda.device(x.device):
+        stream = _native.stream_of(x.device)
+        _native.call(
+            "lf_expert_linear_input_grad", dtype, grad.data_ptr(), row_stride(grad), weight.data_ptr(),
+            expert_stride(weight), weight.stride(1), offsets.data_ptr(), E, R, N, K, grad_x.data_ptr(), K, stream,
+        )
+        _native.call(
+            "lf_expert_linear_weight_grad", dtype, grad.data_ptr(), row_stride(grad), x.data_ptr(), row_stride(x),
+            x.shape[0], None if rows is None else rows.data_ptr(), offsets.data_ptr(), E, R, N, K,
+            _native.dtype_code(weight_grad_dtype), grad_weight.data_ptr(), stream,
+        )
+    return grad_x, grad_weight
