@@ -459,13 +459,16 @@ int lf_combine_experts_backward(int32_t dtype, const void* grad, int64_t grad_st
  * for an empty group) theirs or FP32 (out_dtype).  An i(r) outside [0, x_rows) reads a zero row.
  * dx is by row: lf_combine_experts with weights = NULL adds it up by token.
  * Widths are multiples of 8; x, dy and W 16-byte aligned with strides that are multiples of 8.
- * One launch each, no workspace.
+ * With rows, groups of many rows and the weight gradient copy x's rows in order into `workspace`
+ * first: lf_expert_linear_workspace_bytes bytes, 16-byte aligned, not initialised (0: none needed).
  */
+int64_t lf_expert_linear_workspace_bytes(int32_t num_experts, int64_t num_rows, int64_t width,
+                                         int32_t weight_grad);
 int lf_expert_linear(int32_t dtype, const void* x, int64_t x_stride, int64_t x_rows,
                      const int32_t* rows, const void* w, int64_t w_expert_stride,
                      int64_t w_row_stride, const int32_t* offsets, int32_t num_experts,
                      int64_t num_rows, int64_t out_width, int64_t width, void* y,
-                     int64_t y_stride, void* stream);
+                     int64_t y_stride, void* workspace, int64_t workspace_bytes, void* stream);
 int lf_expert_linear_input_grad(int32_t dtype, const void* dy, int64_t dy_stride, const void* w,
                                 int64_t w_expert_stride, int64_t w_row_stride,
                                 const int32_t* offsets, int32_t num_experts, int64_t num_rows,
@@ -475,7 +478,7 @@ int lf_expert_linear_weight_grad(int32_t dtype, const void* dy, int64_t dy_strid
                                  int64_t x_stride, int64_t x_rows, const int32_t* rows,
                                  const int32_t* offsets, int32_t num_experts, int64_t num_rows,
                                  int64_t out_width, int64_t width, int32_t out_dtype, void* dw,
-                                 void* stream);
+                                 void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
  * MXFP4: blocks of 32 values along a row share 2^e, e = floor(log2 max|x|) - 2 (>= -127), held

@@ -11,15 +11,18 @@
 // rows of padding, and a lane's neighbours are neighbours in the output row: a warp stores 32
 // adjacent features of one row at a time.
 //
-//   mode      A (lanes)                     B (columns)                 contraction
-//   forward   W[e], K-major                 x rows, K-major, gathered   K
-//   input     W[e], MN-major (k on lanes)   dy rows, K-major            N
-//   weight    x rows, MN-major, gathered    dy rows, MN-major           the group's rows
+//   mode      A (lanes)                     B (columns)          contraction
+//   forward   W[e], K-major                 x rows, K-major      K
+//   input     W[e], MN-major (k on lanes)   dy rows, K-major     N
+//   weight    x rows, MN-major              dy rows, MN-major    the group's rows
 //
-// Nothing is transposed or gathered in memory: MN-major operands are read as they lie through
-// the shared-memory descriptor, and x's rows by token come with gather4 loads.  Steps past K, N
-// or a group's last row read zeros (out of bounds for the tensor map, or a row index that is),
-// so a neighbouring group's infinities never reach a sum.
+// Nothing is transposed in memory: MN-major operands are read as they lie through the
+// shared-memory descriptor.  Steps past K, N or a group's last row read zeros (out of bounds for
+// the tensor map, or a row index that is), so a neighbouring group's infinities never reach a
+// sum.  x's rows by token: the narrow tiles fetch them with gather4 loads.  Those move about one
+// 128-byte row per 20 cycles and SM, a third of what the wide tiles take (8 experts, 16384 rows,
+// 4096 -> 14336: 4340 us against 1475 with rows in order), so for these gather_rows_kernel
+// copies the rows into the caller's workspace first (2 x 134 MB there, some 45 us).
 //
 // Per CTA: warp 0 loads 64-deep stages into a ring, warp 1 issues the MMAs and owns the TMEM
 // (two accumulators, so a tile's stores overlap the next tile's MMAs), warps 2-5 store.  The
@@ -44,6 +47,7 @@ enum Mode { kForward = 0, kInput = 1, kWeight = 2 };
 constexpr int kStep = 64;             // contraction per stage: 128 bytes
 constexpr int kABytes = 128 * 128;    // 128 features x 128 bytes (K-major), or two 64-feature boxes of 64 steps
 constexpr int kMaxSplit = 8;
+constexpr int kChunkBytes = 32 * 64;  // 32 columns x 32 features of a warp, 16 bits
 
 struct GParams {
   const int32_t* offsets;  // [E + 1]
@@ -55,9 +59,10 @@ struct GParams {
   int N;     // weight: columns of D (dy's features)
   int out_type, elem_bf16, split;
   CUtensorMap a_map;     // forward: W boxes 64 k x 128 n; input: 64 k x 64 n; weight: x boxes 64 k x 64 rows
+  CUtensorMap a_small;   // weight: 64 k x 8 rows
   CUtensorMap a_gather;  // weight: single x rows of 64 k
-  CUtensorMap b_map;     // forward / input: 64 wide x 64 rows; weight: dy boxes 64 n x 64 rows
-  CUtensorMap b_small;   // forward / input: 64 wide x 8 rows
+  CUtensorMap b_map;     // rows of x or dy, boxes 64 wide x 64 rows
+  CUtensorMap b_small;   // 64 wide x 8 rows
   CUtensorMap b_gather;  // forward: single x rows; weight: single dy rows
 };
 
@@ -65,7 +70,7 @@ template <int kCtas, int kNT>
 struct Shape {
   static constexpr int kBRows = kNT / kCtas;  // a CTA's share of the columns
   static constexpr int kStageBytes = kABytes + kBRows * 128;
-  static constexpr int kPartBytes = kCtas == 1 ? kNT * 128 * 4 : 0;
+  static constexpr int kPartBytes = kCtas == 1 ? kNT * 128 * 4 : 4 * kChunkBytes;  // sums, or the stores' staging
   static constexpr int kStages = 6;
   static constexpr int kColumns = 2 * kNT;  // TMEM
 };
@@ -122,6 +127,45 @@ __device__ __forceinline__ void store_typed(const GParams& p, int64_t at, float 
   if (p.out_type == LF_BF16) store_out<bf16_t>(p.out, at, v);
   else if (p.out_type == LF_F16) store_out<f16_t>(p.out, at, v);
   else store_out<f32_t>(p.out, at, v);
+}
+
+// Columns c0 .. c0 + 31 of this warp's 32 features as 16-bit values to global memory.  The
+// accumulator is read in the fragment shape whose transpose stmatrix writes, so that a column's
+// 32 features (64 bytes) lie together in the warp's staging, 16-byte chunks swizzled by column;
+// each store instruction then writes eight columns.  `dst`: feature 0 of column c0.
+__device__ __forceinline__ void store_chunk(uint32_t taddr, bool live, uint32_t staging, int bf16, uint8_t* dst,
+                                            int64_t pitch, int columns, int features, int lane) {
+  uint32_t r[32];
+  if (live) {
+    ld_fragments(taddr, r);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) r[i] = 0;
+  }
+  __syncwarp();  // the previous chunk has left the staging
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {  // eight columns each
+    uint32_t m[4];
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {  // eight features each
+      const uint32_t lo = r[(h >> 1) * 16 + 4 * j + 2 * (h & 1)], hi = r[(h >> 1) * 16 + 4 * j + 2 * (h & 1) + 1];
+      if (bf16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(m[h]) : "f"(__uint_as_float(hi)), "f"(__uint_as_float(lo)));
+      else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(m[h]) : "f"(__uint_as_float(hi)), "f"(__uint_as_float(lo)));
+    }
+    const int col = 8 * j + (lane & 7), chunk = lane >> 3;
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(
+                     staging + uint32_t(col * 64 + ((chunk ^ (col >> 1 & 3)) << 4))),
+                 "r"(m[0]), "r"(m[1]), "r"(m[2]), "r"(m[3])
+                 : "memory");
+  }
+  __syncwarp();
+  const int chunk = lane & 3;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int col = 8 * i + (lane >> 2);
+    const uint4 v = lds16(staging + uint32_t(col * 64 + ((chunk ^ (col >> 1 & 3)) << 4)));
+    if (col < columns && 8 * chunk < features) *reinterpret_cast<uint4*>(dst + col * pitch + 16 * chunk) = v;
+  }
 }
 
 template <int kMode, int kCtas, int kNT>
@@ -216,7 +260,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(const __grid_const
       my_steps(x, &ks0, &ks1);
       // Forward: this lane's four rows of the tile (fixed over the steps).
       int row4[4];
-      if (kMode == kForward && p.rows) {
+      if (kMode == kForward && kCtas == 1 && p.rows) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int r = n_cta + 4 * lane + i;
@@ -224,48 +268,40 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(const __grid_const
           row4[i] = src >= 0 && src < p.x_rows ? src : p.x_rows;
         }
       }
-      // Weight: this lane's four rows of each step, one step ahead (lanes 0-15 the first box, 16-31 the second).
-      auto step_rows = [&](int ks, int (&r4)[4], int (&d4)[4]) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = x.lo + ks * kStep + 4 * (lane & 15) + i;
-          const bool in = r < x.hi;
-          const int src = in ? (p.rows ? p.rows[r] : r) : -1;
-          r4[i] = src >= 0 && src < p.x_rows ? src : p.x_rows;
-          d4[i] = in ? r : p.R;
-        }
-      };
-      int x4[4], d4[4], x4n[4], d4n[4];
-      if (kMode == kWeight && ks0 < ks1) step_rows(ks0, x4n, d4n);
-      const uint32_t bytes = kCtas * (kABytes + uint32_t(share) * 128u);
+      const uint32_t whole = kCtas * (kABytes + uint32_t(share) * 128u);
       bool ok = true;
       for (int ks = ks0; ks < ks1; ++ks, ++it) {
         const int st = it % kStages;
-        if (kMode == kWeight) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) x4[i] = x4n[i], d4[i] = d4n[i];
-          if (ks + 1 < ks1) step_rows(ks + 1, x4n, d4n);
-        }
         ok = __all_sync(0xffffffffu, wait_or_abort(&empty[st], (uint32_t(it / kStages) & 1u) ^ 1u, abort));
         if (!ok) break;
         const uint32_t a = smem_u32(ring + st * S::kStageBytes), b = a + kABytes;
         const uint32_t bar = kCtas == 2 ? mapa(&full[st], 0) : smem_u32(&full[st]);
+        const int c = ks * kStep;
+        // Weight: the rows of this step; the last one is loaded by 8 rows up to a multiple of 16.
+        const int left = kMode == kWeight ? min(kStep, x.hi - x.lo - c) : kStep;
+        const uint32_t bytes = left == kStep ? whole : whole / kStep * uint32_t(round_up(left, 16));
         if (lane == 0 && rank * (kCtas - 1) == 0) mbar_arrive_expect_tx(&full[st], bytes);
         __syncwarp();
-        const int c = ks * kStep;
         if (kMode == kWeight) {
-          const int box = lane >> 4;
-          const bool tail = x.lo + c + kStep > x.hi;
-          if (p.rows || tail) {
-            gather4<kCtas>(a + box * 8192 + (lane & 15) * 512, &p.a_gather, m_cta + 64 * box, x4, bar);
-          } else if (lane < 2) {
-            load_2d<kCtas>(a + lane * 8192, &p.a_map, m_cta + 64 * lane, x.lo + c, bar);
-          }
-          if (box * 64 < share) {
-            if (tail) {
-              gather4<kCtas>(b + box * 8192 + (lane & 15) * 512, &p.b_gather, n_cta + 64 * box, d4, bar);
-            } else if ((lane & 15) == 2) {
-              load_2d<kCtas>(b + box * 8192, &p.b_map, n_cta + 64 * box, x.lo + c, bar);
+          // Boxes of 64 features: two of x (lanes 0-15), one or two of dy (lanes 16-31).
+          const bool is_x = lane < 16;
+          const int box = lane >> 3 & 1, unit = lane & 7;
+          const int col = (is_x ? m_cta : n_cta) + 64 * box;
+          const uint32_t dst = (is_x ? a : b) + box * 8192 + unit * 1024;
+          const int r = x.lo + c + 8 * unit;
+          if (is_x || box * 64 < share) {
+            if (left == kStep) {
+              if (unit == 0) load_2d<kCtas>(dst, is_x ? &p.a_map : &p.b_map, col, r, bar);
+            } else if (8 * unit + 8 <= left) {
+              load_2d<kCtas>(dst, is_x ? &p.a_small : &p.b_small, col, r, bar);
+            } else if (8 * unit < round_up(left, 16)) {  // rows past the group's last read zeros
+#pragma unroll
+              for (int q = 0; q < 2; ++q) {
+                int r4[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) r4[i] = r + 4 * q + i < x.hi ? r + 4 * q + i : is_x ? p.x_rows : p.R;
+                gather4<kCtas>(dst + q * 512, is_x ? &p.a_gather : &p.b_gather, col, r4, bar);
+              }
             }
           }
         } else {
@@ -274,7 +310,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(const __grid_const
           } else if (lane < 2) {
             load_3d<kCtas>(a + lane * 8192, &p.a_map, m_cta + 64 * lane, c, x.e, bar);
           }
-          if (kMode == kForward && p.rows) {
+          if (kMode == kForward && kCtas == 1 && p.rows) {
             if (4 * lane < share) gather4<kCtas>(b + lane * 512, &p.b_gather, c, row4, bar);
           } else {
             const int big = share / 64;  // boxes of 64 rows, then of 8
@@ -321,9 +357,11 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(const __grid_const
           const uint64_t ad = kMode == kForward ? sw128_desc(sa) : mn_desc(sa);
           const uint64_t bd = kMode == kWeight ? mn_desc(sa + kABytes) : sw128_desc(sa + kABytes);
           constexpr int kAStep = kMode == kForward ? 2 : 128, kBStep = kMode == kWeight ? 128 : 2;
+          const int subs = kMode == kWeight ? min(kStep, round_up(x.hi - x.lo - ks * kStep, 16)) / 16 : kStep / 16;
 #pragma unroll
           for (int k = 0; k < kStep / 16; ++k)
-            mma_f16<kCtas>(d, ad + kAStep * k, bd + kBStep * k, idesc, (ks > ks0 || k > 0) ? 1u : 0u);
+            if (kMode != kWeight || k < subs)
+              mma_f16<kCtas>(d, ad + kAStep * k, bd + kBStep * k, idesc, (ks > ks0 || k > 0) ? 1u : 0u);
           commit<kCtas>(&empty[st]);
         }
         if (!ok) break;
@@ -338,6 +376,8 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(const __grid_const
     // ------------------------------------------------------------ stores
     const int quarter = warp & 3;
     const uint32_t lanes = uint32_t(quarter * 32) << 16;
+    const uint32_t staging = smem_u32(part) + uint32_t(quarter * kChunkBytes);
+    const bool vector = p.out_type != LF_F32 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0 && p.out_stride % 8 == 0;
     int count = 0, parts = 0;
     for (int t = first; t < tiles; t += stride) {
       const Tile x = tile_of<kMode, kCtas, kNT>(p, bounds, starts, t);
@@ -394,13 +434,21 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(const __grid_const
         __syncwarp();
         if (lane < cluster) arrive_cluster(mapa(part_empty, lane));
       } else {
-        for (int c0 = 0; c0 < x.nt; c0 += 16) {
-          uint32_t r[16];
-          if (live) tc_ld16(d + uint32_t(c0), r);
+        if (vector) {
+          const int f0 = f - lane;
+          uint8_t* dst = static_cast<uint8_t*>(p.out) + (row0 * p.out_stride + f0) * 2;
+          for (int c0 = 0; c0 < x.valid; c0 += 32)
+            store_chunk(d + uint32_t(c0), live, staging, p.out_type == LF_BF16, dst + c0 * p.out_stride * 2,
+                        p.out_stride * 2, x.valid - c0, p.M - f0, lane);
+        } else {
+          for (int c0 = 0; c0 < x.nt; c0 += 16) {
+            uint32_t r[16];
+            if (live) tc_ld16(d + uint32_t(c0), r);
 #pragma unroll
-          for (int j = 0; j < 16; ++j)
-            if (f < p.M && c0 + j < x.valid)
-              store_typed(p, (row0 + c0 + j) * p.out_stride + f, live ? __uint_as_float(r[j]) : 0.f);
+            for (int j = 0; j < 16; ++j)
+              if (f < p.M && c0 + j < x.valid)
+                store_typed(p, (row0 + c0 + j) * p.out_stride + f, live ? __uint_as_float(r[j]) : 0.f);
+          }
         }
         if (live) release();
       }
@@ -413,6 +461,47 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(const __grid_const
     tc_fence_after();
     free_tmem<kCtas>(tmem, S::kColumns);
   }
+}
+
+// out[r] = x[rows[r]], zeros for an index outside x: 16 bytes a thread and step, four in flight.
+__global__ void __launch_bounds__(256) gather_rows_kernel(const uint4* x, int64_t stride, int x_rows,
+                                                          const int32_t* rows, int chunks, int64_t total, uint4* out) {
+  pdl_wait();
+  const int64_t first = int64_t(blockIdx.x) * 1024 + threadIdx.x;
+  uint4 v[4];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const int64_t i = first + u * 256;
+    if (i >= total) continue;
+    const int64_t r = i / chunks;
+    const int src = rows[r];
+    v[u] = src >= 0 && src < x_rows ? x[src * stride + (i - r * chunks)] : make_uint4(0, 0, 0, 0);
+  }
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    if (first + u * 256 < total) out[first + u * 256] = v[u];
+}
+
+int gather_rows(const void* x, int64_t x_stride, int64_t x_rows, const int32_t* rows, int64_t R, int64_t width,
+                void* out, void* stream, const char* what) {
+  cudaLaunchConfig_t config = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = attr;
+  config.numAttrs = 1;
+  const int64_t total = R * (width / 8);
+  config.gridDim = dim3(unsigned((total + 1023) / 1024));
+  config.blockDim = dim3(256);
+  config.stream = static_cast<cudaStream_t>(stream);
+  const cudaError_t err =
+      cudaLaunchKernelEx(&config, gather_rows_kernel, static_cast<const uint4*>(x), x_stride / 8, int(x_rows), rows,
+                         int(width / 8), total, static_cast<uint4*>(out));
+  if (err != cudaSuccess) {
+    last_error() = std::string(what) + ": " + cudaGetErrorString(err);
+    return LF_E_CUDA;
+  }
+  return LF_OK;
 }
 
 template <int kMode, int kCtas, int kNT>
@@ -447,6 +536,7 @@ int choose_split(int64_t tiles, int steps) {
 }
 
 constexpr int kWideRows = 256, kNarrowRows = 64;
+constexpr char kNoWorkspace[] = "expert_linear: workspace missing, too small or not 16-byte aligned (see lf_expert_linear_workspace_bytes)";
 
 int check_sizes(const char* what, int dtype, int E, int64_t R, int64_t N, int64_t K) {
   const int64_t limit = int64_t(1) << 31;
@@ -488,10 +578,12 @@ CUtensorMapDataType map_type(int dtype) {
 }
 
 // Groups of up to 64 rows on average take the narrow tiles.
+bool narrow(int64_t E, int64_t R) { return R <= kNarrowRows * (E < R ? E : R); }
+
 template <int kMode>
 int launch_rows(GParams& p, void* stream, const char* what) {
   const int64_t groups = p.E < p.R ? p.E : p.R;
-  if (p.R <= kNarrowRows * groups) {
+  if (narrow(p.E, p.R)) {
     const int64_t mt = ceil_div(p.M, 128);
     const int64_t tiles = mt * (groups + p.R / kNarrowRows);  // at most
     p.split = choose_split(mt * groups, ceil_div(p.C, kStep));
@@ -519,10 +611,16 @@ int grouped_wait_timeouts(unsigned int* value, int reset) {
 
 using namespace lfb;
 
+extern "C" int64_t lf_expert_linear_workspace_bytes(int32_t num_experts, int64_t num_rows, int64_t width,
+                                                    int32_t weight_grad) {
+  if (num_experts < 1 || num_rows < 0 || width < 1) return -1;
+  return weight_grad || !narrow(num_experts, num_rows) ? num_rows * width * 2 : 0;
+}
+
 extern "C" int lf_expert_linear(int32_t dtype, const void* x, int64_t x_stride, int64_t x_rows, const int32_t* rows,
                                 const void* w, int64_t w_expert_stride, int64_t w_row_stride, const int32_t* offsets,
                                 int32_t num_experts, int64_t num_rows, int64_t out_width, int64_t width, void* y,
-                                int64_t y_stride, void* stream) {
+                                int64_t y_stride, void* workspace, int64_t workspace_bytes, void* stream) {
   const char* what = "expert_linear";
   if (int rc = check_sizes(what, dtype, num_experts, num_rows, out_width, width)) return rc;
   if (num_rows == 0) return LF_OK;
@@ -531,6 +629,14 @@ extern "C" int lf_expert_linear(int32_t dtype, const void* x, int64_t x_stride, 
     return fail(LF_E_INVALID, "expert_linear: W must be 16-byte aligned with strides that are multiples of 8, y's rows must not overlap");
   if (x_rows < 1 || x_rows >= (int64_t(1) << 31) - 1 || (!rows && x_rows < num_rows) || !good_rows(x, x_stride, width))
     return fail(LF_E_INVALID, "expert_linear: x must have rows, 16-byte aligned, with a stride that is a multiple of 8");
+  if (rows) {
+    const int64_t need = lf_expert_linear_workspace_bytes(num_experts, num_rows, width, 0);
+    if (need) {
+      if (!workspace || workspace_bytes < need || !aligned16(workspace)) return fail(LF_E_INVALID, kNoWorkspace);
+      if (int rc = gather_rows(x, x_stride, x_rows, rows, num_rows, width, workspace, stream, what)) return rc;
+      x = workspace, x_stride = width, x_rows = num_rows, rows = nullptr;
+    }
+  }
   GParams p{};
   p.offsets = offsets, p.rows = rows, p.out = y, p.out_stride = y_stride;
   p.E = num_experts, p.R = int(num_rows), p.x_rows = int(x_rows);
@@ -570,7 +676,7 @@ extern "C" int lf_expert_linear_weight_grad(int32_t dtype, const void* dy, int64
                                             int64_t x_stride, int64_t x_rows, const int32_t* rows,
                                             const int32_t* offsets, int32_t num_experts, int64_t num_rows,
                                             int64_t out_width, int64_t width, int32_t out_dtype, void* dw,
-                                            void* stream) {
+                                            void* workspace, int64_t workspace_bytes, void* stream) {
   const char* what = "expert_linear_weight_grad";
   if (int rc = check_sizes(what, dtype, num_experts, num_rows, out_width, width)) return rc;
   if (out_dtype != dtype && out_dtype != LF_F32)
@@ -584,14 +690,21 @@ extern "C" int lf_expert_linear_weight_grad(int32_t dtype, const void* dy, int64
   if (!offsets || x_rows < 1 || x_rows >= (int64_t(1) << 31) - 1 || (!rows && x_rows < num_rows) ||
       !good_rows(x, x_stride, width) || !good_rows(dy, dy_stride, out_width))
     return fail(LF_E_INVALID, "expert_linear_weight_grad: x and dy must have rows, 16-byte aligned, with strides that are multiples of 8");
+  if (rows) {
+    if (!workspace || workspace_bytes < num_rows * width * 2 || !aligned16(workspace)) return fail(LF_E_INVALID, kNoWorkspace);
+    if (int rc = gather_rows(x, x_stride, x_rows, rows, num_rows, width, workspace, stream, what)) return rc;
+    x = workspace, x_stride = width, x_rows = num_rows;
+  }
   GParams p{};
-  p.offsets = offsets, p.rows = rows, p.out = dw, p.out_stride = width;
+  p.offsets = offsets, p.out = dw, p.out_stride = width;
   p.E = num_experts, p.R = int(num_rows), p.x_rows = int(x_rows);
   p.M = int(width), p.N = int(out_width), p.out_type = out_dtype, p.elem_bf16 = dtype == LF_BF16, p.split = 1;
   const CUtensorMapDataType type = map_type(dtype);
   if (!encode_rows(&p.a_map, type, x, width, x_rows, x_stride, 64) ||
+      !encode_rows(&p.a_small, type, x, width, x_rows, x_stride, 8) ||
       !encode_rows(&p.a_gather, type, x, width, x_rows, x_stride, 1) ||
       !encode_rows(&p.b_map, type, dy, out_width, num_rows, dy_stride, 64) ||
+      !encode_rows(&p.b_small, type, dy, out_width, num_rows, dy_stride, 8) ||
       !encode_rows(&p.b_gather, type, dy, out_width, num_rows, dy_stride, 1))
     return fail(LF_E_CUDA, "expert_linear_weight_grad: cuTensorMapEncodeTiled failed");
   const int64_t tiles = int64_t(ceil_div(p.M, 256)) * ceil_div(p.N, kWideRows) * num_experts;

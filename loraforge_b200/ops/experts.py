@@ -292,13 +292,23 @@ def expert_linear(x, weight, offsets, *, rows=None, out=None):
         if tuple(out.shape) != (R, N):
             raise ValueError("out must be [rows, out features]")
         output_is_distinct(out, (x, weight, offsets) if rows is None else (x, weight, offsets, rows))
+    workspace, room = _gather_room(x, rows, E, R, K, False)
     with torch.cuda.device(x.device):
         _native.call(
             "lf_expert_linear", _native.dtype_code(x.dtype), x.data_ptr(), row_stride(x), x.shape[0],
             None if rows is None else rows.data_ptr(), weight.data_ptr(), expert_stride(weight), weight.stride(1),
-            offsets.data_ptr(), E, R, N, K, out.data_ptr(), row_stride(out), _native.stream_of(x.device),
+            offsets.data_ptr(), E, R, N, K, out.data_ptr(), row_stride(out),
+            None if workspace is None else workspace.data_ptr(), room, _native.stream_of(x.device),
         )
     return out
+
+
+def _gather_room(x, rows, E: int, R: int, K: int, weight_grad: bool):
+    """Scratch for x's rows in order, where the kernels want them so: (tensor or None, bytes)."""
+    import torch
+
+    room = 0 if rows is None else _native.expert_linear_workspace_bytes(E, R, K, weight_grad)
+    return (torch.empty(room, dtype=torch.uint8, device=x.device) if room else None), room
 
 
 def expert_linear_backward(grad, x, weight, offsets, *, rows=None, weight_grad_dtype=None):
@@ -325,6 +335,7 @@ def expert_linear_backward(grad, x, weight, offsets, *, rows=None, weight_grad_d
     grad_x = torch.empty((R, K), dtype=x.dtype, device=x.device)
     grad_weight = torch.empty((E, N, K), dtype=weight_grad_dtype, device=x.device)
     dtype = _native.dtype_code(x.dtype)
+    workspace, room = _gather_room(x, rows, E, R, K, True)
     with torch.cuda.device(x.device):
         stream = _native.stream_of(x.device)
         _native.call(
@@ -334,6 +345,7 @@ def expert_linear_backward(grad, x, weight, offsets, *, rows=None, weight_grad_d
         _native.call(
             "lf_expert_linear_weight_grad", dtype, grad.data_ptr(), row_stride(grad), x.data_ptr(), row_stride(x),
             x.shape[0], None if rows is None else rows.data_ptr(), offsets.data_ptr(), E, R, N, K,
-            _native.dtype_code(weight_grad_dtype), grad_weight.data_ptr(), stream,
+            _native.dtype_code(weight_grad_dtype), grad_weight.data_ptr(),
+            None if workspace is None else workspace.data_ptr(), room, stream,
         )
     return grad_x, grad_weight

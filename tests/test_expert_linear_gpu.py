@@ -221,5 +221,7 @@ def test_refusals():
         expert_linear_backward(grad[:3], x, w, offsets, rows=rows)
     with pytest.raises(ValueError, match="weight_grad_dtype"):
         expert_linear_backward(grad, x, w, offsets, rows=rows, weight_grad_dtype=torch.float16)
+    with pytest.raises(RuntimeError, match="workspace"):
+        _native.call("lf_expert_linear", 2, 16, 64, 4, 16, 16, 4096, 64, 16, 1, 100, 64, 64, 16, 64, None, 0, None)
     with pytest.raises(RuntimeError, match="experts"):
-        _native.call("lf_expert_linear", 2, 16, 64, 4, None, 16, 4096, 64, 16, 2000, 4, 64, 64, 16, 64, None)
+        _native.call("lf_expert_linear", 2, 16, 64, 4, None, 16, 4096, 64, 16, 2000, 4, 64, 64, 16, 64, None, 0, None)
