@@ -493,6 +493,23 @@ int lf_mxfp4_dequantize(int32_t dtype, const uint8_t* codes, const uint8_t* scal
                         int64_t width, void* out, void* stream);
 
 /*
+ * Expert products of MXFP4 operands (codes and scales as lf_mxfp4_quantize leaves them), FP32
+ * sums on the block-scaled tensor cores, one rounding to out_dtype:
+ *   y[r, n] = sum_k x[i(r), k] w[e, n, k]  for rows r of group e, as in lf_expert_linear.
+ * x [x_rows, width], w [num_experts, out_width, width], both contiguous; width a multiple of 32.
+ * With rows, groups of many rows copy x's codes in order into `workspace` first:
+ * lf_expert_linear_mxfp4_workspace_bytes bytes, 16-byte aligned, not initialised.
+ */
+int64_t lf_expert_linear_mxfp4_workspace_bytes(int32_t num_experts, int64_t num_rows,
+                                               int64_t width);
+int lf_expert_linear_mxfp4(int32_t out_dtype, const uint8_t* x_codes, const uint8_t* x_scales,
+                           int64_t x_rows, const int32_t* rows, const uint8_t* w_codes,
+                           const uint8_t* w_scales, const int32_t* offsets, int32_t num_experts,
+                           int64_t num_rows, int64_t out_width, int64_t width, void* y,
+                           int64_t y_stride, void* workspace, int64_t workspace_bytes,
+                           void* stream);
+
+/*
  * Number of bounded device-side waits (mbarrier polls in the bulk-copy kernels)
  * that expired since the last reset; a non-zero count means a kernel gave up and
  * skipped work instead of hanging.  Synchronous; reset != 0 clears the counter.

@@ -21,7 +21,7 @@ INCLUDE = PACKAGE.parent / "include"
 LIBDIR = PACKAGE / "_lib"
 LIBRARY = LIBDIR / "liblfb200.so"
 SOURCES = ("capi.cu", "grouping.cu", "shrink.cu", "expand.cu", "sgmv.cu", "sgmv_prefill.cu", "base_gemm.cu",
-           "peer.cu", "experts.cu", "grouped_gemm.cu", "mxfp4.cu")
+           "peer.cu", "experts.cu", "grouped_gemm.cu", "mxfp4.cu", "mx_gemm.cu")
 ARCH = ("-gencode", "arch=compute_100a,code=sm_100a")
 FLAGS = ("-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr")
 

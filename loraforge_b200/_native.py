@@ -104,6 +104,9 @@ SIGNATURES = {
     "lf_expert_linear_weight_grad": [
         _i32, _p, _i64, _p, _i64, _i64, _p, _p, _i32, _i64, _i64, _i64, _i32, _p, _p, _i64, _p,
     ],
+    "lf_expert_linear_mxfp4": [
+        _i32, _p, _p, _i64, _p, _p, _p, _p, _i32, _i64, _i64, _i64, _p, _i64, _p, _i64, _p,
+    ],
     "lf_mxfp4_quantize": [_i32, _p, _i64, _i64, _i64, _p, _p, _p],
     "lf_mxfp4_dequantize": [_i32, _p, _p, _i64, _i64, _p, _p],
 }
@@ -117,7 +120,7 @@ def exported_symbols() -> tuple[str, ...]:
     return ("lf_version", "lf_last_error_string", "lf_fused_workspace_floats",
             "lf_sgmv_prefill_workspace_floats", "lf_lora_base_gemm_workspace_floats",
             "lf_peer_buffer_bytes", "lf_peer_handle_bytes", "lf_route_experts_workspace_ints",
-            "lf_expert_linear_workspace_bytes", *SIGNATURES)
+            "lf_expert_linear_workspace_bytes", "lf_expert_linear_mxfp4_workspace_bytes", *SIGNATURES)
 
 
 def library() -> ctypes.CDLL:
@@ -153,6 +156,8 @@ def library() -> ctypes.CDLL:
             lib.lf_route_experts_workspace_ints.argtypes = [_i64, _i32]
             lib.lf_expert_linear_workspace_bytes.restype = ctypes.c_int64
             lib.lf_expert_linear_workspace_bytes.argtypes = [_i32, _i64, _i64, _i32]
+            lib.lf_expert_linear_mxfp4_workspace_bytes.restype = ctypes.c_int64
+            lib.lf_expert_linear_mxfp4_workspace_bytes.argtypes = [_i32, _i64, _i64]
             _lib = lib
     return _lib
 
@@ -201,6 +206,14 @@ def route_experts_workspace_ints(num_tokens: int, num_experts: int) -> int:
 def expert_linear_workspace_bytes(num_experts: int, num_rows: int, width: int, weight_grad: bool = False) -> int:
     """Workspace bytes of lf_expert_linear (or its weight gradient) with row indices."""
     n = library().lf_expert_linear_workspace_bytes(num_experts, num_rows, width, 1 if weight_grad else 0)
+    if n < 0:
+        raise ValueError("invalid sizes for the expert workspace")
+    return n
+
+
+def expert_linear_mxfp4_workspace_bytes(num_experts: int, num_rows: int, width: int) -> int:
+    """Workspace bytes of lf_expert_linear_mxfp4 with row indices."""
+    n = library().lf_expert_linear_mxfp4_workspace_bytes(num_experts, num_rows, width)
     if n < 0:
         raise ValueError("invalid sizes for the expert workspace")
     return n

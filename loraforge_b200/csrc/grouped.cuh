@@ -18,7 +18,7 @@ namespace grouped {
 using namespace tc;
 
 constexpr int kMaxExperts = 1024;
-constexpr int kThreads = 192;  // warp 0 loads, warp 1 MMA, warps 2-5 epilogue (TMEM lane quarter = warp & 3)
+constexpr int kMaxWarps = 10;
 
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
@@ -198,7 +198,7 @@ __device__ __forceinline__ int scan_threads(int v, int* carry, int* part, Op&& o
   if (lane == 31) part[warp] = v;
   __syncthreads();
   int before = *carry, all = *carry;
-  for (int w = 0; w < kThreads / 32; ++w) {
+  for (int w = 0; w < int(blockDim.x) / 32; ++w) {
     if (w < warp) before = op(before, part[w]);
     all = op(all, part[w]);
   }
@@ -214,14 +214,14 @@ template <typename F>
 __device__ void list_tiles(const int32_t* offsets, int E, int R, int* bounds, int* starts, int* part, F&& tiles_of) {
   const int tid = threadIdx.x;
   int largest = 0, total = 0;
-  for (int e0 = 0; e0 <= E; e0 += kThreads) {
+  for (int e0 = 0; e0 <= E; e0 += int(blockDim.x)) {
     const int e = e0 + tid;
     const int v = scan_threads(e <= E ? min(max(offsets[e], 0), R) : 0, &largest, part,
                                [](int a, int b) { return max(a, b); });
     if (e <= E) bounds[e] = v;
   }
   __syncthreads();
-  for (int e0 = 0; e0 < E; e0 += kThreads) {
+  for (int e0 = 0; e0 < E; e0 += int(blockDim.x)) {
     const int e = e0 + tid;
     const int n = e < E ? tiles_of(bounds[e + 1] - bounds[e]) : 0;
     const int v = scan_threads(n, &total, part, [](int a, int b) { return a + b; });
@@ -289,8 +289,159 @@ inline int sm_count(int* sms) {
   return LF_OK;
 }
 
+// ------------------------------------------------------------------ stores
+constexpr int kMaxSplit = 8;
+constexpr int kChunkBytes = 32 * 64;  // 32 columns x 32 features of a warp, 16 bits
+
+// Rows of `features` values, `stride` apart, of type LF_F32, LF_F16 or LF_BF16.
+struct Output {
+  void* data;
+  int64_t stride;
+  int features, type;
+};
+
+__device__ __forceinline__ void store_value(const Output& o, int64_t at, float v) {
+  if (o.type == LF_BF16) static_cast<__nv_bfloat16*>(o.data)[at] = __float2bfloat16_rn(v);
+  else if (o.type == LF_F16) static_cast<__half*>(o.data)[at] = __float2half_rn(v);
+  else static_cast<float*>(o.data)[at] = v;
+}
+
+// Zeros to rows [first, R), spread over the grid.
+__device__ __forceinline__ void zero_rows(const Output& o, int first, int R) {
+  const int size = o.type == LF_F32 ? 4 : 2;
+  const int64_t bytes = int64_t(o.features) * size;
+  for (int64_t r = first + int64_t(blockIdx.x); r < R; r += gridDim.x) {
+    uint8_t* row = static_cast<uint8_t*>(o.data) + r * o.stride * size;
+    if (((reinterpret_cast<uintptr_t>(row) | uintptr_t(bytes)) & 15) == 0) {
+      for (int64_t i = threadIdx.x * 16; i < bytes; i += blockDim.x * 16)
+        *reinterpret_cast<uint4*>(row + i) = make_uint4(0, 0, 0, 0);
+    } else {
+      for (int64_t i = threadIdx.x * 2; i < bytes; i += blockDim.x * 2) *reinterpret_cast<uint16_t*>(row + i) = 0;
+    }
+  }
+}
+
+// Columns c0 .. c0 + 31 of this warp's 32 features as 16-bit values to global memory.  The
+// accumulator is read in the fragment shape whose transpose stmatrix writes, so that a column's
+// 32 features (64 bytes) lie together in the warp's staging, 16-byte chunks swizzled by column;
+// each store instruction then writes eight columns.  `dst`: feature 0 of column c0.
+__device__ __forceinline__ void store_chunk(uint32_t taddr, bool live, uint32_t staging, int bf16, uint8_t* dst,
+                                            int64_t pitch, int columns, int features, int lane) {
+  uint32_t r[32];
+  if (live) {
+    ld_fragments(taddr, r);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) r[i] = 0;
+  }
+  __syncwarp();  // the previous chunk has left the staging
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {  // eight columns each
+    uint32_t m[4];
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {  // eight features each
+      const uint32_t lo = r[(h >> 1) * 16 + 4 * j + 2 * (h & 1)], hi = r[(h >> 1) * 16 + 4 * j + 2 * (h & 1) + 1];
+      if (bf16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(m[h]) : "f"(__uint_as_float(hi)), "f"(__uint_as_float(lo)));
+      else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(m[h]) : "f"(__uint_as_float(hi)), "f"(__uint_as_float(lo)));
+    }
+    const int col = 8 * j + (lane & 7), chunk = lane >> 3;
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(
+                     staging + uint32_t(col * 64 + ((chunk ^ (col >> 1 & 3)) << 4))),
+                 "r"(m[0]), "r"(m[1]), "r"(m[2]), "r"(m[3])
+                 : "memory");
+  }
+  __syncwarp();
+  const int chunk = lane & 3;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int col = 8 * i + (lane >> 2);
+    const uint4 v = lds16(staging + uint32_t(col * 64 + ((chunk ^ (col >> 1 & 3)) << 4)));
+    if (col < columns && 8 * chunk < features) *reinterpret_cast<uint4*>(dst + col * pitch + 16 * chunk) = v;
+  }
+}
+
+// A tile's columns 0 .. valid - 1 of this warp's features f0 .. f0 + 31 (TMEM address `d`; zeros
+// unless live) to rows row0 + column.
+__device__ __forceinline__ void store_whole(const Output& o, uint32_t d, bool live, int f0, int64_t row0, int nt,
+                                            int valid, uint32_t staging, int lane) {
+  if (o.type != LF_F32 && (reinterpret_cast<uintptr_t>(o.data) & 15) == 0 && o.stride % 8 == 0 && o.features % 8 == 0) {
+    uint8_t* dst = static_cast<uint8_t*>(o.data) + (row0 * o.stride + f0) * 2;
+    for (int c0 = 0; c0 < valid; c0 += 32)
+      store_chunk(d + uint32_t(c0), live, staging, o.type == LF_BF16, dst + c0 * o.stride * 2, o.stride * 2, valid - c0,
+                  o.features - f0, lane);
+  } else {
+    for (int c0 = 0; c0 < nt; c0 += 16) {
+      uint32_t r[16];
+      if (live) tc_ld16(d + uint32_t(c0), r);
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (f0 + lane < o.features && c0 + j < valid)
+          store_value(o, (row0 + c0 + j) * o.stride + f0 + lane, live ? __uint_as_float(r[j]) : 0.f);
+    }
+  }
+}
+
+// The same for a contraction split over the cluster's CTAs: the partial sums go to this CTA's
+// `part` [columns][128 features], then every CTA adds a share of the columns over all CTAs in
+// rank order.  `parts`: how often the caller came here before.  False after an expired wait.
+template <typename F>
+__device__ __forceinline__ bool store_split(const Output& o, uint32_t d, bool live, int f0, int64_t row0, int nt,
+                                            int valid, float* part, uint64_t* part_full, uint64_t* part_empty,
+                                            int parts, int cluster, int rank, int quarter, int lane,
+                                            volatile int* abort, F&& release) {
+  if (!__all_sync(0xffffffffu, wait_cluster(part_empty, (uint32_t(parts) & 1u) ^ 1u, abort))) return false;
+  float* mine = part + quarter * 32 + lane;
+  for (int c0 = 0; c0 < nt; c0 += 16) {
+    uint32_t r[16];
+    if (live) tc_ld16(d + uint32_t(c0), r);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) mine[(c0 + j) * 128] = live ? __uint_as_float(r[j]) : 0.f;
+  }
+  release();
+  __syncwarp();
+  if (lane < cluster) arrive_cluster(mapa(part_full, lane));
+  if (!__all_sync(0xffffffffu, wait_cluster(part_full, uint32_t(parts) & 1u, abort))) return false;
+  uint32_t peer[kMaxSplit];
+#pragma unroll
+  for (int q = 0; q < kMaxSplit; ++q)
+    if (q < cluster) peer[q] = mapa(mine, q);
+  for (int c = rank; c < valid; c += cluster) {
+    float v[kMaxSplit], sum = 0.f;
+#pragma unroll
+    for (int q = 0; q < kMaxSplit; ++q)
+      if (q < cluster) v[q] = lds_cluster(peer[q] + uint32_t(c) * 512u);
+#pragma unroll
+    for (int q = 0; q < kMaxSplit; ++q)
+      if (q < cluster) sum += v[q];
+    if (f0 + lane < o.features) store_value(o, (row0 + c) * o.stride + f0 + lane, sum);
+  }
+  __syncwarp();
+  if (lane < cluster) arrive_cluster(mapa(part_empty, lane));
+  return true;
+}
+
+// Waves of clusters times a CTA's share of a tile, for a split of S: the least wins, smaller S on
+// a tie.  A share has at least `least_steps` steps.
+inline int choose_split(int64_t tiles, int steps, int least_steps) {
+  int sms = 148, best = 1;
+  sm_count(&sms);
+  double least = 1e30;
+  for (int s = 1; s <= kMaxSplit; s *= 2) {
+    if (s > 1 && steps < least_steps * s) break;
+    const int64_t clusters = sms / s;
+    const double cost = double((tiles + clusters - 1) / clusters) / s;
+    if (cost < 0.95 * least) {
+      least = cost;
+      best = s;
+    }
+  }
+  return best;
+}
+
+// ------------------------------------------------------------------ launch
 template <typename P>
-int launch_clusters(void (*kernel)(P), int grid, int cluster, int smem, void* stream, const char* what, const P& p) {
+int launch_clusters(void (*kernel)(P), int grid, int threads, int cluster, int smem, void* stream, const char* what,
+                    const P& p) {
   cudaLaunchConfig_t config = {};
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -302,7 +453,7 @@ int launch_clusters(void (*kernel)(P), int grid, int cluster, int smem, void* st
   config.attrs = attr;
   config.numAttrs = 2;
   config.gridDim = dim3(grid);
-  config.blockDim = dim3(kThreads);
+  config.blockDim = dim3(threads);
   config.dynamicSmemBytes = smem;
   config.stream = static_cast<cudaStream_t>(stream);
   const cudaError_t err = cudaLaunchKernelEx(&config, kernel, p);

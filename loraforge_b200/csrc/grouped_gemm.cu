@@ -34,8 +34,8 @@
 //           partial sums are added in rank order through distributed shared memory.
 //
 // Every wait is bounded (tma.cuh): an expiry stops every role at its next wait.
+#include "experts.cuh"
 #include "grouped.cuh"
-#include "sgmv.cuh"
 
 namespace lfb {
 namespace {
@@ -44,20 +44,18 @@ using namespace grouped;
 
 enum Mode { kForward = 0, kInput = 1, kWeight = 2 };
 
+constexpr int kThreads = 192;         // warp 0 loads, warp 1 MMA, warps 2-5 store (TMEM lane quarter = warp & 3)
 constexpr int kStep = 64;             // contraction per stage: 128 bytes
 constexpr int kABytes = 128 * 128;    // 128 features x 128 bytes (K-major), or two 64-feature boxes of 64 steps
-constexpr int kMaxSplit = 8;
-constexpr int kChunkBytes = 32 * 64;  // 32 columns x 32 features of a warp, 16 bits
 
 struct GParams {
   const int32_t* offsets;  // [E + 1]
   const int32_t* rows;     // [R] or null
-  void* out;
-  int64_t out_stride;
+  Output out;
   int E, R, x_rows;
   int M, C;  // output features, contraction (forward K, input N; weight: the groups' rows)
   int N;     // weight: columns of D (dy's features)
-  int out_type, elem_bf16, split;
+  int elem_bf16, split;
   CUtensorMap a_map;     // forward: W boxes 64 k x 128 n; input: 64 k x 64 n; weight: x boxes 64 k x 64 rows
   CUtensorMap a_small;   // weight: 64 k x 8 rows
   CUtensorMap a_gather;  // weight: single x rows of 64 k
@@ -119,55 +117,6 @@ __device__ __forceinline__ Tile tile_of(const GParams& p, const int* bounds, con
   return x;
 }
 
-template <typename O>
-__device__ __forceinline__ void store_out(void* out, int64_t at, float v) {
-  static_cast<typename O::storage*>(out)[at] = O::from_float(v);
-}
-__device__ __forceinline__ void store_typed(const GParams& p, int64_t at, float v) {
-  if (p.out_type == LF_BF16) store_out<bf16_t>(p.out, at, v);
-  else if (p.out_type == LF_F16) store_out<f16_t>(p.out, at, v);
-  else store_out<f32_t>(p.out, at, v);
-}
-
-// Columns c0 .. c0 + 31 of this warp's 32 features as 16-bit values to global memory.  The
-// accumulator is read in the fragment shape whose transpose stmatrix writes, so that a column's
-// 32 features (64 bytes) lie together in the warp's staging, 16-byte chunks swizzled by column;
-// each store instruction then writes eight columns.  `dst`: feature 0 of column c0.
-__device__ __forceinline__ void store_chunk(uint32_t taddr, bool live, uint32_t staging, int bf16, uint8_t* dst,
-                                            int64_t pitch, int columns, int features, int lane) {
-  uint32_t r[32];
-  if (live) {
-    ld_fragments(taddr, r);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 32; ++i) r[i] = 0;
-  }
-  __syncwarp();  // the previous chunk has left the staging
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {  // eight columns each
-    uint32_t m[4];
-#pragma unroll
-    for (int h = 0; h < 4; ++h) {  // eight features each
-      const uint32_t lo = r[(h >> 1) * 16 + 4 * j + 2 * (h & 1)], hi = r[(h >> 1) * 16 + 4 * j + 2 * (h & 1) + 1];
-      if (bf16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(m[h]) : "f"(__uint_as_float(hi)), "f"(__uint_as_float(lo)));
-      else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(m[h]) : "f"(__uint_as_float(hi)), "f"(__uint_as_float(lo)));
-    }
-    const int col = 8 * j + (lane & 7), chunk = lane >> 3;
-    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(
-                     staging + uint32_t(col * 64 + ((chunk ^ (col >> 1 & 3)) << 4))),
-                 "r"(m[0]), "r"(m[1]), "r"(m[2]), "r"(m[3])
-                 : "memory");
-  }
-  __syncwarp();
-  const int chunk = lane & 3;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int col = 8 * i + (lane >> 2);
-    const uint4 v = lds16(staging + uint32_t(col * 64 + ((chunk ^ (col >> 1 & 3)) << 4)));
-    if (col < columns && 8 * chunk < features) *reinterpret_cast<uint4*>(dst + col * pitch + 16 * chunk) = v;
-  }
-}
-
 template <int kMode, int kCtas, int kNT>
 __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(const __grid_constant__ GParams p) {
   using S = Shape<kCtas, kNT>;
@@ -222,19 +171,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(const __grid_const
   const int tiles = starts[p.E];
   const int first = int(blockIdx.x) / cluster, stride = int(gridDim.x) / cluster;
 
-  if (kMode != kWeight) {  // rows of no group
-    const int64_t bytes = int64_t(p.M) * (p.out_type == LF_F32 ? 4 : 2);
-    const int64_t pitch = p.out_stride * (p.out_type == LF_F32 ? 4 : 2);
-    for (int64_t r = bounds[p.E] + int64_t(blockIdx.x); r < p.R; r += gridDim.x) {
-      uint8_t* row = static_cast<uint8_t*>(p.out) + r * pitch;
-      if (((reinterpret_cast<uintptr_t>(row) | uintptr_t(bytes)) & 15) == 0) {
-        for (int64_t i = tid * 16; i < bytes; i += kThreads * 16)
-          *reinterpret_cast<uint4*>(row + i) = make_uint4(0, 0, 0, 0);
-      } else {
-        for (int64_t i = tid * 2; i < bytes; i += kThreads * 2) *reinterpret_cast<uint16_t*>(row + i) = 0;
-      }
-    }
-  }
+  if (kMode != kWeight) zero_rows(p.out, bounds[p.E], p.R);
 
   // The steps of a tile that this CTA takes.
   auto my_steps = [&](const Tile& x, int* ks0, int* ks1) {
@@ -377,7 +314,6 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(const __grid_const
     const int quarter = warp & 3;
     const uint32_t lanes = uint32_t(quarter * 32) << 16;
     const uint32_t staging = smem_u32(part) + uint32_t(quarter * kChunkBytes);
-    const bool vector = p.out_type != LF_F32 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0 && p.out_stride % 8 == 0;
     int count = 0, parts = 0;
     for (int t = first; t < tiles; t += stride) {
       const Tile x = tile_of<kMode, kCtas, kNT>(p, bounds, starts, t);
@@ -391,66 +327,24 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(const __grid_const
         tc_fence_after();
       }
       const uint32_t d = tmem + lanes + uint32_t(ab * kNT);
-      const int f = x.m0 + (kCtas == 2 ? rank * 128 : 0) + quarter * 32 + lane;
+      const int f0 = x.m0 + (kCtas == 2 ? rank * 128 : 0) + quarter * 32;
       const int64_t row0 = kMode == kWeight ? int64_t(x.e) * p.N + x.n0 : x.n0;
       auto release = [&]() {
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) {
+        if (live && lane == 0) {
           if (kCtas == 2) arrive_cluster(mapa(&acc_empty[ab], 0));
           else mbar_arrive(&acc_empty[ab]);
         }
       };
       if (kCtas == 1 && cluster > 1) {
-        // Partial sums to this CTA's buffer, then every CTA adds a share of the columns in rank order.
-        if (!__all_sync(0xffffffffu, wait_cluster(part_empty, (uint32_t(parts) & 1u) ^ 1u, abort))) break;
-        for (int c0 = 0; c0 < x.nt; c0 += 16) {
-          uint32_t r[16];
-          if (live) tc_ld16(d + uint32_t(c0), r);
-#pragma unroll
-          for (int j = 0; j < 16; ++j)
-            part[(c0 + j) * 128 + quarter * 32 + lane] = live ? __uint_as_float(r[j]) : 0.f;
-        }
-        if (live) release();
-        __syncwarp();
-        if (lane < cluster) arrive_cluster(mapa(part_full, lane));
-        if (!__all_sync(0xffffffffu, wait_cluster(part_full, uint32_t(parts) & 1u, abort))) break;
+        if (!store_split(p.out, d, live, f0, row0, x.nt, x.valid, part, part_full, part_empty, parts, cluster, rank,
+                         quarter, lane, abort, release))
+          break;
         ++parts;
-        const uint32_t own = smem_u32(part) + uint32_t(quarter * 32 + lane) * 4u;
-        uint32_t peer[kMaxSplit];
-#pragma unroll
-        for (int q = 0; q < kMaxSplit; ++q)
-          if (q < cluster) asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer[q]) : "r"(own), "r"(q));
-        for (int c = rank; c < x.valid; c += cluster) {
-          float v[kMaxSplit], sum = 0.f;
-#pragma unroll
-          for (int q = 0; q < kMaxSplit; ++q)
-            if (q < cluster) v[q] = lds_cluster(peer[q] + uint32_t(c) * 512u);
-#pragma unroll
-          for (int q = 0; q < kMaxSplit; ++q)
-            if (q < cluster) sum += v[q];
-          if (f < p.M) store_typed(p, (row0 + c) * p.out_stride + f, sum);
-        }
-        __syncwarp();
-        if (lane < cluster) arrive_cluster(mapa(part_empty, lane));
       } else {
-        if (vector) {
-          const int f0 = f - lane;
-          uint8_t* dst = static_cast<uint8_t*>(p.out) + (row0 * p.out_stride + f0) * 2;
-          for (int c0 = 0; c0 < x.valid; c0 += 32)
-            store_chunk(d + uint32_t(c0), live, staging, p.out_type == LF_BF16, dst + c0 * p.out_stride * 2,
-                        p.out_stride * 2, x.valid - c0, p.M - f0, lane);
-        } else {
-          for (int c0 = 0; c0 < x.nt; c0 += 16) {
-            uint32_t r[16];
-            if (live) tc_ld16(d + uint32_t(c0), r);
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-              if (f < p.M && c0 + j < x.valid)
-                store_typed(p, (row0 + c0 + j) * p.out_stride + f, live ? __uint_as_float(r[j]) : 0.f);
-          }
-        }
-        if (live) release();
+        store_whole(p.out, d, live, f0, row0, x.nt, x.valid, staging, lane);
+        release();
       }
     }
   }
@@ -482,28 +376,6 @@ __global__ void __launch_bounds__(256) gather_rows_kernel(const uint4* x, int64_
     if (first + u * 256 < total) out[first + u * 256] = v[u];
 }
 
-int gather_rows(const void* x, int64_t x_stride, int64_t x_rows, const int32_t* rows, int64_t R, int64_t width,
-                void* out, void* stream, const char* what) {
-  cudaLaunchConfig_t config = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  config.attrs = attr;
-  config.numAttrs = 1;
-  const int64_t total = R * (width / 8);
-  config.gridDim = dim3(unsigned((total + 1023) / 1024));
-  config.blockDim = dim3(256);
-  config.stream = static_cast<cudaStream_t>(stream);
-  const cudaError_t err =
-      cudaLaunchKernelEx(&config, gather_rows_kernel, static_cast<const uint4*>(x), x_stride / 8, int(x_rows), rows,
-                         int(width / 8), total, static_cast<uint4*>(out));
-  if (err != cudaSuccess) {
-    last_error() = std::string(what) + ": " + cudaGetErrorString(err);
-    return LF_E_CUDA;
-  }
-  return LF_OK;
-}
-
 template <int kMode, int kCtas, int kNT>
 int launch_grouped(const GParams& p, int64_t tiles, void* stream, const char* what) {
   using S = Shape<kCtas, kNT>;
@@ -515,24 +387,7 @@ int launch_grouped(const GParams& p, int64_t tiles, void* stream, const char* wh
   const int smem = 1024 + S::kStages * S::kStageBytes + S::kPartBytes + 256 + int(sizeof(int)) * (8 + 2 * (p.E + 1));
   static int flags[64] = {};
   if (int rc = ensure_smem(grouped_kernel<kMode, kCtas, kNT>, smem, flags)) return rc;
-  return launch_clusters(grouped_kernel<kMode, kCtas, kNT>, int(grid), cluster, smem, stream, what, p);
-}
-
-// Waves of clusters times a CTA's share of a tile, for a split of S: the least wins, smaller S on a tie.
-int choose_split(int64_t tiles, int steps) {
-  int sms = 148, best = 1;
-  sm_count(&sms);
-  double least = 1e30;
-  for (int s = 1; s <= kMaxSplit; s *= 2) {
-    if (s > 1 && steps < 4 * s) break;
-    const int64_t clusters = sms / s;
-    const double cost = double((tiles + clusters - 1) / clusters) / s;
-    if (cost < 0.95 * least) {
-      least = cost;
-      best = s;
-    }
-  }
-  return best;
+  return launch_clusters(grouped_kernel<kMode, kCtas, kNT>, int(grid), kThreads, cluster, smem, stream, what, p);
 }
 
 constexpr int kWideRows = 256, kNarrowRows = 64;
@@ -586,7 +441,7 @@ int launch_rows(GParams& p, void* stream, const char* what) {
   if (narrow(p.E, p.R)) {
     const int64_t mt = ceil_div(p.M, 128);
     const int64_t tiles = mt * (groups + p.R / kNarrowRows);  // at most
-    p.split = choose_split(mt * groups, ceil_div(p.C, kStep));
+    p.split = choose_split(mt * groups, ceil_div(p.C, kStep), 4);
     return launch_grouped<kMode, 1, kNarrowRows>(p, tiles, stream, what);
   }
   p.split = 1;
@@ -595,6 +450,28 @@ int launch_rows(GParams& p, void* stream, const char* what) {
 }
 
 }  // namespace
+
+int gather_rows(const void* x, int64_t x_stride, int64_t x_rows, const int32_t* rows, int64_t R, int64_t width,
+                void* out, void* stream, const char* what) {
+  cudaLaunchConfig_t config = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = attr;
+  config.numAttrs = 1;
+  const int64_t total = R * (width / 8);
+  config.gridDim = dim3(unsigned((total + 1023) / 1024));
+  config.blockDim = dim3(256);
+  config.stream = static_cast<cudaStream_t>(stream);
+  const cudaError_t err =
+      cudaLaunchKernelEx(&config, gather_rows_kernel, static_cast<const uint4*>(x), x_stride / 8, int(x_rows), rows,
+                         int(width / 8), total, static_cast<uint4*>(out));
+  if (err != cudaSuccess) {
+    last_error() = std::string(what) + ": " + cudaGetErrorString(err);
+    return LF_E_CUDA;
+  }
+  return LF_OK;
+}
 
 int grouped_wait_timeouts(unsigned int* value, int reset) {
   if (cudaMemcpyFromSymbol(value, g_lf_wait_timeouts, sizeof(*value)) != cudaSuccess)
@@ -638,9 +515,9 @@ extern "C" int lf_expert_linear(int32_t dtype, const void* x, int64_t x_stride, 
     }
   }
   GParams p{};
-  p.offsets = offsets, p.rows = rows, p.out = y, p.out_stride = y_stride;
+  p.offsets = offsets, p.rows = rows, p.out = {y, y_stride, int(out_width), dtype};
   p.E = num_experts, p.R = int(num_rows), p.x_rows = int(x_rows);
-  p.M = int(out_width), p.C = int(width), p.out_type = dtype, p.elem_bf16 = dtype == LF_BF16;
+  p.M = int(out_width), p.C = int(width), p.elem_bf16 = dtype == LF_BF16;
   const CUtensorMapDataType type = map_type(dtype);
   if (!encode_weights(&p.a_map, type, w, width, out_width, num_experts, w_row_stride, w_expert_stride, 128) ||
       !encode_rows(&p.b_map, type, x, width, x_rows, x_stride, 64) ||
@@ -661,9 +538,9 @@ extern "C" int lf_expert_linear_input_grad(int32_t dtype, const void* dy, int64_
       w_expert_stride < (out_width - 1) * w_row_stride + width || !good_rows(dy, dy_stride, out_width))
     return fail(LF_E_INVALID, "expert_linear_input_grad: W and dy must be 16-byte aligned with strides that are multiples of 8, dx's rows must not overlap");
   GParams p{};
-  p.offsets = offsets, p.out = dx, p.out_stride = dx_stride;
+  p.offsets = offsets, p.out = {dx, dx_stride, int(width), dtype};
   p.E = num_experts, p.R = int(num_rows), p.x_rows = int(num_rows);
-  p.M = int(width), p.C = int(out_width), p.out_type = dtype, p.elem_bf16 = dtype == LF_BF16;
+  p.M = int(width), p.C = int(out_width), p.elem_bf16 = dtype == LF_BF16;
   const CUtensorMapDataType type = map_type(dtype);
   if (!encode_weights(&p.a_map, type, w, width, out_width, num_experts, w_row_stride, w_expert_stride, 64) ||
       !encode_rows(&p.b_map, type, dy, out_width, num_rows, dy_stride, 64) ||
@@ -696,9 +573,9 @@ extern "C" int lf_expert_linear_weight_grad(int32_t dtype, const void* dy, int64
     x = workspace, x_stride = width, x_rows = num_rows;
   }
   GParams p{};
-  p.offsets = offsets, p.out = dw, p.out_stride = width;
+  p.offsets = offsets, p.out = {dw, width, int(width), out_dtype};
   p.E = num_experts, p.R = int(num_rows), p.x_rows = int(x_rows);
-  p.M = int(width), p.N = int(out_width), p.out_type = out_dtype, p.elem_bf16 = dtype == LF_BF16, p.split = 1;
+  p.M = int(width), p.N = int(out_width), p.elem_bf16 = dtype == LF_BF16, p.split = 1;
   const CUtensorMapDataType type = map_type(dtype);
   if (!encode_rows(&p.a_map, type, x, width, x_rows, x_stride, 64) ||
       !encode_rows(&p.a_small, type, x, width, x_rows, x_stride, 8) ||

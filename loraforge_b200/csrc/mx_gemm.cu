@@ -1,0 +1,512 @@
+// Expert products of MXFP4 activations and weights on the block-scaled tensor cores:
+//
+//   y[r, n] = sum over blocks b of 32 of 2^(sx[i(r), b] + sw[e, n, b] - 254)
+//             sum over k in b of qx[i(r), k] qw[e, n, k]
+//
+// for rows offsets[e] <= r < offsets[e+1], i(r) = rows[r] or r.  tcgen05.mma kind::mxf4 takes
+// the 4-bit codes as they lie (K-major, 64 a step) and one scale byte for 32 of them, and sums
+// in FP32; a product of two codes and two powers of two is exact.
+//
+// The tiles are those of the 16-bit products (grouped_gemm.cu): features on the TMEM lanes,
+// rows on the columns, CTA pairs with 256 features x up to 224 rows, or single CTAs with 128 x
+// 64 whose contraction may be split over a cluster.  224, not 256, rows: two accumulators of 224
+// columns leave 64 TMEM columns for the scales.
+//
+// Scales.  The tensor core wants them in TMEM: for 128 operand rows and 128 codes a row, four
+// columns in which lane l of column j holds the four bytes of row 32 j + l, the same in every
+// quarter of the lanes.  Four warps read them row by row (32 bytes of a row, a thread and four
+// stages: a whole sector), write them to the stage as the 512-byte blocks that tcgen05.cp
+// copies, and the MMA thread issues the copies before the stage's MMAs.  The copies go to two
+// sets of columns in turn; a set is written again when the MMAs that read it are done.
+//
+// Per CTA: warp 0 loads codes (TMA), warp 1 MMA and TMEM, warps 2-5 store, warps 6-9 scales.
+// Every wait is bounded (tma.cuh): an expiry stops every role at its next wait.
+#include "experts.cuh"
+#include "grouped.cuh"
+
+namespace lfb {
+namespace {
+
+using namespace grouped;
+
+constexpr int kThreads = 320;
+constexpr int kStep = 256;           // codes per stage: 128 bytes a row
+constexpr int kABytes = 128 * 128;
+constexpr int kSuper = 4;            // stages whose scales a thread loads at once (32 bytes a row)
+
+struct MxParams {
+  const int32_t* offsets;  // [E + 1]
+  const int32_t* rows;     // [R] or null: row of x (and of its scales)
+  Output out;
+  const uint8_t* x_scales;  // [x_rows][blocks]
+  const uint8_t* w_scales;  // [E][N][blocks]
+  int E, R, x_rows, N, K, blocks;
+  int x_align, w_align;  // 16, 8 or 1: alignment of every row of the scales
+  int gathered;          // codes are in the rows' order already
+  int split;
+  CUtensorMap w_map;      // 128 bytes x 128 rows
+  CUtensorMap x_map;      // 128 bytes x 16 rows
+  CUtensorMap x_small;    // 128 bytes x 8 rows
+  CUtensorMap x_gather;   // single rows
+};
+
+template <int kCtas, int kNT>
+struct Shape {
+  static constexpr int kBRows = kNT / kCtas;
+  static constexpr int kHalves = (kNT + 127) / 128;              // scale blocks of 128 rows of x
+  static constexpr int kScaleBytes = 2 * 512 * (1 + kHalves);    // two groups of 128 codes a stage
+  static constexpr int kStageBytes = (kABytes + kBRows * 128 + kScaleBytes + 1023) / 1024 * 1024;
+  static constexpr int kPartBytes = kCtas == 1 ? kNT * 128 * 4 : 4 * kChunkBytes;
+  static constexpr int kStages = kCtas == 2 ? 6 : 7;
+  static constexpr int kScaleColumns = 2 * (4 + 4 * kHalves);    // a set
+  static constexpr int kColumns = kCtas == 2 ? 512 : 256;        // TMEM
+  static_assert(2 * kNT + 2 * kScaleColumns <= kColumns, "TMEM");
+};
+
+__device__ __forceinline__ uint32_t instruction(int m, int n, int scale_id) {
+  return (uint32_t(scale_id) << 4) | (1u << 7) | (1u << 10) | (uint32_t(n >> 3) << 17) | (1u << 23) |
+         (uint32_t(m >> 7) << 27) | (uint32_t(scale_id) << 29);
+}
+
+template <int kCtas>
+__device__ __forceinline__ void mma_mxf4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb,
+                                         uint32_t accumulate) {
+  if constexpr (kCtas == 1) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
+        " tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+        : "memory");
+  }
+}
+
+// 512 bytes (32 rows of 16) to four TMEM columns, repeated in the four quarters of the lanes;
+// in a pair, each CTA from its own shared memory to its own TMEM.
+template <int kCtas>
+__device__ __forceinline__ void copy_scales(uint32_t taddr, uint32_t saddr) {
+  // No swizzle, groups of 8 rows 128 bytes apart.
+  const uint64_t desc = uint64_t((saddr & 0x3FFFFu) >> 4) | (uint64_t(1) << 16) | (uint64_t(128 >> 4) << 32) | (uint64_t(1) << 46);
+  if constexpr (kCtas == 1)
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+  else
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+
+// Arrive on this CTA's `bar` alone.
+template <int kCtas>
+__device__ __forceinline__ void commit_here(uint64_t* bar) {
+  if constexpr (kCtas == 1)
+    tc_commit(bar);
+  else
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+                 : "memory");
+}
+
+struct Tile {
+  int e, m0, n0, nt, valid, hi;
+};
+
+template <int kCtas, int kNT>
+__device__ __forceinline__ Tile tile_of(const MxParams& p, const int* bounds, const int* starts, int t) {
+  Tile x;
+  x.e = group_of(starts, p.E, t);
+  const int lo = bounds[x.e];
+  x.hi = bounds[x.e + 1];
+  const int nt = ceil_div(x.hi - lo, kNT);
+  int m, n;
+  place_tile(t - starts[x.e], ceil_div(p.N, 128 * kCtas), nt, &m, &n);
+  x.m0 = m * 128 * kCtas;
+  const int each = round_up(ceil_div(x.hi - lo, nt), 16);
+  x.n0 = lo + n * each;
+  x.valid = min(each, x.hi - x.n0);
+  x.nt = round_up(x.valid, 16);
+  return x;
+}
+
+// 32 scale bytes from byte k0 of a row of `blocks`; zeros past the row and where row is null.
+__device__ __forceinline__ void load_scales(const uint8_t* row, int k0, int blocks, int align, uint32_t (&s)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) s[i] = 0;
+  if (!row) return;
+  if (align == 16 && k0 + 32 <= blocks) {
+    const uint4 a = *reinterpret_cast<const uint4*>(row + k0), b = *reinterpret_cast<const uint4*>(row + k0 + 16);
+    s[0] = a.x, s[1] = a.y, s[2] = a.z, s[3] = a.w, s[4] = b.x, s[5] = b.y, s[6] = b.z, s[7] = b.w;
+  } else if (align >= 8) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (k0 + 8 * i < blocks) {
+        const uint2 v = *reinterpret_cast<const uint2*>(row + k0 + 8 * i);
+        s[2 * i] = v.x, s[2 * i + 1] = v.y;
+      }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (k0 + i < blocks) s[i >> 2] |= uint32_t(row[k0 + i]) << (8 * (i & 3));
+  }
+}
+
+template <int kCtas, int kNT>
+__global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__ MxParams p) {
+  using S = Shape<kCtas, kNT>;
+  constexpr int kStages = S::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = align1024(smem_raw);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  uint8_t* ring = smem;  // stage: W codes, x codes, scales of W (two groups), of x (two groups x halves)
+  float* part = reinterpret_cast<float*>(ring + kStages * S::kStageBytes);
+  uint64_t* full = reinterpret_cast<uint64_t*>(ring + kStages * S::kStageBytes + S::kPartBytes);
+  uint64_t* empty = full + kStages;
+  uint64_t* acc_full = empty + kStages;
+  uint64_t* acc_empty = acc_full + 2;
+  uint64_t* set_done = acc_empty + 2;
+  uint64_t* part_full = set_done + 2;
+  uint64_t* part_empty = part_full + 1;
+  uint64_t* fin = part_empty + 1;
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(fin + 1);
+  volatile int* abort = reinterpret_cast<volatile int*>(tslot + 1);
+  int* scan = reinterpret_cast<int*>(tslot + 2);
+  int* bounds = scan + kMaxWarps;  // [E + 1]
+  int* starts = bounds + p.E + 1;  // [E + 1]
+
+  const int cluster = kCtas == 2 ? 2 : p.split;
+  const int rank = cluster > 1 ? int(cluster_rank()) : 0;
+  const bool leader = rank * (kCtas - 1) == 0;
+  if (tid == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&full[i], 1 + 4 * kCtas);  // the codes' bytes and the scale warps
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_empty[i], 4 * kCtas);
+      mbar_init(&set_done[i], 1);
+    }
+    mbar_init(part_full, 4 * cluster);
+    mbar_init(part_empty, 4 * cluster);
+    mbar_init(fin, 1);
+    fence_mbar_init();
+    *abort = 0;
+  }
+  if (warp == 1) alloc_tmem<kCtas>(tslot, S::kColumns);
+  pdl_wait();
+  const int mtiles = ceil_div(p.N, 128 * kCtas);
+  list_tiles(p.offsets, p.E, p.R, bounds, starts, scan, [&](int rows) { return mtiles * ceil_div(rows, kNT); });
+  tc_fence_before();
+  __syncthreads();
+  if (cluster > 1) cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = *tslot;
+  const int tiles = starts[p.E];
+  const int first = int(blockIdx.x) / cluster, stride = int(gridDim.x) / cluster;
+  zero_rows(p.out, bounds[p.E], p.R);
+
+  // The steps this CTA takes of every tile, in whole groups of kSuper.
+  const int steps = ceil_div(p.K, kStep);
+  int ks0 = 0, ks1 = steps;
+  if (kCtas == 1 && cluster > 1) {
+    const int each = round_up(ceil_div(steps, cluster), kSuper);
+    ks0 = min(steps, rank * each);
+    ks1 = min(steps, ks0 + each);
+  }
+  const bool live = ks1 > ks0;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ codes
+    int it = 0;
+    for (int t = first; t < tiles && live; t += stride) {
+      const Tile x = tile_of<kCtas, kNT>(p, bounds, starts, t);
+      const int m_cta = x.m0 + (kCtas == 2 ? rank * 128 : 0);
+      const int share = x.nt / kCtas;
+      const int n_cta = x.n0 + (kCtas == 2 ? rank * share : 0);
+      const bool by_row = kCtas == 1 && p.rows && !p.gathered;
+      int row4[4];
+      if (by_row) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = n_cta + 4 * lane + i;
+          const int src = 4 * lane + i < share && r < x.hi ? p.rows[r] : -1;
+          row4[i] = src >= 0 && src < p.x_rows ? src : p.x_rows;
+        }
+      }
+      const uint32_t bytes = kCtas * (kABytes + uint32_t(share) * 128u);
+      bool ok = true;
+      for (int ks = ks0; ks < ks1; ++ks, ++it) {
+        const int st = it % kStages;
+        ok = __all_sync(0xffffffffu, wait_or_abort(&empty[st], (uint32_t(it / kStages) & 1u) ^ 1u, abort));
+        if (!ok) break;
+        const uint32_t a = smem_u32(ring + st * S::kStageBytes), b = a + kABytes;
+        const uint32_t bar = kCtas == 2 ? mapa(&full[st], 0) : smem_u32(&full[st]);
+        if (lane == 0 && leader) mbar_arrive_expect_tx(&full[st], bytes);
+        __syncwarp();
+        const int c = ks * 128;  // bytes along K
+        if (lane == 0) load_3d<kCtas>(a, &p.w_map, c, m_cta, x.e, bar);
+        if (by_row) {
+          if (4 * lane < share) gather4<kCtas>(b + lane * 512, &p.x_gather, c, row4, bar);
+        } else {
+          const int big = share / 16, i = lane - 1;
+          if (i >= 0 && i < big) load_2d<kCtas>(b + i * 2048, &p.x_map, c, n_cta + 16 * i, bar);
+          else if (i == big && share % 16) load_2d<kCtas>(b + big * 2048, &p.x_small, c, n_cta + 16 * big, bar);
+        }
+      }
+      if (!ok) break;
+    }
+    // A pair's CTA stays until the commits that arrive here from the other CTA have.
+    if (kCtas == 2)
+      for (int j = max(0, it - kStages); j < it; ++j) wait_or_abort(&empty[j % kStages], uint32_t(j / kStages) & 1u, abort);
+    // No load may still be landing when the CTA exits: after an expired wait, give them time.
+    if (*abort && lane == 0 && leader)
+      for (int j = max(0, it - kStages); j < it; ++j) mbar_wait(&full[j % kStages], uint32_t(j / kStages) & 1u);
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA thread
+    if (lane == 0 && leader) {
+      int it = 0, count = 0;
+      for (int t = first; t < tiles && live; t += stride) {
+        const Tile x = tile_of<kCtas, kNT>(p, bounds, starts, t);
+        const int ab = count & 1;
+        if (!wait_cluster(&acc_empty[ab], (uint32_t(count >> 1) & 1u) ^ 1u, abort)) break;
+        ++count;
+        tc_fence_after();
+        const uint32_t d = tmem + uint32_t(ab * kNT);
+        const uint32_t idesc0 = instruction(128 * kCtas, x.nt, 0), idesc1 = instruction(128 * kCtas, x.nt, 2);
+        bool ok = true;
+        for (int ks = ks0; ks < ks1; ++ks, ++it) {
+          const int st = it % kStages, set = it & 1;
+          ok = wait_cluster(&full[st], uint32_t(it / kStages) & 1u, abort) &&
+               wait_or_abort(&set_done[set], (uint32_t(it >> 1) & 1u) ^ 1u, abort);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t sa = smem_u32(ring + st * S::kStageBytes);
+          const uint32_t sc = sa + kABytes + S::kBRows * 128;
+          const uint32_t ts = tmem + uint32_t(2 * kNT + set * S::kScaleColumns);  // W: 2 x 4 columns, then x
+#pragma unroll
+          for (int i = 0; i < 2 * (1 + S::kHalves); ++i) copy_scales<kCtas>(ts + 4 * i, sc + 512 * i);
+          const uint64_t ad = sw128_desc(sa), bd = sw128_desc(sa + kABytes);
+#pragma unroll
+          for (int k = 0; k < kStep / 64; ++k)
+            mma_mxf4<kCtas>(d, ad + 2 * k, bd + 2 * k, k & 1 ? idesc1 : idesc0, ts + 4 * (k >> 1),
+                            ts + 8 + 4 * S::kHalves * (k >> 1), (ks > ks0 || k > 0) ? 1u : 0u);
+          commit<kCtas>(&empty[st]);
+          commit_here<kCtas>(&set_done[set]);
+        }
+        if (!ok) break;
+        commit<kCtas>(&acc_full[ab]);
+      }
+      // Every arrival on this CTA's barriers has landed, and after an expired wait every MMA has retired.
+      for (int j = max(0, it - 2); j < it; ++j) wait_or_abort(&set_done[j & 1], uint32_t(j >> 1) & 1u, abort);
+      if (*abort) {
+        commit_here<kCtas>(fin);
+        mbar_wait(fin, 0);
+      }
+    }
+  } else if (warp < 6) {
+    // ------------------------------------------------------------ stores
+    const int quarter = warp & 3;
+    const uint32_t lanes = uint32_t(quarter * 32) << 16;
+    const uint32_t staging = smem_u32(part) + uint32_t(quarter * kChunkBytes);
+    int count = 0;
+    for (int t = first; t < tiles; t += stride, ++count) {
+      const Tile x = tile_of<kCtas, kNT>(p, bounds, starts, t);
+      const int ab = count & 1;
+      if (live) {
+        if (!__all_sync(0xffffffffu, wait_or_abort(&acc_full[ab], uint32_t(count >> 1) & 1u, abort))) break;
+        tc_fence_after();
+      }
+      const uint32_t d = tmem + lanes + uint32_t(ab * kNT);
+      const int f0 = x.m0 + (kCtas == 2 ? rank * 128 : 0) + quarter * 32;
+      auto release = [&]() {
+        tc_fence_before();
+        __syncwarp();
+        if (live && lane == 0) {
+          if (kCtas == 2) arrive_cluster(mapa(&acc_empty[ab], 0));
+          else mbar_arrive(&acc_empty[ab]);
+        }
+      };
+      if (kCtas == 1 && cluster > 1) {
+        if (!store_split(p.out, d, live, f0, x.n0, x.nt, x.valid, part, part_full, part_empty, count, cluster, rank,
+                         quarter, lane, abort, release))
+          break;
+      } else {
+        store_whole(p.out, d, live, f0, x.n0, x.nt, x.valid, staging, lane);
+        release();
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ scales
+    constexpr int kRows = 1 + S::kHalves;  // rows a thread reads: one of W, one of each half of the tile's rows
+    const int i = tid - 192;
+    int it = 0;
+    for (int t = first; t < tiles && live; t += stride) {
+      const Tile x = tile_of<kCtas, kNT>(p, bounds, starts, t);
+      const uint8_t* row[kRows];
+      const int n = x.m0 + (kCtas == 2 ? rank * 128 : 0) + i;
+      row[0] = n < p.N ? p.w_scales + (int64_t(x.e) * p.N + n) * p.blocks : nullptr;
+#pragma unroll
+      for (int h = 0; h < S::kHalves; ++h) {
+        const int r = x.n0 + 128 * h + i;
+        const int src = 128 * h + i < x.valid ? (p.rows ? p.rows[r] : r) : -1;
+        row[1 + h] = src >= 0 && src < p.x_rows ? p.x_scales + int64_t(src) * p.blocks : nullptr;
+      }
+      uint32_t next[kRows][8];
+#pragma unroll
+      for (int q = 0; q < kRows; ++q) load_scales(row[q], ks0 * 8, p.blocks, q ? p.x_align : p.w_align, next[q]);
+      bool ok = true;
+      for (int k0 = ks0; k0 < ks1 && ok; k0 += kSuper) {
+        uint32_t now[kRows][8];
+#pragma unroll
+        for (int q = 0; q < kRows; ++q) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) now[q][j] = next[q][j];
+        }
+        if (k0 + kSuper < ks1) {
+#pragma unroll
+          for (int q = 0; q < kRows; ++q) load_scales(row[q], (k0 + kSuper) * 8, p.blocks, q ? p.x_align : p.w_align, next[q]);
+        }
+#pragma unroll
+        for (int j = 0; j < kSuper; ++j) {
+          if (k0 + j >= ks1 || !ok) continue;
+          const int st = it % kStages;
+          ok = __all_sync(0xffffffffu, wait_or_abort(&empty[st], (uint32_t(it / kStages) & 1u) ^ 1u, abort));
+          ++it;
+          if (!ok) continue;
+          const uint32_t sc = smem_u32(ring + st * S::kStageBytes) + kABytes + S::kBRows * 128 +
+                              uint32_t((i & 31) * 16 + (i >> 5) * 4);
+#pragma unroll
+          for (int q = 0; q < kRows; ++q) {
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+              // W: group g at block g; x: group g, half h at block 2 + g * halves + h.
+              const uint32_t block = q == 0 ? g : 2 + g * S::kHalves + (q - 1);
+              asm volatile("st.shared.b32 [%0], %1;" ::"r"(sc + block * 512), "r"(now[q][2 * j + g]) : "memory");
+            }
+          }
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            if (kCtas == 2) arrive_cluster(mapa(&full[st], 0));
+            else mbar_arrive(&full[st]);
+          }
+        }
+      }
+      if (!ok) break;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (cluster > 1) cluster_sync();
+  if (warp == 1) {
+    tc_fence_after();
+    free_tmem<kCtas>(tmem, S::kColumns);
+  }
+}
+
+constexpr int kWideRows = 224, kNarrowRows = 64;
+
+bool narrow(int64_t E, int64_t R) { return R <= kNarrowRows * (E < R ? E : R); }
+
+template <int kCtas, int kNT>
+int launch_mx(const MxParams& p, int64_t tiles, void* stream) {
+  using S = Shape<kCtas, kNT>;
+  int sms = 0;
+  if (int rc = sm_count(&sms)) return rc;
+  const int cluster = kCtas == 2 ? 2 : p.split;
+  int64_t grid = int64_t(sms / cluster) * cluster;
+  if (tiles * cluster < grid) grid = tiles * cluster;
+  const int smem = 1024 + S::kStages * S::kStageBytes + S::kPartBytes + 256 +
+                   int(sizeof(int)) * (kMaxWarps + 2 + 2 * (p.E + 1));
+  static int flags[64] = {};
+  if (int rc = ensure_smem(mx_kernel<kCtas, kNT>, smem, flags)) return rc;
+  return launch_clusters(mx_kernel<kCtas, kNT>, int(grid), kThreads, cluster, smem, stream, "expert_linear_mxfp4", p);
+}
+
+bool encode_codes(CUtensorMap* map, const void* p, int64_t bytes, int64_t rows, int box_rows) {
+  const cuuint64_t dims[2] = {cuuint64_t(bytes), cuuint64_t(rows)};
+  const cuuint64_t strides[1] = {cuuint64_t(bytes)};
+  const cuuint32_t box[2] = {128, cuuint32_t(box_rows)};
+  return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, p, dims, strides, box);
+}
+
+int row_alignment(const void* p, int blocks) {
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(p) | uintptr_t(blocks);
+  return bits & 7 ? 1 : bits & 15 ? 8 : 16;
+}
+
+}  // namespace
+
+int mx_wait_timeouts(unsigned int* value, int reset) {
+  if (cudaMemcpyFromSymbol(value, g_lf_wait_timeouts, sizeof(*value)) != cudaSuccess)
+    return check_launch("device_wait_timeouts (MXFP4 products)");
+  if (reset && *value) {
+    const unsigned int zero = 0;
+    if (cudaMemcpyToSymbol(g_lf_wait_timeouts, &zero, sizeof(zero)) != cudaSuccess)
+      return check_launch("device_wait_timeouts (MXFP4 products)");
+  }
+  return LF_OK;
+}
+
+}  // namespace lfb
+
+using namespace lfb;
+
+extern "C" int64_t lf_expert_linear_mxfp4_workspace_bytes(int32_t num_experts, int64_t num_rows, int64_t width) {
+  if (num_experts < 1 || num_rows < 0 || width < 1) return -1;
+  return narrow(num_experts, num_rows) ? 0 : num_rows * (width / 2);
+}
+
+extern "C" int lf_expert_linear_mxfp4(int32_t out_dtype, const uint8_t* x_codes, const uint8_t* x_scales,
+                                      int64_t x_rows, const int32_t* rows, const uint8_t* w_codes,
+                                      const uint8_t* w_scales, const int32_t* offsets, int32_t num_experts,
+                                      int64_t num_rows, int64_t out_width, int64_t width, void* y, int64_t y_stride,
+                                      void* workspace, int64_t workspace_bytes, void* stream) {
+  const int64_t limit = int64_t(1) << 31;
+  if (out_dtype < LF_F32 || out_dtype > LF_BF16) return fail(LF_E_INVALID, "expert_linear_mxfp4: unknown output type");
+  if (num_experts < 1 || num_experts > kMaxExperts || num_rows < 0 || num_rows >= limit - 256 || out_width < 1 ||
+      out_width >= limit - 256 || width < 32 || width % 32 || width >= limit - 256 ||
+      (num_rows / kNarrowRows + num_experts + 1) * (out_width / 128 + 1) >= limit)
+    return fail(LF_E_INVALID, "expert_linear_mxfp4: needs 1..1024 experts, a width that is a multiple of 32, and rows and tiles that fit int32");
+  if (num_rows == 0) return LF_OK;
+  if (!x_codes || !x_scales || !w_codes || !w_scales || !offsets || !y || y_stride < out_width || !aligned16(x_codes) ||
+      !aligned16(w_codes))
+    return fail(LF_E_INVALID, "expert_linear_mxfp4: null buffer, codes not 16-byte aligned, or y's rows overlap");
+  if (x_rows < 1 || x_rows >= limit - 1 || (!rows && x_rows < num_rows))
+    return fail(LF_E_INVALID, "expert_linear_mxfp4: x has too few rows");
+  MxParams p{};
+  p.offsets = offsets, p.rows = rows, p.out = {y, y_stride, int(out_width), out_dtype};
+  p.x_scales = x_scales, p.w_scales = w_scales;
+  p.E = num_experts, p.R = int(num_rows), p.x_rows = int(x_rows), p.N = int(out_width), p.K = int(width);
+  p.blocks = int(width / 32);
+  p.x_align = row_alignment(x_scales, p.blocks), p.w_align = row_alignment(w_scales, p.blocks);
+  const bool few = narrow(num_experts, num_rows);
+  int64_t code_rows = x_rows;
+  if (rows && !few) {
+    const int64_t need = lf_expert_linear_mxfp4_workspace_bytes(num_experts, num_rows, width);
+    if (!workspace || workspace_bytes < need || !aligned16(workspace))
+      return fail(LF_E_INVALID, "expert_linear_mxfp4: workspace missing, too small or not 16-byte aligned "
+                                "(see lf_expert_linear_mxfp4_workspace_bytes)");
+    // Rows of width / 2 bytes as rows of width / 4 16-bit values.
+    if (int rc = gather_rows(x_codes, width / 4, x_rows, rows, num_rows, width / 4, workspace, stream, "expert_linear_mxfp4"))
+      return rc;
+    x_codes = static_cast<const uint8_t*>(workspace), code_rows = num_rows, p.gathered = 1;
+  }
+  const cuuint64_t dims[3] = {cuuint64_t(width / 2), cuuint64_t(out_width), cuuint64_t(num_experts)};
+  const cuuint64_t strides[2] = {cuuint64_t(width / 2), cuuint64_t(width / 2) * cuuint64_t(out_width)};
+  const cuuint32_t box[3] = {128, 128, 1};
+  if (!encode_map(&p.w_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, w_codes, dims, strides, box) ||
+      !encode_codes(&p.x_map, x_codes, width / 2, code_rows, 16) ||
+      !encode_codes(&p.x_small, x_codes, width / 2, code_rows, 8) ||
+      !encode_codes(&p.x_gather, x_codes, width / 2, code_rows, 1))
+    return fail(LF_E_CUDA, "expert_linear_mxfp4: cuTensorMapEncodeTiled failed");
+  const int64_t groups = num_experts < num_rows ? num_experts : num_rows;
+  if (few) {
+    const int64_t mt = ceil_div(p.N, 128);
+    p.split = choose_split(mt * groups, ceil_div(p.K, kStep), kSuper);
+    return launch_mx<1, kNarrowRows>(p, mt * (groups + num_rows / kNarrowRows), stream);
+  }
+  p.split = 1;
+  return launch_mx<2, kWideRows>(p, int64_t(ceil_div(p.N, 256)) * (groups + num_rows / kWideRows), stream);
+}

@@ -52,6 +52,7 @@
 #include <string>
 
 #include "launch.cuh"
+#include "experts.cuh"
 #include "sgmv.cuh"
 #include "tma.cuh"
 
@@ -1736,9 +1737,10 @@ extern "C" int lf_device_wait_timeouts(int32_t* count, int32_t reset) {
     return check_launch("device_wait_timeouts");
   unsigned int prefill = 0;
   if (int rc = prefill_wait_timeouts(&prefill, reset)) return rc;
-  unsigned int grouped = 0;
+  unsigned int grouped = 0, mx = 0;
   if (int rc = grouped_wait_timeouts(&grouped, reset)) return rc;
-  if (count) *count = int32_t(value + prefill + grouped);
+  if (int rc = mx_wait_timeouts(&mx, reset)) return rc;
+  if (count) *count = int32_t(value + prefill + grouped + mx);
   if (reset) {
     const unsigned int zero = 0;
     if (cudaMemcpyToSymbol(g_lf_wait_timeouts, &zero, sizeof(zero)) != cudaSuccess)

@@ -47,7 +47,5 @@ int prefill_launch(const void* x, int64_t x_stride, const void* a, const void* b
 
 // Expired bounded waits counted by the prefill kernels' translation unit (synchronous).
 int prefill_wait_timeouts(unsigned int* value, int reset);
-// The same for grouped_gemm.cu.
-int grouped_wait_timeouts(unsigned int* value, int reset);
 
 }  // namespace lfb

@@ -12,7 +12,8 @@ from __future__ import annotations
 from typing import NamedTuple
 
 from loraforge_b200 import _native
-from loraforge_b200.ops.experts import cuda_tensor, packed_table
+from loraforge_b200.ops._contract import output_is_distinct
+from loraforge_b200.ops.experts import MAX_EXPERTS, cuda_tensor, group_tables, packed_table, row_matrix, row_stride
 
 BLOCK = 32
 
@@ -82,4 +83,44 @@ def mxfp4_dequantize(x: MxTensor, dtype=None):
     with torch.cuda.device(out.device):
         _native.call("lf_mxfp4_dequantize", _native.dtype_code(dtype), x.codes.data_ptr(), x.scales.data_ptr(),
                      out.numel() // shape[-1], shape[-1], out.data_ptr(), _native.stream_of(out.device))
+    return out
+
+
+def expert_linear_mxfp4(x: MxTensor, weight: MxTensor, offsets, *, rows=None, dtype=None, out=None):
+    """``expert_linear`` of MXFP4 operands on the block-scaled tensor cores.
+
+    ``x`` [T, K] and ``weight`` [E, N, K] are MxTensors; ``offsets`` int32 [E + 1] and ``rows``
+    int32 [R] as in ``expert_linear`` (one expert and offsets (0, T) give a dense product).
+    Sums are FP32, rounded once to ``dtype`` (FP32 / FP16 / BF16, default BF16 or out's); rows of
+    no group are zeros.  Returns y [R, N] (``out`` when given).
+    """
+    import torch
+
+    T, K = check_mx(x, "x", 2)
+    device = x.codes.device
+    E, N, width = check_mx(weight, "weight", 3, device)
+    if width != K:
+        raise ValueError("x's width must be the weight's")
+    if not 1 <= E <= MAX_EXPERTS or N < 1:
+        raise ValueError(f"weight must be [experts, out, in] with 1..{MAX_EXPERTS} experts")
+    R = group_tables(offsets, rows, E, T, device)
+    kinds = (torch.float32, torch.float16, torch.bfloat16)
+    if dtype is not None and dtype not in kinds:
+        raise ValueError("dtype must be float32, float16 or bfloat16")
+    if out is None:
+        out = torch.empty((R, N), dtype=torch.bfloat16 if dtype is None else dtype, device=device)
+    else:
+        row_matrix(out, "out", kinds if dtype is None else (dtype,), device)
+        if tuple(out.shape) != (R, N):
+            raise ValueError("out must be [rows, out features]")
+        output_is_distinct(out, (*x, *weight, offsets) if rows is None else (*x, *weight, offsets, rows))
+    room = 0 if rows is None else _native.expert_linear_mxfp4_workspace_bytes(E, R, K)
+    workspace = torch.empty(room, dtype=torch.uint8, device=device) if room else None
+    with torch.cuda.device(device):
+        _native.call(
+            "lf_expert_linear_mxfp4", _native.dtype_code(out.dtype), x.codes.data_ptr(), x.scales.data_ptr(), T,
+            None if rows is None else rows.data_ptr(), weight.codes.data_ptr(), weight.scales.data_ptr(),
+            offsets.data_ptr(), E, R, N, K, out.data_ptr(), row_stride(out),
+            None if workspace is None else workspace.data_ptr(), room, _native.stream_of(device),
+        )
     return out
