@@ -497,11 +497,13 @@ int lf_mxfp4_dequantize(int32_t dtype, const uint8_t* codes, const uint8_t* scal
  * sums on the block-scaled tensor cores, one rounding to out_dtype:
  *   y[r, n] = sum_k x[i(r), k] w[e, n, k]  for rows r of group e, as in lf_expert_linear.
  * x [x_rows, width], w [num_experts, out_width, width], both contiguous; width a multiple of 32.
- * With rows, groups of many rows copy x's codes in order into `workspace` first:
- * lf_expert_linear_mxfp4_workspace_bytes bytes, 16-byte aligned, not initialised.
+ * Groups of many rows lay out the scales (and with rows x's codes, in order) in `workspace`
+ * first: lf_expert_linear_mxfp4_workspace_bytes bytes, 16-byte aligned, not initialised (0: none
+ * needed; by_rows: whether rows is given).
  */
 int64_t lf_expert_linear_mxfp4_workspace_bytes(int32_t num_experts, int64_t num_rows,
-                                               int64_t width);
+                                               int64_t out_width, int64_t width,
+                                               int32_t by_rows);
 int lf_expert_linear_mxfp4(int32_t out_dtype, const uint8_t* x_codes, const uint8_t* x_scales,
                            int64_t x_rows, const int32_t* rows, const uint8_t* w_codes,
                            const uint8_t* w_scales, const int32_t* offsets, int32_t num_experts,

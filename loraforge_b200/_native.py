@@ -157,7 +157,7 @@ def library() -> ctypes.CDLL:
             lib.lf_expert_linear_workspace_bytes.restype = ctypes.c_int64
             lib.lf_expert_linear_workspace_bytes.argtypes = [_i32, _i64, _i64, _i32]
             lib.lf_expert_linear_mxfp4_workspace_bytes.restype = ctypes.c_int64
-            lib.lf_expert_linear_mxfp4_workspace_bytes.argtypes = [_i32, _i64, _i64]
+            lib.lf_expert_linear_mxfp4_workspace_bytes.argtypes = [_i32, _i64, _i64, _i64, _i32]
             _lib = lib
     return _lib
 
@@ -211,9 +211,10 @@ def expert_linear_workspace_bytes(num_experts: int, num_rows: int, width: int, w
     return n
 
 
-def expert_linear_mxfp4_workspace_bytes(num_experts: int, num_rows: int, width: int) -> int:
-    """Workspace bytes of lf_expert_linear_mxfp4 with row indices."""
-    n = library().lf_expert_linear_mxfp4_workspace_bytes(num_experts, num_rows, width)
+def expert_linear_mxfp4_workspace_bytes(num_experts: int, num_rows: int, out_width: int, width: int,
+                                        by_rows: bool) -> int:
+    """Workspace bytes of lf_expert_linear_mxfp4 (by_rows: with row indices)."""
+    n = library().lf_expert_linear_mxfp4_workspace_bytes(num_experts, num_rows, out_width, width, 1 if by_rows else 0)
     if n < 0:
         raise ValueError("invalid sizes for the expert workspace")
     return n

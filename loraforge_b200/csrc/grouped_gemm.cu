@@ -376,6 +376,28 @@ __global__ void __launch_bounds__(256) gather_rows_kernel(const uint4* x, int64_
     if (first + u * 256 < total) out[first + u * 256] = v[u];
 }
 
+int gather_rows(const void* x, int64_t x_stride, int64_t x_rows, const int32_t* rows, int64_t R, int64_t width,
+                void* out, void* stream, const char* what) {
+  cudaLaunchConfig_t config = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = attr;
+  config.numAttrs = 1;
+  const int64_t total = R * (width / 8);
+  config.gridDim = dim3(unsigned((total + 1023) / 1024));
+  config.blockDim = dim3(256);
+  config.stream = static_cast<cudaStream_t>(stream);
+  const cudaError_t err =
+      cudaLaunchKernelEx(&config, gather_rows_kernel, static_cast<const uint4*>(x), x_stride / 8, int(x_rows), rows,
+                         int(width / 8), total, static_cast<uint4*>(out));
+  if (err != cudaSuccess) {
+    last_error() = std::string(what) + ": " + cudaGetErrorString(err);
+    return LF_E_CUDA;
+  }
+  return LF_OK;
+}
+
 template <int kMode, int kCtas, int kNT>
 int launch_grouped(const GParams& p, int64_t tiles, void* stream, const char* what) {
   using S = Shape<kCtas, kNT>;
@@ -450,28 +472,6 @@ int launch_rows(GParams& p, void* stream, const char* what) {
 }
 
 }  // namespace
-
-int gather_rows(const void* x, int64_t x_stride, int64_t x_rows, const int32_t* rows, int64_t R, int64_t width,
-                void* out, void* stream, const char* what) {
-  cudaLaunchConfig_t config = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  config.attrs = attr;
-  config.numAttrs = 1;
-  const int64_t total = R * (width / 8);
-  config.gridDim = dim3(unsigned((total + 1023) / 1024));
-  config.blockDim = dim3(256);
-  config.stream = static_cast<cudaStream_t>(stream);
-  const cudaError_t err =
-      cudaLaunchKernelEx(&config, gather_rows_kernel, static_cast<const uint4*>(x), x_stride / 8, int(x_rows), rows,
-                         int(width / 8), total, static_cast<uint4*>(out));
-  if (err != cudaSuccess) {
-    last_error() = std::string(what) + ": " + cudaGetErrorString(err);
-    return LF_E_CUDA;
-  }
-  return LF_OK;
-}
 
 int grouped_wait_timeouts(unsigned int* value, int reset) {
   if (cudaMemcpyFromSymbol(value, g_lf_wait_timeouts, sizeof(*value)) != cudaSuccess)

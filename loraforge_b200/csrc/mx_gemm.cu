@@ -14,12 +14,16 @@
 //
 // Scales.  The tensor core wants them in TMEM: for 128 operand rows and 128 codes a row, four
 // columns in which lane l of column j holds the four bytes of row 32 j + l, the same in every
-// quarter of the lanes.  Four warps read them row by row (32 bytes of a row, a thread and four
-// stages: a whole sector), write them to the stage as the 512-byte blocks that tcgen05.cp
-// copies, and the MMA thread issues the copies before the stage's MMAs.  The copies go to two
-// sets of columns in turn; a set is written again when the MMAs that read it are done.
+// quarter of the lanes.  tcgen05.cp writes them there from blocks of 512 bytes in shared memory;
+// the MMA thread issues the copies before the stage's MMAs, to two sets of columns in turn, and a
+// set is written again when the MMAs that read it are done.  The blocks of a stage come
+//   wide    by TMA, from blocks that pack_kernel laid out in the workspace before (scales of
+//           28672 x 4096 weights: 3.7 MB each way).  Warps that read the scales and tell the
+//           pair's first CTA stage by stage cost 0.7 us a stage, against 0.25 for its MMAs;
+//   narrow  from four warps that read them row by row: 32 bytes of a row (a whole sector) for a
+//           thread and four stages, one such group ahead, also across tiles.
 //
-// Per CTA: warp 0 loads codes (TMA), warp 1 MMA and TMEM, warps 2-5 store, warps 6-9 scales.
+// Per CTA: warp 0 loads (TMA), warp 1 MMA and TMEM, warps 2-5 store, narrow: warps 6-9 scales.
 // Every wait is bounded (tma.cuh): an expiry stops every role at its next wait.
 #include "experts.cuh"
 #include "grouped.cuh"
@@ -29,7 +33,6 @@ namespace {
 
 using namespace grouped;
 
-constexpr int kThreads = 320;
 constexpr int kStep = 256;           // codes per stage: 128 bytes a row
 constexpr int kABytes = 128 * 128;
 constexpr int kSuper = 4;            // stages whose scales a thread loads at once (32 bytes a row)
@@ -42,12 +45,14 @@ struct MxParams {
   const uint8_t* w_scales;  // [E][N][blocks]
   int E, R, x_rows, N, K, blocks;
   int x_align, w_align;  // 16, 8 or 1: alignment of every row of the scales
-  int gathered;          // codes are in the rows' order already
+  int groups;            // wide: groups of 128 codes in the packed scales, an even number
   int split;
   CUtensorMap w_map;      // 128 bytes x 128 rows
   CUtensorMap x_map;      // 128 bytes x 16 rows
   CUtensorMap x_small;    // 128 bytes x 8 rows
   CUtensorMap x_gather;   // single rows
+  CUtensorMap w_blocks;   // wide: packed scales, 512 bytes x 2 blocks
+  CUtensorMap x_blocks;   // 512 bytes x 4 blocks
 };
 
 template <int kCtas, int kNT>
@@ -58,6 +63,7 @@ struct Shape {
   static constexpr int kStageBytes = (kABytes + kBRows * 128 + kScaleBytes + 1023) / 1024 * 1024;
   static constexpr int kPartBytes = kCtas == 1 ? kNT * 128 * 4 : 4 * kChunkBytes;
   static constexpr int kStages = kCtas == 2 ? 6 : 7;
+  static constexpr int kThreads = kCtas == 2 ? 192 : 320;
   static constexpr int kScaleColumns = 2 * (4 + 4 * kHalves);    // a set
   static constexpr int kColumns = kCtas == 2 ? 512 : 256;        // TMEM
   static_assert(2 * kNT + 2 * kScaleColumns <= kColumns, "TMEM");
@@ -110,6 +116,7 @@ __device__ __forceinline__ void commit_here(uint64_t* bar) {
 
 struct Tile {
   int e, m0, n0, nt, valid, hi;
+  int row_tile;  // among the row tiles of all groups
 };
 
 template <int kCtas, int kNT>
@@ -118,9 +125,10 @@ __device__ __forceinline__ Tile tile_of(const MxParams& p, const int* bounds, co
   x.e = group_of(starts, p.E, t);
   const int lo = bounds[x.e];
   x.hi = bounds[x.e + 1];
-  const int nt = ceil_div(x.hi - lo, kNT);
+  const int mt = ceil_div(p.N, 128 * kCtas), nt = ceil_div(x.hi - lo, kNT);
   int m, n;
-  place_tile(t - starts[x.e], ceil_div(p.N, 128 * kCtas), nt, &m, &n);
+  place_tile(t - starts[x.e], mt, nt, &m, &n);
+  x.row_tile = starts[x.e] / mt + n;
   x.m0 = m * 128 * kCtas;
   const int each = round_up(ceil_div(x.hi - lo, nt), 16);
   x.n0 = lo + n * each;
@@ -152,7 +160,7 @@ __device__ __forceinline__ void load_scales(const uint8_t* row, int k0, int bloc
 }
 
 template <int kCtas, int kNT>
-__global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__ MxParams p) {
+__global__ void __launch_bounds__(Shape<kCtas, kNT>::kThreads, 1) mx_kernel(const __grid_constant__ MxParams p) {
   using S = Shape<kCtas, kNT>;
   constexpr int kStages = S::kStages;
   extern __shared__ uint8_t smem_raw[];
@@ -179,7 +187,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
   const bool leader = rank * (kCtas - 1) == 0;
   if (tid == 0) {
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(&full[i], 1 + 4 * kCtas);  // the codes' bytes and the scale warps
+      mbar_init(&full[i], kCtas == 2 ? 1 : 1 + 4);  // the loads' bytes, narrow: and the scale warps
       mbar_init(&empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -224,7 +232,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
       const int m_cta = x.m0 + (kCtas == 2 ? rank * 128 : 0);
       const int share = x.nt / kCtas;
       const int n_cta = x.n0 + (kCtas == 2 ? rank * share : 0);
-      const bool by_row = kCtas == 1 && p.rows && !p.gathered;
+      const bool by_row = kCtas == 1 && p.rows;
       int row4[4];
       if (by_row) {
 #pragma unroll
@@ -234,7 +242,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
           row4[i] = src >= 0 && src < p.x_rows ? src : p.x_rows;
         }
       }
-      const uint32_t bytes = kCtas * (kABytes + uint32_t(share) * 128u);
+      const uint32_t bytes = kCtas * (kABytes + uint32_t(share) * 128u + (kCtas == 2 ? uint32_t(S::kScaleBytes) : 0u));
       bool ok = true;
       for (int ks = ks0; ks < ks1; ++ks, ++it) {
         const int st = it % kStages;
@@ -246,6 +254,12 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
         __syncwarp();
         const int c = ks * 128;  // bytes along K
         if (lane == 0) load_3d<kCtas>(a, &p.w_map, c, m_cta, x.e, bar);
+        if (kCtas == 2 && lane >= 30) {
+          const uint32_t sc = b + S::kBRows * 128;
+          const int wb = (x.e * ceil_div(p.N, 256) * 2 + m_cta / 128) * p.groups + 2 * ks;
+          if (lane == 30) load_2d<kCtas>(sc, &p.w_blocks, 0, wb, bar);
+          else load_2d<kCtas>(sc + 1024, &p.x_blocks, 0, (x.row_tile * p.groups + 2 * ks) * 2, bar);
+        }
         if (by_row) {
           if (4 * lane < share) gather4<kCtas>(b + lane * 512, &p.x_gather, c, row4, bar);
         } else {
@@ -277,7 +291,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
         bool ok = true;
         for (int ks = ks0; ks < ks1; ++ks, ++it) {
           const int st = it % kStages, set = it & 1;
-          ok = wait_cluster(&full[st], uint32_t(it / kStages) & 1u, abort) &&
+          ok = wait_or_abort(&full[st], uint32_t(it / kStages) & 1u, abort) &&
                wait_or_abort(&set_done[set], (uint32_t(it >> 1) & 1u) ^ 1u, abort);
           if (!ok) break;
           tc_fence_after();
@@ -336,64 +350,64 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
         release();
       }
     }
-  } else {
+  } else if constexpr (kCtas == 1) {
     // ------------------------------------------------------------ scales
-    constexpr int kRows = 1 + S::kHalves;  // rows a thread reads: one of W, one of each half of the tile's rows
+    constexpr int kRows = 2;  // rows a thread reads: one of W and one of the tile's
     const int i = tid - 192;
-    int it = 0;
-    for (int t = first; t < tiles && live; t += stride) {
+    const uint8_t* row[kRows] = {nullptr, nullptr};
+    auto rows_of = [&](int t) {
       const Tile x = tile_of<kCtas, kNT>(p, bounds, starts, t);
-      const uint8_t* row[kRows];
-      const int n = x.m0 + (kCtas == 2 ? rank * 128 : 0) + i;
+      const int n = x.m0 + i, r = x.n0 + i;
       row[0] = n < p.N ? p.w_scales + (int64_t(x.e) * p.N + n) * p.blocks : nullptr;
+      const int src = i < x.valid ? (p.rows ? p.rows[r] : r) : -1;
+      row[1] = src >= 0 && src < p.x_rows ? p.x_scales + int64_t(src) * p.blocks : nullptr;
+    };
+    uint32_t next[kRows][8];
+    auto load = [&](int k0) {
 #pragma unroll
-      for (int h = 0; h < S::kHalves; ++h) {
-        const int r = x.n0 + 128 * h + i;
-        const int src = 128 * h + i < x.valid ? (p.rows ? p.rows[r] : r) : -1;
-        row[1 + h] = src >= 0 && src < p.x_rows ? p.x_scales + int64_t(src) * p.blocks : nullptr;
+      for (int q = 0; q < kRows; ++q) load_scales(row[q], k0 * 8, p.blocks, q ? p.x_align : p.w_align, next[q]);
+    };
+    int it = 0, t = first, k0 = ks0;
+    bool ok = live && t < tiles;
+    if (ok) {
+      rows_of(t);
+      load(k0);
+    }
+    while (ok) {
+      uint32_t now[kRows][8];
+#pragma unroll
+      for (int q = 0; q < kRows; ++q) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) now[q][j] = next[q][j];
       }
-      uint32_t next[kRows][8];
+      const int todo = min(kSuper, ks1 - k0);
+      k0 += kSuper;
+      if (k0 >= ks1) {
+        k0 = ks0;
+        t += stride;
+        if (t < tiles) rows_of(t);
+      }
+      if (t < tiles) load(k0);
 #pragma unroll
-      for (int q = 0; q < kRows; ++q) load_scales(row[q], ks0 * 8, p.blocks, q ? p.x_align : p.w_align, next[q]);
-      bool ok = true;
-      for (int k0 = ks0; k0 < ks1 && ok; k0 += kSuper) {
-        uint32_t now[kRows][8];
+      for (int j = 0; j < kSuper; ++j) {
+        if (j >= todo || !ok) continue;
+        const int st = it % kStages;
+        ok = __all_sync(0xffffffffu, wait_or_abort(&empty[st], (uint32_t(it / kStages) & 1u) ^ 1u, abort));
+        ++it;
+        if (!ok) continue;
+        const uint32_t sc = smem_u32(ring + st * S::kStageBytes) + kABytes + S::kBRows * 128 +
+                            uint32_t((i & 31) * 16 + (i >> 5) * 4);
 #pragma unroll
         for (int q = 0; q < kRows; ++q) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) now[q][j] = next[q][j];
+          for (int g = 0; g < 2; ++g)
+            asm volatile("st.shared.b32 [%0], %1;" ::"r"(sc + uint32_t(2 * q + g) * 512u), "r"(now[q][2 * j + g]) : "memory");
         }
-        if (k0 + kSuper < ks1) {
-#pragma unroll
-          for (int q = 0; q < kRows; ++q) load_scales(row[q], (k0 + kSuper) * 8, p.blocks, q ? p.x_align : p.w_align, next[q]);
-        }
-#pragma unroll
-        for (int j = 0; j < kSuper; ++j) {
-          if (k0 + j >= ks1 || !ok) continue;
-          const int st = it % kStages;
-          ok = __all_sync(0xffffffffu, wait_or_abort(&empty[st], (uint32_t(it / kStages) & 1u) ^ 1u, abort));
-          ++it;
-          if (!ok) continue;
-          const uint32_t sc = smem_u32(ring + st * S::kStageBytes) + kABytes + S::kBRows * 128 +
-                              uint32_t((i & 31) * 16 + (i >> 5) * 4);
-#pragma unroll
-          for (int q = 0; q < kRows; ++q) {
-#pragma unroll
-            for (int g = 0; g < 2; ++g) {
-              // W: group g at block g; x: group g, half h at block 2 + g * halves + h.
-              const uint32_t block = q == 0 ? g : 2 + g * S::kHalves + (q - 1);
-              asm volatile("st.shared.b32 [%0], %1;" ::"r"(sc + block * 512), "r"(now[q][2 * j + g]) : "memory");
-            }
-          }
-          fence_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            if (kCtas == 2) arrive_cluster(mapa(&full[st], 0));
-            else mbar_arrive(&full[st]);
-          }
-        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full[st]);
       }
-      if (!ok) break;
+      ok = ok && t < tiles;
     }
   }
   tc_fence_before();
@@ -409,6 +423,95 @@ constexpr int kWideRows = 224, kNarrowRows = 64;
 
 bool narrow(int64_t E, int64_t R) { return R <= kNarrowRows * (E < R ? E : R); }
 
+// The wide tiles' workspace: W's scales as blocks [expert][128 features][group of 128 codes],
+// x's as [row tile][group][half], and x's codes in the rows' order.
+struct PackParams {
+  const int32_t* offsets;
+  const int32_t* rows;
+  const uint8_t* x_scales;
+  const uint8_t* w_scales;
+  const uint4* x_codes;  // null: in order already
+  uint8_t *w_blocks, *x_blocks;
+  uint4* codes;
+  int E, R, x_rows, N, blocks, groups, words;  // words: 16-byte words of a row of codes
+  int w_tasks, x_tasks, words4;                // CUDA blocks for each part; words4: 4-byte reads of scales allowed
+};
+
+__device__ __forceinline__ uint32_t scale_word(const uint8_t* row, int k, int blocks, bool words) {
+  if (!row || k >= blocks) return 0;
+  if (words) return *reinterpret_cast<const uint32_t*>(row + k);
+  uint32_t v = 0;
+  for (int i = 0; i < 4 && k + i < blocks; ++i) v |= uint32_t(row[k + i]) << (8 * i);
+  return v;
+}
+
+constexpr int kPackThreads = 256;
+
+// One CUDA block writes the scale blocks of 128 features, or of a row tile (2 x 128 rows), a warp
+// one 512-byte block at a time: lane l takes rows l, l + 32, l + 64, l + 96.  Or it moves 1024
+// 16-byte words of codes.
+template <int kNT>
+__global__ void __launch_bounds__(kPackThreads) pack_kernel(const __grid_constant__ PackParams p) {
+  __shared__ int scan[kMaxWarps];
+  extern __shared__ int tables[];
+  pdl_wait();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  int task = blockIdx.x;
+  if (task < p.w_tasks) {
+    const int mb = ceil_div(p.N, 256) * 2, e = task / mb, n0 = (task % mb) * 128 + lane;
+    const uint8_t* row[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      row[j] = n0 + 32 * j < p.N ? p.w_scales + (int64_t(e) * p.N + n0 + 32 * j) * p.blocks : nullptr;
+    uint4* out = reinterpret_cast<uint4*>(p.w_blocks + int64_t(task) * p.groups * 512) + lane;
+    for (int g = warp; g < p.groups; g += kPackThreads / 32)
+      out[g * 32] = make_uint4(scale_word(row[0], 4 * g, p.blocks, p.words4), scale_word(row[1], 4 * g, p.blocks, p.words4),
+                               scale_word(row[2], 4 * g, p.blocks, p.words4), scale_word(row[3], 4 * g, p.blocks, p.words4));
+    return;
+  }
+  task -= p.w_tasks;
+  if (task < p.x_tasks) {
+    int* bounds = tables;
+    int* starts = bounds + p.E + 1;
+    list_tiles(p.offsets, p.E, p.R, bounds, starts, scan, [](int rows) { return ceil_div(rows, kNT); });
+    if (task >= starts[p.E]) return;
+    const int e = group_of(starts, p.E, task), lo = bounds[e], hi = bounds[e + 1];
+    const int each = round_up(ceil_div(hi - lo, ceil_div(hi - lo, kNT)), 16);
+    const int n0 = lo + (task - starts[e]) * each, valid = min(each, hi - n0);
+    const uint8_t* row[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int r = lane + 32 * j;
+      const int src = r < valid ? (p.rows ? p.rows[n0 + r] : n0 + r) : -1;
+      row[j] = src >= 0 && src < p.x_rows ? p.x_scales + int64_t(src) * p.blocks : nullptr;
+    }
+    uint4* out = reinterpret_cast<uint4*>(p.x_blocks + int64_t(task) * p.groups * 1024) + lane;
+    for (int g = warp; g < p.groups; g += kPackThreads / 32) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        out[(g * 2 + h) * 32] =
+            make_uint4(scale_word(row[4 * h], 4 * g, p.blocks, p.words4), scale_word(row[4 * h + 1], 4 * g, p.blocks, p.words4),
+                       scale_word(row[4 * h + 2], 4 * g, p.blocks, p.words4), scale_word(row[4 * h + 3], 4 * g, p.blocks, p.words4));
+    }
+    return;
+  }
+  task -= p.x_tasks;
+  const int64_t total = int64_t(p.R) * p.words;
+  const int64_t at = int64_t(task) * (4 * kPackThreads) + tid;
+  uint4 v[4];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const int64_t i = at + u * kPackThreads;
+    if (i >= total) continue;
+    const int64_t r = i / p.words;
+    const int src = p.rows[r];
+    v[u] = src >= 0 && src < p.x_rows ? p.x_codes[int64_t(src) * p.words + (i - r * p.words)] : make_uint4(0, 0, 0, 0);
+  }
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    if (at + u * kPackThreads < total) p.codes[at + u * kPackThreads] = v[u];
+}
+
 template <int kCtas, int kNT>
 int launch_mx(const MxParams& p, int64_t tiles, void* stream) {
   using S = Shape<kCtas, kNT>;
@@ -421,7 +524,7 @@ int launch_mx(const MxParams& p, int64_t tiles, void* stream) {
                    int(sizeof(int)) * (kMaxWarps + 2 + 2 * (p.E + 1));
   static int flags[64] = {};
   if (int rc = ensure_smem(mx_kernel<kCtas, kNT>, smem, flags)) return rc;
-  return launch_clusters(mx_kernel<kCtas, kNT>, int(grid), kThreads, cluster, smem, stream, "expert_linear_mxfp4", p);
+  return launch_clusters(mx_kernel<kCtas, kNT>, int(grid), S::kThreads, cluster, smem, stream, "expert_linear_mxfp4", p);
 }
 
 bool encode_codes(CUtensorMap* map, const void* p, int64_t bytes, int64_t rows, int box_rows) {
@@ -429,6 +532,32 @@ bool encode_codes(CUtensorMap* map, const void* p, int64_t bytes, int64_t rows, 
   const cuuint64_t strides[1] = {cuuint64_t(bytes)};
   const cuuint32_t box[2] = {128, cuuint32_t(box_rows)};
   return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, p, dims, strides, box);
+}
+
+// 512-byte scale blocks, `box_blocks` at a time.
+bool encode_blocks(CUtensorMap* map, const void* p, int64_t blocks, int box_blocks) {
+  const PFN_cuTensorMapEncodeTiled_v12000 encode = map_encoder();
+  const cuuint64_t dims[2] = {128, cuuint64_t(blocks)};
+  const cuuint64_t strides[1] = {512};
+  const cuuint32_t box[2] = {128, cuuint32_t(box_blocks)}, ones[2] = {1, 1};
+  return encode && encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void*>(p), dims, strides, box, ones,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Sizes of the wide tiles' workspace: 512-byte blocks of W's and of x's scales, then codes.
+struct Workspace {
+  int groups;
+  int64_t row_tiles, w_blocks, x_blocks, bytes;
+};
+Workspace workspace_of(int64_t E, int64_t R, int64_t N, int64_t K, bool gather) {
+  Workspace w{};
+  w.groups = 2 * int((K + kStep - 1) / kStep);
+  w.row_tiles = (E < R ? E : R) + R / kWideRows;  // at most
+  w.w_blocks = E * ((N + 255) / 256) * 2 * w.groups;
+  w.x_blocks = w.row_tiles * w.groups * 2;
+  w.bytes = (w.w_blocks + w.x_blocks) * 512 + (gather ? R * (K / 2) : 0);
+  return w;
 }
 
 int row_alignment(const void* p, int blocks) {
@@ -453,9 +582,10 @@ int mx_wait_timeouts(unsigned int* value, int reset) {
 
 using namespace lfb;
 
-extern "C" int64_t lf_expert_linear_mxfp4_workspace_bytes(int32_t num_experts, int64_t num_rows, int64_t width) {
-  if (num_experts < 1 || num_rows < 0 || width < 1) return -1;
-  return narrow(num_experts, num_rows) ? 0 : num_rows * (width / 2);
+extern "C" int64_t lf_expert_linear_mxfp4_workspace_bytes(int32_t num_experts, int64_t num_rows, int64_t out_width,
+                                                          int64_t width, int32_t by_rows) {
+  if (num_experts < 1 || num_rows < 0 || out_width < 1 || width < 1) return -1;
+  return narrow(num_experts, num_rows) ? 0 : workspace_of(num_experts, num_rows, out_width, width, by_rows != 0).bytes;
 }
 
 extern "C" int lf_expert_linear_mxfp4(int32_t out_dtype, const uint8_t* x_codes, const uint8_t* x_scales,
@@ -483,15 +613,29 @@ extern "C" int lf_expert_linear_mxfp4(int32_t out_dtype, const uint8_t* x_codes,
   p.x_align = row_alignment(x_scales, p.blocks), p.w_align = row_alignment(w_scales, p.blocks);
   const bool few = narrow(num_experts, num_rows);
   int64_t code_rows = x_rows;
-  if (rows && !few) {
-    const int64_t need = lf_expert_linear_mxfp4_workspace_bytes(num_experts, num_rows, width);
-    if (!workspace || workspace_bytes < need || !aligned16(workspace))
+  if (!few) {
+    const Workspace w = workspace_of(num_experts, num_rows, out_width, width, rows != nullptr);
+    if (!workspace || workspace_bytes < w.bytes || !aligned16(workspace))
       return fail(LF_E_INVALID, "expert_linear_mxfp4: workspace missing, too small or not 16-byte aligned "
                                 "(see lf_expert_linear_mxfp4_workspace_bytes)");
-    // Rows of width / 2 bytes as rows of width / 4 16-bit values.
-    if (int rc = gather_rows(x_codes, width / 4, x_rows, rows, num_rows, width / 4, workspace, stream, "expert_linear_mxfp4"))
+    if (w.w_blocks >= limit || w.x_blocks >= limit)
+      return fail(LF_E_INVALID, "expert_linear_mxfp4: too many scale blocks");
+    PackParams k{};
+    k.offsets = offsets, k.rows = rows, k.x_scales = x_scales, k.w_scales = w_scales;
+    k.w_blocks = static_cast<uint8_t*>(workspace), k.x_blocks = k.w_blocks + w.w_blocks * 512;
+    k.codes = reinterpret_cast<uint4*>(k.x_blocks + w.x_blocks * 512);
+    k.x_codes = reinterpret_cast<const uint4*>(x_codes);
+    k.E = p.E, k.R = p.R, k.x_rows = p.x_rows, k.N = p.N, k.blocks = p.blocks, k.groups = w.groups;
+    k.words = int(width / 32), k.w_tasks = int(w.w_blocks / w.groups), k.x_tasks = int(w.row_tiles);
+    k.words4 = ((reinterpret_cast<uintptr_t>(x_scales) | reinterpret_cast<uintptr_t>(w_scales) | uintptr_t(p.blocks)) & 3) == 0;
+    const int64_t moves = rows ? (num_rows * k.words + 4 * kPackThreads - 1) / (4 * kPackThreads) : 0;
+    if (int rc = launch_clusters(pack_kernel<kWideRows>, int(k.w_tasks + k.x_tasks + moves), kPackThreads, 1,
+                                 int(sizeof(int)) * 2 * (p.E + 1), stream, "expert_linear_mxfp4 (scales)", k))
       return rc;
-    x_codes = static_cast<const uint8_t*>(workspace), code_rows = num_rows, p.gathered = 1;
+    if (rows) x_codes = reinterpret_cast<const uint8_t*>(k.codes), code_rows = num_rows;
+    p.groups = w.groups;
+    if (!encode_blocks(&p.w_blocks, k.w_blocks, w.w_blocks, 2) || !encode_blocks(&p.x_blocks, k.x_blocks, w.x_blocks, 4))
+      return fail(LF_E_CUDA, "expert_linear_mxfp4: cuTensorMapEncodeTiled failed");
   }
   const cuuint64_t dims[3] = {cuuint64_t(width / 2), cuuint64_t(out_width), cuuint64_t(num_experts)};
   const cuuint64_t strides[2] = {cuuint64_t(width / 2), cuuint64_t(width / 2) * cuuint64_t(out_width)};

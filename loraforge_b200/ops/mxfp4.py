@@ -114,7 +114,7 @@ def expert_linear_mxfp4(x: MxTensor, weight: MxTensor, offsets, *, rows=None, dt
         if tuple(out.shape) != (R, N):
             raise ValueError("out must be [rows, out features]")
         output_is_distinct(out, (*x, *weight, offsets) if rows is None else (*x, *weight, offsets, rows))
-    room = 0 if rows is None else _native.expert_linear_mxfp4_workspace_bytes(E, R, K)
+    room = _native.expert_linear_mxfp4_workspace_bytes(E, R, N, K, rows is not None)
     workspace = torch.empty(room, dtype=torch.uint8, device=device) if room else None
     with torch.cuda.device(device):
         _native.call(
