@@ -59,9 +59,10 @@ struct GParams {
   CUtensorMap a_map;     // forward: W boxes 64 k x 128 n; input: 64 k x 64 n; weight: x boxes 64 k x 64 rows
   CUtensorMap a_small;   // weight: 64 k x 8 rows
   CUtensorMap a_gather;  // weight: single x rows of 64 k
-  CUtensorMap b_map;     // rows of x or dy, boxes 64 wide x 64 rows
-  CUtensorMap b_small;   // 64 wide x 8 rows
+  CUtensorMap b_map;     // weight: dy boxes 64 n x 64 rows
+  CUtensorMap b_small;   // weight: 64 n x 8 rows
   CUtensorMap b_gather;  // forward: single x rows; weight: single dy rows
+  CUtensorMap b_rows[8]; // forward / input: rows of x or dy, 64 wide x 16, 32, .. 128 rows
 };
 
 template <int kCtas, int kNT>
@@ -205,7 +206,8 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(const __grid_const
           row4[i] = src >= 0 && src < p.x_rows ? src : p.x_rows;
         }
       }
-      const uint32_t whole = kCtas * (kABytes + uint32_t(share) * 128u);
+      const bool boxed = kMode != kWeight && !(kMode == kForward && kCtas == 1 && p.rows);
+      const uint32_t whole = kCtas * (kABytes + uint32_t(boxed ? round_up(share, 16) : share) * 128u);
       bool ok = true;
       for (int ks = ks0; ks < ks1; ++ks, ++it) {
         const int st = it % kStages;
@@ -250,14 +252,9 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(const __grid_const
           if (kMode == kForward && kCtas == 1 && p.rows) {
             if (4 * lane < share) gather4<kCtas>(b + lane * 512, &p.b_gather, c, row4, bar);
           } else {
-            const int big = share / 64;  // boxes of 64 rows, then of 8
-            const int i = lane - 2;
-            if (i >= 0 && i < big) {
-              load_2d<kCtas>(b + i * 8192, &p.b_map, c, n_cta + 64 * i, bar);
-            } else if (i >= big && i - big < (share - big * 64) / 8) {
-              const int r = big * 64 + (i - big) * 8;
-              load_2d<kCtas>(b + r * 128, &p.b_small, c, n_cta + r, bar);
-            }
+            // One box of the share's rows in steps of 16: small boxes cost the copy engine near
+            // 0.1 us each, whatever their size (rows past the share are loaded and not used).
+            if (lane == 2) load_2d<kCtas>(b, &p.b_rows[ceil_div(share, 16) - 1], c, n_cta, bar);
           }
         }
       }
@@ -442,6 +439,13 @@ bool encode_rows(CUtensorMap* map, CUtensorMapDataType type, const void* p, int6
   return encode_map(map, type, 2, p, dims, strides, box);
 }
 
+bool encode_row_boxes(CUtensorMap (&maps)[8], CUtensorMapDataType type, const void* p, int64_t width, int64_t rows,
+                      int64_t stride) {
+  bool ok = true;
+  for (int i = 0; i < 8 && ok; ++i) ok = encode_rows(&maps[i], type, p, width, rows, stride, 16 * (i + 1));
+  return ok;
+}
+
 bool encode_weights(CUtensorMap* map, CUtensorMapDataType type, const void* w, int64_t K, int64_t N, int64_t E,
                     int64_t row_stride, int64_t expert_stride, int box_rows) {
   const cuuint64_t dims[3] = {cuuint64_t(K), cuuint64_t(N), cuuint64_t(E)};
@@ -520,8 +524,7 @@ extern "C" int lf_expert_linear(int32_t dtype, const void* x, int64_t x_stride, 
   p.M = int(out_width), p.C = int(width), p.elem_bf16 = dtype == LF_BF16;
   const CUtensorMapDataType type = map_type(dtype);
   if (!encode_weights(&p.a_map, type, w, width, out_width, num_experts, w_row_stride, w_expert_stride, 128) ||
-      !encode_rows(&p.b_map, type, x, width, x_rows, x_stride, 64) ||
-      !encode_rows(&p.b_small, type, x, width, x_rows, x_stride, 8) ||
+      !encode_row_boxes(p.b_rows, type, x, width, x_rows, x_stride) ||
       !encode_rows(&p.b_gather, type, x, width, x_rows, x_stride, 1))
     return fail(LF_E_CUDA, "expert_linear: cuTensorMapEncodeTiled failed");
   return launch_rows<kForward>(p, stream, what);
@@ -543,8 +546,7 @@ extern "C" int lf_expert_linear_input_grad(int32_t dtype, const void* dy, int64_
   p.M = int(width), p.C = int(out_width), p.elem_bf16 = dtype == LF_BF16;
   const CUtensorMapDataType type = map_type(dtype);
   if (!encode_weights(&p.a_map, type, w, width, out_width, num_experts, w_row_stride, w_expert_stride, 64) ||
-      !encode_rows(&p.b_map, type, dy, out_width, num_rows, dy_stride, 64) ||
-      !encode_rows(&p.b_small, type, dy, out_width, num_rows, dy_stride, 8))
+      !encode_row_boxes(p.b_rows, type, dy, out_width, num_rows, dy_stride))
     return fail(LF_E_CUDA, "expert_linear_input_grad: cuTensorMapEncodeTiled failed");
   return launch_rows<kInput>(p, stream, what);
 }

@@ -48,8 +48,7 @@ struct MxParams {
   int groups;            // wide: groups of 128 codes in the packed scales, an even number
   int split;
   CUtensorMap w_map;      // 128 bytes x 128 rows
-  CUtensorMap x_map;      // 128 bytes x 16 rows
-  CUtensorMap x_small;    // 128 bytes x 8 rows
+  CUtensorMap x_map[7];   // 128 bytes x 16, 32, .. 112 rows
   CUtensorMap x_gather;   // single rows
   CUtensorMap w_blocks;   // wide: packed scales, 512 bytes x 2 blocks
   CUtensorMap x_blocks;   // 512 bytes x 4 blocks
@@ -242,7 +241,7 @@ __global__ void __launch_bounds__(Shape<kCtas, kNT>::kThreads, 1) mx_kernel(cons
           row4[i] = src >= 0 && src < p.x_rows ? src : p.x_rows;
         }
       }
-      const uint32_t bytes = kCtas * (kABytes + uint32_t(share) * 128u + (kCtas == 2 ? uint32_t(S::kScaleBytes) : 0u));
+      const uint32_t bytes = kCtas * (kABytes + uint32_t(by_row ? share : round_up(share, 16)) * 128u + (kCtas == 2 ? uint32_t(S::kScaleBytes) : 0u));
       bool ok = true;
       for (int ks = ks0; ks < ks1; ++ks, ++it) {
         const int st = it % kStages;
@@ -263,9 +262,9 @@ __global__ void __launch_bounds__(Shape<kCtas, kNT>::kThreads, 1) mx_kernel(cons
         if (by_row) {
           if (4 * lane < share) gather4<kCtas>(b + lane * 512, &p.x_gather, c, row4, bar);
         } else {
-          const int big = share / 16, i = lane - 1;
-          if (i >= 0 && i < big) load_2d<kCtas>(b + i * 2048, &p.x_map, c, n_cta + 16 * i, bar);
-          else if (i == big && share % 16) load_2d<kCtas>(b + big * 2048, &p.x_small, c, n_cta + 16 * big, bar);
+          // One box of the share's rows in steps of 16: small boxes cost the copy engine near
+          // 0.1 us each, whatever their size (rows past the share are loaded and not used).
+          if (lane == 1) load_2d<kCtas>(b, &p.x_map[ceil_div(share, 16) - 1], c, n_cta, bar);
         }
       }
       if (!ok) break;
@@ -641,10 +640,11 @@ extern "C" int lf_expert_linear_mxfp4(int32_t out_dtype, const uint8_t* x_codes,
   const cuuint64_t strides[2] = {cuuint64_t(width / 2), cuuint64_t(width / 2) * cuuint64_t(out_width)};
   const cuuint32_t box[3] = {128, 128, 1};
   if (!encode_map(&p.w_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, w_codes, dims, strides, box) ||
-      !encode_codes(&p.x_map, x_codes, width / 2, code_rows, 16) ||
-      !encode_codes(&p.x_small, x_codes, width / 2, code_rows, 8) ||
       !encode_codes(&p.x_gather, x_codes, width / 2, code_rows, 1))
     return fail(LF_E_CUDA, "expert_linear_mxfp4: cuTensorMapEncodeTiled failed");
+  for (int i = 0; i < 7; ++i)
+    if (!encode_codes(&p.x_map[i], x_codes, width / 2, code_rows, 16 * (i + 1)))
+      return fail(LF_E_CUDA, "expert_linear_mxfp4: cuTensorMapEncodeTiled failed");
   const int64_t groups = num_experts < num_rows ? num_experts : num_rows;
   if (few) {
     const int64_t mt = ceil_div(p.N, 128);
