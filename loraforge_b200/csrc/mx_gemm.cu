@@ -8,22 +8,22 @@
 // in FP32; a product of two codes and two powers of two is exact.
 //
 // The tiles are those of the 16-bit products (grouped_gemm.cu): features on the TMEM lanes,
-// rows on the columns, CTA pairs with 256 features x up to 224 rows, or single CTAs with 128 x
-// 64 whose contraction may be split over a cluster.  224, not 256, rows: two accumulators of 224
-// columns leave 64 TMEM columns for the scales.
+// rows on the columns, CTA pairs with 256 features x up to 208 rows, or single CTAs with 128 x
+// 64 whose contraction may be split over a cluster.  208, not 256, rows: two accumulators of 208
+// columns leave 96 TMEM columns for four sets of scales.
 //
 // Scales.  The tensor core wants them in TMEM: for 128 operand rows and 128 codes a row, four
 // columns in which lane l of column j holds the four bytes of row 32 j + l, the same in every
-// quarter of the lanes.  tcgen05.cp writes them there from blocks of 512 bytes in shared memory;
-// the MMA thread issues the copies before the stage's MMAs, to two sets of columns in turn, and a
-// set is written again when the MMAs that read it are done.  The blocks of a stage come
-//   wide    by TMA, from blocks that pack_kernel laid out in the workspace before (scales of
-//           28672 x 4096 weights: 3.7 MB each way).  Warps that read the scales and tell the
-//           pair's first CTA stage by stage cost 0.7 us a stage, against 0.25 for its MMAs;
-//   narrow  from four warps that read them row by row: 32 bytes of a row (a whole sector) for a
-//           thread and four stages, one such group ahead, also across tiles.
+// quarter of the lanes.  Four warps, one a quarter, bring them there from blocks of 512 bytes in
+// shared memory, to four sets of columns in turn (a stage each), and tell the MMA thread.
+// tcgen05.cp would do that without them, but each copy of a block holds up the MMAs for some 33 ns,
+// six of them near 0.2 us a wide stage whose MMAs take 0.22.  The blocks of a stage come
+//   wide    by bulk copies, from blocks that pack_kernel laid out in the workspace before (scales
+//           of 28672 x 4096 weights: 3.7 MB each way);
+//   narrow  from the same four warps, which read them row by row: 32 bytes of a row (a whole
+//           sector) for a thread and four stages, one such group ahead, also across tiles.
 //
-// Per CTA: warp 0 loads (TMA), warp 1 MMA and TMEM, warps 2-5 store, narrow: warps 6-9 scales.
+// Per CTA: warp 0 loads (TMA), warp 1 MMA and TMEM, warps 2-5 store, warps 6-9 scales.
 // Every wait is bounded (tma.cuh): an expiry stops every role at its next wait.
 #include "experts.cuh"
 #include "grouped.cuh"
@@ -33,8 +33,10 @@ namespace {
 
 using namespace grouped;
 
+constexpr int kThreads = 320;
 constexpr int kStep = 256;           // codes per stage: 128 bytes a row
 constexpr int kABytes = 128 * 128;
+constexpr int kSets = 4;             // sets of TMEM columns that the stages' scales go to in turn
 constexpr int kSuper = 4;            // stages whose scales a thread loads at once (32 bytes a row)
 
 struct MxParams {
@@ -45,27 +47,26 @@ struct MxParams {
   const uint8_t* w_scales;  // [E][N][blocks]
   int E, R, x_rows, N, K, blocks;
   int x_align, w_align;  // 16, 8 or 1: alignment of every row of the scales
-  int groups;            // wide: groups of 128 codes in the packed scales, an even number
+  const uint8_t* w_blocks;  // wide: packed scales
+  const uint8_t* x_blocks;
+  int groups;            // of 128 codes in them, an even number
   int split;
   CUtensorMap w_map;      // 128 bytes x 128 rows
   CUtensorMap x_map[7];   // 128 bytes x 16, 32, .. 112 rows
   CUtensorMap x_gather;   // single rows
-  CUtensorMap w_blocks;   // wide: packed scales, 512 bytes x 2 blocks
-  CUtensorMap x_blocks;   // 512 bytes x 4 blocks
 };
 
 template <int kCtas, int kNT>
 struct Shape {
-  static constexpr int kBRows = kNT / kCtas;
+  static constexpr int kBRows = round_up(kNT / kCtas, 16);  // a CTA's share of the rows, loaded by 16
   static constexpr int kHalves = (kNT + 127) / 128;              // scale blocks of 128 rows of x
   static constexpr int kScaleBytes = 2 * 512 * (1 + kHalves);    // two groups of 128 codes a stage
   static constexpr int kStageBytes = (kABytes + kBRows * 128 + kScaleBytes + 1023) / 1024 * 1024;
   static constexpr int kPartBytes = kCtas == 1 ? kNT * 128 * 4 : 4 * kChunkBytes;
   static constexpr int kStages = kCtas == 2 ? 6 : 7;
-  static constexpr int kThreads = kCtas == 2 ? 192 : 320;
   static constexpr int kScaleColumns = 2 * (4 + 4 * kHalves);    // a set
   static constexpr int kColumns = kCtas == 2 ? 512 : 256;        // TMEM
-  static_assert(2 * kNT + 2 * kScaleColumns <= kColumns, "TMEM");
+  static_assert(2 * kNT + kSets * kScaleColumns <= kColumns, "TMEM");
 };
 
 __device__ __forceinline__ uint32_t instruction(int m, int n, int scale_id) {
@@ -91,26 +92,23 @@ __device__ __forceinline__ void mma_mxf4(uint32_t d, uint64_t a, uint64_t b, uin
   }
 }
 
-// 512 bytes (32 rows of 16) to four TMEM columns, repeated in the four quarters of the lanes;
-// in a pair, each CTA from its own shared memory to its own TMEM.
-template <int kCtas>
-__device__ __forceinline__ void copy_scales(uint32_t taddr, uint32_t saddr) {
-  // No swizzle, groups of 8 rows 128 bytes apart.
-  const uint64_t desc = uint64_t((saddr & 0x3FFFFu) >> 4) | (uint64_t(1) << 16) | (uint64_t(128 >> 4) << 32) | (uint64_t(1) << 46);
-  if constexpr (kCtas == 1)
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
-  else
-    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
-}
-
-// Arrive on this CTA's `bar` alone.
-template <int kCtas>
-__device__ __forceinline__ void commit_here(uint64_t* bar) {
-  if constexpr (kCtas == 1)
-    tc_commit(bar);
-  else
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+// Columns taddr .. taddr + 4 n - 1 of this warp's lane quarter from n blocks of 512 bytes, lane l's
+// 16 bytes at l * 16.
+template <int n>
+__device__ __forceinline__ void store_scales(uint32_t taddr, uint32_t blocks, int lane) {
+  static_assert(n == 4 || n == 6, "two groups of one block of W and one or two of x");
+#pragma unroll
+  for (int i = 0; i < n; i += 2) {
+    const uint4 a = lds16(blocks + i * 512 + lane * 16), b = lds16(blocks + i * 512 + 512 + lane * 16);
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr + 4 * i),
+                 "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w)
                  : "memory");
+  }
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+// Arrive on a barrier of the cluster after tcgen05 operations (which the fence before it orders).
+__device__ __forceinline__ void arrive_cluster_relaxed(uint32_t bar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 struct Tile {
@@ -159,7 +157,7 @@ __device__ __forceinline__ void load_scales(const uint8_t* row, int k0, int bloc
 }
 
 template <int kCtas, int kNT>
-__global__ void __launch_bounds__(Shape<kCtas, kNT>::kThreads, 1) mx_kernel(const __grid_constant__ MxParams p) {
+__global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__ MxParams p) {
   using S = Shape<kCtas, kNT>;
   constexpr int kStages = S::kStages;
   extern __shared__ uint8_t smem_raw[];
@@ -171,8 +169,9 @@ __global__ void __launch_bounds__(Shape<kCtas, kNT>::kThreads, 1) mx_kernel(cons
   uint64_t* empty = full + kStages;
   uint64_t* acc_full = empty + kStages;
   uint64_t* acc_empty = acc_full + 2;
-  uint64_t* set_done = acc_empty + 2;
-  uint64_t* part_full = set_done + 2;
+  uint64_t* blocks_full = acc_empty + 2;      // a stage's scale blocks are here
+  uint64_t* set_full = blocks_full + kStages;  // a set of scale columns is written, in both CTAs
+  uint64_t* part_full = set_full + kSets;
   uint64_t* part_empty = part_full + 1;
   uint64_t* fin = part_empty + 1;
   uint32_t* tslot = reinterpret_cast<uint32_t*>(fin + 1);
@@ -186,14 +185,15 @@ __global__ void __launch_bounds__(Shape<kCtas, kNT>::kThreads, 1) mx_kernel(cons
   const bool leader = rank * (kCtas - 1) == 0;
   if (tid == 0) {
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(&full[i], kCtas == 2 ? 1 : 1 + 4);  // the loads' bytes, narrow: and the scale warps
+      mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
+      mbar_init(&blocks_full[i], kCtas == 2 ? 1 : 4);  // the copies' bytes, or the four warps that write them
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&acc_full[i], 1);
       mbar_init(&acc_empty[i], 4 * kCtas);
-      mbar_init(&set_done[i], 1);
     }
+    for (int i = 0; i < kSets; ++i) mbar_init(&set_full[i], 4 * kCtas);
     mbar_init(part_full, 4 * cluster);
     mbar_init(part_empty, 4 * cluster);
     mbar_init(fin, 1);
@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(Shape<kCtas, kNT>::kThreads, 1) mx_kernel(cons
           row4[i] = src >= 0 && src < p.x_rows ? src : p.x_rows;
         }
       }
-      const uint32_t bytes = kCtas * (kABytes + uint32_t(by_row ? share : round_up(share, 16)) * 128u + (kCtas == 2 ? uint32_t(S::kScaleBytes) : 0u));
+      const uint32_t bytes = kCtas * (kABytes + uint32_t(by_row ? share : round_up(share, 16)) * 128u);
       bool ok = true;
       for (int ks = ks0; ks < ks1; ++ks, ++it) {
         const int st = it % kStages;
@@ -253,11 +253,12 @@ __global__ void __launch_bounds__(Shape<kCtas, kNT>::kThreads, 1) mx_kernel(cons
         __syncwarp();
         const int c = ks * 128;  // bytes along K
         if (lane == 0) load_3d<kCtas>(a, &p.w_map, c, m_cta, x.e, bar);
-        if (kCtas == 2 && lane >= 30) {
-          const uint32_t sc = b + S::kBRows * 128;
-          const int wb = (x.e * ceil_div(p.N, 256) * 2 + m_cta / 128) * p.groups + 2 * ks;
-          if (lane == 30) load_2d<kCtas>(sc, &p.w_blocks, 0, wb, bar);
-          else load_2d<kCtas>(sc + 1024, &p.x_blocks, 0, (x.row_tile * p.groups + 2 * ks) * 2, bar);
+        if (kCtas == 2 && lane == 31) {
+          uint8_t* sc = ring + st * S::kStageBytes + kABytes + S::kBRows * 128;
+          const int64_t wb = int64_t(x.e * ceil_div(p.N, 256) * 2 + m_cta / 128) * p.groups + 2 * ks;
+          mbar_arrive_expect_tx(&blocks_full[st], S::kScaleBytes);
+          bulk_g2s(sc, p.w_blocks + wb * 512, 1024, &blocks_full[st]);
+          bulk_g2s(sc + 1024, p.x_blocks + (int64_t(x.row_tile) * p.groups + 2 * ks) * 1024, 2048, &blocks_full[st]);
         }
         if (by_row) {
           if (4 * lane < share) gather4<kCtas>(b + lane * 512, &p.x_gather, c, row4, bar);
@@ -273,8 +274,11 @@ __global__ void __launch_bounds__(Shape<kCtas, kNT>::kThreads, 1) mx_kernel(cons
     if (kCtas == 2)
       for (int j = max(0, it - kStages); j < it; ++j) wait_or_abort(&empty[j % kStages], uint32_t(j / kStages) & 1u, abort);
     // No load may still be landing when the CTA exits: after an expired wait, give them time.
-    if (*abort && lane == 0 && leader)
-      for (int j = max(0, it - kStages); j < it; ++j) mbar_wait(&full[j % kStages], uint32_t(j / kStages) & 1u);
+    if (*abort && lane == 0)
+      for (int j = max(0, it - kStages); j < it; ++j) {
+        if (leader) mbar_wait(&full[j % kStages], uint32_t(j / kStages) & 1u);
+        if (kCtas == 2) mbar_wait(&blocks_full[j % kStages], uint32_t(j / kStages) & 1u);
+      }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA thread
     if (lane == 0 && leader) {
@@ -284,36 +288,29 @@ __global__ void __launch_bounds__(Shape<kCtas, kNT>::kThreads, 1) mx_kernel(cons
         const int ab = count & 1;
         if (!wait_cluster(&acc_empty[ab], (uint32_t(count >> 1) & 1u) ^ 1u, abort)) break;
         ++count;
-        tc_fence_after();
         const uint32_t d = tmem + uint32_t(ab * kNT);
         const uint32_t idesc0 = instruction(128 * kCtas, x.nt, 0), idesc1 = instruction(128 * kCtas, x.nt, 2);
         bool ok = true;
         for (int ks = ks0; ks < ks1; ++ks, ++it) {
-          const int st = it % kStages, set = it & 1;
+          const int st = it % kStages, set = it % kSets;
           ok = wait_or_abort(&full[st], uint32_t(it / kStages) & 1u, abort) &&
-               wait_or_abort(&set_done[set], (uint32_t(it >> 1) & 1u) ^ 1u, abort);
+               wait_cluster(&set_full[set], uint32_t(it / kSets) & 1u, abort);
           if (!ok) break;
           tc_fence_after();
           const uint32_t sa = smem_u32(ring + st * S::kStageBytes);
-          const uint32_t sc = sa + kABytes + S::kBRows * 128;
           const uint32_t ts = tmem + uint32_t(2 * kNT + set * S::kScaleColumns);  // W: 2 x 4 columns, then x
-#pragma unroll
-          for (int i = 0; i < 2 * (1 + S::kHalves); ++i) copy_scales<kCtas>(ts + 4 * i, sc + 512 * i);
           const uint64_t ad = sw128_desc(sa), bd = sw128_desc(sa + kABytes);
 #pragma unroll
           for (int k = 0; k < kStep / 64; ++k)
             mma_mxf4<kCtas>(d, ad + 2 * k, bd + 2 * k, k & 1 ? idesc1 : idesc0, ts + 4 * (k >> 1),
                             ts + 8 + 4 * S::kHalves * (k >> 1), (ks > ks0 || k > 0) ? 1u : 0u);
           commit<kCtas>(&empty[st]);
-          commit_here<kCtas>(&set_done[set]);
         }
         if (!ok) break;
         commit<kCtas>(&acc_full[ab]);
       }
-      // Every arrival on this CTA's barriers has landed, and after an expired wait every MMA has retired.
-      for (int j = max(0, it - 2); j < it; ++j) wait_or_abort(&set_done[j & 1], uint32_t(j >> 1) & 1u, abort);
-      if (*abort) {
-        commit_here<kCtas>(fin);
+      if (*abort) {  // every MMA has retired before the TMEM columns are released
+        commit<kCtas>(fin);
         mbar_wait(fin, 0);
       }
     }
@@ -349,64 +346,86 @@ __global__ void __launch_bounds__(Shape<kCtas, kNT>::kThreads, 1) mx_kernel(cons
         release();
       }
     }
-  } else if constexpr (kCtas == 1) {
+  } else {
     // ------------------------------------------------------------ scales
-    constexpr int kRows = 2;  // rows a thread reads: one of W and one of the tile's
-    const int i = tid - 192;
-    const uint8_t* row[kRows] = {nullptr, nullptr};
-    auto rows_of = [&](int t) {
-      const Tile x = tile_of<kCtas, kNT>(p, bounds, starts, t);
-      const int n = x.m0 + i, r = x.n0 + i;
-      row[0] = n < p.N ? p.w_scales + (int64_t(x.e) * p.N + n) * p.blocks : nullptr;
-      const int src = i < x.valid ? (p.rows ? p.rows[r] : r) : -1;
-      row[1] = src >= 0 && src < p.x_rows ? p.x_scales + int64_t(src) * p.blocks : nullptr;
-    };
-    uint32_t next[kRows][8];
-    auto load = [&](int k0) {
-#pragma unroll
-      for (int q = 0; q < kRows; ++q) load_scales(row[q], k0 * 8, p.blocks, q ? p.x_align : p.w_align, next[q]);
-    };
-    int it = 0, t = first, k0 = ks0;
-    bool ok = live && t < tiles;
-    if (ok) {
-      rows_of(t);
-      load(k0);
-    }
-    while (ok) {
-      uint32_t now[kRows][8];
-#pragma unroll
-      for (int q = 0; q < kRows; ++q) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) now[q][j] = next[q][j];
+    const uint32_t quarter_set = tmem + (uint32_t((warp & 3) * 32) << 16) + uint32_t(2 * kNT);
+    // Stage `it`'s blocks to its set of columns, once the MMAs of kSets stages ago are done with it.
+    auto to_tmem = [&](int it) {
+      const int before = it - kSets;
+      bool ready = wait_or_abort(&blocks_full[it % kStages], uint32_t(it / kStages) & 1u, abort);
+      if (before >= 0) ready = ready && wait_or_abort(&empty[before % kStages], uint32_t(before / kStages) & 1u, abort);
+      if (!__all_sync(0xffffffffu, ready)) return false;
+      tc_fence_after();
+      store_scales<2 * (1 + S::kHalves)>(quarter_set + uint32_t(it % kSets * S::kScaleColumns),
+                                         smem_u32(ring + it % kStages * S::kStageBytes) + kABytes + S::kBRows * 128, lane);
+      tc_fence_before();
+      if (lane == 0) {
+        if (kCtas == 2) arrive_cluster_relaxed(mapa(&set_full[it % kSets], 0));
+        else mbar_arrive(&set_full[it % kSets]);
       }
-      const int todo = min(kSuper, ks1 - k0);
-      k0 += kSuper;
-      if (k0 >= ks1) {
-        k0 = ks0;
-        t += stride;
-        if (t < tiles) rows_of(t);
-      }
-      if (t < tiles) load(k0);
+      return true;
+    };
+    if constexpr (kCtas == 2) {
+      const int mine = live && first < tiles ? (tiles - first + stride - 1) / stride : 0;
+      for (int it = 0; it < mine * (ks1 - ks0); ++it)
+        if (!to_tmem(it)) break;
+    } else {
+      constexpr int kRows = 2;  // rows a thread reads: one of W and one of the tile's
+      const int i = tid - 192;
+      const uint8_t* row[kRows] = {nullptr, nullptr};
+      auto rows_of = [&](int t) {
+        const Tile x = tile_of<kCtas, kNT>(p, bounds, starts, t);
+        const int n = x.m0 + i, r = x.n0 + i;
+        row[0] = n < p.N ? p.w_scales + (int64_t(x.e) * p.N + n) * p.blocks : nullptr;
+        const int src = i < x.valid ? (p.rows ? p.rows[r] : r) : -1;
+        row[1] = src >= 0 && src < p.x_rows ? p.x_scales + int64_t(src) * p.blocks : nullptr;
+      };
+      uint32_t next[kRows][8];
+      auto load = [&](int k0) {
 #pragma unroll
-      for (int j = 0; j < kSuper; ++j) {
-        if (j >= todo || !ok) continue;
-        const int st = it % kStages;
-        ok = __all_sync(0xffffffffu, wait_or_abort(&empty[st], (uint32_t(it / kStages) & 1u) ^ 1u, abort));
-        ++it;
-        if (!ok) continue;
-        const uint32_t sc = smem_u32(ring + st * S::kStageBytes) + kABytes + S::kBRows * 128 +
-                            uint32_t((i & 31) * 16 + (i >> 5) * 4);
+        for (int q = 0; q < kRows; ++q) load_scales(row[q], k0 * 8, p.blocks, q ? p.x_align : p.w_align, next[q]);
+      };
+      int it = 0, t = first, k0 = ks0;
+      bool ok = live && t < tiles;
+      if (ok) {
+        rows_of(t);
+        load(k0);
+      }
+      while (ok) {
+        uint32_t now[kRows][8];
 #pragma unroll
         for (int q = 0; q < kRows; ++q) {
 #pragma unroll
-          for (int g = 0; g < 2; ++g)
-            asm volatile("st.shared.b32 [%0], %1;" ::"r"(sc + uint32_t(2 * q + g) * 512u), "r"(now[q][2 * j + g]) : "memory");
+          for (int j = 0; j < 8; ++j) now[q][j] = next[q][j];
         }
-        fence_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&full[st]);
+        const int todo = min(kSuper, ks1 - k0);
+        k0 += kSuper;
+        if (k0 >= ks1) {
+          k0 = ks0;
+          t += stride;
+          if (t < tiles) rows_of(t);
+        }
+        if (t < tiles) load(k0);
+#pragma unroll
+        for (int j = 0; j < kSuper; ++j) {
+          if (j >= todo || !ok) continue;
+          const int st = it % kStages;
+          ok = __all_sync(0xffffffffu, wait_or_abort(&empty[st], (uint32_t(it / kStages) & 1u) ^ 1u, abort));
+          const uint32_t sc = smem_u32(ring + st * S::kStageBytes) + kABytes + S::kBRows * 128 +
+                              uint32_t((i & 31) * 16 + (i >> 5) * 4);
+#pragma unroll
+          for (int q = 0; q < kRows; ++q) {
+#pragma unroll
+            for (int g = 0; g < 2; ++g)
+              asm volatile("st.shared.b32 [%0], %1;" ::"r"(sc + uint32_t(2 * q + g) * 512u), "r"(now[q][2 * j + g]) : "memory");
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&blocks_full[st]);
+          ok = ok && to_tmem(it);
+          ++it;
+        }
+        ok = ok && t < tiles;
       }
-      ok = ok && t < tiles;
     }
   }
   tc_fence_before();
@@ -418,7 +437,7 @@ __global__ void __launch_bounds__(Shape<kCtas, kNT>::kThreads, 1) mx_kernel(cons
   }
 }
 
-constexpr int kWideRows = 224, kNarrowRows = 64;
+constexpr int kWideRows = 208, kNarrowRows = 64;
 
 bool narrow(int64_t E, int64_t R) { return R <= kNarrowRows * (E < R ? E : R); }
 
@@ -523,7 +542,7 @@ int launch_mx(const MxParams& p, int64_t tiles, void* stream) {
                    int(sizeof(int)) * (kMaxWarps + 2 + 2 * (p.E + 1));
   static int flags[64] = {};
   if (int rc = ensure_smem(mx_kernel<kCtas, kNT>, smem, flags)) return rc;
-  return launch_clusters(mx_kernel<kCtas, kNT>, int(grid), S::kThreads, cluster, smem, stream, "expert_linear_mxfp4", p);
+  return launch_clusters(mx_kernel<kCtas, kNT>, int(grid), kThreads, cluster, smem, stream, "expert_linear_mxfp4", p);
 }
 
 bool encode_codes(CUtensorMap* map, const void* p, int64_t bytes, int64_t rows, int box_rows) {
@@ -531,17 +550,6 @@ bool encode_codes(CUtensorMap* map, const void* p, int64_t bytes, int64_t rows, 
   const cuuint64_t strides[1] = {cuuint64_t(bytes)};
   const cuuint32_t box[2] = {128, cuuint32_t(box_rows)};
   return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, p, dims, strides, box);
-}
-
-// 512-byte scale blocks, `box_blocks` at a time.
-bool encode_blocks(CUtensorMap* map, const void* p, int64_t blocks, int box_blocks) {
-  const PFN_cuTensorMapEncodeTiled_v12000 encode = map_encoder();
-  const cuuint64_t dims[2] = {128, cuuint64_t(blocks)};
-  const cuuint64_t strides[1] = {512};
-  const cuuint32_t box[2] = {128, cuuint32_t(box_blocks)}, ones[2] = {1, 1};
-  return encode && encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void*>(p), dims, strides, box, ones,
-                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 // Sizes of the wide tiles' workspace: 512-byte blocks of W's and of x's scales, then codes.
@@ -633,8 +641,7 @@ extern "C" int lf_expert_linear_mxfp4(int32_t out_dtype, const uint8_t* x_codes,
       return rc;
     if (rows) x_codes = reinterpret_cast<const uint8_t*>(k.codes), code_rows = num_rows;
     p.groups = w.groups;
-    if (!encode_blocks(&p.w_blocks, k.w_blocks, w.w_blocks, 2) || !encode_blocks(&p.x_blocks, k.x_blocks, w.x_blocks, 4))
-      return fail(LF_E_CUDA, "expert_linear_mxfp4: cuTensorMapEncodeTiled failed");
+    p.w_blocks = k.w_blocks, p.x_blocks = k.x_blocks;
   }
   const cuuint64_t dims[3] = {cuuint64_t(width / 2), cuuint64_t(out_width), cuuint64_t(num_experts)};
   const cuuint64_t strides[2] = {cuuint64_t(width / 2), cuuint64_t(width / 2) * cuuint64_t(out_width)};
