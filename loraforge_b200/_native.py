@@ -171,6 +171,26 @@ def call(name: str, *args) -> None:
         raise RuntimeError(message or f"{name} failed with status {status}")
 
 
+def launch(name: str, index: int, *args) -> None:
+    """``call`` on CUDA device ``index`` with PyTorch's current stream there as the last argument.
+
+    For the operators whose smallest calls are bound by the host: it looks the stream up without
+    making a Stream object, and changes the current device only where it is another one.
+    """
+    import torch
+
+    status_of = getattr(_lib or library(), name)
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch._C._cuda_getDevice() == index:
+        status = status_of(*args, stream)
+    else:
+        with torch.cuda.device(index):
+            status = status_of(*args, stream)
+    if status != 0:
+        message = library().lf_last_error_string().decode(errors="replace")
+        raise RuntimeError(message or f"{name} failed with status {status}")
+
+
 def fused_workspace_floats(num_tokens: int, width: int, num_slices: int, capacity: int) -> int:
     """FP32 workspace size of lf_fused_shrink_expand for these sizes."""
     n = library().lf_fused_workspace_floats(num_tokens, width, num_slices, capacity)
@@ -197,7 +217,7 @@ def lora_base_gemm_workspace_floats(num_tokens: int, width: int, num_slices: int
 
 def route_experts_workspace_ints(num_tokens: int, num_experts: int) -> int:
     """int32 workspace size of lf_route_experts for these sizes."""
-    n = library().lf_route_experts_workspace_ints(num_tokens, num_experts)
+    n = (_lib or library()).lf_route_experts_workspace_ints(num_tokens, num_experts)
     if n < 0:
         raise ValueError("invalid sizes for the routing workspace")
     return n
@@ -205,7 +225,7 @@ def route_experts_workspace_ints(num_tokens: int, num_experts: int) -> int:
 
 def expert_linear_workspace_bytes(num_experts: int, num_rows: int, width: int, weight_grad: bool = False) -> int:
     """Workspace bytes of lf_expert_linear (or its weight gradient) with row indices."""
-    n = library().lf_expert_linear_workspace_bytes(num_experts, num_rows, width, 1 if weight_grad else 0)
+    n = (_lib or library()).lf_expert_linear_workspace_bytes(num_experts, num_rows, width, 1 if weight_grad else 0)
     if n < 0:
         raise ValueError("invalid sizes for the expert workspace")
     return n
@@ -214,7 +234,7 @@ def expert_linear_workspace_bytes(num_experts: int, num_rows: int, width: int, w
 def expert_linear_mxfp4_workspace_bytes(num_experts: int, num_rows: int, out_width: int, width: int,
                                         by_rows: bool) -> int:
     """Workspace bytes of lf_expert_linear_mxfp4 (by_rows: with row indices)."""
-    n = library().lf_expert_linear_mxfp4_workspace_bytes(num_experts, num_rows, out_width, width, 1 if by_rows else 0)
+    n = (_lib or library()).lf_expert_linear_mxfp4_workspace_bytes(num_experts, num_rows, out_width, width, 1 if by_rows else 0)
     if n < 0:
         raise ValueError("invalid sizes for the expert workspace")
     return n
@@ -242,8 +262,12 @@ def stream_of(device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-def dtype_code(dtype) -> int:
-    import torch
+_codes: dict = {}
 
-    codes = {torch.float32: LF_F32, torch.float16: LF_F16, torch.bfloat16: LF_BF16}
-    return codes[dtype]
+
+def dtype_code(dtype) -> int:
+    if not _codes:
+        import torch
+
+        _codes.update({torch.float32: LF_F32, torch.float16: LF_F16, torch.bfloat16: LF_BF16})
+    return _codes[dtype]

@@ -66,6 +66,8 @@ __device__ __forceinline__ void load_logits(const void* logits, int64_t row, int
 
 // Stable sort of this block's slots by expert: base[e] (block b's first row of expert e) from
 // the blocks' counts, then ranks inside the block from per-warp counts.
+// kOwn: `counts` are this block's alone, in the same shared memory as the tables.
+template <bool kOwn>
 __device__ void scatter_slots(const int32_t* experts, const int32_t* counts, int blocks, int block, int64_t slot0,
                               int slots, int64_t all_slots, int E, int k, int32_t* offsets, int32_t* rows,
                               int32_t* positions, int* smem) {
@@ -81,7 +83,7 @@ __device__ void scatter_slots(const int32_t* experts, const int32_t* counts, int
     if (e < E) {
 #pragma unroll 8
       for (int b = 0; b < blocks; ++b) {
-        const int c = __ldcg(counts + int64_t(b) * E + e);
+        const int c = kOwn ? counts[e] : __ldcg(counts + int64_t(b) * E + e);
         total += c;
         before += b < block ? c : 0;
       }
@@ -203,12 +205,12 @@ __global__ void __launch_bounds__(kRouteThreads) route_topk_kernel(
     }
   }
   __syncthreads();
-  for (int e = tid; e < E; e += kRouteThreads) counts[int64_t(blockIdx.x) * E + e] = hist[e];
-  if (gridDim.x == 1) {
-    __syncthreads();
-    scatter_slots(experts, counts, 1, 0, 0, num_tokens * k, int64_t(num_tokens) * k, E, k, offsets, rows, positions,
-                  smem);
+  if (gridDim.x > 1) {
+    for (int e = tid; e < E; e += kRouteThreads) counts[int64_t(blockIdx.x) * E + e] = hist[e];
+    return;
   }
+  scatter_slots<true>(experts, hist, 1, 0, 0, num_tokens * k, int64_t(num_tokens) * k, E, k, offsets, rows, positions,
+                      smem);
 }
 
 __global__ void __launch_bounds__(kRouteThreads) route_scatter_kernel(const int32_t* experts, const int32_t* counts,
@@ -218,7 +220,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_scatter_kernel(const int3
   extern __shared__ int smem[];
   pdl_wait();
   const int t0 = blockIdx.x * block_tokens, t1 = min(num_tokens, t0 + block_tokens);
-  scatter_slots(experts, counts, gridDim.x, blockIdx.x, int64_t(t0) * k, (t1 - t0) * k, int64_t(num_tokens) * k, E, k,
+  scatter_slots<false>(experts, counts, gridDim.x, blockIdx.x, int64_t(t0) * k, (t1 - t0) * k, int64_t(num_tokens) * k, E, k,
                 offsets, rows, positions, smem);
 }
 
@@ -504,7 +506,8 @@ using namespace lfb;
 
 extern "C" int64_t lf_route_experts_workspace_ints(int64_t num_tokens, int32_t num_experts) {
   if (num_tokens < 0 || num_experts < 1 || num_experts > kMaxExperts) return -1;
-  return int64_t(num_tokens ? route_plan(num_tokens).blocks : 1) * num_experts;
+  const int blocks = route_plan(num_tokens).blocks;
+  return blocks > 1 ? int64_t(blocks) * num_experts : 0;
 }
 
 extern "C" int lf_route_experts(int32_t dtype, const void* logits, int64_t logits_stride, int64_t num_tokens,
@@ -524,7 +527,8 @@ extern "C" int lf_route_experts(int32_t dtype, const void* logits, int64_t logit
       return check_launch("route_experts");
     return LF_OK;
   }
-  if (!workspace || workspace_ints < lf_route_experts_workspace_ints(num_tokens, num_experts))
+  const int64_t need = lf_route_experts_workspace_ints(num_tokens, num_experts);
+  if (need && (!workspace || workspace_ints < need))
     return fail(LF_E_INVALID, "route_experts: workspace too small (see lf_route_experts_workspace_ints)");
   const RouteCall call{logits, logits_stride, int(num_tokens), num_experts, top_k,     renormalize ? 1 : 0, scale,
                        weights, experts,      offsets,         rows,        positions, workspace,           stream};

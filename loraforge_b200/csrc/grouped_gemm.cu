@@ -412,6 +412,9 @@ int launch_grouped(const GParams& p, int64_t tiles, void* stream, const char* wh
 constexpr int kWideRows = 256, kNarrowRows = 64;
 constexpr char kNoWorkspace[] = "expert_linear: workspace missing, too small or not 16-byte aligned (see lf_expert_linear_workspace_bytes)";
 
+// Groups of up to 64 rows on average take the narrow tiles.
+bool narrow(int64_t E, int64_t R) { return R <= kNarrowRows * (E < R ? E : R); }
+
 int check_sizes(const char* what, int dtype, int E, int64_t R, int64_t N, int64_t K) {
   const int64_t limit = int64_t(1) << 31;
   if (dtype != LF_BF16 && dtype != LF_F16)
@@ -440,9 +443,9 @@ bool encode_rows(CUtensorMap* map, CUtensorMapDataType type, const void* p, int6
 }
 
 bool encode_row_boxes(CUtensorMap (&maps)[8], CUtensorMapDataType type, const void* p, int64_t width, int64_t rows,
-                      int64_t stride) {
+                      int64_t stride, bool few) {
   bool ok = true;
-  for (int i = 0; i < 8 && ok; ++i) ok = encode_rows(&maps[i], type, p, width, rows, stride, 16 * (i + 1));
+  for (int i = 0; i < (few ? kNarrowRows / 16 : 8) && ok; ++i) ok = encode_rows(&maps[i], type, p, width, rows, stride, 16 * (i + 1));
   return ok;
 }
 
@@ -457,9 +460,6 @@ bool encode_weights(CUtensorMap* map, CUtensorMapDataType type, const void* w, i
 CUtensorMapDataType map_type(int dtype) {
   return dtype == LF_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
 }
-
-// Groups of up to 64 rows on average take the narrow tiles.
-bool narrow(int64_t E, int64_t R) { return R <= kNarrowRows * (E < R ? E : R); }
 
 template <int kMode>
 int launch_rows(GParams& p, void* stream, const char* what) {
@@ -524,8 +524,8 @@ extern "C" int lf_expert_linear(int32_t dtype, const void* x, int64_t x_stride, 
   p.M = int(out_width), p.C = int(width), p.elem_bf16 = dtype == LF_BF16;
   const CUtensorMapDataType type = map_type(dtype);
   if (!encode_weights(&p.a_map, type, w, width, out_width, num_experts, w_row_stride, w_expert_stride, 128) ||
-      !encode_row_boxes(p.b_rows, type, x, width, x_rows, x_stride) ||
-      !encode_rows(&p.b_gather, type, x, width, x_rows, x_stride, 1))
+      (rows ? !encode_rows(&p.b_gather, type, x, width, x_rows, x_stride, 1)
+            : !encode_row_boxes(p.b_rows, type, x, width, x_rows, x_stride, narrow(num_experts, num_rows))))
     return fail(LF_E_CUDA, "expert_linear: cuTensorMapEncodeTiled failed");
   return launch_rows<kForward>(p, stream, what);
 }
@@ -546,7 +546,7 @@ extern "C" int lf_expert_linear_input_grad(int32_t dtype, const void* dy, int64_
   p.M = int(width), p.C = int(out_width), p.elem_bf16 = dtype == LF_BF16;
   const CUtensorMapDataType type = map_type(dtype);
   if (!encode_weights(&p.a_map, type, w, width, out_width, num_experts, w_row_stride, w_expert_stride, 64) ||
-      !encode_row_boxes(p.b_rows, type, dy, out_width, num_rows, dy_stride))
+      !encode_row_boxes(p.b_rows, type, dy, out_width, num_rows, dy_stride, narrow(num_experts, num_rows)))
     return fail(LF_E_CUDA, "expert_linear_input_grad: cuTensorMapEncodeTiled failed");
   return launch_rows<kInput>(p, stream, what);
 }

@@ -646,12 +646,12 @@ extern "C" int lf_expert_linear_mxfp4(int32_t out_dtype, const uint8_t* x_codes,
   const cuuint64_t dims[3] = {cuuint64_t(width / 2), cuuint64_t(out_width), cuuint64_t(num_experts)};
   const cuuint64_t strides[2] = {cuuint64_t(width / 2), cuuint64_t(width / 2) * cuuint64_t(out_width)};
   const cuuint32_t box[3] = {128, 128, 1};
-  if (!encode_map(&p.w_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, w_codes, dims, strides, box) ||
-      !encode_codes(&p.x_gather, x_codes, width / 2, code_rows, 1))
-    return fail(LF_E_CUDA, "expert_linear_mxfp4: cuTensorMapEncodeTiled failed");
-  for (int i = 0; i < 7; ++i)
-    if (!encode_codes(&p.x_map[i], x_codes, width / 2, code_rows, 16 * (i + 1)))
-      return fail(LF_E_CUDA, "expert_linear_mxfp4: cuTensorMapEncodeTiled failed");
+  bool ok = encode_map(&p.w_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, w_codes, dims, strides, box);
+  if (rows && few) ok = ok && encode_codes(&p.x_gather, x_codes, width / 2, code_rows, 1);
+  else
+    for (int i = 0; i < (few ? kNarrowRows / 16 : 7) && ok; ++i)
+      ok = encode_codes(&p.x_map[i], x_codes, width / 2, code_rows, 16 * (i + 1));
+  if (!ok) return fail(LF_E_CUDA, "expert_linear_mxfp4: cuTensorMapEncodeTiled failed");
   const int64_t groups = num_experts < num_rows ? num_experts : num_rows;
   if (few) {
     const int64_t mt = ceil_div(p.N, 128);

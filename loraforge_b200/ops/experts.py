@@ -10,10 +10,11 @@ Each forward has an explicit gradient (``*_backward``).  The reference has no co
 
 from __future__ import annotations
 
+from functools import lru_cache
 from typing import NamedTuple
 
 from loraforge_b200 import _native
-from loraforge_b200.ops._contract import INT32_LIMIT, first_failure, output_is_distinct
+from loraforge_b200.ops._contract import INT32_LIMIT, output_is_distinct
 
 MAX_EXPERTS = 1024
 MAX_TOP_K = 32
@@ -29,43 +30,52 @@ class ExpertRouting(NamedTuple):
     positions: object  # int32 [T, k]: row of each slot or -1
 
 
-def cuda_tensor(value, name: str, ndim: int, dtypes, device=None) -> None:
-    """A CUDA tensor of rank `ndim` and one of `dtypes`, int32-indexable, on `device` if given."""
+@lru_cache(maxsize=1)
+def _kinds():
+    """(torch.Tensor, 16-bit types, floating types), looked up once."""
     import torch
 
-    if not isinstance(value, torch.Tensor):
+    halves = (torch.float16, torch.bfloat16)
+    return torch.Tensor, halves, (torch.float32, *halves)
+
+
+def cuda_tensor(value, name: str, ndim: int, dtypes, index: int | None = None) -> int:
+    """A CUDA tensor of rank `ndim` and one of `dtypes`, int32-indexable, on CUDA device `index`
+    if given; the index of its device."""
+    if not isinstance(value, _kinds()[0]):
         raise TypeError(f"{name} must be a torch.Tensor")
     if value.ndim != ndim or value.dtype not in dtypes:
         raise ValueError(f"{name} must be {ndim}D with dtype {' or '.join(str(d) for d in dtypes)}")
-    if max(value.shape, default=0) >= INT32_LIMIT:
+    if value.numel() >= INT32_LIMIT and max(value.shape) >= INT32_LIMIT:
         raise ValueError(f"{name} dimensions must fit signed int32 indexing")
-    if value.device.type != "cuda" or (device is not None and value.device != device):
+    found = value.get_device() if value.is_cuda else -1
+    if found < 0 or (index is not None and found != index):
         raise ValueError(f"{name} must be on the same CUDA GPU")
+    return found
 
 
-def row_matrix(value, name: str, dtypes, device=None) -> None:
+def row_matrix(value, name: str, dtypes, index: int | None = None) -> int:
     """A 2-D `cuda_tensor` of rows that do not overlap, with unit column stride."""
-    cuda_tensor(value, name, 2, dtypes, device)
-    if value.shape[0] > 1 and value.stride(0) < value.shape[1] or (value.shape[1] > 1 and value.stride(1) != 1):
-        raise ValueError(f"{name} must have unit column stride and rows that do not overlap")
+    index = cuda_tensor(value, name, 2, dtypes, index)
+    if not value.is_contiguous():
+        rows, width = value.shape
+        step, unit = value.stride()
+        if (rows > 1 and step < width) or (width > 1 and unit != 1):
+            raise ValueError(f"{name} must have unit column stride and rows that do not overlap")
+    return index
 
 
 def row_stride(t) -> int:
     """Row stride of a `row_matrix` (a one-row tensor's own stride says nothing)."""
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+    rows, width = t.shape
+    return t.stride(0) if rows > 1 else width
 
 
-def packed_table(value, name: str, shape, device, dtype) -> None:
+def packed_table(value, name: str, shape, index: int, dtype) -> None:
     """A contiguous table of exactly `shape`."""
-    cuda_tensor(value, name, len(shape), (dtype,), device)
-    if tuple(value.shape) != tuple(shape) or not value.is_contiguous():
+    cuda_tensor(value, name, len(shape), (dtype,), index)
+    if value.shape != shape or not value.is_contiguous():
         raise ValueError(f"{name} must be contiguous with shape {tuple(shape)}")
-
-
-def _floats():
-    import torch
-
-    return (torch.float32, torch.float16, torch.bfloat16)
 
 
 def _scale(value) -> float:
@@ -88,39 +98,35 @@ def route_experts(logits, top_k: int, *, renormalize: bool = True, scale: float 
     """
     import torch
 
-    row_matrix(logits, "logits", _floats())
+    index = row_matrix(logits, "logits", _kinds()[2])
     T, E = logits.shape
     if type(top_k) is not int or not 1 <= top_k <= min(E, MAX_TOP_K):
         raise ValueError(f"top_k must be in 1..min(experts, {MAX_TOP_K})")
-    first_failure((
-        (E > MAX_EXPERTS, f"at most {MAX_EXPERTS} experts"),
-        (T * top_k >= INT32_LIMIT, "tokens * top_k must fit signed int32 indexing"),
-        (type(renormalize) is not bool, "renormalize must be a bool"),
-    ))
+    if E > MAX_EXPERTS:
+        raise ValueError(f"at most {MAX_EXPERTS} experts")
+    if T * top_k >= INT32_LIMIT:
+        raise ValueError("tokens * top_k must fit signed int32 indexing")
+    if type(renormalize) is not bool:
+        raise ValueError("renormalize must be a bool")
     scale = _scale(scale)
-    device = logits.device
     if out is None:
-        out = ExpertRouting(
-            torch.empty((T, top_k), dtype=torch.float32, device=device),
-            torch.empty((T, top_k), dtype=torch.int32, device=device),
-            torch.empty(E + 1, dtype=torch.int32, device=device),
-            torch.empty(T * top_k, dtype=torch.int32, device=device),
-            torch.empty((T, top_k), dtype=torch.int32, device=device),
-        )
+        # The four tables of T * k entries are parts of one allocation.
+        parts = torch.unsafe_split_with_sizes(logits.new_empty((4 * T, top_k), dtype=torch.int32), (T, T, T, T))
+        out = ExpertRouting(parts[0].view(torch.float32), parts[1], logits.new_empty(E + 1, dtype=torch.int32),
+                            parts[2].view(-1), parts[3])
     else:
         for name, shape, dtype in (("weights", (T, top_k), torch.float32), ("experts", (T, top_k), torch.int32),
                                    ("offsets", (E + 1,), torch.int32), ("rows", (T * top_k,), torch.int32),
                                    ("positions", (T, top_k), torch.int32)):
-            packed_table(getattr(out, name), f"out.{name}", shape, device, dtype)
+            packed_table(getattr(out, name), f"out.{name}", shape, index, dtype)
             output_is_distinct(getattr(out, name), (logits,))
-    workspace = torch.empty(_native.route_experts_workspace_ints(T, E), dtype=torch.int32, device=device)
-    with torch.cuda.device(device):
-        _native.call(
-            "lf_route_experts", _native.dtype_code(logits.dtype), logits.data_ptr(), row_stride(logits), T, E, top_k,
-            int(renormalize), scale, out.weights.data_ptr(), out.experts.data_ptr(), out.offsets.data_ptr(),
-            out.rows.data_ptr(), out.positions.data_ptr(), workspace.data_ptr(), workspace.numel(),
-            _native.stream_of(device),
-        )
+    room = _native.route_experts_workspace_ints(T, E)
+    workspace = logits.new_empty(room, dtype=torch.int32) if room else None
+    _native.launch(
+        "lf_route_experts", index, _native.dtype_code(logits.dtype), logits.data_ptr(), row_stride(logits), T, E, top_k,
+        renormalize, scale, out.weights.data_ptr(), out.experts.data_ptr(), out.offsets.data_ptr(),
+        out.rows.data_ptr(), out.positions.data_ptr(), workspace.data_ptr() if room else None, room,
+    )
     return out
 
 
@@ -133,40 +139,40 @@ def route_experts_backward(logits, routing: ExpertRouting, grad_weights, *, reno
     """
     import torch
 
-    row_matrix(logits, "logits", _floats())
+    index = row_matrix(logits, "logits", _kinds()[2])
     T, E = logits.shape
     if not isinstance(routing, ExpertRouting):
         raise TypeError("routing must be the ExpertRouting of the forward call")
-    device = logits.device
-    cuda_tensor(routing.weights, "routing.weights", 2, (torch.float32,), device)
+    cuda_tensor(routing.weights, "routing.weights", 2, (torch.float32,), index)
     k = routing.weights.shape[1]
-    packed_table(routing.weights, "routing.weights", (T, k), device, torch.float32)
-    packed_table(routing.experts, "routing.experts", (T, k), device, torch.int32)
-    row_matrix(grad_weights, "grad_weights", (torch.float32,), device)
-    first_failure((
-        (tuple(grad_weights.shape) != (T, k), "grad_weights must have the weights' shape"),
-        (not 1 <= k <= min(E, MAX_TOP_K) or E > MAX_EXPERTS, "routing does not fit the logits"),
-        (type(renormalize) is not bool, "renormalize must be a bool"),
-    ))
+    packed_table(routing.weights, "routing.weights", (T, k), index, torch.float32)
+    packed_table(routing.experts, "routing.experts", (T, k), index, torch.int32)
+    row_matrix(grad_weights, "grad_weights", (torch.float32,), index)
+    if grad_weights.shape != (T, k):
+        raise ValueError("grad_weights must have the weights' shape")
+    if not 1 <= k <= min(E, MAX_TOP_K) or E > MAX_EXPERTS:
+        raise ValueError("routing does not fit the logits")
+    if type(renormalize) is not bool:
+        raise ValueError("renormalize must be a bool")
     scale = _scale(scale)
-    grad = torch.empty((T, E), dtype=logits.dtype, device=device)
-    with torch.cuda.device(device):
-        _native.call(
-            "lf_route_experts_backward", _native.dtype_code(logits.dtype), logits.data_ptr(), row_stride(logits),
-            routing.weights.data_ptr(), routing.experts.data_ptr(), grad_weights.data_ptr(), row_stride(grad_weights),
-            T, E, k, int(renormalize), scale, grad.data_ptr(), E, _native.stream_of(device),
-        )
+    grad = logits.new_empty((T, E))
+    _native.launch(
+        "lf_route_experts_backward", index, _native.dtype_code(logits.dtype), logits.data_ptr(), row_stride(logits),
+        routing.weights.data_ptr(), routing.experts.data_ptr(), grad_weights.data_ptr(), row_stride(grad_weights),
+        T, E, k, renormalize, scale, grad.data_ptr(), E,
+    )
     return grad
 
 
-def _combine_tables(positions, weights, device):
+def _combine_tables(positions, weights, index: int):
     import torch
 
-    cuda_tensor(positions, "positions", 2, (torch.int32,), device)
+    cuda_tensor(positions, "positions", 2, (torch.int32,), index)
     T, k = positions.shape
-    packed_table(positions, "positions", (T, k), device, torch.int32)
+    if not positions.is_contiguous():
+        raise ValueError("positions must be contiguous")
     if weights is not None:
-        packed_table(weights, "weights", (T, k), device, torch.float32)
+        packed_table(weights, "weights", (T, k), index, torch.float32)
     if not 1 <= k <= MAX_TOP_K or T * k >= INT32_LIMIT:
         raise ValueError(f"positions must have 1..{MAX_TOP_K} columns and fit signed int32 indexing")
     return T, k
@@ -179,25 +185,22 @@ def combine_experts(y, weights, positions, *, out=None):
     a gather), ``positions`` int32 [T, k]; a position outside [0, R) adds nothing, so a token
     without experts gets zeros.
     """
-    import torch
-
-    row_matrix(y, "y", _floats())
-    T, k = _combine_tables(positions, weights, y.device)
-    if y.shape[1] < 1:
+    index = row_matrix(y, "y", _kinds()[2])
+    T, k = _combine_tables(positions, weights, index)
+    R, N = y.shape
+    if N < 1:
         raise ValueError("y must have at least one column")
     if out is None:
-        out = torch.empty((T, y.shape[1]), dtype=y.dtype, device=y.device)
+        out = y.new_empty((T, N))
     else:
-        row_matrix(out, "out", (y.dtype,), y.device)
-        if tuple(out.shape) != (T, y.shape[1]):
+        row_matrix(out, "out", (y.dtype,), index)
+        if out.shape != (T, N):
             raise ValueError("out must be [tokens, width]")
         output_is_distinct(out, (y, positions) if weights is None else (y, positions, weights))
-    with torch.cuda.device(y.device):
-        _native.call(
-            "lf_combine_experts", _native.dtype_code(y.dtype), y.data_ptr(), row_stride(y), y.shape[0],
-            None if weights is None else weights.data_ptr(), positions.data_ptr(), T, k, y.shape[1], out.data_ptr(),
-            row_stride(out), _native.stream_of(y.device),
-        )
+    _native.launch(
+        "lf_combine_experts", index, _native.dtype_code(y.dtype), y.data_ptr(), row_stride(y), R,
+        None if weights is None else weights.data_ptr(), positions.data_ptr(), T, k, N, out.data_ptr(), row_stride(out),
+    )
     return out
 
 
@@ -210,63 +213,59 @@ def combine_experts_backward(grad, y, weights, positions):
     """
     import torch
 
-    row_matrix(y, "y", _floats())
-    T, k = _combine_tables(positions, weights, y.device)
-    row_matrix(grad, "grad", (y.dtype,), y.device)
-    if tuple(grad.shape) != (T, y.shape[1]) or y.shape[1] < 1:
+    index = row_matrix(y, "y", _kinds()[2])
+    T, k = _combine_tables(positions, weights, index)
+    R, N = y.shape
+    row_matrix(grad, "grad", (y.dtype,), index)
+    if grad.shape != (T, N) or N < 1:
         raise ValueError("grad must be [tokens, width]")
-    grad_y = torch.empty(tuple(y.shape), dtype=y.dtype, device=y.device)
-    grad_weights = None if weights is None else torch.empty((T, k), dtype=torch.float32, device=y.device)
-    with torch.cuda.device(y.device):
-        _native.call(
-            "lf_combine_experts_backward", _native.dtype_code(y.dtype), grad.data_ptr(), row_stride(grad),
-            y.data_ptr(), row_stride(y), y.shape[0], None if weights is None else weights.data_ptr(),
-            positions.data_ptr(), T, k, y.shape[1], grad_y.data_ptr(), y.shape[1],
-            None if weights is None else grad_weights.data_ptr(), _native.stream_of(y.device),
-        )
+    grad_y = y.new_empty((R, N))
+    grad_weights = None if weights is None else y.new_empty((T, k), dtype=torch.float32)
+    _native.launch(
+        "lf_combine_experts_backward", index, _native.dtype_code(y.dtype), grad.data_ptr(), row_stride(grad),
+        y.data_ptr(), row_stride(y), R, None if weights is None else weights.data_ptr(), positions.data_ptr(), T, k, N,
+        grad_y.data_ptr(), N, None if weights is None else grad_weights.data_ptr(),
+    )
     return grad_y, grad_weights
 
 
-def _halves():
-    import torch
-
-    return (torch.float16, torch.bfloat16)
-
-
-def _operand(value, name: str, dtypes, device=None) -> None:
+def _operand(value, name: str, dtypes, index: int | None = None) -> int:
     """A row matrix that TMA can read: aligned, its row stride a multiple of 8."""
-    row_matrix(value, name, dtypes, device)
-    if value.shape[1] < 8 or value.shape[1] % 8 or (value.shape[0] > 1 and value.stride(0) % 8) or value.data_ptr() % 16:
+    index = row_matrix(value, name, dtypes, index)
+    rows, width = value.shape
+    if width < 8 or width % 8 or (rows > 1 and value.stride(0) % 8) or value.data_ptr() % 16:
         raise ValueError(f"{name} must be 16-byte aligned with a width and row stride that are multiples of 8")
+    return index
 
 
-def _expert_weight(weight, dtype, device) -> None:
-    cuda_tensor(weight, "weight", 3, (dtype,), device)
+def _expert_weight(weight, dtype, index: int) -> tuple:
+    """(experts, out, in, expert stride, row stride) of a weight tensor that TMA can read."""
+    cuda_tensor(weight, "weight", 3, (dtype,), index)
     E, N, K = weight.shape
     if not 1 <= E <= MAX_EXPERTS or N < 8 or N % 8 or K < 8 or K % 8:
         raise ValueError(f"weight must be [experts, out, in] with 1..{MAX_EXPERTS} experts and widths that are multiples of 8")
-    if (weight.stride(2) != 1 or weight.stride(1) % 8 or weight.stride(1) < K or weight.data_ptr() % 16
-            or (E > 1 and (weight.stride(0) % 8 or weight.stride(0) < (N - 1) * weight.stride(1) + K))):
+    by_expert, by_row, unit = weight.stride()
+    if E == 1:  # a single expert's own stride says nothing
+        by_expert = N * by_row
+    if unit != 1 or by_row % 8 or by_row < K or weight.data_ptr() % 16 or by_expert % 8 or by_expert < (N - 1) * by_row + K:
         raise ValueError("weight must be 16-byte aligned with unit inner stride and outer strides that are multiples of 8")
+    return E, N, K, by_expert, by_row
 
 
-def expert_stride(weight) -> int:
-    """Stride between experts (a single expert's own stride says nothing)."""
-    return weight.stride(0) if weight.shape[0] > 1 else weight.shape[1] * weight.stride(1)
-
-
-def group_tables(offsets, rows, num_experts: int, x_rows: int, device) -> int:
+def group_tables(offsets, rows, num_experts: int, x_rows: int, index: int) -> int:
     """Checks ``offsets`` [E + 1] and ``rows`` [R] (or None); the number of rows R."""
     import torch
 
-    packed_table(offsets, "offsets", (num_experts + 1,), device, torch.int32)
+    packed_table(offsets, "offsets", (num_experts + 1,), index, torch.int32)
     if rows is None:
         return x_rows
-    cuda_tensor(rows, "rows", 1, (torch.int32,), device)
-    packed_table(rows, "rows", (rows.numel(),), device, torch.int32)
-    if rows.numel() and not x_rows:
+    cuda_tensor(rows, "rows", 1, (torch.int32,), index)
+    R = rows.numel()
+    if not rows.is_contiguous():
+        raise ValueError("rows must be contiguous")
+    if R and not x_rows:
         raise ValueError("x must have at least one row")
-    return rows.numel()
+    return R
 
 
 def expert_linear(x, weight, offsets, *, rows=None, out=None):
@@ -277,29 +276,25 @@ def expert_linear(x, weight, offsets, *, rows=None, out=None):
     ``rows``, x's own rows are the sorted ones.  Sums are FP32, rounded once; rows of no group
     are zeros.  Returns y [R, N] (``out`` when given).
     """
-    import torch
-
-    _operand(x, "x", _halves())
-    _expert_weight(weight, x.dtype, x.device)
-    E, N, K = weight.shape
-    if x.shape[1] != K:
+    index = _operand(x, "x", _kinds()[1])
+    E, N, K, by_expert, by_row = _expert_weight(weight, x.dtype, index)
+    T, width = x.shape
+    if width != K:
         raise ValueError("x's width must be the weight's")
-    R = group_tables(offsets, rows, E, x.shape[0], x.device)
+    R = group_tables(offsets, rows, E, T, index)
     if out is None:
-        out = torch.empty((R, N), dtype=x.dtype, device=x.device)
+        out = x.new_empty((R, N))
     else:
-        row_matrix(out, "out", (x.dtype,), x.device)
-        if tuple(out.shape) != (R, N):
+        row_matrix(out, "out", (x.dtype,), index)
+        if out.shape != (R, N):
             raise ValueError("out must be [rows, out features]")
         output_is_distinct(out, (x, weight, offsets) if rows is None else (x, weight, offsets, rows))
     workspace, room = _gather_room(x, rows, E, R, K, False)
-    with torch.cuda.device(x.device):
-        _native.call(
-            "lf_expert_linear", _native.dtype_code(x.dtype), x.data_ptr(), row_stride(x), x.shape[0],
-            None if rows is None else rows.data_ptr(), weight.data_ptr(), expert_stride(weight), weight.stride(1),
-            offsets.data_ptr(), E, R, N, K, out.data_ptr(), row_stride(out),
-            None if workspace is None else workspace.data_ptr(), room, _native.stream_of(x.device),
-        )
+    _native.launch(
+        "lf_expert_linear", index, _native.dtype_code(x.dtype), x.data_ptr(), row_stride(x), T,
+        None if rows is None else rows.data_ptr(), weight.data_ptr(), by_expert, by_row, offsets.data_ptr(), E, R, N, K,
+        out.data_ptr(), row_stride(out), workspace.data_ptr() if room else None, room,
+    )
     return out
 
 
@@ -308,7 +303,7 @@ def _gather_room(x, rows, E: int, R: int, K: int, weight_grad: bool):
     import torch
 
     room = 0 if rows is None else _native.expert_linear_workspace_bytes(E, R, K, weight_grad)
-    return (torch.empty(room, dtype=torch.uint8, device=x.device) if room else None), room
+    return (x.new_empty(room, dtype=torch.uint8) if room else None), room
 
 
 def expert_linear_backward(grad, x, weight, offsets, *, rows=None, weight_grad_dtype=None):
@@ -320,32 +315,29 @@ def expert_linear_backward(grad, x, weight, offsets, *, rows=None, weight_grad_d
     """
     import torch
 
-    _operand(x, "x", _halves())
-    _expert_weight(weight, x.dtype, x.device)
-    _operand(grad, "grad", (x.dtype,), x.device)
-    E, N, K = weight.shape
-    if x.shape[1] != K:
+    index = _operand(x, "x", _kinds()[1])
+    E, N, K, by_expert, by_row = _expert_weight(weight, x.dtype, index)
+    _operand(grad, "grad", (x.dtype,), index)
+    T, width = x.shape
+    if width != K:
         raise ValueError("x's width must be the weight's")
-    R = group_tables(offsets, rows, E, x.shape[0], x.device)
-    if tuple(grad.shape) != (R, N):
+    R = group_tables(offsets, rows, E, T, index)
+    if grad.shape != (R, N):
         raise ValueError("grad must be [rows, out features]")
     weight_grad_dtype = x.dtype if weight_grad_dtype is None else weight_grad_dtype
     if weight_grad_dtype not in (x.dtype, torch.float32):
         raise ValueError("weight_grad_dtype must be the operands' type or float32")
-    grad_x = torch.empty((R, K), dtype=x.dtype, device=x.device)
-    grad_weight = torch.empty((E, N, K), dtype=weight_grad_dtype, device=x.device)
-    dtype = _native.dtype_code(x.dtype)
+    grad_x = x.new_empty((R, K))
+    grad_weight = x.new_empty((E, N, K), dtype=weight_grad_dtype)
+    dtype, stride = _native.dtype_code(x.dtype), row_stride(grad)
+    _native.launch(
+        "lf_expert_linear_input_grad", index, dtype, grad.data_ptr(), stride, weight.data_ptr(), by_expert, by_row,
+        offsets.data_ptr(), E, R, N, K, grad_x.data_ptr(), K,
+    )
     workspace, room = _gather_room(x, rows, E, R, K, True)
-    with torch.cuda.device(x.device):
-        stream = _native.stream_of(x.device)
-        _native.call(
-            "lf_expert_linear_input_grad", dtype, grad.data_ptr(), row_stride(grad), weight.data_ptr(),
-            expert_stride(weight), weight.stride(1), offsets.data_ptr(), E, R, N, K, grad_x.data_ptr(), K, stream,
-        )
-        _native.call(
-            "lf_expert_linear_weight_grad", dtype, grad.data_ptr(), row_stride(grad), x.data_ptr(), row_stride(x),
-            x.shape[0], None if rows is None else rows.data_ptr(), offsets.data_ptr(), E, R, N, K,
-            _native.dtype_code(weight_grad_dtype), grad_weight.data_ptr(),
-            None if workspace is None else workspace.data_ptr(), room, stream,
-        )
+    _native.launch(
+        "lf_expert_linear_weight_grad", index, dtype, grad.data_ptr(), stride, x.data_ptr(), row_stride(x), T,
+        None if rows is None else rows.data_ptr(), offsets.data_ptr(), E, R, N, K,
+        _native.dtype_code(weight_grad_dtype), grad_weight.data_ptr(), workspace.data_ptr() if room else None, room,
+    )
     return grad_x, grad_weight

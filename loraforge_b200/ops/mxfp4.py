@@ -13,7 +13,7 @@ from typing import NamedTuple
 
 from loraforge_b200 import _native
 from loraforge_b200.ops._contract import output_is_distinct
-from loraforge_b200.ops.experts import MAX_EXPERTS, cuda_tensor, group_tables, packed_table, row_matrix, row_stride
+from loraforge_b200.ops.experts import MAX_EXPERTS, _kinds, cuda_tensor, group_tables, packed_table, row_matrix, row_stride
 
 BLOCK = 32
 
@@ -25,18 +25,19 @@ class MxTensor(NamedTuple):
     scales: object  # uint8 [..., K / 32]
 
 
-def check_mx(value, name: str, ndim: int, device=None) -> tuple:
-    """The shape [..., K] of a contiguous MxTensor of rank `ndim` on `device` if given."""
+def check_mx(value, name: str, ndim: int, index: int | None = None) -> tuple:
+    """(shape [..., K], device index) of a contiguous MxTensor of rank `ndim`, on `index` if given."""
     import torch
 
     if not isinstance(value, MxTensor):
         raise TypeError(f"{name} must be an MxTensor")
-    cuda_tensor(value.codes, f"{name}.codes", ndim, (torch.uint8,), device)
-    *rows, half = value.codes.shape
-    if half < BLOCK // 2 or half % (BLOCK // 2) or not value.codes.is_contiguous() or value.codes.data_ptr() % 16:
+    codes = value.codes
+    index = cuda_tensor(codes, f"{name}.codes", ndim, (torch.uint8,), index)
+    *rows, half = codes.shape
+    if half < BLOCK // 2 or half % (BLOCK // 2) or not codes.is_contiguous() or codes.data_ptr() % 16:
         raise ValueError(f"{name}.codes must be contiguous and 16-byte aligned with rows of whole blocks of {BLOCK}")
-    packed_table(value.scales, f"{name}.scales", (*rows, half * 2 // BLOCK), value.codes.device, torch.uint8)
-    return (*rows, 2 * half)
+    packed_table(value.scales, f"{name}.scales", (*rows, half * 2 // BLOCK), index, torch.uint8)
+    return (*rows, 2 * half), index
 
 
 def mxfp4_quantize(x) -> MxTensor:
@@ -48,24 +49,21 @@ def mxfp4_quantize(x) -> MxTensor:
 
     if not isinstance(x, torch.Tensor):
         raise TypeError("x must be a torch.Tensor")
-    cuda_tensor(x, "x", max(x.ndim, 1), (torch.float32, torch.float16, torch.bfloat16))
-    K = x.shape[-1]
+    index = cuda_tensor(x, "x", max(x.ndim, 1), _kinds()[2])
+    *shape, K = x.shape
     if K < BLOCK or K % BLOCK:
         raise ValueError(f"x's last dimension must be a positive multiple of {BLOCK}")
-    shape = tuple(x.shape[:-1])
-    if x.ndim == 2 and x.shape[0] > 1:
-        rows, stride = x.shape[0], x.stride(0)
+    rows, stride = x.numel() // K, K
+    if not x.is_contiguous():
+        if x.ndim != 2:
+            raise ValueError("x must be contiguous unless it is 2D")
+        stride = x.stride(0)
         if x.stride(1) != 1 or stride < K:
             raise ValueError("x must have unit column stride and rows that do not overlap")
-    else:
-        rows, stride = x.numel() // K, K
-        if not x.is_contiguous():
-            raise ValueError("x must be contiguous unless it is 2D")
-    codes = torch.empty((*shape, K // 2), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((*shape, K // BLOCK), dtype=torch.uint8, device=x.device)
-    with torch.cuda.device(x.device):
-        _native.call("lf_mxfp4_quantize", _native.dtype_code(x.dtype), x.data_ptr(), stride, rows, K,
-                     codes.data_ptr(), scales.data_ptr(), _native.stream_of(x.device))
+    codes = x.new_empty((*shape, K // 2), dtype=torch.uint8)
+    scales = x.new_empty((*shape, K // BLOCK), dtype=torch.uint8)
+    _native.launch("lf_mxfp4_quantize", index, _native.dtype_code(x.dtype), x.data_ptr(), stride, rows, K,
+                   codes.data_ptr(), scales.data_ptr())
     return MxTensor(codes, scales)
 
 
@@ -74,15 +72,14 @@ def mxfp4_dequantize(x: MxTensor, dtype=None):
     import torch
 
     dtype = torch.bfloat16 if dtype is None else dtype
-    if dtype not in (torch.float32, torch.float16, torch.bfloat16):
+    if dtype not in _kinds()[2]:
         raise ValueError("dtype must be float32, float16 or bfloat16")
     if not isinstance(x, MxTensor):
         raise TypeError("x must be an MxTensor")
-    shape = check_mx(x, "x", getattr(x.codes, "ndim", 1))
-    out = torch.empty(shape, dtype=dtype, device=x.codes.device)
-    with torch.cuda.device(out.device):
-        _native.call("lf_mxfp4_dequantize", _native.dtype_code(dtype), x.codes.data_ptr(), x.scales.data_ptr(),
-                     out.numel() // shape[-1], shape[-1], out.data_ptr(), _native.stream_of(out.device))
+    shape, index = check_mx(x, "x", getattr(x.codes, "ndim", 1))
+    out = x.codes.new_empty(shape, dtype=dtype)
+    _native.launch("lf_mxfp4_dequantize", index, _native.dtype_code(dtype), x.codes.data_ptr(), x.scales.data_ptr(),
+                   out.numel() // shape[-1], shape[-1], out.data_ptr())
     return out
 
 
@@ -96,31 +93,27 @@ def expert_linear_mxfp4(x: MxTensor, weight: MxTensor, offsets, *, rows=None, dt
     """
     import torch
 
-    T, K = check_mx(x, "x", 2)
-    device = x.codes.device
-    E, N, width = check_mx(weight, "weight", 3, device)
+    (T, K), index = check_mx(x, "x", 2)
+    E, N, width = check_mx(weight, "weight", 3, index)[0]
     if width != K:
         raise ValueError("x's width must be the weight's")
     if not 1 <= E <= MAX_EXPERTS or N < 1:
         raise ValueError(f"weight must be [experts, out, in] with 1..{MAX_EXPERTS} experts")
-    R = group_tables(offsets, rows, E, T, device)
-    kinds = (torch.float32, torch.float16, torch.bfloat16)
-    if dtype is not None and dtype not in kinds:
+    R = group_tables(offsets, rows, E, T, index)
+    if dtype is not None and dtype not in _kinds()[2]:
         raise ValueError("dtype must be float32, float16 or bfloat16")
     if out is None:
-        out = torch.empty((R, N), dtype=torch.bfloat16 if dtype is None else dtype, device=device)
+        out = x.codes.new_empty((R, N), dtype=torch.bfloat16 if dtype is None else dtype)
     else:
-        row_matrix(out, "out", kinds if dtype is None else (dtype,), device)
-        if tuple(out.shape) != (R, N):
+        row_matrix(out, "out", _kinds()[2] if dtype is None else (dtype,), index)
+        if out.shape != (R, N):
             raise ValueError("out must be [rows, out features]")
         output_is_distinct(out, (*x, *weight, offsets) if rows is None else (*x, *weight, offsets, rows))
     room = _native.expert_linear_mxfp4_workspace_bytes(E, R, N, K, rows is not None)
-    workspace = torch.empty(room, dtype=torch.uint8, device=device) if room else None
-    with torch.cuda.device(device):
-        _native.call(
-            "lf_expert_linear_mxfp4", _native.dtype_code(out.dtype), x.codes.data_ptr(), x.scales.data_ptr(), T,
-            None if rows is None else rows.data_ptr(), weight.codes.data_ptr(), weight.scales.data_ptr(),
-            offsets.data_ptr(), E, R, N, K, out.data_ptr(), row_stride(out),
-            None if workspace is None else workspace.data_ptr(), room, _native.stream_of(device),
-        )
+    workspace = x.codes.new_empty(room) if room else None
+    _native.launch(
+        "lf_expert_linear_mxfp4", index, _native.dtype_code(out.dtype), x.codes.data_ptr(), x.scales.data_ptr(), T,
+        None if rows is None else rows.data_ptr(), weight.codes.data_ptr(), weight.scales.data_ptr(),
+        offsets.data_ptr(), E, R, N, K, out.data_ptr(), row_stride(out), workspace.data_ptr() if room else None, room,
+    )
     return out
