@@ -17,10 +17,13 @@ namespace {
 
 constexpr int kMaxExperts = 1024;
 constexpr int kMaxTopK = 32;
-constexpr int kRouteThreads = 256;
+constexpr int kRouteThreads = 1024;
 constexpr int kRouteWarps = kRouteThreads / 32;
+constexpr int kSortWarps = 8;         // of a block, that rank its slots
 constexpr int kMaxRouteBlocks = 256;  // each block of the scatter adds up the others' counts
 constexpr int kMinBlockTokens = 32;
+constexpr int kBackThreads = 256;
+constexpr int sort_bytes(int E) { return int(sizeof(int)) * E * (1 + kSortWarps); }
 
 template <typename T>
 __device__ __forceinline__ float load_value(const void* p, int64_t i);
@@ -71,23 +74,36 @@ template <bool kOwn>
 __device__ void scatter_slots(const int32_t* experts, const int32_t* counts, int blocks, int block, int64_t slot0,
                               int slots, int64_t all_slots, int E, int k, int32_t* offsets, int32_t* rows,
                               int32_t* positions, int* smem) {
-  int* base = smem;            // [E + 1]
-  int* wcount = smem + E + 1;  // [kRouteWarps][E]
+  int* base = smem;                     // [E]: rows before expert e's, then before this block's of e
+  int* wcount = base + E;               // [kSortWarps][E]
+  int* sums = wcount;                   // [parts][2][E] before that: all rows of e, those of earlier blocks
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, threads = blockDim.x;
   __shared__ int warp_total[kRouteWarps];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  // Rows of the experts before e, plus those of e in the blocks before this one.
+  // Counts of the blocks, in up to four parts of them at a time.
+  const int parts = kOwn ? 1 : max(1, min(kSortWarps / 2, threads / E));
+  const int each = (blocks + parts - 1) / parts;
+  for (int i = tid; i < parts * E; i += threads) {
+    const int part = i / E, e = i - part * E;
+    int total = 0, before = 0;
+#pragma unroll 16
+    for (int b = part * each; b < min(blocks, part * each + each); ++b) {
+      const int c = kOwn ? counts[e] : __ldcg(counts + int64_t(b) * E + e);
+      total += c;
+      before += b < block ? c : 0;
+    }
+    sums[(2 * part) * E + e] = total;
+    sums[(2 * part + 1) * E + e] = before;
+  }
+  __syncthreads();
   int carry = 0;
-  for (int e0 = 0; e0 < E; e0 += kRouteThreads) {
+  for (int e0 = 0; e0 < E; e0 += threads) {
     const int e = e0 + tid;
     int total = 0, before = 0;
-    if (e < E) {
-#pragma unroll 8
-      for (int b = 0; b < blocks; ++b) {
-        const int c = kOwn ? counts[e] : __ldcg(counts + int64_t(b) * E + e);
-        total += c;
-        before += b < block ? c : 0;
+    if (e < E)
+      for (int part = 0; part < parts; ++part) {
+        total += sums[(2 * part) * E + e];
+        before += sums[(2 * part + 1) * E + e];
       }
-    }
     int scan = total;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -97,28 +113,32 @@ __device__ void scatter_slots(const int32_t* experts, const int32_t* counts, int
     if (lane == 31) warp_total[warp] = scan;
     __syncthreads();
     int prefix = carry;
-    for (int w = 0; w < warp; ++w) prefix += warp_total[w];
+    for (int w = 0; w < threads / 32; ++w) {
+      if (w < warp) prefix += warp_total[w];
+      carry += warp_total[w];
+    }
     if (e < E) {
       base[e] = prefix + scan - total + before;
       if (block == 0) offsets[e] = prefix + scan - total;
     }
-    for (int w = 0; w < kRouteWarps; ++w) carry += warp_total[w];
     __syncthreads();
   }
   if (block == 0 && tid == 0) offsets[E] = carry;
-  // Each warp counts its contiguous part of the slots.
-  const int part = (slots + kRouteWarps - 1) / kRouteWarps;
-  const int lo = min(slots, warp * part), hi = min(slots, lo + part);
-  for (int i = tid; i < kRouteWarps * E; i += kRouteThreads) wcount[i] = 0;
+  // The first kSortWarps warps count their contiguous parts of the slots.
+  const int part = (slots + kSortWarps - 1) / kSortWarps;
+  const bool sorts = warp < kSortWarps;
+  const int lo = sorts ? min(slots, warp * part) : 0, hi = sorts ? min(slots, lo + part) : 0;
+  for (int i = tid; i < kSortWarps * E; i += threads) wcount[i] = 0;
   __syncthreads();
   for (int s = lo + lane; s < hi; s += 32) {
     const int e = experts[slot0 + s];
     if (e >= 0) atomicAdd(&wcount[warp * E + e], 1);
   }
   __syncthreads();
-  for (int e = tid; e < E; e += kRouteThreads) {
+  for (int e = tid; e < E; e += threads) {
     int at = base[e];
-    for (int w = 0; w < kRouteWarps; ++w) {
+#pragma unroll
+    for (int w = 0; w < kSortWarps; ++w) {
       const int c = wcount[w * E + e];
       wcount[w * E + e] = at;
       at += c;
@@ -140,13 +160,13 @@ __device__ void scatter_slots(const int32_t* experts, const int32_t* counts, int
     }
   }
   // Rows of no slot.
-  for (int64_t r = carry + int64_t(block) * kRouteThreads + tid; r < all_slots; r += int64_t(blocks) * kRouteThreads)
-    rows[r] = -1;
+  for (int64_t r = carry + int64_t(block) * threads + tid; r < all_slots; r += int64_t(blocks) * threads) rows[r] = -1;
 }
 
 // One warp a token: k times the largest remaining logit.  A lane keeps the best of its own
 // V logits and looks through them again only after it lost it.  With one block the slots
 // are sorted in the same launch, else the block leaves its counts for route_scatter_kernel.
+// Bound by the latency of the k picks, so a block has a warp for each of its 32 tokens.
 template <typename T, int V>
 __global__ void __launch_bounds__(kRouteThreads) route_topk_kernel(
     const void* logits, int64_t stride, int num_tokens, int E, int k, int renormalize, float scale, int block_tokens,
@@ -154,11 +174,11 @@ __global__ void __launch_bounds__(kRouteThreads) route_topk_kernel(
   extern __shared__ int smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   int* hist = smem;
-  for (int e = tid; e < E; e += kRouteThreads) hist[e] = 0;
+  for (int e = tid; e < E; e += blockDim.x) hist[e] = 0;
   pdl_wait();
   __syncthreads();
   const int t0 = blockIdx.x * block_tokens, t1 = min(num_tokens, t0 + block_tokens);
-  for (int t = t0 + warp; t < t1; t += kRouteWarps) {
+  for (int t = t0 + warp; t < t1; t += blockDim.x / 32) {
     float v[V];
     load_logits<T, V>(logits, int64_t(t) * stride, E, lane, v);
     uint32_t taken = 0;
@@ -206,7 +226,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_topk_kernel(
   }
   __syncthreads();
   if (gridDim.x > 1) {
-    for (int e = tid; e < E; e += kRouteThreads) counts[int64_t(blockIdx.x) * E + e] = hist[e];
+    for (int e = tid; e < E; e += blockDim.x) counts[int64_t(blockIdx.x) * E + e] = hist[e];
     return;
   }
   scatter_slots<true>(experts, hist, 1, 0, 0, num_tokens * k, int64_t(num_tokens) * k, E, k, offsets, rows, positions,
@@ -227,13 +247,13 @@ __global__ void __launch_bounds__(kRouteThreads) route_scatter_kernel(const int3
 // dl_i = w_i (g_i - d) for the taken experts, with d = sum_j w_j g_j / scale, and for the
 // others 0 (renormalised weights) or -scale . p_i . d.  One warp a token.
 template <typename T, int V>
-__global__ void __launch_bounds__(kRouteThreads) route_backward_kernel(
+__global__ void __launch_bounds__(kBackThreads) route_backward_kernel(
     const void* logits, int64_t stride, const float* weights, const int32_t* experts, const float* grad,
     int64_t grad_stride, int num_tokens, int E, int k, int renormalize, float scale, void* grad_logits,
     int64_t out_stride) {
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t t = int64_t(blockIdx.x) * kRouteWarps + warp;
+  const int64_t t = int64_t(blockIdx.x) * (kBackThreads / 32) + warp;
   if (t >= num_tokens) return;
   const int e = lane < k ? experts[t * k + lane] : -1;
   const bool live = e >= 0 && e < E;
@@ -468,8 +488,8 @@ struct RouteCall {
   template <typename D, int V>
   int operator()() const {
     const RoutePlan plan = route_plan(T);
-    const int smem = int(sizeof(int)) * (E + 1 + kRouteWarps * E);
-    return launch_pdl(route_topk_kernel<D, V>, dim3(plan.blocks), kRouteThreads, smem, stream, "route_experts", logits,
+    const int threads = T > kSortWarps ? kRouteThreads : kSortWarps * 32;
+    return launch_pdl(route_topk_kernel<D, V>, dim3(plan.blocks), threads, sort_bytes(E), stream, "route_experts", logits,
                       stride, T, E, k, renormalize, scale, plan.block_tokens, weights, experts, offsets, rows,
                       positions, counts);
   }
@@ -489,7 +509,7 @@ struct RouteBackwardCall {
   void* stream;
   template <typename D, int V>
   int operator()() const {
-    return launch_pdl(route_backward_kernel<D, V>, dim3((T + kRouteWarps - 1) / kRouteWarps), kRouteThreads, 0, stream,
+    return launch_pdl(route_backward_kernel<D, V>, dim3((T + kBackThreads / 32 - 1) / (kBackThreads / 32)), kBackThreads, 0, stream,
                       "route_experts_backward", logits, stride, weights, experts, grad, grad_stride, T, E, k,
                       renormalize, scale, out, out_stride);
   }
@@ -535,8 +555,7 @@ extern "C" int lf_route_experts(int32_t dtype, const void* logits, int64_t logit
   if (int rc = with_type(dtype, num_experts, call)) return rc;
   const RoutePlan plan = route_plan(num_tokens);
   if (plan.blocks == 1) return LF_OK;
-  const int smem = int(sizeof(int)) * (num_experts + 1 + kRouteWarps * num_experts);
-  return launch_pdl(route_scatter_kernel, dim3(plan.blocks), kRouteThreads, smem, stream, "route_experts (sort)",
+  return launch_pdl(route_scatter_kernel, dim3(plan.blocks), kRouteThreads, sort_bytes(num_experts), stream, "route_experts (sort)",
                     static_cast<const int32_t*>(experts), static_cast<const int32_t*>(workspace), int(num_tokens),
                     int(num_experts), int(top_k), plan.block_tokens, offsets, rows, positions);
 }
