@@ -7,31 +7,20 @@
 // division is by a power of two, so nothing is rounded but the code itself.  A block with an
 // infinity or a NaN gets scale byte 255 (NaN) and codes 0.
 //
-// Both kernels are bound by HBM: 4.25 bits a value on one side, 16 or 32 on the other.  A
-// thread takes 8 values (one or two 16-byte loads, 4 bytes of codes), so that four
-// neighbouring lanes share a block and every access of a warp is contiguous.
+// Both kernels are bound by HBM: 4.25 bits a value on one side, 16 or 32 on the other.  In the
+// quantiser a thread takes 16 values, so two neighbouring lanes share a block: with 8 values a
+// thread the address arithmetic, the shuffles and the scale's stores of every 8 values made it
+// issue-bound (28672 x 4096 BF16: 82 us).  Magnitudes of 16-bit types are compared in pairs.
 #include "launch.cuh"
 
 namespace lfb {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kPerThread = 4;  // groups of 8 values in flight a thread
+constexpr int kPerThread = 4;  // dequantiser: groups of 8 values in flight a thread
+constexpr int kUnits = 2;      // quantiser: units of 16 values in flight a thread
 
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
-template <typename T, bool kVector>
-__device__ __forceinline__ void load8(const typename T::storage* p, float* f) {
-  if (!kVector) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = T::to_float(p[i]);
-  } else if constexpr (sizeof(typename T::storage) == 4) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
-  } else {
-    unpack8<T>(*reinterpret_cast<const uint4*>(p), f);
-  }
-}
 
 // Eight values as E2M1 codes, the first in the lowest nibble (nearest even, saturating).
 __device__ __forceinline__ uint32_t e2m1x8(const float* v) {
@@ -45,42 +34,89 @@ __device__ __forceinline__ uint32_t e2m1x8(const float* v) {
   return codes;
 }
 
-// groups: groups of 8 values in all, per_row of them a row; a row of x starts at row * stride.
-// Rows without gaps are one long row.  Every lane of a block's four takes part together:
-// groups is a multiple of 4.
+// 16 values of T in 16-byte words, their FP32 values, and the bits of the largest magnitude as
+// FP32, where an infinity or a NaN ends at 0x7f800000 or above.
+template <typename T>
+struct Unit {  // 16-bit types
+  static constexpr int kWords = 2;
+  static __device__ __forceinline__ void values(const uint4 (&q)[2], float* f) {
+    unpack8<T>(q[0], f);
+    unpack8<T>(q[1], f + 8);
+  }
+  static __device__ __forceinline__ uint32_t peak(const uint4 (&q)[2]) {
+    // Magnitudes order like their bits, so two halves compare at once.
+    const uint32_t w[8] = {q[0].x, q[0].y, q[0].z, q[0].w, q[1].x, q[1].y, q[1].z, q[1].w};
+    uint32_t m = w[0] & 0x7fff7fffu;
+#pragma unroll
+    for (int i = 1; i < 8; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+    const uint32_t top = max(m & 0xffffu, m >> 16);
+    typename T::storage h;
+    *reinterpret_cast<uint16_t*>(&h) = uint16_t(top);
+    return __float_as_uint(T::to_float(h)) & 0x7fffffffu;
+  }
+};
+template <>
+struct Unit<f32_t> {
+  static constexpr int kWords = 4;
+  static __device__ __forceinline__ void values(const uint4 (&q)[4], float* f) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[4 * i] = __uint_as_float(q[i].x), f[4 * i + 1] = __uint_as_float(q[i].y);
+      f[4 * i + 2] = __uint_as_float(q[i].z), f[4 * i + 3] = __uint_as_float(q[i].w);
+    }
+  }
+  static __device__ __forceinline__ uint32_t peak(const uint4 (&q)[4]) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      m = max(m, max(max(q[i].x & 0x7fffffffu, q[i].y & 0x7fffffffu), max(q[i].z & 0x7fffffffu, q[i].w & 0x7fffffffu)));
+    return m;
+  }
+};
+
+// units: units of 16 values in all, per_row of them a row; a row of x starts at row * stride.
+// Rows without gaps are one long row.  units is even, so both lanes of a block take part.
 template <typename T, bool kVector>
 __global__ void __launch_bounds__(kThreads) quantize_kernel(const typename T::storage* x, int64_t stride,
-                                                            int64_t per_row, int64_t groups, uint32_t* codes,
+                                                            int64_t per_row, int64_t units, uint2* codes,
                                                             uint8_t* scales) {
+  using U = Unit<T>;
   pdl_wait();
-  const int64_t first = int64_t(blockIdx.x) * (kThreads * kPerThread) + threadIdx.x;
-  float v[kPerThread][8];
+  const int64_t first = int64_t(blockIdx.x) * (kThreads * kUnits);
+  const int live = int(min(units - first, int64_t(kThreads * kUnits)));  // units of this block
+  uint4 q[kUnits][U::kWords];
 #pragma unroll
-  for (int u = 0; u < kPerThread; ++u) {
-    const int64_t g = first + u * kThreads;
-    if (g >= groups) continue;
-    const int64_t row = g < per_row ? 0 : g / per_row;
-    load8<T, kVector>(x + row * stride + (g - row * per_row) * 8, v[u]);
+  for (int u = 0; u < kUnits; ++u) {
+    const int i = u * kThreads + threadIdx.x;
+    if (i >= live) continue;
+    const int64_t unit = first + i;
+    const int64_t row = per_row == units ? 0 : unit / per_row;
+    const typename T::storage* src = x + row * stride + (unit - row * per_row) * 16;
+    if (kVector) {
+#pragma unroll
+      for (int w = 0; w < U::kWords; ++w) q[u][w] = reinterpret_cast<const uint4*>(src)[w];
+    } else {
+      typename T::storage* dst = reinterpret_cast<typename T::storage*>(q[u]);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) dst[j] = src[j];
+    }
   }
 #pragma unroll
-  for (int u = 0; u < kPerThread; ++u) {
-    const int64_t g = first + u * kThreads;
-    uint32_t peak = 0;  // the largest magnitude's bits order like the magnitudes
-    if (g < groups) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) peak = max(peak, __float_as_uint(v[u][i]) & 0x7fffffffu);
-    }
+  for (int u = 0; u < kUnits; ++u) {
+    const int i = u * kThreads + threadIdx.x;
+    uint32_t peak = i < live ? U::peak(q[u]) : 0;
     peak = max(peak, __shfl_xor_sync(0xffffffffu, peak, 1));
-    peak = max(peak, __shfl_xor_sync(0xffffffffu, peak, 2));
-    if (g >= groups) continue;
+    if (i >= live) continue;
     const bool finite = peak < 0x7f800000u;
     const int scale = finite ? max(int(peak >> 23) - 2, 0) : 255;
     const float inverse = __uint_as_float(uint32_t(254 - scale) << 23);  // 2^(127 - scale), exact
-    float w[8];
+    float f[16];
+    U::values(q[u], f);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = finite ? v[u][i] * inverse : 0.f;
-    codes[g] = e2m1x8(w);
-    if ((g & 3) == 0) scales[g >> 2] = uint8_t(scale);
+    for (int j = 0; j < 16; ++j) f[j] *= inverse;
+    const uint2 c = make_uint2(e2m1x8(f), e2m1x8(f + 8));
+    (codes + first)[i] = finite ? c : make_uint2(0, 0);
+    if ((i & 1) == 0) (scales + first / 2)[i >> 1] = uint8_t(scale);
   }
 }
 
@@ -124,14 +160,14 @@ __global__ void __launch_bounds__(kThreads) dequantize_kernel(const uint32_t* co
 }
 
 template <typename... Params, typename... Args>
-int launch_flat(void (*kernel)(Params...), int64_t groups, void* stream, const char* what, Args... args) {
+int launch_flat(void (*kernel)(Params...), int64_t blocks, void* stream, const char* what, Args... args) {
   cudaLaunchConfig_t config = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   config.attrs = attr;
   config.numAttrs = 1;
-  config.gridDim = dim3(unsigned((groups + kThreads * kPerThread - 1) / (kThreads * kPerThread)));
+  config.gridDim = dim3(unsigned(blocks));
   config.blockDim = dim3(kThreads);
   config.stream = static_cast<cudaStream_t>(stream);
   const cudaError_t err = cudaLaunchKernelEx(&config, kernel, args...);
@@ -147,15 +183,16 @@ int launch_quantize(const void* x, int64_t stride, int64_t rows, int64_t width, 
                     void* stream) {
   using S = typename T::storage;
   const bool flat = stride == width || rows == 1;
-  const int64_t groups = rows * (width / 8), per_row = flat ? groups : width / 8;
+  const int64_t units = rows * (width / 16), per_row = flat ? units : width / 16;
   const bool vec = aligned16(x) && (rows == 1 || stride * int64_t(sizeof(S)) % 16 == 0);
-  return launch_flat(vec ? quantize_kernel<T, true> : quantize_kernel<T, false>, groups, stream, "mxfp4_quantize",
-                     static_cast<const S*>(x), stride, per_row, groups, reinterpret_cast<uint32_t*>(codes), scales);
+  return launch_flat(vec ? quantize_kernel<T, true> : quantize_kernel<T, false>,
+                     (units + kThreads * kUnits - 1) / (kThreads * kUnits), stream, "mxfp4_quantize",
+                     static_cast<const S*>(x), stride, per_row, units, reinterpret_cast<uint2*>(codes), scales);
 }
 
 template <typename T>
 int launch_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t groups, void* out, void* stream) {
-  return launch_flat(dequantize_kernel<T>, groups, stream, "mxfp4_dequantize",
+  return launch_flat(dequantize_kernel<T>, (groups + kThreads * kPerThread - 1) / (kThreads * kPerThread), stream, "mxfp4_dequantize",
                      reinterpret_cast<const uint32_t*>(codes), scales, groups,
                      static_cast<typename T::storage*>(out));
 }
