@@ -360,22 +360,22 @@ __device__ __forceinline__ void store_chunk(uint32_t taddr, bool live, uint32_t 
   }
 }
 
-// A tile's columns 0 .. valid - 1 of this warp's features f0 .. f0 + 31 (TMEM address `d`; zeros
-// unless live) to rows row0 + column.
-__device__ __forceinline__ void store_whole(const Output& o, uint32_t d, bool live, int f0, int64_t row0, int nt,
+// A tile's columns 0 .. valid - 1 of this warp's features f0 .. f0 + 31, those below `end` (TMEM
+// address `d`; zeros unless live), to rows row0 + column.
+__device__ __forceinline__ void store_whole(const Output& o, uint32_t d, bool live, int f0, int end, int64_t row0, int nt,
                                             int valid, uint32_t staging, int lane) {
   if (o.type != LF_F32 && (reinterpret_cast<uintptr_t>(o.data) & 15) == 0 && o.stride % 8 == 0 && o.features % 8 == 0) {
     uint8_t* dst = static_cast<uint8_t*>(o.data) + (row0 * o.stride + f0) * 2;
     for (int c0 = 0; c0 < valid; c0 += 32)
       store_chunk(d + uint32_t(c0), live, staging, o.type == LF_BF16, dst + c0 * o.stride * 2, o.stride * 2, valid - c0,
-                  o.features - f0, lane);
+                  end - f0, lane);
   } else {
     for (int c0 = 0; c0 < nt; c0 += 16) {
       uint32_t r[16];
       if (live) tc_ld16(d + uint32_t(c0), r);
 #pragma unroll
       for (int j = 0; j < 16; ++j)
-        if (f0 + lane < o.features && c0 + j < valid)
+        if (f0 + lane < end && c0 + j < valid)
           store_value(o, (row0 + c0 + j) * o.stride + f0 + lane, live ? __uint_as_float(r[j]) : 0.f);
     }
   }
@@ -385,7 +385,7 @@ __device__ __forceinline__ void store_whole(const Output& o, uint32_t d, bool li
 // `part` [columns][128 features], then every CTA adds a share of the columns over all CTAs in
 // rank order.  `parts`: how often the caller came here before.  False after an expired wait.
 template <typename F>
-__device__ __forceinline__ bool store_split(const Output& o, uint32_t d, bool live, int f0, int64_t row0, int nt,
+__device__ __forceinline__ bool store_split(const Output& o, uint32_t d, bool live, int f0, int end, int64_t row0, int nt,
                                             int valid, float* part, uint64_t* part_full, uint64_t* part_empty,
                                             int parts, int cluster, int rank, int quarter, int lane,
                                             volatile int* abort, F&& release) {
@@ -413,26 +413,39 @@ __device__ __forceinline__ bool store_split(const Output& o, uint32_t d, bool li
 #pragma unroll
     for (int q = 0; q < kMaxSplit; ++q)
       if (q < cluster) sum += v[q];
-    if (f0 + lane < o.features) store_value(o, (row0 + c) * o.stride + f0 + lane, sum);
+    if (f0 + lane < end) store_value(o, (row0 + c) * o.stride + f0 + lane, sum);
   }
   __syncwarp();
   if (lane < cluster) arrive_cluster(mapa(part_empty, lane));
   return true;
 }
 
-// Waves of clusters times a CTA's share of a tile, for a split of S: the least wins, smaller S on
-// a tie.  A share has at least `least_steps` steps.
-inline int choose_split(int64_t tiles, int steps, int least_steps) {
-  int sms = 148, best = 1;
+// How the narrow kernels cut the work: `height` features a tile (the MMA always takes 128 lanes;
+// rows of A past the height are neither loaded nor stored) and the contraction over `split` CTAs.
+struct Cut {
+  int height, split;
+};
+
+// The cut with the least time for `groups` groups of one row tile each and `steps` stages.  What
+// costs is the bytes of the weights a CTA streams, height x stages of 128 bytes at some 44 GB/s:
+// 2.9 ns each, the unit here.  Whole waves count (896 tiles of 128 over 148 CTAs are 7 waves for
+// 6.05 waves' work; 1024 tiles of 112 are 6.9).  A tile costs 0.5 us more, and where a cluster adds
+// up its parts 4 us that only other tiles' loads cover.
+inline Cut choose_cut(int64_t groups, int M, int steps, int least_steps, bool any_height) {
+  int sms = 148;
   sm_count(&sms);
+  Cut best{128, 1};
   double least = 1e30;
-  for (int s = 1; s <= kMaxSplit; s *= 2) {
-    if (s > 1 && steps < least_steps * s) break;
-    const int64_t clusters = sms / s;
-    const double cost = double((tiles + clusters - 1) / clusters) / s;
-    if (cost < 0.95 * least) {
-      least = cost;
-      best = s;
+  for (int s = 1; s <= kMaxSplit && (s == 1 || steps >= least_steps * s); s *= 2) {
+    for (int h = 128; h >= (any_height ? 64 : 128); h -= 8) {
+      const int64_t tiles = groups * ceil_div(M, h), clusters = sms / s;
+      const double waves = double((tiles + clusters - 1) / clusters), joined = s > 1 ? 1400 : 0;
+      const double tile = double(h) * ceil_div(steps, s) + 170;
+      const double cost = waves * (tile > joined ? tile : joined) + joined;
+      if (cost < 0.98 * least) {
+        least = cost;
+        best = {h, s};
+      }
     }
   }
   return best;

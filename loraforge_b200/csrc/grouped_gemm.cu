@@ -55,7 +55,7 @@ struct GParams {
   int E, R, x_rows;
   int M, C;  // output features, contraction (forward K, input N; weight: the groups' rows)
   int N;     // weight: columns of D (dy's features)
-  int elem_bf16, split;
+  int elem_bf16, height, split;
   CUtensorMap a_map;     // forward: W boxes 64 k x 128 n; input: 64 k x 64 n; weight: x boxes 64 k x 64 rows
   CUtensorMap a_small;   // weight: 64 k x 8 rows
   CUtensorMap a_gather;  // weight: single x rows of 64 k
@@ -87,7 +87,7 @@ __device__ __forceinline__ uint32_t instruction(int bf16, int a_mn, int b_mn, in
 }
 
 struct Tile {
-  int e, m0, n0, nt, valid, steps;  // n0: first row (forward, input) or feature of dy; valid columns
+  int e, m0, end, n0, nt, valid, steps;  // features m0 .. end - 1; n0: first row (forward, input) or feature of dy; valid columns
   int lo, hi;                       // the group's rows
 };
 
@@ -97,12 +97,13 @@ __device__ __forceinline__ Tile tile_of(const GParams& p, const int* bounds, con
   x.e = group_of(starts, p.E, t);
   x.lo = bounds[x.e];
   x.hi = bounds[x.e + 1];
-  const int mt = ceil_div(p.M, 128 * kCtas);
+  const int mt = ceil_div(p.M, p.height * kCtas);
   const int columns = kMode == kWeight ? p.N : x.hi - x.lo;
   const int nt = ceil_div(columns, kNT);
   int m, n;
   place_tile(t - starts[x.e], mt, nt, &m, &n);
-  x.m0 = m * 128 * kCtas;
+  x.m0 = m * p.height * kCtas;
+  x.end = min(p.M, x.m0 + p.height * kCtas);
   if (kMode == kWeight) {
     x.n0 = n * kNT;
     x.valid = min(kNT, p.N - x.n0);
@@ -160,7 +161,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(const __grid_const
   }
   if (warp == 1) alloc_tmem<kCtas>(tslot, S::kColumns);
   pdl_wait();
-  const int mtiles = ceil_div(p.M, 128 * kCtas);
+  const int mtiles = ceil_div(p.M, p.height * kCtas);
   list_tiles(p.offsets, p.E, p.R, bounds, starts, scan, [&](int rows) {
     return mtiles * ceil_div(kMode == kWeight ? p.N : rows, kNT);
   });
@@ -207,7 +208,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(const __grid_const
         }
       }
       const bool boxed = kMode != kWeight && !(kMode == kForward && kCtas == 1 && p.rows);
-      const uint32_t whole = kCtas * (kABytes + uint32_t(boxed ? round_up(share, 16) : share) * 128u);
+      const uint32_t whole = kCtas * (uint32_t(p.height) * 128u + uint32_t(boxed ? round_up(share, 16) : share) * 128u);
       bool ok = true;
       for (int ks = ks0; ks < ks1; ++ks, ++it) {
         const int st = it % kStages;
@@ -335,12 +336,12 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(const __grid_const
         }
       };
       if (kCtas == 1 && cluster > 1) {
-        if (!store_split(p.out, d, live, f0, row0, x.nt, x.valid, part, part_full, part_empty, parts, cluster, rank,
+        if (!store_split(p.out, d, live, f0, x.end, row0, x.nt, x.valid, part, part_full, part_empty, parts, cluster, rank,
                          quarter, lane, abort, release))
           break;
         ++parts;
       } else {
-        store_whole(p.out, d, live, f0, row0, x.nt, x.valid, staging, lane);
+        store_whole(p.out, d, live, f0, x.end, row0, x.nt, x.valid, staging, lane);
         release();
       }
     }
@@ -461,16 +462,25 @@ CUtensorMapDataType map_type(int dtype) {
   return dtype == LF_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
 }
 
+struct Weights {
+  const void* data;
+  int64_t K, N, row_stride, expert_stride;
+};
+
 template <int kMode>
-int launch_rows(GParams& p, void* stream, const char* what) {
+int launch_rows(GParams& p, CUtensorMapDataType type, const Weights& w, void* stream, const char* what) {
   const int64_t groups = p.E < p.R ? p.E : p.R;
   if (narrow(p.E, p.R)) {
-    const int64_t mt = ceil_div(p.M, 128);
-    const int64_t tiles = mt * (groups + p.R / kNarrowRows);  // at most
-    p.split = choose_split(mt * groups, ceil_div(p.C, kStep), 4);
+    const Cut cut = choose_cut(groups, p.M, ceil_div(p.C, kStep), 4, kMode == kForward);  // input: boxes of 64 features
+    p.height = cut.height, p.split = cut.split;
+    if (kMode == kForward && !encode_weights(&p.a_map, type, w.data, w.K, w.N, p.E, w.row_stride, w.expert_stride, cut.height))
+      return fail(LF_E_CUDA, (std::string(what) + ": cuTensorMapEncodeTiled failed").c_str());
+    const int64_t tiles = ceil_div(p.M, cut.height) * (groups + p.R / kNarrowRows);  // at most
     return launch_grouped<kMode, 1, kNarrowRows>(p, tiles, stream, what);
   }
-  p.split = 1;
+  p.height = 128, p.split = 1;
+  if (kMode == kForward && !encode_weights(&p.a_map, type, w.data, w.K, w.N, p.E, w.row_stride, w.expert_stride, 128))
+    return fail(LF_E_CUDA, (std::string(what) + ": cuTensorMapEncodeTiled failed").c_str());
   const int64_t tiles = int64_t(ceil_div(p.M, 256)) * (groups + p.R / kWideRows);
   return launch_grouped<kMode, 2, kWideRows>(p, tiles, stream, what);
 }
@@ -523,11 +533,10 @@ extern "C" int lf_expert_linear(int32_t dtype, const void* x, int64_t x_stride, 
   p.E = num_experts, p.R = int(num_rows), p.x_rows = int(x_rows);
   p.M = int(out_width), p.C = int(width), p.elem_bf16 = dtype == LF_BF16;
   const CUtensorMapDataType type = map_type(dtype);
-  if (!encode_weights(&p.a_map, type, w, width, out_width, num_experts, w_row_stride, w_expert_stride, 128) ||
-      (rows ? !encode_rows(&p.b_gather, type, x, width, x_rows, x_stride, 1)
+  if ((rows ? !encode_rows(&p.b_gather, type, x, width, x_rows, x_stride, 1)
             : !encode_row_boxes(p.b_rows, type, x, width, x_rows, x_stride, narrow(num_experts, num_rows))))
     return fail(LF_E_CUDA, "expert_linear: cuTensorMapEncodeTiled failed");
-  return launch_rows<kForward>(p, stream, what);
+  return launch_rows<kForward>(p, type, {w, width, out_width, w_row_stride, w_expert_stride}, stream, what);
 }
 
 extern "C" int lf_expert_linear_input_grad(int32_t dtype, const void* dy, int64_t dy_stride, const void* w,
@@ -548,7 +557,7 @@ extern "C" int lf_expert_linear_input_grad(int32_t dtype, const void* dy, int64_
   if (!encode_weights(&p.a_map, type, w, width, out_width, num_experts, w_row_stride, w_expert_stride, 64) ||
       !encode_row_boxes(p.b_rows, type, dy, out_width, num_rows, dy_stride, narrow(num_experts, num_rows)))
     return fail(LF_E_CUDA, "expert_linear_input_grad: cuTensorMapEncodeTiled failed");
-  return launch_rows<kInput>(p, stream, what);
+  return launch_rows<kInput>(p, type, {w, width, out_width, w_row_stride, w_expert_stride}, stream, what);
 }
 
 extern "C" int lf_expert_linear_weight_grad(int32_t dtype, const void* dy, int64_t dy_stride, const void* x,
@@ -577,7 +586,7 @@ extern "C" int lf_expert_linear_weight_grad(int32_t dtype, const void* dy, int64
   GParams p{};
   p.offsets = offsets, p.out = {dw, width, int(width), out_dtype};
   p.E = num_experts, p.R = int(num_rows), p.x_rows = int(x_rows);
-  p.M = int(width), p.N = int(out_width), p.elem_bf16 = dtype == LF_BF16, p.split = 1;
+  p.M = int(width), p.N = int(out_width), p.elem_bf16 = dtype == LF_BF16, p.height = 128, p.split = 1;
   const CUtensorMapDataType type = map_type(dtype);
   if (!encode_rows(&p.a_map, type, x, width, x_rows, x_stride, 64) ||
       !encode_rows(&p.a_small, type, x, width, x_rows, x_stride, 8) ||

@@ -50,7 +50,7 @@ struct MxParams {
   const uint8_t* w_blocks;  // wide: packed scales
   const uint8_t* x_blocks;
   int groups;            // of 128 codes in them, an even number
-  int split;
+  int height, split;
   CUtensorMap w_map;      // 128 bytes x 128 rows
   CUtensorMap x_map[7];   // 128 bytes x 16, 32, .. 112 rows
   CUtensorMap x_gather;   // single rows
@@ -112,7 +112,7 @@ __device__ __forceinline__ void arrive_cluster_relaxed(uint32_t bar) {
 }
 
 struct Tile {
-  int e, m0, n0, nt, valid, hi;
+  int e, m0, end, n0, nt, valid, hi;
   int row_tile;  // among the row tiles of all groups
 };
 
@@ -122,11 +122,12 @@ __device__ __forceinline__ Tile tile_of(const MxParams& p, const int* bounds, co
   x.e = group_of(starts, p.E, t);
   const int lo = bounds[x.e];
   x.hi = bounds[x.e + 1];
-  const int mt = ceil_div(p.N, 128 * kCtas), nt = ceil_div(x.hi - lo, kNT);
+  const int mt = ceil_div(p.N, p.height * kCtas), nt = ceil_div(x.hi - lo, kNT);
   int m, n;
   place_tile(t - starts[x.e], mt, nt, &m, &n);
   x.row_tile = starts[x.e] / mt + n;
-  x.m0 = m * 128 * kCtas;
+  x.m0 = m * p.height * kCtas;
+  x.end = min(p.N, x.m0 + p.height * kCtas);
   const int each = round_up(ceil_div(x.hi - lo, nt), 16);
   x.n0 = lo + n * each;
   x.valid = min(each, x.hi - x.n0);
@@ -202,7 +203,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
   }
   if (warp == 1) alloc_tmem<kCtas>(tslot, S::kColumns);
   pdl_wait();
-  const int mtiles = ceil_div(p.N, 128 * kCtas);
+  const int mtiles = ceil_div(p.N, p.height * kCtas);
   list_tiles(p.offsets, p.E, p.R, bounds, starts, scan, [&](int rows) { return mtiles * ceil_div(rows, kNT); });
   tc_fence_before();
   __syncthreads();
@@ -241,7 +242,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
           row4[i] = src >= 0 && src < p.x_rows ? src : p.x_rows;
         }
       }
-      const uint32_t bytes = kCtas * (kABytes + uint32_t(by_row ? share : round_up(share, 16)) * 128u);
+      const uint32_t bytes = kCtas * (uint32_t(p.height) * 128u + uint32_t(by_row ? share : round_up(share, 16)) * 128u);
       bool ok = true;
       for (int ks = ks0; ks < ks1; ++ks, ++it) {
         const int st = it % kStages;
@@ -338,11 +339,11 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
         }
       };
       if (kCtas == 1 && cluster > 1) {
-        if (!store_split(p.out, d, live, f0, x.n0, x.nt, x.valid, part, part_full, part_empty, count, cluster, rank,
+        if (!store_split(p.out, d, live, f0, x.end, x.n0, x.nt, x.valid, part, part_full, part_empty, count, cluster, rank,
                          quarter, lane, abort, release))
           break;
       } else {
-        store_whole(p.out, d, live, f0, x.n0, x.nt, x.valid, staging, lane);
+        store_whole(p.out, d, live, f0, x.end, x.n0, x.nt, x.valid, staging, lane);
         release();
       }
     }
@@ -376,7 +377,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
       auto rows_of = [&](int t) {
         const Tile x = tile_of<kCtas, kNT>(p, bounds, starts, t);
         const int n = x.m0 + i, r = x.n0 + i;
-        row[0] = n < p.N ? p.w_scales + (int64_t(x.e) * p.N + n) * p.blocks : nullptr;
+        row[0] = n < x.end ? p.w_scales + (int64_t(x.e) * p.N + n) * p.blocks : nullptr;
         const int src = i < x.valid ? (p.rows ? p.rows[r] : r) : -1;
         row[1] = src >= 0 && src < p.x_rows ? p.x_scales + int64_t(src) * p.blocks : nullptr;
       };
@@ -645,19 +646,16 @@ extern "C" int lf_expert_linear_mxfp4(int32_t out_dtype, const uint8_t* x_codes,
   }
   const cuuint64_t dims[3] = {cuuint64_t(width / 2), cuuint64_t(out_width), cuuint64_t(num_experts)};
   const cuuint64_t strides[2] = {cuuint64_t(width / 2), cuuint64_t(width / 2) * cuuint64_t(out_width)};
-  const cuuint32_t box[3] = {128, 128, 1};
+  const int64_t groups = num_experts < num_rows ? num_experts : num_rows;
+  const Cut cut = few ? choose_cut(groups, p.N, ceil_div(p.K, kStep), kSuper, true) : Cut{128, 1};
+  p.height = cut.height, p.split = cut.split;
+  const cuuint32_t box[3] = {128, cuuint32_t(cut.height), 1};
   bool ok = encode_map(&p.w_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, w_codes, dims, strides, box);
   if (rows && few) ok = ok && encode_codes(&p.x_gather, x_codes, width / 2, code_rows, 1);
   else
     for (int i = 0; i < (few ? kNarrowRows / 16 : 7) && ok; ++i)
       ok = encode_codes(&p.x_map[i], x_codes, width / 2, code_rows, 16 * (i + 1));
   if (!ok) return fail(LF_E_CUDA, "expert_linear_mxfp4: cuTensorMapEncodeTiled failed");
-  const int64_t groups = num_experts < num_rows ? num_experts : num_rows;
-  if (few) {
-    const int64_t mt = ceil_div(p.N, 128);
-    p.split = choose_split(mt * groups, ceil_div(p.K, kStep), kSuper);
-    return launch_mx<1, kNarrowRows>(p, mt * (groups + num_rows / kNarrowRows), stream);
-  }
-  p.split = 1;
+  if (few) return launch_mx<1, kNarrowRows>(p, ceil_div(p.N, cut.height) * (groups + num_rows / kNarrowRows), stream);
   return launch_mx<2, kWideRows>(p, int64_t(ceil_div(p.N, 256)) * (groups + num_rows / kWideRows), stream);
 }
