@@ -15,7 +15,7 @@
 // Scales.  The tensor core wants them in TMEM: for 128 operand rows and 128 codes a row, four
 // columns in which lane l of column j holds the four bytes of row 32 j + l, the same in every
 // quarter of the lanes.  Four warps, one a quarter, bring them there from blocks of 512 bytes in
-// shared memory, to four sets of columns in turn (a stage each), and tell the MMA thread.
+// shared memory, to several sets of columns in turn (a stage each), and tell the MMA thread.
 // tcgen05.cp would do that without them, but each copy of a block holds up the MMAs for some 33 ns,
 // six of them near 0.2 us a wide stage whose MMAs take 0.22.  The blocks of a stage come
 //   wide    by bulk copies, from blocks that pack_kernel laid out in the workspace before (scales
@@ -36,7 +36,6 @@ using namespace grouped;
 constexpr int kThreads = 320;
 constexpr int kStep = 256;           // codes per stage: 128 bytes a row
 constexpr int kABytes = 128 * 128;
-constexpr int kSets = 4;             // sets of TMEM columns that the stages' scales go to in turn
 constexpr int kSuper = 4;            // stages whose scales a thread loads at once (32 bytes a row)
 
 struct MxParams {
@@ -64,7 +63,8 @@ struct Shape {
   static constexpr int kStageBytes = (kABytes + kBRows * 128 + kScaleBytes + 1023) / 1024 * 1024;
   static constexpr int kPartBytes = kCtas == 1 ? kNT * 128 * 4 : 4 * kChunkBytes;
   static constexpr int kStages = kCtas == 2 ? 6 : 7;
-  static constexpr int kScaleColumns = 2 * (4 + 4 * kHalves);    // a set
+  static constexpr int kScaleColumns = 2 * (4 + 4 * kHalves);    // a set of TMEM columns for a stage's scales
+  static constexpr int kSets = kCtas == 2 ? 4 : kStages;         // that the stages use in turn
   static constexpr int kColumns = kCtas == 2 ? 512 : 256;        // TMEM
   static_assert(2 * kNT + kSets * kScaleColumns <= kColumns, "TMEM");
 };
@@ -160,7 +160,7 @@ __device__ __forceinline__ void load_scales(const uint8_t* row, int k0, int bloc
 template <int kCtas, int kNT>
 __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__ MxParams p) {
   using S = Shape<kCtas, kNT>;
-  constexpr int kStages = S::kStages;
+  constexpr int kStages = S::kStages, kSets = S::kSets;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align1024(smem_raw);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -408,10 +408,10 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
         }
         if (t < tiles) load(k0);
 #pragma unroll
-        for (int j = 0; j < kSuper; ++j) {
+        for (int j = 0; j < kSuper; ++j) {  // all four stages' blocks first: one exchange's latency for four
           if (j >= todo || !ok) continue;
-          const int st = it % kStages;
-          ok = __all_sync(0xffffffffu, wait_or_abort(&empty[st], (uint32_t(it / kStages) & 1u) ^ 1u, abort));
+          const int st = (it + j) % kStages;
+          ok = __all_sync(0xffffffffu, wait_or_abort(&empty[st], (uint32_t((it + j) / kStages) & 1u) ^ 1u, abort));
           const uint32_t sc = smem_u32(ring + st * S::kStageBytes) + kABytes + S::kBRows * 128 +
                               uint32_t((i & 31) * 16 + (i >> 5) * 4);
 #pragma unroll
@@ -422,9 +422,8 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
           }
           __syncwarp();
           if (lane == 0) mbar_arrive(&blocks_full[st]);
-          ok = ok && to_tmem(it);
-          ++it;
         }
+        for (int j = 0; j < todo && ok; ++j, ++it) ok = to_tmem(it);
         ok = ok && t < tiles;
       }
     }
