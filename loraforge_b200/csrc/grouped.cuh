@@ -20,6 +20,11 @@ using namespace tc;
 constexpr int kMaxExperts = 1024;
 constexpr int kMaxWarps = 10;
 
+// Stages that fit beside `other` bytes of shared memory (and the tables of kMaxExperts groups).
+constexpr int stages_of(int stage_bytes, int other) {
+  return (227 * 1024 - 1024 - 512 - 4 * (kMaxWarps + 2 + 2 * (kMaxExperts + 1)) - other) / stage_bytes;
+}
+
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // ------------------------------------------------------------------ clusters

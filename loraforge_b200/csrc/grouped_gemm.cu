@@ -29,8 +29,8 @@
 // grid is persistent and computes its tile list from `offsets` on the device.
 //
 //   wide    CTA pairs (cta_group::2), 256 x 256 tiles: each CTA loads half of both operands.
-//   narrow  one CTA, 128 features x up to 64 rows, for groups of few rows, where the weights'
-//           bytes are the cost; the contraction can be split over a cluster of CTAs, whose
+//   narrow  one CTA, up to 128 features x up to 32 or 64 rows, for groups of few rows, where the
+//           weights' bytes are the cost (32: four more stages for the weights in flight); the contraction can be split over a cluster of CTAs, whose
 //           partial sums are added in rank order through distributed shared memory.
 //
 // Every wait is bounded (tma.cuh): an expiry stops every role at its next wait.
@@ -70,7 +70,7 @@ struct Shape {
   static constexpr int kBRows = kNT / kCtas;  // a CTA's share of the columns
   static constexpr int kStageBytes = kABytes + kBRows * 128;
   static constexpr int kPartBytes = kCtas == 1 ? kNT * 128 * 4 : 4 * kChunkBytes;  // sums, or the stores' staging
-  static constexpr int kStages = 6;
+  static constexpr int kStages = stages_of(kStageBytes, kPartBytes);  // what is in flight hides some 2 us a load
   static constexpr int kColumns = 2 * kNT;  // TMEM
 };
 
@@ -208,7 +208,8 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(const __grid_const
         }
       }
       const bool boxed = kMode != kWeight && !(kMode == kForward && kCtas == 1 && p.rows);
-      const uint32_t whole = kCtas * (uint32_t(p.height) * 128u + uint32_t(boxed ? round_up(share, 16) : share) * 128u);
+      const int loaded = kMode == kWeight ? share : boxed ? round_up(share, 16) : round_up(x.valid, 4);
+      const uint32_t whole = kCtas * uint32_t(p.height + loaded) * 128u;
       bool ok = true;
       for (int ks = ks0; ks < ks1; ++ks, ++it) {
         const int st = it % kStages;
@@ -251,7 +252,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(const __grid_const
             load_3d<kCtas>(a + lane * 8192, &p.a_map, m_cta + 64 * lane, c, x.e, bar);
           }
           if (kMode == kForward && kCtas == 1 && p.rows) {
-            if (4 * lane < share) gather4<kCtas>(b + lane * 512, &p.b_gather, c, row4, bar);
+            if (4 * lane < x.valid) gather4<kCtas>(b + lane * 512, &p.b_gather, c, row4, bar);
           } else {
             // One box of the share's rows in steps of 16: small boxes cost the copy engine near
             // 0.1 us each, whatever their size (rows past the share are loaded and not used).
@@ -404,13 +405,13 @@ int launch_grouped(const GParams& p, int64_t tiles, void* stream, const char* wh
   const int cluster = kCtas == 2 ? 2 : p.split;
   int64_t grid = int64_t(sms / cluster) * cluster;
   if (tiles * cluster < grid) grid = tiles * cluster;
-  const int smem = 1024 + S::kStages * S::kStageBytes + S::kPartBytes + 256 + int(sizeof(int)) * (8 + 2 * (p.E + 1));
+  const int smem = 1024 + S::kStages * S::kStageBytes + S::kPartBytes + 512 + int(sizeof(int)) * (kMaxWarps + 2 + 2 * (p.E + 1));
   static int flags[64] = {};
   if (int rc = ensure_smem(grouped_kernel<kMode, kCtas, kNT>, smem, flags)) return rc;
   return launch_clusters(grouped_kernel<kMode, kCtas, kNT>, int(grid), kThreads, cluster, smem, stream, what, p);
 }
 
-constexpr int kWideRows = 256, kNarrowRows = 64;
+constexpr int kWideRows = 256, kNarrowRows = 64, kFewRows = 32;
 constexpr char kNoWorkspace[] = "expert_linear: workspace missing, too small or not 16-byte aligned (see lf_expert_linear_workspace_bytes)";
 
 // Groups of up to 64 rows on average take the narrow tiles.
@@ -426,7 +427,7 @@ int check_sizes(const char* what, int dtype, int E, int64_t R, int64_t N, int64_
                 (std::string(what) + ": needs 1..1024 experts, widths that are multiples of 8, and rows that fit int32").c_str());
   // Tiles are counted in int32, also those of narrow tiles.
   const int64_t m = (N > K ? N : K) / 128 + 1;
-  if ((R / kNarrowRows + E + 1) * m >= limit || (N / kWideRows + 1) * (K / 256 + 1) * int64_t(E) >= limit)
+  if ((R / kFewRows + E + 1) * m >= limit || (N / kWideRows + 1) * (K / 256 + 1) * int64_t(E) >= limit)
     return fail(LF_E_INVALID, (std::string(what) + ": too many tiles").c_str());
   return LF_OK;
 }
@@ -475,8 +476,9 @@ int launch_rows(GParams& p, CUtensorMapDataType type, const Weights& w, void* st
     p.height = cut.height, p.split = cut.split;
     if (kMode == kForward && !encode_weights(&p.a_map, type, w.data, w.K, w.N, p.E, w.row_stride, w.expert_stride, cut.height))
       return fail(LF_E_CUDA, (std::string(what) + ": cuTensorMapEncodeTiled failed").c_str());
-    const int64_t tiles = ceil_div(p.M, cut.height) * (groups + p.R / kNarrowRows);  // at most
-    return launch_grouped<kMode, 1, kNarrowRows>(p, tiles, stream, what);
+    const int64_t mt = ceil_div(p.M, cut.height);  // tiles: at most
+    if (p.R <= kFewRows / 2 * groups) return launch_grouped<kMode, 1, kFewRows>(p, mt * (groups + p.R / kFewRows), stream, what);
+    return launch_grouped<kMode, 1, kNarrowRows>(p, mt * (groups + p.R / kNarrowRows), stream, what);
   }
   p.height = 128, p.split = 1;
   if (kMode == kForward && !encode_weights(&p.a_map, type, w.data, w.K, w.N, p.E, w.row_stride, w.expert_stride, 128))

@@ -8,20 +8,24 @@
 // in FP32; a product of two codes and two powers of two is exact.
 //
 // The tiles are those of the 16-bit products (grouped_gemm.cu): features on the TMEM lanes,
-// rows on the columns, CTA pairs with 256 features x up to 208 rows, or single CTAs with 128 x
-// 64 whose contraction may be split over a cluster.  208, not 256, rows: two accumulators of 208
+// rows on the columns, CTA pairs with 256 features x up to 208 rows, or single CTAs with up to
+// 128 x 32 or 64 whose contraction may be split over a cluster.  208, not 256, rows: two accumulators of 208
 // columns leave 96 TMEM columns for four sets of scales.
 //
 // Scales.  The tensor core wants them in TMEM: for 128 operand rows and 128 codes a row, four
 // columns in which lane l of column j holds the four bytes of row 32 j + l, the same in every
-// quarter of the lanes.  Four warps, one a quarter, bring them there from blocks of 512 bytes in
-// shared memory, to several sets of columns in turn (a stage each), and tell the MMA thread.
-// tcgen05.cp would do that without them, but each copy of a block holds up the MMAs for some 33 ns,
-// six of them near 0.2 us a wide stage whose MMAs take 0.22.  The blocks of a stage come
-//   wide    by bulk copies, from blocks that pack_kernel laid out in the workspace before (scales
-//           of 28672 x 4096 weights: 3.7 MB each way);
-//   narrow  from the same four warps, which read them row by row: 32 bytes of a row (a whole
-//           sector) for a thread and four stages, one such group ahead, also across tiles.
+// quarter of the lanes.  Four warps, one a quarter, write them there, to several sets of columns
+// in turn (a stage each), and tell the MMA thread.  tcgen05.cp would do that without them, but each
+// copy of 512 bytes holds up the MMAs for some 33 ns, six of them near 0.2 us a wide stage whose
+// MMAs take 0.22.
+//   wide    the warps read them from shared memory, where a stage's come by bulk copies from
+//           blocks that pack_kernel laid out in the workspace before (the scales of
+//           28672 x 4096 weights: 3.7 MB each way).  Row by row from global memory, the warps
+//           were slower than the MMAs.
+//   narrow  every warp reads all rows itself (three of four times from a cache): 32 bytes, a
+//           whole sector, of each row for four stages, one such group ahead, also across tiles,
+//           and up to 16 stages before the MMAs.  W's are asked into L2 a tile before: from HBM
+//           under load they took some 2 us, 0.45 a stage, where the codes need 0.33.
 //
 // Per CTA: warp 0 loads (TMA), warp 1 MMA and TMEM, warps 2-5 store, warps 6-9 scales.
 // Every wait is bounded (tma.cuh): an expiry stops every role at its next wait.
@@ -59,13 +63,13 @@ template <int kCtas, int kNT>
 struct Shape {
   static constexpr int kBRows = round_up(kNT / kCtas, 16);  // a CTA's share of the rows, loaded by 16
   static constexpr int kHalves = (kNT + 127) / 128;              // scale blocks of 128 rows of x
-  static constexpr int kScaleBytes = 2 * 512 * (1 + kHalves);    // two groups of 128 codes a stage
+  static constexpr int kScaleBytes = kCtas == 2 ? 2 * 512 * (1 + kHalves) : 0;  // blocks of two groups of 128 codes
   static constexpr int kStageBytes = (kABytes + kBRows * 128 + kScaleBytes + 1023) / 1024 * 1024;
   static constexpr int kPartBytes = kCtas == 1 ? kNT * 128 * 4 : 4 * kChunkBytes;
-  static constexpr int kStages = kCtas == 2 ? 6 : 7;
-  static constexpr int kScaleColumns = 2 * (4 + 4 * kHalves);    // a set of TMEM columns for a stage's scales
-  static constexpr int kSets = kCtas == 2 ? 4 : kStages;         // that the stages use in turn
-  static constexpr int kColumns = kCtas == 2 ? 512 : 256;        // TMEM
+  static constexpr int kStages = stages_of(kStageBytes, kPartBytes);
+  static constexpr int kScaleColumns = 2 * (4 + 4 * kHalves);  // a set of TMEM columns for a stage's scales
+  static constexpr int kSets = kCtas == 2 ? 4 : 16;            // that the stages use in turn
+  static constexpr int kColumns = 512;                         // TMEM
   static_assert(2 * kNT + kSets * kScaleColumns <= kColumns, "TMEM");
 };
 
@@ -170,9 +174,10 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
   uint64_t* empty = full + kStages;
   uint64_t* acc_full = empty + kStages;
   uint64_t* acc_empty = acc_full + 2;
-  uint64_t* blocks_full = acc_empty + 2;      // a stage's scale blocks are here
+  uint64_t* blocks_full = acc_empty + 2;      // wide: a stage's scale blocks are here
   uint64_t* set_full = blocks_full + kStages;  // a set of scale columns is written, in both CTAs
-  uint64_t* part_full = set_full + kSets;
+  uint64_t* set_done = set_full + kSets;       // narrow: the MMAs are done with it
+  uint64_t* part_full = set_done + kSets;
   uint64_t* part_empty = part_full + 1;
   uint64_t* fin = part_empty + 1;
   uint32_t* tslot = reinterpret_cast<uint32_t*>(fin + 1);
@@ -188,13 +193,16 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
-      mbar_init(&blocks_full[i], kCtas == 2 ? 1 : 4);  // the copies' bytes, or the four warps that write them
+      mbar_init(&blocks_full[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&acc_full[i], 1);
       mbar_init(&acc_empty[i], 4 * kCtas);
     }
-    for (int i = 0; i < kSets; ++i) mbar_init(&set_full[i], 4 * kCtas);
+    for (int i = 0; i < kSets; ++i) {
+      mbar_init(&set_full[i], 4 * kCtas);
+      mbar_init(&set_done[i], 1);
+    }
     mbar_init(part_full, 4 * cluster);
     mbar_init(part_empty, 4 * cluster);
     mbar_init(fin, 1);
@@ -242,7 +250,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
           row4[i] = src >= 0 && src < p.x_rows ? src : p.x_rows;
         }
       }
-      const uint32_t bytes = kCtas * (uint32_t(p.height) * 128u + uint32_t(by_row ? share : round_up(share, 16)) * 128u);
+      const uint32_t bytes = kCtas * uint32_t(p.height + (by_row ? round_up(x.valid, 4) : round_up(share, 16))) * 128u;
       bool ok = true;
       for (int ks = ks0; ks < ks1; ++ks, ++it) {
         const int st = it % kStages;
@@ -262,7 +270,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
           bulk_g2s(sc + 1024, p.x_blocks + (int64_t(x.row_tile) * p.groups + 2 * ks) * 1024, 2048, &blocks_full[st]);
         }
         if (by_row) {
-          if (4 * lane < share) gather4<kCtas>(b + lane * 512, &p.x_gather, c, row4, bar);
+          if (4 * lane < x.valid) gather4<kCtas>(b + lane * 512, &p.x_gather, c, row4, bar);
         } else {
           // One box of the share's rows in steps of 16: small boxes cost the copy engine near
           // 0.1 us each, whatever their size (rows past the share are loaded and not used).
@@ -306,6 +314,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
             mma_mxf4<kCtas>(d, ad + 2 * k, bd + 2 * k, k & 1 ? idesc1 : idesc0, ts + 4 * (k >> 1),
                             ts + 8 + 4 * S::kHalves * (k >> 1), (ks > ks0 || k > 0) ? 1u : 0u);
           commit<kCtas>(&empty[st]);
+          if (kCtas == 1) commit<kCtas>(&set_done[set]);
         }
         if (!ok) break;
         commit<kCtas>(&acc_full[ab]);
@@ -350,41 +359,50 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
   } else {
     // ------------------------------------------------------------ scales
     const uint32_t quarter_set = tmem + (uint32_t((warp & 3) * 32) << 16) + uint32_t(2 * kNT);
-    // Stage `it`'s blocks to its set of columns, once the MMAs of kSets stages ago are done with it.
-    auto to_tmem = [&](int it) {
-      const int before = it - kSets;
-      bool ready = wait_or_abort(&blocks_full[it % kStages], uint32_t(it / kStages) & 1u, abort);
-      if (before >= 0) ready = ready && wait_or_abort(&empty[before % kStages], uint32_t(before / kStages) & 1u, abort);
-      if (!__all_sync(0xffffffffu, ready)) return false;
-      tc_fence_after();
-      store_scales<2 * (1 + S::kHalves)>(quarter_set + uint32_t(it % kSets * S::kScaleColumns),
-                                         smem_u32(ring + it % kStages * S::kStageBytes) + kABytes + S::kBRows * 128, lane);
-      tc_fence_before();
-      if (lane == 0) {
-        if (kCtas == 2) arrive_cluster_relaxed(mapa(&set_full[it % kSets], 0));
-        else mbar_arrive(&set_full[it % kSets]);
-      }
-      return true;
-    };
     if constexpr (kCtas == 2) {
-      const int mine = live && first < tiles ? (tiles - first + stride - 1) / stride : 0;
-      for (int it = 0; it < mine * (ks1 - ks0); ++it)
-        if (!to_tmem(it)) break;
+      const int mine = first < tiles ? (tiles - first + stride - 1) / stride : 0;
+      for (int it = 0; it < mine * steps; ++it) {
+        const int before = it - kSets, st = it % kStages, set = it % kSets;
+        bool ready = wait_or_abort(&blocks_full[st], uint32_t(it / kStages) & 1u, abort);
+        if (before >= 0) ready = ready && wait_or_abort(&empty[before % kStages], uint32_t(before / kStages) & 1u, abort);
+        if (!__all_sync(0xffffffffu, ready)) break;
+        tc_fence_after();
+        store_scales<2 * (1 + S::kHalves)>(quarter_set + uint32_t(set * S::kScaleColumns),
+                                           smem_u32(ring + st * S::kStageBytes) + kABytes + S::kBRows * 128, lane);
+        tc_fence_before();
+        if (lane == 0) arrive_cluster_relaxed(mapa(&set_full[set], 0));
+      }
     } else {
-      constexpr int kRows = 2;  // rows a thread reads: one of W and one of the tile's
-      const int i = tid - 192;
-      const uint8_t* row[kRows] = {nullptr, nullptr};
+      constexpr int kXRows = kNT / 32;
+      const uint8_t *w_row[4], *x_row[kXRows];  // this lane's of every 32 rows
+      const uint8_t* ahead = nullptr;            // one of W's rows a tile later
       auto rows_of = [&](int t) {
+        ahead = nullptr;
+        if (t + stride < tiles) {
+          const Tile y = tile_of<kCtas, kNT>(p, bounds, starts, t + stride);
+          const int n = y.m0 + 32 * (warp & 3) + lane;
+          if (n < y.end) ahead = p.w_scales + (int64_t(y.e) * p.N + n) * p.blocks;
+        }
         const Tile x = tile_of<kCtas, kNT>(p, bounds, starts, t);
-        const int n = x.m0 + i, r = x.n0 + i;
-        row[0] = n < x.end ? p.w_scales + (int64_t(x.e) * p.N + n) * p.blocks : nullptr;
-        const int src = i < x.valid ? (p.rows ? p.rows[r] : r) : -1;
-        row[1] = src >= 0 && src < p.x_rows ? p.x_scales + int64_t(src) * p.blocks : nullptr;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int n = x.m0 + 32 * j + lane;
+          w_row[j] = n < x.end ? p.w_scales + (int64_t(x.e) * p.N + n) * p.blocks : nullptr;
+        }
+#pragma unroll
+        for (int j = 0; j < kXRows; ++j) {
+          const int r = 32 * j + lane;
+          const int src = r < x.valid ? (p.rows ? p.rows[x.n0 + r] : x.n0 + r) : -1;
+          x_row[j] = src >= 0 && src < p.x_rows ? p.x_scales + int64_t(src) * p.blocks : nullptr;
+        }
       };
-      uint32_t next[kRows][8];
+      uint32_t w_next[4][8], x_next[kXRows][8];
       auto load = [&](int k0) {
 #pragma unroll
-        for (int q = 0; q < kRows; ++q) load_scales(row[q], k0 * 8, p.blocks, q ? p.x_align : p.w_align, next[q]);
+        for (int j = 0; j < 4; ++j) load_scales(w_row[j], k0 * 8, p.blocks, p.w_align, w_next[j]);
+#pragma unroll
+        for (int j = 0; j < kXRows; ++j) load_scales(x_row[j], k0 * 8, p.blocks, p.x_align, x_next[j]);
+        if (ahead && k0 * 8 < p.blocks) asm volatile("prefetch.global.L2 [%0];" ::"l"(ahead + k0 * 8));
       };
       int it = 0, t = first, k0 = ks0;
       bool ok = live && t < tiles;
@@ -393,11 +411,13 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
         load(k0);
       }
       while (ok) {
-        uint32_t now[kRows][8];
+        uint32_t w_now[4][8], x_now[kXRows][8];
 #pragma unroll
-        for (int q = 0; q < kRows; ++q) {
+        for (int i = 0; i < 8; ++i) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) now[q][j] = next[q][j];
+          for (int j = 0; j < 4; ++j) w_now[j][i] = w_next[j][i];
+#pragma unroll
+          for (int j = 0; j < kXRows; ++j) x_now[j][i] = x_next[j][i];
         }
         const int todo = min(kSuper, ks1 - k0);
         k0 += kSuper;
@@ -408,22 +428,25 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
         }
         if (t < tiles) load(k0);
 #pragma unroll
-        for (int j = 0; j < kSuper; ++j) {  // all four stages' blocks first: one exchange's latency for four
+        for (int j = 0; j < kSuper; ++j) {
           if (j >= todo || !ok) continue;
-          const int st = (it + j) % kStages;
-          ok = __all_sync(0xffffffffu, wait_or_abort(&empty[st], (uint32_t((it + j) / kStages) & 1u) ^ 1u, abort));
-          const uint32_t sc = smem_u32(ring + st * S::kStageBytes) + kABytes + S::kBRows * 128 +
-                              uint32_t((i & 31) * 16 + (i >> 5) * 4);
-#pragma unroll
-          for (int q = 0; q < kRows; ++q) {
-#pragma unroll
-            for (int g = 0; g < 2; ++g)
-              asm volatile("st.shared.b32 [%0], %1;" ::"r"(sc + uint32_t(2 * q + g) * 512u), "r"(now[q][2 * j + g]) : "memory");
-          }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&blocks_full[st]);
+          const int set = it % kSets;
+          ok = __all_sync(0xffffffffu, wait_or_abort(&set_done[set], (uint32_t(it / kSets) & 1u) ^ 1u, abort));
+          if (!ok) continue;
+          tc_fence_after();
+          // Groups 2 j and 2 j + 1 of W, then of x; columns past the tile's rows are not read.
+          asm volatile(
+              "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %11, %12, "
+              "%13, %14, %14};\n tcgen05.wait::st.sync.aligned;" ::"r"(quarter_set + uint32_t(set * S::kScaleColumns)),
+              "r"(w_now[0][2 * j]), "r"(w_now[1][2 * j]), "r"(w_now[2][2 * j]), "r"(w_now[3][2 * j]),
+              "r"(w_now[0][2 * j + 1]), "r"(w_now[1][2 * j + 1]), "r"(w_now[2][2 * j + 1]), "r"(w_now[3][2 * j + 1]),
+              "r"(x_now[0][2 * j]), "r"(x_now[kXRows - 1][2 * j]), "r"(0), "r"(x_now[0][2 * j + 1]),
+              "r"(x_now[kXRows - 1][2 * j + 1]), "r"(0)
+              : "memory");
+          tc_fence_before();
+          if (lane == 0) mbar_arrive(&set_full[set]);
+          ++it;
         }
-        for (int j = 0; j < todo && ok; ++j, ++it) ok = to_tmem(it);
         ok = ok && t < tiles;
       }
     }
@@ -437,7 +460,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
   }
 }
 
-constexpr int kWideRows = 208, kNarrowRows = 64;
+constexpr int kWideRows = 208, kNarrowRows = 64, kFewRows = 32;
 
 bool narrow(int64_t E, int64_t R) { return R <= kNarrowRows * (E < R ? E : R); }
 
@@ -538,7 +561,7 @@ int launch_mx(const MxParams& p, int64_t tiles, void* stream) {
   const int cluster = kCtas == 2 ? 2 : p.split;
   int64_t grid = int64_t(sms / cluster) * cluster;
   if (tiles * cluster < grid) grid = tiles * cluster;
-  const int smem = 1024 + S::kStages * S::kStageBytes + S::kPartBytes + 256 +
+  const int smem = 1024 + S::kStages * S::kStageBytes + S::kPartBytes + 512 +
                    int(sizeof(int)) * (kMaxWarps + 2 + 2 * (p.E + 1));
   static int flags[64] = {};
   if (int rc = ensure_smem(mx_kernel<kCtas, kNT>, smem, flags)) return rc;
@@ -604,7 +627,7 @@ extern "C" int lf_expert_linear_mxfp4(int32_t out_dtype, const uint8_t* x_codes,
   if (out_dtype < LF_F32 || out_dtype > LF_BF16) return fail(LF_E_INVALID, "expert_linear_mxfp4: unknown output type");
   if (num_experts < 1 || num_experts > kMaxExperts || num_rows < 0 || num_rows >= limit - 256 || out_width < 1 ||
       out_width >= limit - 256 || width < 32 || width % 32 || width >= limit - 256 ||
-      (num_rows / kNarrowRows + num_experts + 1) * (out_width / 128 + 1) >= limit)
+      (num_rows / kFewRows + num_experts + 1) * (out_width / 64 + 1) >= limit)
     return fail(LF_E_INVALID, "expert_linear_mxfp4: needs 1..1024 experts, a width that is a multiple of 32, and rows and tiles that fit int32");
   if (num_rows == 0) return LF_OK;
   if (!x_codes || !x_scales || !w_codes || !w_scales || !offsets || !y || y_stride < out_width || !aligned16(x_codes) ||
@@ -655,6 +678,10 @@ extern "C" int lf_expert_linear_mxfp4(int32_t out_dtype, const uint8_t* x_codes,
     for (int i = 0; i < (few ? kNarrowRows / 16 : 7) && ok; ++i)
       ok = encode_codes(&p.x_map[i], x_codes, width / 2, code_rows, 16 * (i + 1));
   if (!ok) return fail(LF_E_CUDA, "expert_linear_mxfp4: cuTensorMapEncodeTiled failed");
-  if (few) return launch_mx<1, kNarrowRows>(p, ceil_div(p.N, cut.height) * (groups + num_rows / kNarrowRows), stream);
+  if (few) {
+    const int64_t mt = ceil_div(p.N, cut.height);  // tiles: at most
+    if (num_rows <= kFewRows / 2 * groups) return launch_mx<1, kFewRows>(p, mt * (groups + num_rows / kFewRows), stream);
+    return launch_mx<1, kNarrowRows>(p, mt * (groups + num_rows / kNarrowRows), stream);
+  }
   return launch_mx<2, kWideRows>(p, int64_t(ceil_div(p.N, 256)) * (groups + num_rows / kWideRows), stream);
 }
