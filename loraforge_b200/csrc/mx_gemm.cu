@@ -23,9 +23,9 @@
 //           28672 x 4096 weights: 3.7 MB each way).  Row by row from global memory, the warps
 //           were slower than the MMAs.
 //   narrow  every warp reads all rows itself (three of four times from a cache): 32 bytes, a
-//           whole sector, of each row for four stages, one such group ahead, also across tiles,
-//           and up to 16 stages before the MMAs.  W's are asked into L2 a tile before: from HBM
-//           under load they took some 2 us, 0.45 a stage, where the codes need 0.33.
+//           whole sector, of each row for four stages, one such group ahead, also across tiles.
+// A narrow tile's MMAs have N = 32 at least: with 16 they were slower (eight 14336 x 4096 experts,
+// 16 rows: 60 us against 63).
 //
 // Per CTA: warp 0 loads (TMA), warp 1 MMA and TMEM, warps 2-5 store, warps 6-9 scales.
 // Every wait is bounded (tma.cuh): an expiry stops every role at its next wait.
@@ -68,7 +68,7 @@ struct Shape {
   static constexpr int kPartBytes = kCtas == 1 ? kNT * 128 * 4 : 4 * kChunkBytes;
   static constexpr int kStages = stages_of(kStageBytes, kPartBytes);
   static constexpr int kScaleColumns = 2 * (4 + 4 * kHalves);  // a set of TMEM columns for a stage's scales
-  static constexpr int kSets = kCtas == 2 ? 4 : 16;            // that the stages use in turn
+  static constexpr int kSets = kCtas == 2 ? 4 : kStages;       // that the stages use in turn
   static constexpr int kColumns = 512;                         // TMEM
   static_assert(2 * kNT + kSets * kScaleColumns <= kColumns, "TMEM");
 };
@@ -135,7 +135,7 @@ __device__ __forceinline__ Tile tile_of(const MxParams& p, const int* bounds, co
   const int each = round_up(ceil_div(x.hi - lo, nt), 16);
   x.n0 = lo + n * each;
   x.valid = min(each, x.hi - x.n0);
-  x.nt = round_up(x.valid, 16);
+  x.nt = round_up(x.valid, kCtas == 1 ? 32 : 16);
   return x;
 }
 
@@ -176,8 +176,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
   uint64_t* acc_empty = acc_full + 2;
   uint64_t* blocks_full = acc_empty + 2;      // wide: a stage's scale blocks are here
   uint64_t* set_full = blocks_full + kStages;  // a set of scale columns is written, in both CTAs
-  uint64_t* set_done = set_full + kSets;       // narrow: the MMAs are done with it
-  uint64_t* part_full = set_done + kSets;
+  uint64_t* part_full = set_full + kSets;
   uint64_t* part_empty = part_full + 1;
   uint64_t* fin = part_empty + 1;
   uint32_t* tslot = reinterpret_cast<uint32_t*>(fin + 1);
@@ -199,10 +198,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
       mbar_init(&acc_full[i], 1);
       mbar_init(&acc_empty[i], 4 * kCtas);
     }
-    for (int i = 0; i < kSets; ++i) {
-      mbar_init(&set_full[i], 4 * kCtas);
-      mbar_init(&set_done[i], 1);
-    }
+    for (int i = 0; i < kSets; ++i) mbar_init(&set_full[i], 4 * kCtas);
     mbar_init(part_full, 4 * cluster);
     mbar_init(part_empty, 4 * cluster);
     mbar_init(fin, 1);
@@ -238,7 +234,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
     for (int t = first; t < tiles && live; t += stride) {
       const Tile x = tile_of<kCtas, kNT>(p, bounds, starts, t);
       const int m_cta = x.m0 + (kCtas == 2 ? rank * 128 : 0);
-      const int share = x.nt / kCtas;
+      const int share = kCtas == 1 ? x.valid : x.nt / kCtas;
       const int n_cta = x.n0 + (kCtas == 2 ? rank * share : 0);
       const bool by_row = kCtas == 1 && p.rows;
       int row4[4];
@@ -314,7 +310,6 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
             mma_mxf4<kCtas>(d, ad + 2 * k, bd + 2 * k, k & 1 ? idesc1 : idesc0, ts + 4 * (k >> 1),
                             ts + 8 + 4 * S::kHalves * (k >> 1), (ks > ks0 || k > 0) ? 1u : 0u);
           commit<kCtas>(&empty[st]);
-          if (kCtas == 1) commit<kCtas>(&set_done[set]);
         }
         if (!ok) break;
         commit<kCtas>(&acc_full[ab]);
@@ -375,14 +370,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
     } else {
       constexpr int kXRows = kNT / 32;
       const uint8_t *w_row[4], *x_row[kXRows];  // this lane's of every 32 rows
-      const uint8_t* ahead = nullptr;            // one of W's rows a tile later
       auto rows_of = [&](int t) {
-        ahead = nullptr;
-        if (t + stride < tiles) {
-          const Tile y = tile_of<kCtas, kNT>(p, bounds, starts, t + stride);
-          const int n = y.m0 + 32 * (warp & 3) + lane;
-          if (n < y.end) ahead = p.w_scales + (int64_t(y.e) * p.N + n) * p.blocks;
-        }
         const Tile x = tile_of<kCtas, kNT>(p, bounds, starts, t);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -402,7 +390,6 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
         for (int j = 0; j < 4; ++j) load_scales(w_row[j], k0 * 8, p.blocks, p.w_align, w_next[j]);
 #pragma unroll
         for (int j = 0; j < kXRows; ++j) load_scales(x_row[j], k0 * 8, p.blocks, p.x_align, x_next[j]);
-        if (ahead && k0 * 8 < p.blocks) asm volatile("prefetch.global.L2 [%0];" ::"l"(ahead + k0 * 8));
       };
       int it = 0, t = first, k0 = ks0;
       bool ok = live && t < tiles;
@@ -430,8 +417,8 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
 #pragma unroll
         for (int j = 0; j < kSuper; ++j) {
           if (j >= todo || !ok) continue;
-          const int set = it % kSets;
-          ok = __all_sync(0xffffffffu, wait_or_abort(&set_done[set], (uint32_t(it / kSets) & 1u) ^ 1u, abort));
+          const int set = it % kSets;  // free when the MMAs of its stage are done
+          ok = __all_sync(0xffffffffu, wait_or_abort(&empty[set], (uint32_t(it / kSets) & 1u) ^ 1u, abort));
           if (!ok) continue;
           tc_fence_after();
           // Groups 2 j and 2 j + 1 of W, then of x; columns past the tile's rows are not read.
@@ -475,22 +462,44 @@ struct PackParams {
   uint8_t *w_blocks, *x_blocks;
   uint4* codes;
   int E, R, x_rows, N, blocks, groups, words;  // words: 16-byte words of a row of codes
-  int w_tasks, x_tasks, words4;                // CUDA blocks for each part; words4: 4-byte reads of scales allowed
+  int w_tasks, x_tasks;                        // CUDA blocks for each part
+  int align;                                   // 16, 4 or 1: alignment of every row of the scales
 };
 
-__device__ __forceinline__ uint32_t scale_word(const uint8_t* row, int k, int blocks, bool words) {
-  if (!row || k >= blocks) return 0;
-  if (words) return *reinterpret_cast<const uint32_t*>(row + k);
-  uint32_t v = 0;
-  for (int i = 0; i < 4 && k + i < blocks; ++i) v |= uint32_t(row[k + i]) << (8 * i);
-  return v;
+// Four bytes each of groups g .. g + 3 of a row; zeros past it and where row is null.
+__device__ __forceinline__ uint4 scale_words(const uint8_t* row, int g, int blocks, int align) {
+  uint32_t v[4] = {0, 0, 0, 0};
+  const int k = 4 * g;
+  if (!row) return make_uint4(0, 0, 0, 0);
+  if (align == 16 && k + 16 <= blocks) return *reinterpret_cast<const uint4*>(row + k);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (align >= 4) {
+      if (k + 4 * i < blocks) v[i] = *reinterpret_cast<const uint32_t*>(row + k + 4 * i);
+    } else {
+      for (int j = 0; j < 4; ++j)
+        if (k + 4 * i + j < blocks) v[i] |= uint32_t(row[k + 4 * i + j]) << (8 * j);
+    }
+  }
+  return make_uint4(v[0], v[1], v[2], v[3]);
+}
+
+// Blocks of groups g .. g + 3 (`pitch` uint4 apart, those below `groups`): lane l takes rows l, l + 32,
+// l + 64 and l + 96, 16 bytes of each, and writes their words for each group.
+__device__ __forceinline__ void pack_groups(const uint8_t* const (&row)[4], int g, int blocks, int align, int groups,
+                                            uint4* out, int pitch) {
+  const uint4 a = scale_words(row[0], g, blocks, align), b = scale_words(row[1], g, blocks, align);
+  const uint4 c = scale_words(row[2], g, blocks, align), d = scale_words(row[3], g, blocks, align);
+  out[0] = make_uint4(a.x, b.x, c.x, d.x);
+  if (g + 1 < groups) out[pitch] = make_uint4(a.y, b.y, c.y, d.y);
+  if (g + 2 < groups) out[2 * pitch] = make_uint4(a.z, b.z, c.z, d.z);
+  if (g + 3 < groups) out[3 * pitch] = make_uint4(a.w, b.w, c.w, d.w);
 }
 
 constexpr int kPackThreads = 256;
 
 // One CUDA block writes the scale blocks of 128 features, or of a row tile (2 x 128 rows), a warp
-// one 512-byte block at a time: lane l takes rows l, l + 32, l + 64, l + 96.  Or it moves 1024
-// 16-byte words of codes.
+// those of four groups at a time.  Or it moves 1024 16-byte words of codes.
 template <int kNT>
 __global__ void __launch_bounds__(kPackThreads) pack_kernel(const __grid_constant__ PackParams p) {
   __shared__ int scan[kMaxWarps];
@@ -505,9 +514,8 @@ __global__ void __launch_bounds__(kPackThreads) pack_kernel(const __grid_constan
     for (int j = 0; j < 4; ++j)
       row[j] = n0 + 32 * j < p.N ? p.w_scales + (int64_t(e) * p.N + n0 + 32 * j) * p.blocks : nullptr;
     uint4* out = reinterpret_cast<uint4*>(p.w_blocks + int64_t(task) * p.groups * 512) + lane;
-    for (int g = warp; g < p.groups; g += kPackThreads / 32)
-      out[g * 32] = make_uint4(scale_word(row[0], 4 * g, p.blocks, p.words4), scale_word(row[1], 4 * g, p.blocks, p.words4),
-                               scale_word(row[2], 4 * g, p.blocks, p.words4), scale_word(row[3], 4 * g, p.blocks, p.words4));
+    for (int g = 4 * warp; g < p.groups; g += kPackThreads / 8)
+      pack_groups(row, g, p.blocks, p.align, p.groups, out + g * 32, 32);
     return;
   }
   task -= p.w_tasks;
@@ -519,20 +527,17 @@ __global__ void __launch_bounds__(kPackThreads) pack_kernel(const __grid_constan
     const int e = group_of(starts, p.E, task), lo = bounds[e], hi = bounds[e + 1];
     const int each = round_up(ceil_div(hi - lo, ceil_div(hi - lo, kNT)), 16);
     const int n0 = lo + (task - starts[e]) * each, valid = min(each, hi - n0);
-    const uint8_t* row[8];
+    const uint8_t* row[2][4];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int r = lane + 32 * j;
       const int src = r < valid ? (p.rows ? p.rows[n0 + r] : n0 + r) : -1;
-      row[j] = src >= 0 && src < p.x_rows ? p.x_scales + int64_t(src) * p.blocks : nullptr;
+      row[j >> 2][j & 3] = src >= 0 && src < p.x_rows ? p.x_scales + int64_t(src) * p.blocks : nullptr;
     }
     uint4* out = reinterpret_cast<uint4*>(p.x_blocks + int64_t(task) * p.groups * 1024) + lane;
-    for (int g = warp; g < p.groups; g += kPackThreads / 32) {
+    for (int g = 4 * warp; g < p.groups; g += kPackThreads / 8) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        out[(g * 2 + h) * 32] =
-            make_uint4(scale_word(row[4 * h], 4 * g, p.blocks, p.words4), scale_word(row[4 * h + 1], 4 * g, p.blocks, p.words4),
-                       scale_word(row[4 * h + 2], 4 * g, p.blocks, p.words4), scale_word(row[4 * h + 3], 4 * g, p.blocks, p.words4));
+      for (int h = 0; h < 2; ++h) pack_groups(row[h], g, p.blocks, p.align, p.groups, out + (g * 2 + h) * 32, 64);
     }
     return;
   }
@@ -657,7 +662,8 @@ extern "C" int lf_expert_linear_mxfp4(int32_t out_dtype, const uint8_t* x_codes,
     k.x_codes = reinterpret_cast<const uint4*>(x_codes);
     k.E = p.E, k.R = p.R, k.x_rows = p.x_rows, k.N = p.N, k.blocks = p.blocks, k.groups = w.groups;
     k.words = int(width / 32), k.w_tasks = int(w.w_blocks / w.groups), k.x_tasks = int(w.row_tiles);
-    k.words4 = ((reinterpret_cast<uintptr_t>(x_scales) | reinterpret_cast<uintptr_t>(w_scales) | uintptr_t(p.blocks)) & 3) == 0;
+    const uintptr_t bits = reinterpret_cast<uintptr_t>(x_scales) | reinterpret_cast<uintptr_t>(w_scales) | uintptr_t(p.blocks);
+    k.align = bits & 3 ? 1 : bits & 15 ? 4 : 16;
     const int64_t moves = rows ? (num_rows * k.words + 4 * kPackThreads - 1) / (4 * kPackThreads) : 0;
     if (int rc = launch_clusters(pack_kernel<kWideRows>, int(k.w_tasks + k.x_tasks + moves), kPackThreads, 1,
                                  int(sizeof(int)) * 2 * (p.E + 1), stream, "expert_linear_mxfp4 (scales)", k))
