@@ -159,8 +159,8 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(const __grid_const
     fence_mbar_init();
     *abort = 0;
   }
-  if (warp == 1) alloc_tmem<kCtas>(tslot, S::kColumns);
   pdl_wait();
+  if (warp == 1) alloc_tmem<kCtas>(tslot, S::kColumns);  // not while waiting for a grid that may want some too
   const int mtiles = ceil_div(p.M, p.height * kCtas);
   list_tiles(p.offsets, p.E, p.R, bounds, starts, scan, [&](int rows) {
     return mtiles * ceil_div(kMode == kWeight ? p.N : rows, kNT);
