@@ -236,9 +236,10 @@ __device__ void list_tiles(const int32_t* offsets, int E, int R, int* bounds, in
   __syncthreads();
 }
 
-// The group of tile t: the last e with starts[e] <= t (empty groups share their successor's start).
-__device__ __forceinline__ int group_of(const int* starts, int E, int t) {
-  int lo = 0, hi = E - 1;
+// The group of tile t, e at least: the last with starts[e] <= t (empty groups share their
+// successor's start).
+__device__ __forceinline__ int group_of(const int* starts, int E, int t, int e = 0) {
+  int lo = e, hi = E - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
     if (starts[mid] <= t) lo = mid;
@@ -247,15 +248,47 @@ __device__ __forceinline__ int group_of(const int* starts, int E, int t) {
   return lo;
 }
 
-// Order of a group's tiles (m feature tiles x n row tiles): bands of up to eight row tiles,
-// inside a band row tiles fastest, so that the CTAs of a wave share both operands in L2.
+// Walks one CTA's tiles t = first, first + stride, ...: a group's mt feature tiles x nt column tiles in
+// bands of up to eight column tiles, inside a band column tiles fastest, so that the CTAs of a
+// wave share both operands in L2.  What holds for a group is kept from tile to tile and the
+// divisions are multiplications by a reciprocal: between two tiles nothing covers this.
 constexpr int kBand = 8;
-__device__ __forceinline__ void place_tile(int q, int mt, int nt, int* m, int* n) {
-  const int band = q / (kBand * mt), width = min(kBand, nt - band * kBand);
-  const int w = q - band * kBand * mt;
-  *m = w / width;
-  *n = band * kBand + w % width;
-}
+struct Bands {
+  int mt;            // feature tiles
+  uint64_t by_band;  // 2^64 / (kBand * mt), rounded up: exact for dividends below 2^32
+};
+inline Bands bands_of(int mt) { return {mt, ~0ull / (uint64_t(kBand) * uint64_t(mt)) + 1}; }
+
+struct Walk {
+  int e, m, n;         // group, feature tile, column tile
+  int lo, hi, nt;      // the group's rows, its column tiles
+  int start, end;      // its first tile, and the tile after its last
+  uint32_t by_last;    // 2^32 / the columns of its last band, rounded up: exact for dividends below 2^29
+
+  __device__ __forceinline__ Walk() : e(-1), end(-1) {}
+  // Moves to tile t; true when it is the first one here of its group.  columns_of(rows): the number
+  // of column tiles.
+  template <typename F>
+  __device__ __forceinline__ bool go(const Bands& bands, const int* bounds, const int* starts, int E, int t,
+                                     F&& columns_of) {
+    const bool moved = t >= end;
+    if (moved) {
+      e = group_of(starts, E, t, e + 1);
+      lo = bounds[e];
+      hi = bounds[e + 1];
+      start = starts[e];
+      end = starts[e + 1];
+      nt = columns_of(hi - lo);
+      if (nt % kBand > 1) by_last = 0xffffffffu / uint32_t(nt % kBand) + 1;
+    }
+    const uint32_t q = uint32_t(t - start), band = nt <= kBand ? 0 : uint32_t(__umul64hi(q, bands.by_band));
+    const uint32_t w = q - band * uint32_t(kBand * bands.mt);
+    const int width = min(kBand, nt - int(band) * kBand);
+    m = width == kBand ? int(w / kBand) : width == 1 ? int(w) : int(__umulhi(w, by_last));
+    n = int(band) * kBand + int(w) - m * width;
+    return moved;
+  }
+};
 
 // ------------------------------------------------------------------ host
 inline PFN_cuTensorMapEncodeTiled_v12000 map_encoder() {

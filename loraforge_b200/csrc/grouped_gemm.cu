@@ -56,6 +56,7 @@ struct GParams {
   int M, C;  // output features, contraction (forward K, input N; weight: the groups' rows)
   int N;     // weight: columns of D (dy's features)
   int elem_bf16, height, split;
+  Bands bands;
   CUtensorMap a_map;     // forward: W boxes 64 k x 128 n; input: 64 k x 64 n; weight: x boxes 64 k x 64 rows
   CUtensorMap a_small;   // weight: 64 k x 8 rows
   CUtensorMap a_gather;  // weight: single x rows of 64 k
@@ -87,37 +88,36 @@ __device__ __forceinline__ uint32_t instruction(int bf16, int a_mn, int b_mn, in
 }
 
 struct Tile {
-  int e, m0, end, n0, nt, valid, steps;  // features m0 .. end - 1; n0: first row (forward, input) or feature of dy; valid columns
-  int lo, hi;                       // the group's rows
+  int e, m0, end, n0, nt, valid, steps;  // features m0 .. end - 1; n0: first row (forward, input) or feature of dy
+  int lo, hi;                            // the group's rows
 };
 
+// A role's walk over its CTA's tiles.
 template <int kMode, int kCtas, int kNT>
-__device__ __forceinline__ Tile tile_of(const GParams& p, const int* bounds, const int* starts, int t) {
-  Tile x;
-  x.e = group_of(starts, p.E, t);
-  x.lo = bounds[x.e];
-  x.hi = bounds[x.e + 1];
-  const int mt = ceil_div(p.M, p.height * kCtas);
-  const int columns = kMode == kWeight ? p.N : x.hi - x.lo;
-  const int nt = ceil_div(columns, kNT);
-  int m, n;
-  place_tile(t - starts[x.e], mt, nt, &m, &n);
-  x.m0 = m * p.height * kCtas;
-  x.end = min(p.M, x.m0 + p.height * kCtas);
-  if (kMode == kWeight) {
-    x.n0 = n * kNT;
-    x.valid = min(kNT, p.N - x.n0);
-    x.nt = round_up(x.valid, kNT / 2);  // whole 64-feature boxes in each CTA
-    x.steps = ceil_div(x.hi - x.lo, kStep);
-  } else {
-    const int each = round_up(ceil_div(columns, nt), 16);  // the group's rows in even tiles
-    x.n0 = x.lo + n * each;
-    x.valid = min(each, x.hi - x.n0);
-    x.nt = round_up(x.valid, 16);
-    x.steps = ceil_div(p.C, kStep);
+struct Tiles {
+  Walk walk;
+  int each;  // rows of the group's column tiles
+  __device__ __forceinline__ Tile at(const GParams& p, const int* bounds, const int* starts, int t) {
+    if (walk.go(p.bands, bounds, starts, p.E, t, [&](int rows) { return ceil_div(kMode == kWeight ? p.N : rows, kNT); }))
+      each = round_up(walk.nt == 1 ? walk.hi - walk.lo : ceil_div(walk.hi - walk.lo, walk.nt), 16);  // the group's rows in even tiles
+    Tile x;
+    x.e = walk.e, x.lo = walk.lo, x.hi = walk.hi;
+    x.m0 = walk.m * p.height * kCtas;
+    x.end = min(p.M, x.m0 + p.height * kCtas);
+    if (kMode == kWeight) {
+      x.n0 = walk.n * kNT;
+      x.valid = min(kNT, p.N - x.n0);
+      x.nt = round_up(x.valid, kNT / 2);  // whole 64-feature boxes in each CTA
+      x.steps = ceil_div(x.hi - x.lo, kStep);
+    } else {
+      x.n0 = x.lo + walk.n * each;
+      x.valid = min(each, x.hi - x.n0);
+      x.nt = round_up(x.valid, 16);
+      x.steps = ceil_div(p.C, kStep);
+    }
+    return x;
   }
-  return x;
-}
+};
 
 template <int kMode, int kCtas, int kNT>
 __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(const __grid_constant__ GParams p) {
@@ -159,9 +159,10 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(const __grid_const
     fence_mbar_init();
     *abort = 0;
   }
+  Tiles<kMode, kCtas, kNT> walk;
   pdl_wait();
   if (warp == 1) alloc_tmem<kCtas>(tslot, S::kColumns);  // not while waiting for a grid that may want some too
-  const int mtiles = ceil_div(p.M, p.height * kCtas);
+  const int mtiles = p.bands.mt;
   list_tiles(p.offsets, p.E, p.R, bounds, starts, scan, [&](int rows) {
     return mtiles * ceil_div(kMode == kWeight ? p.N : rows, kNT);
   });
@@ -191,7 +192,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(const __grid_const
     // ------------------------------------------------------------ loads
     int it = 0;
     for (int t = first; t < tiles; t += stride) {
-      const Tile x = tile_of<kMode, kCtas, kNT>(p, bounds, starts, t);
+      const Tile x = walk.at(p, bounds, starts, t);
       const int m_cta = x.m0 + (kCtas == 2 ? rank * 128 : 0);
       const int share = x.nt / kCtas;  // columns this CTA loads
       const int n_cta = x.n0 + (kCtas == 2 ? rank * share : 0);
@@ -273,7 +274,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(const __grid_const
     if (lane == 0 && rank * (kCtas - 1) == 0) {
       int it = 0, count = 0;
       for (int t = first; t < tiles; t += stride) {
-        const Tile x = tile_of<kMode, kCtas, kNT>(p, bounds, starts, t);
+        const Tile x = walk.at(p, bounds, starts, t);
         int ks0, ks1;
         my_steps(x, &ks0, &ks1);
         if (ks0 >= ks1) continue;
@@ -315,7 +316,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(const __grid_const
     const uint32_t staging = smem_u32(part) + uint32_t(quarter * kChunkBytes);
     int count = 0, parts = 0;
     for (int t = first; t < tiles; t += stride) {
-      const Tile x = tile_of<kMode, kCtas, kNT>(p, bounds, starts, t);
+      const Tile x = walk.at(p, bounds, starts, t);
       int ks0, ks1;
       my_steps(x, &ks0, &ks1);
       const bool live = ks1 > ks0;
@@ -398,8 +399,9 @@ int gather_rows(const void* x, int64_t x_stride, int64_t x_rows, const int32_t* 
 }
 
 template <int kMode, int kCtas, int kNT>
-int launch_grouped(const GParams& p, int64_t tiles, void* stream, const char* what) {
+int launch_grouped(GParams& p, int64_t tiles, void* stream, const char* what) {
   using S = Shape<kCtas, kNT>;
+  p.bands = bands_of(ceil_div(p.M, p.height * kCtas));
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
   const int cluster = kCtas == 2 ? 2 : p.split;

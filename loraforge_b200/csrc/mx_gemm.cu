@@ -54,6 +54,7 @@ struct MxParams {
   const uint8_t* x_blocks;
   int groups;            // of 128 codes in them, an even number
   int height, split;
+  Bands bands;
   CUtensorMap w_map;      // 128 bytes x 128 rows
   CUtensorMap x_map[7];   // 128 bytes x 16, 32, .. 112 rows
   CUtensorMap x_gather;   // single rows
@@ -120,24 +121,27 @@ struct Tile {
   int row_tile;  // among the row tiles of all groups
 };
 
+// A role's walk over its CTA's tiles.
 template <int kCtas, int kNT>
-__device__ __forceinline__ Tile tile_of(const MxParams& p, const int* bounds, const int* starts, int t) {
-  Tile x;
-  x.e = group_of(starts, p.E, t);
-  const int lo = bounds[x.e];
-  x.hi = bounds[x.e + 1];
-  const int mt = ceil_div(p.N, p.height * kCtas), nt = ceil_div(x.hi - lo, kNT);
-  int m, n;
-  place_tile(t - starts[x.e], mt, nt, &m, &n);
-  x.row_tile = starts[x.e] / mt + n;
-  x.m0 = m * p.height * kCtas;
-  x.end = min(p.N, x.m0 + p.height * kCtas);
-  const int each = round_up(ceil_div(x.hi - lo, nt), 16);
-  x.n0 = lo + n * each;
-  x.valid = min(each, x.hi - x.n0);
-  x.nt = round_up(x.valid, kCtas == 1 ? 32 : 16);
-  return x;
-}
+struct Tiles {
+  Walk walk;
+  int each, row_tiles;  // rows of the group's row tiles; row tiles of the groups before it
+  __device__ __forceinline__ Tile at(const MxParams& p, const int* bounds, const int* starts, int t) {
+    if (walk.go(p.bands, bounds, starts, p.E, t, [](int rows) { return ceil_div(rows, kNT); })) {
+      each = round_up(walk.nt == 1 ? walk.hi - walk.lo : ceil_div(walk.hi - walk.lo, walk.nt), 16);
+      if (kCtas == 2) row_tiles = walk.start / p.bands.mt;
+    }
+    Tile x;
+    x.e = walk.e, x.hi = walk.hi;
+    x.m0 = walk.m * p.height * kCtas;
+    x.end = min(p.N, x.m0 + p.height * kCtas);
+    x.row_tile = row_tiles + walk.n;
+    x.n0 = walk.lo + walk.n * each;
+    x.valid = min(each, x.hi - x.n0);
+    x.nt = round_up(x.valid, kCtas == 1 ? 32 : 16);
+    return x;
+  }
+};
 
 // 32 scale bytes from byte k0 of a row of `blocks`; zeros past the row and where row is null.
 __device__ __forceinline__ void load_scales(const uint8_t* row, int k0, int blocks, int align, uint32_t (&s)[8]) {
@@ -205,9 +209,10 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
     fence_mbar_init();
     *abort = 0;
   }
+  Tiles<kCtas, kNT> walk;
   pdl_wait();
   if (warp == 1) alloc_tmem<kCtas>(tslot, S::kColumns);  // not while waiting for a grid that may want some too
-  const int mtiles = ceil_div(p.N, p.height * kCtas);
+  const int mtiles = p.bands.mt;
   list_tiles(p.offsets, p.E, p.R, bounds, starts, scan, [&](int rows) { return mtiles * ceil_div(rows, kNT); });
   tc_fence_before();
   __syncthreads();
@@ -232,7 +237,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
     // ------------------------------------------------------------ codes
     int it = 0;
     for (int t = first; t < tiles && live; t += stride) {
-      const Tile x = tile_of<kCtas, kNT>(p, bounds, starts, t);
+      const Tile x = walk.at(p, bounds, starts, t);
       const int m_cta = x.m0 + (kCtas == 2 ? rank * 128 : 0);
       const int share = kCtas == 1 ? x.valid : x.nt / kCtas;
       const int n_cta = x.n0 + (kCtas == 2 ? rank * share : 0);
@@ -289,7 +294,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
     if (lane == 0 && leader) {
       int it = 0, count = 0;
       for (int t = first; t < tiles && live; t += stride) {
-        const Tile x = tile_of<kCtas, kNT>(p, bounds, starts, t);
+        const Tile x = walk.at(p, bounds, starts, t);
         const int ab = count & 1;
         if (!wait_cluster(&acc_empty[ab], (uint32_t(count >> 1) & 1u) ^ 1u, abort)) break;
         ++count;
@@ -326,7 +331,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
     const uint32_t staging = smem_u32(part) + uint32_t(quarter * kChunkBytes);
     int count = 0;
     for (int t = first; t < tiles; t += stride, ++count) {
-      const Tile x = tile_of<kCtas, kNT>(p, bounds, starts, t);
+      const Tile x = walk.at(p, bounds, starts, t);
       const int ab = count & 1;
       if (live) {
         if (!__all_sync(0xffffffffu, wait_or_abort(&acc_full[ab], uint32_t(count >> 1) & 1u, abort))) break;
@@ -371,7 +376,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
       constexpr int kXRows = kNT / 32;
       const uint8_t *w_row[4], *x_row[kXRows];  // this lane's of every 32 rows
       auto rows_of = [&](int t) {
-        const Tile x = tile_of<kCtas, kNT>(p, bounds, starts, t);
+        const Tile x = walk.at(p, bounds, starts, t);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int n = x.m0 + 32 * j + lane;
@@ -559,8 +564,9 @@ __global__ void __launch_bounds__(kPackThreads) pack_kernel(const __grid_constan
 }
 
 template <int kCtas, int kNT>
-int launch_mx(const MxParams& p, int64_t tiles, void* stream) {
+int launch_mx(MxParams& p, int64_t tiles, void* stream) {
   using S = Shape<kCtas, kNT>;
+  p.bands = bands_of(ceil_div(p.N, p.height * kCtas));
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
   const int cluster = kCtas == 2 ? 2 : p.split;
