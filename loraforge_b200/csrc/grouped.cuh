@@ -26,6 +26,9 @@ constexpr int stages_of(int stage_bytes, int other) {
 }
 
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// Called by a kernel that prepares the next one's operands, after its own pdl_wait: the next one
+// starts, may read whatever was complete before this kernel, and waits before it reads the rest.
+__device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 // ------------------------------------------------------------------ clusters
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -154,6 +157,14 @@ __device__ __forceinline__ void load_3d(uint32_t dst, const CUtensorMap* map, in
         : "memory");
   }
 }
+// A box on its way into L2.
+__device__ __forceinline__ void prefetch_3d(const CUtensorMap* map, int c0, int c1, int c2) {
+  asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(c0), "r"(c1), "r"(c2)
+               : "memory");
+}
+constexpr int kAhead = 16;  // stages of W asked into L2 while the operands' other half is prepared
 // Four rows of one box width, from columns c0 on; a row index past the tensor reads zeros.
 template <int kCtas>
 __device__ __forceinline__ void gather4(uint32_t dst, const CUtensorMap* map, int c0, const int (&r)[4], uint32_t bar) {

@@ -56,6 +56,7 @@ struct GParams {
   int M, C;  // output features, contraction (forward K, input N; weight: the groups' rows)
   int N;     // weight: columns of D (dy's features)
   int elem_bf16, height, split;
+  int prepared;  // the grid before this one only put x's rows in order: all else can be read before it ends
   Bands bands;
   CUtensorMap a_map;     // forward: W boxes 64 k x 128 n; input: 64 k x 64 n; weight: x boxes 64 k x 64 rows
   CUtensorMap a_small;   // weight: 64 k x 8 rows
@@ -160,7 +161,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(const __grid_const
     *abort = 0;
   }
   Tiles<kMode, kCtas, kNT> walk;
-  pdl_wait();
+  if (!p.prepared) pdl_wait();
   if (warp == 1) alloc_tmem<kCtas>(tslot, S::kColumns);  // not while waiting for a grid that may want some too
   const int mtiles = p.bands.mt;
   list_tiles(p.offsets, p.E, p.R, bounds, starts, scan, [&](int rows) {
@@ -190,6 +191,16 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(const __grid_const
 
   if (warp == 0) {
     // ------------------------------------------------------------ loads
+    if (p.prepared) {
+      if (kMode == kForward && lane == 0 && first < tiles) {
+        const Tile x = walk.at(p, bounds, starts, first);
+        for (int ks = 0; ks < min(x.steps, kAhead); ++ks)
+          prefetch_3d(&p.a_map, ks * kStep, x.m0 + (kCtas == 2 ? rank * 128 : 0), x.e);
+      }
+      __syncwarp();
+      walk = {};
+      pdl_wait();
+    }
     int it = 0;
     for (int t = first; t < tiles; t += stride) {
       const Tile x = walk.at(p, bounds, starts, t);
@@ -361,6 +372,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(const __grid_const
 __global__ void __launch_bounds__(256) gather_rows_kernel(const uint4* x, int64_t stride, int x_rows,
                                                           const int32_t* rows, int chunks, int64_t total, uint4* out) {
   pdl_wait();
+  pdl_launch_dependents();
   const int64_t first = int64_t(blockIdx.x) * 1024 + threadIdx.x;
   uint4 v[4];
 #pragma unroll
@@ -524,15 +536,17 @@ extern "C" int lf_expert_linear(int32_t dtype, const void* x, int64_t x_stride, 
     return fail(LF_E_INVALID, "expert_linear: W must be 16-byte aligned with strides that are multiples of 8, y's rows must not overlap");
   if (x_rows < 1 || x_rows >= (int64_t(1) << 31) - 1 || (!rows && x_rows < num_rows) || !good_rows(x, x_stride, width))
     return fail(LF_E_INVALID, "expert_linear: x must have rows, 16-byte aligned, with a stride that is a multiple of 8");
+  int prepared = 0;
   if (rows) {
     const int64_t need = lf_expert_linear_workspace_bytes(num_experts, num_rows, width, 0);
     if (need) {
       if (!workspace || workspace_bytes < need || !aligned16(workspace)) return fail(LF_E_INVALID, kNoWorkspace);
       if (int rc = gather_rows(x, x_stride, x_rows, rows, num_rows, width, workspace, stream, what)) return rc;
-      x = workspace, x_stride = width, x_rows = num_rows, rows = nullptr;
+      x = workspace, x_stride = width, x_rows = num_rows, rows = nullptr, prepared = 1;
     }
   }
   GParams p{};
+  p.prepared = prepared;
   p.offsets = offsets, p.rows = rows, p.out = {y, y_stride, int(out_width), dtype};
   p.E = num_experts, p.R = int(num_rows), p.x_rows = int(x_rows);
   p.M = int(out_width), p.C = int(width), p.elem_bf16 = dtype == LF_BF16;
@@ -588,6 +602,7 @@ extern "C" int lf_expert_linear_weight_grad(int32_t dtype, const void* dy, int64
     x = workspace, x_stride = width, x_rows = num_rows;
   }
   GParams p{};
+  p.prepared = rows != nullptr;
   p.offsets = offsets, p.out = {dw, width, int(width), out_dtype};
   p.E = num_experts, p.R = int(num_rows), p.x_rows = int(x_rows);
   p.M = int(width), p.N = int(out_width), p.elem_bf16 = dtype == LF_BF16, p.height = 128, p.split = 1;

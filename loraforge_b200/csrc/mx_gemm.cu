@@ -210,7 +210,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
     *abort = 0;
   }
   Tiles<kCtas, kNT> walk;
-  pdl_wait();
+  if (kCtas == 1) pdl_wait();  // wide: the grid before is pack_kernel, and all but what it packs can be read before it ends
   if (warp == 1) alloc_tmem<kCtas>(tslot, S::kColumns);  // not while waiting for a grid that may want some too
   const int mtiles = p.bands.mt;
   list_tiles(p.offsets, p.E, p.R, bounds, starts, scan, [&](int rows) { return mtiles * ceil_div(rows, kNT); });
@@ -235,6 +235,15 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
 
   if (warp == 0) {
     // ------------------------------------------------------------ codes
+    if (kCtas == 2) {
+      if (lane == 0 && first < tiles) {
+        const Tile x = walk.at(p, bounds, starts, first);
+        for (int ks = 0; ks < min(steps, kAhead); ++ks) prefetch_3d(&p.w_map, ks * 128, x.m0 + rank * 128, x.e);
+      }
+      __syncwarp();
+      walk = {};
+      pdl_wait();
+    }
     int it = 0;
     for (int t = first; t < tiles && live; t += stride) {
       const Tile x = walk.at(p, bounds, starts, t);
@@ -510,6 +519,7 @@ __global__ void __launch_bounds__(kPackThreads) pack_kernel(const __grid_constan
   __shared__ int scan[kMaxWarps];
   extern __shared__ int tables[];
   pdl_wait();
+  pdl_launch_dependents();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   int task = blockIdx.x;
   if (task < p.w_tasks) {
