@@ -50,7 +50,7 @@ __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
 }
 __device__ __forceinline__ float lds_cluster(uint32_t addr) {
   float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr));  // the barriers around order it
   return v;
 }
 __device__ __forceinline__ bool try_wait_cluster(uint64_t* bar, uint32_t parity) {
@@ -327,17 +327,6 @@ inline bool encode_map(CUtensorMap* map, CUtensorMapDataType type, int ndim, con
                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-inline int sm_count(int* sms) {
-  static int known[64] = {};
-  int device = 0;
-  if (cudaGetDevice(&device) != cudaSuccess) return check_launch("cudaGetDevice");
-  int& have = known[device & 63];
-  if (!have && cudaDeviceGetAttribute(&have, cudaDevAttrMultiProcessorCount, device) != cudaSuccess)
-    return check_launch("cudaDeviceGetAttribute");
-  *sms = have;
-  return LF_OK;
-}
-
 // ------------------------------------------------------------------ stores
 constexpr int kMaxSplit = 8;
 constexpr int kChunkBytes = 32 * 64;  // 32 columns x 32 features of a warp, 16 bits
@@ -454,20 +443,36 @@ __device__ __forceinline__ bool store_split(const Output& o, uint32_t d, bool li
 #pragma unroll
   for (int q = 0; q < kMaxSplit; ++q)
     if (q < cluster) peer[q] = mapa(mine, q);
-  for (int c = rank; c < valid; c += cluster) {
-    float v[kMaxSplit], sum = 0.f;
+  for (int c0 = rank; c0 < valid; c0 += 4 * cluster) {  // four columns' loads in flight
+    float sum[4];
 #pragma unroll
-    for (int q = 0; q < kMaxSplit; ++q)
-      if (q < cluster) v[q] = lds_cluster(peer[q] + uint32_t(c) * 512u);
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t at = uint32_t(min(c0 + i * cluster, valid - 1)) * 512u;
+      float v[kMaxSplit];
 #pragma unroll
-    for (int q = 0; q < kMaxSplit; ++q)
-      if (q < cluster) sum += v[q];
-    if (f0 + lane < end) store_value(o, (row0 + c) * o.stride + f0 + lane, sum);
+      for (int q = 0; q < kMaxSplit; ++q)
+        if (q < cluster) v[q] = lds_cluster(peer[q] + at);
+      sum[i] = 0.f;
+#pragma unroll
+      for (int q = 0; q < kMaxSplit; ++q)
+        if (q < cluster) sum[i] += v[q];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int c = c0 + i * cluster;
+      if (c < valid && f0 + lane < end) store_value(o, (row0 + c) * o.stride + f0 + lane, sum[i]);
+    }
   }
   __syncwarp();
   if (lane < cluster) arrive_cluster(mapa(part_empty, lane));
   return true;
 }
+
+// Rows by index: with at most `most` a group on average the loads gather them, else they are put in
+// order first.  A gather4 fetches four rows of a stage and costs nothing beside the weights until
+// there are too many: two in the 16-bit products (64 experts of 2048 x 2048: 2 rows each 84 us
+// against 83 with rows in order, 16 rows 97 against 86), four in the MXFP4 ones.
+inline bool gather_in_loads(int64_t E, int64_t R, int most) { return R <= most * (E < R ? E : R); }
 
 // How the narrow kernels cut the work: `height` features a tile (the MMA always takes 128 lanes;
 // rows of A past the height are neither loaded nor stored) and the contraction over `split` CTAs.
@@ -475,21 +480,51 @@ struct Cut {
   int height, split;
 };
 
+// How many clusters of 1, 2, .. kMaxSplit CTAs the device holds at a time (148 SMs, one CTA each: 33 of
+// 4, 15 of 8, as clusters stay inside a GPC).  More in a persistent grid would run in a second wave.
+struct Clusters {
+  int at_once[kMaxSplit + 1];
+};
+template <typename P>
+int clusters_of(void (*kernel)(P), int threads, int smem, Clusters* out) {
+  static Clusters known[64] = {};
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return check_launch("cudaGetDevice");
+  Clusters& have = known[device & 63];
+  for (int s = 1; s <= kMaxSplit && !have.at_once[kMaxSplit]; ++s) {
+    cudaLaunchConfig_t config = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = s;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    config.attrs = attr;
+    config.numAttrs = 1;
+    config.gridDim = dim3(s);
+    config.blockDim = dim3(threads);
+    config.dynamicSmemBytes = smem;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &config) != cudaSuccess)
+      return check_launch("cudaOccupancyMaxActiveClusters");
+    have.at_once[s] = n > 0 ? n : 1;
+  }
+  *out = have;
+  return LF_OK;
+}
+
 // The cut with the least time for `groups` groups of one row tile each and `steps` stages.  What
 // costs is the bytes of the weights a CTA streams, height x stages of 128 bytes at some 44 GB/s:
 // 2.9 ns each, the unit here.  Whole waves count (896 tiles of 128 over 148 CTAs are 7 waves for
 // 6.05 waves' work; 1024 tiles of 112 are 6.9).  A tile costs 0.5 us more, and where a cluster adds
-// up its parts 4 us that only other tiles' loads cover.
-inline Cut choose_cut(int64_t groups, int M, int steps, int least_steps, bool any_height) {
-  int sms = 148;
-  sm_count(&sms);
+// up its parts 4 us that only other tiles' loads cover.  A CTA's steps are a multiple of `whole`.
+inline Cut choose_cut(const Clusters& clusters, int64_t groups, int M, int steps, int whole, bool any_height) {
   Cut best{128, 1};
   double least = 1e30;
-  for (int s = 1; s <= kMaxSplit && (s == 1 || steps >= least_steps * s); s *= 2) {
+  for (int s = 1; s <= kMaxSplit && (s == 1 || steps >= 4 * s); ++s) {
     for (int h = 128; h >= (any_height ? 64 : 128); h -= 8) {
-      const int64_t tiles = groups * ceil_div(M, h), clusters = sms / s;
-      const double waves = double((tiles + clusters - 1) / clusters), joined = s > 1 ? 1400 : 0;
-      const double tile = double(h) * ceil_div(steps, s) + 170;
+      const int64_t tiles = groups * ceil_div(M, h), wave = clusters.at_once[s];
+      const double waves = double((tiles + wave - 1) / wave), joined = s > 1 ? 1400 : 0;
+      const double tile = double(h) * round_up(ceil_div(steps, s), whole) + 170;
       const double cost = waves * (tile > joined ? tile : joined) + joined;
       if (cost < 0.98 * least) {
         least = cost;

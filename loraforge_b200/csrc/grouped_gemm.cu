@@ -19,10 +19,10 @@
 // Nothing is transposed in memory: MN-major operands are read as they lie through the
 // shared-memory descriptor.  Steps past K, N or a group's last row read zeros (out of bounds for
 // the tensor map, or a row index that is), so a neighbouring group's infinities never reach a
-// sum.  x's rows by token: the narrow tiles fetch them with gather4 loads.  Those move about one
+// sum.  x's rows by token: with few rows a group gather4 loads fetch them.  Those move about one
 // 128-byte row per 20 cycles and SM, a third of what the wide tiles take (8 experts, 16384 rows,
-// 4096 -> 14336: 4340 us against 1475 with rows in order), so for these gather_rows_kernel
-// copies the rows into the caller's workspace first (2 x 134 MB there, some 45 us).
+// 4096 -> 14336: 4340 us against 1475 with rows in order), so for more rows gather_rows_kernel
+// copies them into the caller's workspace first (2 x 134 MB there, 35 us).
 //
 // Per CTA: warp 0 loads 64-deep stages into a ring, warp 1 issues the MMAs and owns the TMEM
 // (two accumulators, so a tile's stores overlap the next tile's MMAs), warps 2-5 store.  The
@@ -30,8 +30,9 @@
 //
 //   wide    CTA pairs (cta_group::2), 256 x 256 tiles: each CTA loads half of both operands.
 //   narrow  one CTA, up to 128 features x up to 32 or 64 rows, for groups of few rows, where the
-//           weights' bytes are the cost (32: four more stages for the weights in flight); the contraction can be split over a cluster of CTAs, whose
-//           partial sums are added in rank order through distributed shared memory.
+//           weights' bytes are the cost (32: three more stages of weights in flight); the
+//           contraction can be split over a cluster of CTAs, whose partial sums are added in
+//           rank order through distributed shared memory.
 //
 // Every wait is bounded (tma.cuh): an expiry stops every role at its next wait.
 #include "experts.cuh"
@@ -410,22 +411,32 @@ int gather_rows(const void* x, int64_t x_stride, int64_t x_rows, const int32_t* 
   return LF_OK;
 }
 
-template <int kMode, int kCtas, int kNT>
-int launch_grouped(GParams& p, int64_t tiles, void* stream, const char* what) {
+template <int kCtas, int kNT>
+int smem_of(int E) {
   using S = Shape<kCtas, kNT>;
-  p.bands = bands_of(ceil_div(p.M, p.height * kCtas));
-  int sms = 0;
-  if (int rc = sm_count(&sms)) return rc;
-  const int cluster = kCtas == 2 ? 2 : p.split;
-  int64_t grid = int64_t(sms / cluster) * cluster;
-  if (tiles * cluster < grid) grid = tiles * cluster;
-  const int smem = 1024 + S::kStages * S::kStageBytes + S::kPartBytes + 512 + int(sizeof(int)) * (kMaxWarps + 2 + 2 * (p.E + 1));
-  static int flags[64] = {};
-  if (int rc = ensure_smem(grouped_kernel<kMode, kCtas, kNT>, smem, flags)) return rc;
-  return launch_clusters(grouped_kernel<kMode, kCtas, kNT>, int(grid), kThreads, cluster, smem, stream, what, p);
+  return 1024 + S::kStages * S::kStageBytes + S::kPartBytes + 512 + int(sizeof(int)) * (kMaxWarps + 2 + 2 * (E + 1));
 }
 
-constexpr int kWideRows = 256, kNarrowRows = 64, kFewRows = 32;
+template <int kMode, int kCtas, int kNT>
+int clusters_at_once(Clusters* out) {
+  const auto kernel = grouped_kernel<kMode, kCtas, kNT>;
+  static int flags[64] = {};
+  if (int rc = ensure_smem(kernel, smem_of<kCtas, kNT>(kMaxExperts), flags)) return rc;
+  return clusters_of(kernel, kThreads, smem_of<kCtas, kNT>(kMaxExperts), out);
+}
+
+template <int kMode, int kCtas, int kNT>
+int launch_grouped(GParams& p, int64_t tiles, void* stream, const char* what) {
+  p.bands = bands_of(ceil_div(p.M, p.height * kCtas));
+  const int cluster = kCtas == 2 ? 2 : p.split;
+  Clusters clusters;
+  if (int rc = clusters_at_once<kMode, kCtas, kNT>(&clusters)) return rc;
+  const int64_t most = tiles < clusters.at_once[cluster] ? tiles : clusters.at_once[cluster];
+  return launch_clusters(grouped_kernel<kMode, kCtas, kNT>, int(most * cluster), kThreads, cluster,
+                         smem_of<kCtas, kNT>(p.E), stream, what, p);
+}
+
+constexpr int kWideRows = 256, kNarrowRows = 64, kFewRows = 32, kGatherRows = 8;
 constexpr char kNoWorkspace[] = "expert_linear: workspace missing, too small or not 16-byte aligned (see lf_expert_linear_workspace_bytes)";
 
 // Groups of up to 64 rows on average take the narrow tiles.
@@ -486,7 +497,10 @@ template <int kMode>
 int launch_rows(GParams& p, CUtensorMapDataType type, const Weights& w, void* stream, const char* what) {
   const int64_t groups = p.E < p.R ? p.E : p.R;
   if (narrow(p.E, p.R)) {
-    const Cut cut = choose_cut(groups, p.M, ceil_div(p.C, kStep), 4, kMode == kForward);  // input: boxes of 64 features
+    Clusters clusters;
+    if (int rc = clusters_at_once<kMode, 1, kNarrowRows>(&clusters)) return rc;
+    const int steps = ceil_div(p.C, kStep);
+    const Cut cut = choose_cut(clusters, groups, p.M, steps, 1, kMode == kForward);  // input: boxes of 64 features
     p.height = cut.height, p.split = cut.split;
     if (kMode == kForward && !encode_weights(&p.a_map, type, w.data, w.K, w.N, p.E, w.row_stride, w.expert_stride, cut.height))
       return fail(LF_E_CUDA, (std::string(what) + ": cuTensorMapEncodeTiled failed").c_str());
@@ -521,7 +535,7 @@ using namespace lfb;
 extern "C" int64_t lf_expert_linear_workspace_bytes(int32_t num_experts, int64_t num_rows, int64_t width,
                                                     int32_t weight_grad) {
   if (num_experts < 1 || num_rows < 0 || width < 1) return -1;
-  return weight_grad || !narrow(num_experts, num_rows) ? num_rows * width * 2 : 0;
+  return weight_grad || !gather_in_loads(num_experts, num_rows, kGatherRows) ? num_rows * width * 2 : 0;
 }
 
 extern "C" int lf_expert_linear(int32_t dtype, const void* x, int64_t x_stride, int64_t x_rows, const int32_t* rows,

@@ -54,6 +54,8 @@ struct MxParams {
   const uint8_t* x_blocks;
   int groups;            // of 128 codes in them, an even number
   int height, split;
+  int gathered;  // x's codes (not its scales) are in the rows' order
+  int prepared;  // the grid before is pack_kernel: all but what it packs can be read before it ends
   Bands bands;
   CUtensorMap w_map;      // 128 bytes x 128 rows
   CUtensorMap x_map[7];   // 128 bytes x 16, 32, .. 112 rows
@@ -210,7 +212,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
     *abort = 0;
   }
   Tiles<kCtas, kNT> walk;
-  if (kCtas == 1) pdl_wait();  // wide: the grid before is pack_kernel, and all but what it packs can be read before it ends
+  if (!p.prepared) pdl_wait();
   if (warp == 1) alloc_tmem<kCtas>(tslot, S::kColumns);  // not while waiting for a grid that may want some too
   const int mtiles = p.bands.mt;
   list_tiles(p.offsets, p.E, p.R, bounds, starts, scan, [&](int rows) { return mtiles * ceil_div(rows, kNT); });
@@ -235,10 +237,11 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
 
   if (warp == 0) {
     // ------------------------------------------------------------ codes
-    if (kCtas == 2) {
+    if (p.prepared) {
       if (lane == 0 && first < tiles) {
         const Tile x = walk.at(p, bounds, starts, first);
-        for (int ks = 0; ks < min(steps, kAhead); ++ks) prefetch_3d(&p.w_map, ks * 128, x.m0 + rank * 128, x.e);
+        for (int ks = ks0; ks < min(ks1, ks0 + kAhead); ++ks)
+          prefetch_3d(&p.w_map, ks * 128, x.m0 + (kCtas == 2 ? rank * 128 : 0), x.e);
       }
       __syncwarp();
       walk = {};
@@ -250,7 +253,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
       const int m_cta = x.m0 + (kCtas == 2 ? rank * 128 : 0);
       const int share = kCtas == 1 ? x.valid : x.nt / kCtas;
       const int n_cta = x.n0 + (kCtas == 2 ? rank * share : 0);
-      const bool by_row = kCtas == 1 && p.rows;
+      const bool by_row = kCtas == 1 && p.rows && !p.gathered;
       int row4[4];
       if (by_row) {
 #pragma unroll
@@ -461,7 +464,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
   }
 }
 
-constexpr int kWideRows = 208, kNarrowRows = 64, kFewRows = 32;
+constexpr int kWideRows = 208, kNarrowRows = 64, kFewRows = 32, kGatherRows = 16;
 
 bool narrow(int64_t E, int64_t R) { return R <= kNarrowRows * (E < R ? E : R); }
 
@@ -574,19 +577,28 @@ __global__ void __launch_bounds__(kPackThreads) pack_kernel(const __grid_constan
 }
 
 template <int kCtas, int kNT>
-int launch_mx(MxParams& p, int64_t tiles, void* stream) {
+int smem_of(int E) {
   using S = Shape<kCtas, kNT>;
-  p.bands = bands_of(ceil_div(p.N, p.height * kCtas));
-  int sms = 0;
-  if (int rc = sm_count(&sms)) return rc;
-  const int cluster = kCtas == 2 ? 2 : p.split;
-  int64_t grid = int64_t(sms / cluster) * cluster;
-  if (tiles * cluster < grid) grid = tiles * cluster;
-  const int smem = 1024 + S::kStages * S::kStageBytes + S::kPartBytes + 512 +
-                   int(sizeof(int)) * (kMaxWarps + 2 + 2 * (p.E + 1));
+  return 1024 + S::kStages * S::kStageBytes + S::kPartBytes + 512 + int(sizeof(int)) * (kMaxWarps + 2 + 2 * (E + 1));
+}
+
+template <int kCtas, int kNT>
+int clusters_at_once(Clusters* out) {
+  const auto kernel = mx_kernel<kCtas, kNT>;
   static int flags[64] = {};
-  if (int rc = ensure_smem(mx_kernel<kCtas, kNT>, smem, flags)) return rc;
-  return launch_clusters(mx_kernel<kCtas, kNT>, int(grid), kThreads, cluster, smem, stream, "expert_linear_mxfp4", p);
+  if (int rc = ensure_smem(kernel, smem_of<kCtas, kNT>(kMaxExperts), flags)) return rc;
+  return clusters_of(kernel, kThreads, smem_of<kCtas, kNT>(kMaxExperts), out);
+}
+
+template <int kCtas, int kNT>
+int launch_mx(MxParams& p, int64_t tiles, void* stream) {
+  p.bands = bands_of(ceil_div(p.N, p.height * kCtas));
+  const int cluster = kCtas == 2 ? 2 : p.split;
+  Clusters clusters;
+  if (int rc = clusters_at_once<kCtas, kNT>(&clusters)) return rc;
+  const int64_t most = tiles < clusters.at_once[cluster] ? tiles : clusters.at_once[cluster];
+  return launch_clusters(mx_kernel<kCtas, kNT>, int(most * cluster), kThreads, cluster, smem_of<kCtas, kNT>(p.E), stream,
+                         "expert_linear_mxfp4", p);
 }
 
 bool encode_codes(CUtensorMap* map, const void* p, int64_t bytes, int64_t rows, int box_rows) {
@@ -596,18 +608,20 @@ bool encode_codes(CUtensorMap* map, const void* p, int64_t bytes, int64_t rows, 
   return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, p, dims, strides, box);
 }
 
-// Sizes of the wide tiles' workspace: 512-byte blocks of W's and of x's scales, then codes.
+// Sizes of the workspace: 512-byte blocks of W's and of x's scales (wide tiles), then codes.
 struct Workspace {
   int groups;
   int64_t row_tiles, w_blocks, x_blocks, bytes;
 };
-Workspace workspace_of(int64_t E, int64_t R, int64_t N, int64_t K, bool gather) {
+Workspace workspace_of(int64_t E, int64_t R, int64_t N, int64_t K, bool by_rows) {
   Workspace w{};
-  w.groups = 2 * int((K + kStep - 1) / kStep);
-  w.row_tiles = (E < R ? E : R) + R / kWideRows;  // at most
-  w.w_blocks = E * ((N + 255) / 256) * 2 * w.groups;
-  w.x_blocks = w.row_tiles * w.groups * 2;
-  w.bytes = (w.w_blocks + w.x_blocks) * 512 + (gather ? R * (K / 2) : 0);
+  if (!narrow(E, R)) {
+    w.groups = 2 * int((K + kStep - 1) / kStep);
+    w.row_tiles = (E < R ? E : R) + R / kWideRows;  // at most
+    w.w_blocks = E * ((N + 255) / 256) * 2 * w.groups;
+    w.x_blocks = w.row_tiles * w.groups * 2;
+  }
+  w.bytes = (w.w_blocks + w.x_blocks) * 512 + (by_rows && !gather_in_loads(E, R, kGatherRows) ? R * (K / 2) : 0);
   return w;
 }
 
@@ -636,7 +650,7 @@ using namespace lfb;
 extern "C" int64_t lf_expert_linear_mxfp4_workspace_bytes(int32_t num_experts, int64_t num_rows, int64_t out_width,
                                                           int64_t width, int32_t by_rows) {
   if (num_experts < 1 || num_rows < 0 || out_width < 1 || width < 1) return -1;
-  return narrow(num_experts, num_rows) ? 0 : workspace_of(num_experts, num_rows, out_width, width, by_rows != 0).bytes;
+  return workspace_of(num_experts, num_rows, out_width, width, by_rows != 0).bytes;
 }
 
 extern "C" int lf_expert_linear_mxfp4(int32_t out_dtype, const uint8_t* x_codes, const uint8_t* x_scales,
@@ -664,38 +678,44 @@ extern "C" int lf_expert_linear_mxfp4(int32_t out_dtype, const uint8_t* x_codes,
   p.x_align = row_alignment(x_scales, p.blocks), p.w_align = row_alignment(w_scales, p.blocks);
   const bool few = narrow(num_experts, num_rows);
   int64_t code_rows = x_rows;
-  if (!few) {
-    const Workspace w = workspace_of(num_experts, num_rows, out_width, width, rows != nullptr);
+  const Workspace w = workspace_of(num_experts, num_rows, out_width, width, rows != nullptr);
+  if (w.bytes) {
     if (!workspace || workspace_bytes < w.bytes || !aligned16(workspace))
       return fail(LF_E_INVALID, "expert_linear_mxfp4: workspace missing, too small or not 16-byte aligned "
                                 "(see lf_expert_linear_mxfp4_workspace_bytes)");
     if (w.w_blocks >= limit || w.x_blocks >= limit)
       return fail(LF_E_INVALID, "expert_linear_mxfp4: too many scale blocks");
+    const bool move = rows && !gather_in_loads(num_experts, num_rows, kGatherRows);
     PackParams k{};
     k.offsets = offsets, k.rows = rows, k.x_scales = x_scales, k.w_scales = w_scales;
     k.w_blocks = static_cast<uint8_t*>(workspace), k.x_blocks = k.w_blocks + w.w_blocks * 512;
     k.codes = reinterpret_cast<uint4*>(k.x_blocks + w.x_blocks * 512);
     k.x_codes = reinterpret_cast<const uint4*>(x_codes);
     k.E = p.E, k.R = p.R, k.x_rows = p.x_rows, k.N = p.N, k.blocks = p.blocks, k.groups = w.groups;
-    k.words = int(width / 32), k.w_tasks = int(w.w_blocks / w.groups), k.x_tasks = int(w.row_tiles);
+    k.words = int(width / 32), k.w_tasks = w.groups ? int(w.w_blocks / w.groups) : 0, k.x_tasks = int(w.row_tiles);
     const uintptr_t bits = reinterpret_cast<uintptr_t>(x_scales) | reinterpret_cast<uintptr_t>(w_scales) | uintptr_t(p.blocks);
     k.align = bits & 3 ? 1 : bits & 15 ? 4 : 16;
-    const int64_t moves = rows ? (num_rows * k.words + 4 * kPackThreads - 1) / (4 * kPackThreads) : 0;
+    const int64_t moves = move ? (num_rows * k.words + 4 * kPackThreads - 1) / (4 * kPackThreads) : 0;
     if (int rc = launch_clusters(pack_kernel<kWideRows>, int(k.w_tasks + k.x_tasks + moves), kPackThreads, 1,
                                  int(sizeof(int)) * 2 * (p.E + 1), stream, "expert_linear_mxfp4 (scales)", k))
       return rc;
-    if (rows) x_codes = reinterpret_cast<const uint8_t*>(k.codes), code_rows = num_rows;
-    p.groups = w.groups;
+    if (move) x_codes = reinterpret_cast<const uint8_t*>(k.codes), code_rows = num_rows, p.gathered = 1;
+    p.groups = w.groups, p.prepared = 1;
     p.w_blocks = k.w_blocks, p.x_blocks = k.x_blocks;
   }
   const cuuint64_t dims[3] = {cuuint64_t(width / 2), cuuint64_t(out_width), cuuint64_t(num_experts)};
   const cuuint64_t strides[2] = {cuuint64_t(width / 2), cuuint64_t(width / 2) * cuuint64_t(out_width)};
   const int64_t groups = num_experts < num_rows ? num_experts : num_rows;
-  const Cut cut = few ? choose_cut(groups, p.N, ceil_div(p.K, kStep), kSuper, true) : Cut{128, 1};
+  Cut cut{128, 1};
+  if (few) {
+    Clusters clusters;
+    if (int rc = clusters_at_once<1, kNarrowRows>(&clusters)) return rc;
+    cut = choose_cut(clusters, groups, p.N, ceil_div(p.K, kStep), kSuper, true);
+  }
   p.height = cut.height, p.split = cut.split;
   const cuuint32_t box[3] = {128, cuuint32_t(cut.height), 1};
   bool ok = encode_map(&p.w_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, w_codes, dims, strides, box);
-  if (rows && few) ok = ok && encode_codes(&p.x_gather, x_codes, width / 2, code_rows, 1);
+  if (rows && few && !p.gathered) ok = ok && encode_codes(&p.x_gather, x_codes, width / 2, code_rows, 1);
   else
     for (int i = 0; i < (few ? kNarrowRows / 16 : 7) && ok; ++i)
       ok = encode_codes(&p.x_map[i], x_codes, width / 2, code_rows, 16 * (i + 1));
