@@ -20,9 +20,10 @@ constexpr int kMaxTopK = 32;
 constexpr int kRouteThreads = 1024;
 constexpr int kRouteWarps = kRouteThreads / 32;
 constexpr int kSortWarps = 8;         // of a block, that rank its slots
-constexpr int kMaxRouteBlocks = 256;  // each block of the scatter adds up the others' counts
+constexpr int kMaxRouteBlocks = 148;  // one wave; each block of the sort adds up the others' counts
 constexpr int kMinBlockTokens = 32;
 constexpr int kBackThreads = 256;
+constexpr int route_threads(int values) { return values > 8 ? kRouteThreads / 2 : kRouteThreads; }  // registers
 constexpr int sort_bytes(int E) { return int(sizeof(int)) * E * (1 + kSortWarps); }
 
 template <typename T>
@@ -55,6 +56,11 @@ __device__ __forceinline__ uint32_t order_key(float v) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+__device__ __forceinline__ float key_value(uint32_t key) {
+  return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+}
+constexpr uint32_t kNoKey = 0x007fffffu;  // order_key(-infinity); 0 stands for a logit that was taken
+
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // Lane holds the logits of experts lane, lane + 32, ...
@@ -76,7 +82,7 @@ __device__ void scatter_slots(const int32_t* experts, const int32_t* counts, int
                               int32_t* positions, int* smem) {
   int* base = smem;                     // [E]: rows before expert e's, then before this block's of e
   int* wcount = base + E;               // [kSortWarps][E]
-  int* sums = wcount;                   // [parts][2][E] before that: all rows of e, those of earlier blocks
+  int* found = wcount;                  // [parts][2][E] before that: all rows of e, those of earlier blocks
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, threads = blockDim.x;
   __shared__ int warp_total[kRouteWarps];
   // Counts of the blocks, in up to four parts of them at a time.
@@ -91,8 +97,8 @@ __device__ void scatter_slots(const int32_t* experts, const int32_t* counts, int
       total += c;
       before += b < block ? c : 0;
     }
-    sums[(2 * part) * E + e] = total;
-    sums[(2 * part + 1) * E + e] = before;
+    found[(2 * part) * E + e] = total;
+    found[(2 * part + 1) * E + e] = before;
   }
   __syncthreads();
   int carry = 0;
@@ -101,8 +107,8 @@ __device__ void scatter_slots(const int32_t* experts, const int32_t* counts, int
     int total = 0, before = 0;
     if (e < E)
       for (int part = 0; part < parts; ++part) {
-        total += sums[(2 * part) * E + e];
-        before += sums[(2 * part + 1) * E + e];
+        total += found[(2 * part) * E + e];
+        before += found[(2 * part + 1) * E + e];
       }
     int scan = total;
 #pragma unroll
@@ -112,11 +118,14 @@ __device__ void scatter_slots(const int32_t* experts, const int32_t* counts, int
     }
     if (lane == 31) warp_total[warp] = scan;
     __syncthreads();
-    int prefix = carry;
-    for (int w = 0; w < threads / 32; ++w) {
-      if (w < warp) prefix += warp_total[w];
-      carry += warp_total[w];
+    int sums = lane < threads / 32 ? warp_total[lane] : 0;  // every warp scans the warps' totals
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, sums, d);
+      if (lane >= d) sums += up;
     }
+    const int prefix = carry + (warp ? __shfl_sync(0xffffffffu, sums, warp - 1) : 0);
+    carry += __shfl_sync(0xffffffffu, sums, 31);
     if (e < E) {
       base[e] = prefix + scan - total + before;
       if (block == 0) offsets[e] = prefix + scan - total;
@@ -163,12 +172,12 @@ __device__ void scatter_slots(const int32_t* experts, const int32_t* counts, int
   for (int64_t r = carry + int64_t(block) * threads + tid; r < all_slots; r += int64_t(blocks) * threads) rows[r] = -1;
 }
 
-// One warp a token: k times the largest remaining logit.  A lane keeps the best of its own
-// V logits and looks through them again only after it lost it.  With one block the slots
+// One warp a token: k times the largest remaining logit, as integer keys.  A lane keeps the best
+// of its own V logits and looks through them again only after it lost it.  With one block the slots
 // are sorted in the same launch, else the block leaves its counts for route_scatter_kernel.
 // Bound by the latency of the k picks, so a block has a warp for each of its 32 tokens.
 template <typename T, int V>
-__global__ void __launch_bounds__(kRouteThreads) route_topk_kernel(
+__global__ void __launch_bounds__(route_threads(V)) route_topk_kernel(
     const void* logits, int64_t stride, int num_tokens, int E, int k, int renormalize, float scale, int block_tokens,
     float* weights, int32_t* experts, int32_t* offsets, int32_t* rows, int32_t* positions, int32_t* counts) {
   extern __shared__ int smem[];
@@ -181,36 +190,50 @@ __global__ void __launch_bounds__(kRouteThreads) route_topk_kernel(
   for (int t = t0 + warp; t < t1; t += blockDim.x / 32) {
     float v[V];
     load_logits<T, V>(logits, int64_t(t) * stride, E, lane, v);
-    uint32_t taken = 0;
-    float best = -INFINITY, peak = 0.f, mine = 0.f;
-    int at = 0, my_expert = -1;
-    auto look = [&]() {
-      best = -INFINITY;
-      at = 0;
+    uint32_t keys[V], best;
+    int at;
 #pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (!(taken >> i & 1u) && v[i] > best) {
-          best = v[i];
-          at = i;
+    for (int i = 0; i < V; ++i) keys[i] = order_key(v[i]);
+    auto look = [&]() {  // this lane's largest key, by halves: the lower index of two equal ones stays
+      uint32_t m[V];
+      int where[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) m[i] = keys[i], where[i] = i;
+#pragma unroll
+      for (int d = 1; d < V; d *= 2) {
+#pragma unroll
+        for (int i = 0; i + d < V; i += 2 * d) {
+          const bool up = m[i + d] > m[i];
+          m[i] = up ? m[i + d] : m[i];
+          where[i] = up ? where[i + d] : where[i];
         }
+      }
+      best = m[0];
+      at = where[0];
     };
     look();
+    const uint32_t peak_key = __reduce_max_sync(0xffffffffu, best);
+    const float peak = peak_key > kNoKey ? key_value(peak_key) : 0.f;
+    uint32_t top = peak_key, my_key = 0;
+    int my_expert = -1;
     for (int j = 0; j < k; ++j) {
-      const uint32_t key = order_key(best);
-      const uint32_t top = __reduce_max_sync(0xffffffffu, key);
-      if (top == order_key(-INFINITY)) break;
-      const int e = __reduce_min_sync(0xffffffffu, key == top ? at * 32 + lane : 0x7fffffff);
-      const float value = __shfl_sync(0xffffffffu, best, e & 31);
-      if (j == 0) peak = value;
+      if (top <= kNoKey) break;
+      const unsigned holders = __ballot_sync(0xffffffffu, best == top);
+      int e = __shfl_sync(0xffffffffu, at * 32 + lane, __ffs(holders) - 1);
+      if (holders & (holders - 1)) e = __reduce_min_sync(0xffffffffu, best == top ? at * 32 + lane : 0x7fffffff);
       if (lane == j) {
         my_expert = e;
-        mine = expf(value - peak);
+        my_key = top;
       }
       if (lane == (e & 31)) {
-        taken |= 1u << at;
+#pragma unroll
+        for (int i = 0; i < V; ++i) keys[i] = i == at ? 0 : keys[i];
         look();
       }
+      __syncwarp();
+      top = __reduce_max_sync(0xffffffffu, best);
     }
+    const float mine = my_expert >= 0 ? expf(key_value(my_key) - peak) : 0.f;
     float sum = mine;
     if (!renormalize) {
       sum = 0.f;
@@ -488,7 +511,7 @@ struct RouteCall {
   template <typename D, int V>
   int operator()() const {
     const RoutePlan plan = route_plan(T);
-    const int threads = T > kSortWarps ? kRouteThreads : kSortWarps * 32;
+    const int threads = T > kSortWarps ? route_threads(V) : kSortWarps * 32;
     return launch_pdl(route_topk_kernel<D, V>, dim3(plan.blocks), threads, sort_bytes(E), stream, "route_experts", logits,
                       stride, T, E, k, renormalize, scale, plan.block_tokens, weights, experts, offsets, rows,
                       positions, counts);
