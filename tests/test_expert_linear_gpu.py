@@ -195,6 +195,58 @@ def test_layer_of_experts():
     assert (out - want).norm() <= 2.0**-7 * want.norm()
 
 
+@pytest.mark.parametrize("tokens", [600, 20000])
+def test_a_thousand_experts(tokens):
+    g = torch.Generator(device="cuda").manual_seed(12)
+    r = route_experts(torch.randn(tokens, 1024, generator=g, device="cuda"), 5)
+    x = torch.randn(tokens, 72, generator=g, device="cuda").bfloat16()
+    w = (torch.randn(1024, 40, 72, generator=g, device="cuda") / 8).bfloat16()
+    grad = torch.randn(tokens * 5, 40, generator=g, device="cuda").bfloat16()
+    check_forward(x, w, r.offsets, r.rows, expert_linear(x, w, r.offsets, rows=r.rows))
+    check_backward(grad, x, w, r.offsets, r.rows, *expert_linear_backward(grad, x, w, r.offsets, rows=r.rows))
+
+
+def test_offsets_past_32_bits():
+    # 2.4e9 weights, then 2.2e9 outputs: the last expert's rows against 64 bits.
+    N, K, E = 32768, 24576, 3
+    w = torch.empty(E, N, K, dtype=torch.bfloat16, device="cuda")
+    for e in range(E):
+        w[e].normal_(std=K**-0.5)
+    offsets = torch.tensor([0, 2, 3, 5], dtype=torch.int32, device="cuda")
+    x = torch.randn(5, K, device="cuda").bfloat16()
+    y = expert_linear(x, w, offsets)
+    want, size = x[3:].double() @ w[2, -512:].double().T, x[3:].double().abs() @ w[2, -512:].double().abs().T
+    near(y[3:, -512:], want, size, K)
+    del w, y
+    R, N, K = 70000, 32000, 32
+    x = torch.randn(R, K, device="cuda").bfloat16()
+    w = torch.randn(2, N, K, device="cuda").bfloat16()
+    offsets = torch.tensor([0, 30000, R], dtype=torch.int32, device="cuda")
+    y = expert_linear(x, w, offsets)
+    near(y[-64:], x[-64:].double() @ w[1].double().T, x[-64:].double().abs() @ w[1].double().abs().T, K)
+
+
+@pytest.mark.parametrize("counts", [[3, 0, 2], [40, 300, 90]])
+def test_other_streams_and_captured_graphs(counts):
+    x, w, offsets, rows, grad = make(counts, 136, 200, torch.bfloat16, seed=13)
+    want, want_grads = expert_linear(x, w, offsets, rows=rows), expert_linear_backward(grad, x, w, offsets, rows=rows)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        y = expert_linear(x, w, offsets, rows=rows)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(y, want)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = expert_linear(x, w, offsets, rows=rows)
+        grads = expert_linear_backward(grad, x, w, offsets, rows=rows)
+    y.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, want) and all(torch.equal(a, b) for a, b in zip(grads, want_grads))
+
+
 def test_refusals():
     x, w, offsets, rows, grad = make([4, 4], 64, 64, torch.bfloat16, seed=2)
     with pytest.raises(TypeError, match="weight"):

@@ -156,6 +156,55 @@ def test_output_rows_of_a_wider_buffer():
     assert (wide[:, 96:] == 7).all()
 
 
+@pytest.mark.parametrize("tokens", [600, 20000])
+def test_a_thousand_experts(tokens):
+    g = torch.Generator(device="cuda").manual_seed(12)
+    r = route_experts(torch.randn(tokens, 1024, generator=g, device="cuda"), 5)
+    x, w = random_mx(g, tokens, 96), random_mx(g, 1024, 40, 96)
+    check(x, w, r.offsets, r.rows, expert_linear_mxfp4(x, w, r.offsets, rows=r.rows))
+
+
+def test_offsets_past_32_bits():
+    # 2.4e9 codes' bytes, then 2.2e9 outputs: the last expert's rows against 64 bits.
+    g = torch.Generator(device="cuda").manual_seed(14)
+    E, N, K = 3, 32768, 49152
+    w = random_mx(g, E, N, K)
+    offsets = torch.tensor([0, 2, 3, 5], dtype=torch.int32, device="cuda")
+    x = random_mx(g, 5, K)
+    y = expert_linear_mxfp4(x, w, offsets, dtype=torch.float32)
+    last = MxTensor(w.codes[2, -256:].contiguous(), w.scales[2, -256:].contiguous())
+    xs, ws = values64(x)[3:], values64(last)
+    assert ((y[3:, -256:].double() - xs @ ws.T).abs() <= (xs.abs() @ ws.abs().T) * K * 2.0**-22).all()
+    del w, y
+    R, N, K = 70000, 32000, 32
+    x, w = random_mx(g, R, K), random_mx(g, 2, N, K)
+    offsets = torch.tensor([0, 30000, R], dtype=torch.int32, device="cuda")
+    y = expert_linear_mxfp4(x, w, offsets)
+    xs, ws = values64(MxTensor(x.codes[-64:], x.scales[-64:])), values64(w)[1]
+    far = (y[-64:].double() - xs @ ws.T).abs() - (xs.abs() @ ws.abs().T) * (K * 2.0**-22 + 2.0**-8)
+    assert (far <= 2.0**-24).all()
+
+
+@pytest.mark.parametrize("counts", [[3, 0, 2], [40, 300, 90]])
+def test_other_streams_and_captured_graphs(counts):
+    x, w, offsets, rows = make(counts, 136, 192, seed=13)
+    want = expert_linear_mxfp4(x, w, offsets, rows=rows)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        y = expert_linear_mxfp4(x, w, offsets, rows=rows)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(y, want)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = expert_linear_mxfp4(x, w, offsets, rows=rows)
+    y.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, want)
+
+
 def test_refusals():
     x, w, offsets, rows = make([4, 4], 64, 64, seed=2)
     with pytest.raises(TypeError, match="MxTensor"):
