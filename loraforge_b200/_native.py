@@ -8,6 +8,7 @@ CPU or library computation.
 from __future__ import annotations
 
 import ctypes
+import functools
 import threading
 from pathlib import Path
 
@@ -177,18 +178,26 @@ def launch(name: str, index: int, *args) -> None:
     For the operators whose smallest calls are bound by the host: it looks the stream up without
     making a Stream object, and changes the current device only where it is another one.
     """
-    import torch
-
+    current, stream_on = _device_calls()
     status_of = getattr(_lib or library(), name)
-    stream = torch._C._cuda_getCurrentRawStream(index)
-    if torch._C._cuda_getDevice() == index:
-        status = status_of(*args, stream)
+    if current() == index:
+        status = status_of(*args, stream_on(index))
     else:
+        import torch
+
         with torch.cuda.device(index):
-            status = status_of(*args, stream)
+            status = status_of(*args, stream_on(index))
     if status != 0:
         message = library().lf_last_error_string().decode(errors="replace")
         raise RuntimeError(message or f"{name} failed with status {status}")
+
+
+@functools.lru_cache(maxsize=1)
+def _device_calls():
+    """PyTorch's current device and the raw handle of its current stream on a device."""
+    import torch
+
+    return torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
 def fused_workspace_floats(num_tokens: int, width: int, num_slices: int, capacity: int) -> int:

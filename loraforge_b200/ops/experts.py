@@ -48,8 +48,8 @@ def cuda_tensor(value, name: str, ndim: int, dtypes, index: int | None = None) -
         raise ValueError(f"{name} must be {ndim}D with dtype {' or '.join(str(d) for d in dtypes)}")
     if value.numel() >= INT32_LIMIT and max(value.shape) >= INT32_LIMIT:
         raise ValueError(f"{name} dimensions must fit signed int32 indexing")
-    found = value.get_device() if value.is_cuda else -1
-    if found < 0 or (index is not None and found != index):
+    found = value.get_device()  # -1: the host
+    if found < 0 or not value.is_cuda or (index is not None and found != index):
         raise ValueError(f"{name} must be on the same CUDA GPU")
     return found
 
@@ -72,10 +72,12 @@ def row_stride(t) -> int:
 
 
 def packed_table(value, name: str, shape, index: int, dtype) -> None:
-    """A contiguous table of exactly `shape`."""
+    """A contiguous table of exactly `shape` on CUDA device `index`."""
+    if (isinstance(value, _kinds()[0]) and value.dtype is dtype and value.shape == shape and value.is_contiguous()
+            and value.get_device() == index and value.is_cuda):
+        return
     cuda_tensor(value, name, len(shape), (dtype,), index)
-    if value.shape != shape or not value.is_contiguous():
-        raise ValueError(f"{name} must be contiguous with shape {tuple(shape)}")
+    raise ValueError(f"{name} must be contiguous with shape {tuple(shape)}")
 
 
 def _scale(value) -> float:
@@ -143,7 +145,8 @@ def route_experts_backward(logits, routing: ExpertRouting, grad_weights, *, reno
     T, E = logits.shape
     if not isinstance(routing, ExpertRouting):
         raise TypeError("routing must be the ExpertRouting of the forward call")
-    cuda_tensor(routing.weights, "routing.weights", 2, (torch.float32,), index)
+    if getattr(routing.weights, "ndim", 0) != 2:
+        cuda_tensor(routing.weights, "routing.weights", 2, (torch.float32,), index)
     k = routing.weights.shape[1]
     packed_table(routing.weights, "routing.weights", (T, k), index, torch.float32)
     packed_table(routing.experts, "routing.experts", (T, k), index, torch.int32)
@@ -167,10 +170,10 @@ def route_experts_backward(logits, routing: ExpertRouting, grad_weights, *, reno
 def _combine_tables(positions, weights, index: int):
     import torch
 
-    cuda_tensor(positions, "positions", 2, (torch.int32,), index)
+    if getattr(positions, "ndim", 0) != 2:
+        cuda_tensor(positions, "positions", 2, (torch.int32,), index)
     T, k = positions.shape
-    if not positions.is_contiguous():
-        raise ValueError("positions must be contiguous")
+    packed_table(positions, "positions", (T, k), index, torch.int32)
     if weights is not None:
         packed_table(weights, "weights", (T, k), index, torch.float32)
     if not 1 <= k <= MAX_TOP_K or T * k >= INT32_LIMIT:
@@ -259,10 +262,10 @@ def group_tables(offsets, rows, num_experts: int, x_rows: int, index: int) -> in
     packed_table(offsets, "offsets", (num_experts + 1,), index, torch.int32)
     if rows is None:
         return x_rows
-    cuda_tensor(rows, "rows", 1, (torch.int32,), index)
+    if getattr(rows, "ndim", 0) != 1:
+        cuda_tensor(rows, "rows", 1, (torch.int32,), index)
     R = rows.numel()
-    if not rows.is_contiguous():
-        raise ValueError("rows must be contiguous")
+    packed_table(rows, "rows", (R,), index, torch.int32)
     if R and not x_rows:
         raise ValueError("x must have at least one row")
     return R
