@@ -408,7 +408,7 @@ int lf_peer_sum(const uint64_t* bases, int32_t rank, int32_t world, float* z, in
  *   slot.  Row r in [offsets[e], offsets[e+1]) belongs to expert e and token rows[r];
  *   positions[t, j] is the slot's row or -1; rows beyond offsets[E] are -1.
  * Sizes: 1 <= k <= 32, k <= E <= 1024, T*k < 2^31.  workspace: lf_route_experts_workspace_ints
- * int32 values, not initialised (0: none needed).  One launch up to 32 tokens, else two.
+ * int32 values, not initialised (0: none needed).  One launch up to 64 tokens, else two.
  */
 int64_t lf_route_experts_workspace_ints(int64_t num_tokens, int32_t num_experts);
 int lf_route_experts(int32_t dtype, const void* logits, int64_t logits_stride, int64_t num_tokens,

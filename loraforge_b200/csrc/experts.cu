@@ -21,7 +21,7 @@ constexpr int kRouteThreads = 1024;
 constexpr int kRouteWarps = kRouteThreads / 32;
 constexpr int kSortWarps = 8;         // of a block, that rank its slots
 constexpr int kMaxRouteBlocks = 148;  // one wave; each block of the sort adds up the others' counts
-constexpr int kMinBlockTokens = 32;
+constexpr int kMinBlockTokens = 64;  // two a warp; up to so many the whole call is one launch
 constexpr int kBackThreads = 256;
 constexpr int route_threads(int values) { return values > 8 ? kRouteThreads / 2 : kRouteThreads; }  // registers
 constexpr int sort_bytes(int E) { return int(sizeof(int)) * E * (1 + kSortWarps); }
@@ -175,7 +175,7 @@ __device__ void scatter_slots(const int32_t* experts, const int32_t* counts, int
 // One warp a token: k times the largest remaining logit, as integer keys.  A lane keeps the best
 // of its own V logits and looks through them again only after it lost it.  With one block the slots
 // are sorted in the same launch, else the block leaves its counts for route_scatter_kernel.
-// Bound by the latency of the k picks, so a block has a warp for each of its 32 tokens.
+// Bound by the latency of the k picks, so a block has a warp for every two of its 64 tokens.
 template <typename T, int V>
 __global__ void __launch_bounds__(route_threads(V)) route_topk_kernel(
     const void* logits, int64_t stride, int num_tokens, int E, int k, int renormalize, float scale, int block_tokens,

@@ -44,7 +44,7 @@ def test_sizes_are_checked_on_the_host(entry, args, match):
 
 
 def test_workspace_sizes():
-    assert _native.route_experts_workspace_ints(32, 64) == 0 and _native.route_experts_workspace_ints(33, 64) == 128
+    assert _native.route_experts_workspace_ints(64, 64) == 0 and _native.route_experts_workspace_ints(65, 64) == 128
     assert _native.expert_linear_workspace_bytes(8, 64, 512) == 0  # eight rows a group: gathered by the loads
     assert _native.expert_linear_workspace_bytes(8, 65, 512) == 65 * 1024
     assert _native.expert_linear_workspace_bytes(8, 64, 512, weight_grad=True) == 64 * 1024
