@@ -63,12 +63,15 @@ __device__ __forceinline__ bool try_wait_cluster(uint64_t* bar, uint32_t parity)
       : "memory");
   return done != 0;
 }
-// wait_or_abort for barriers on which other CTAs of the cluster arrive.
-__device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity, volatile int* abort) {
-  if (*abort) return false;
-  if (try_wait_cluster(bar, parity)) return true;
+// Wait for the phase of `bar` with parity `parity`; false, with the CTA's abort word set, when it has
+// not come after kWaitLimitNs, or when another role gave up.  kCluster: other CTAs arrive on it.  The
+// abort word is read only when there is something to wait for: these waits stand between MMAs.
+template <bool kCluster>
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  if (kCluster ? try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity)) return true;
   const uint64_t start = global_timer_ns();
-  while (!try_wait_cluster(bar, parity)) {
+  while (!(kCluster ? try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity))) {
+    if (*abort) return false;
     if (global_timer_ns() - start > kWaitLimitNs) {
       atomicAdd(&g_lf_wait_timeouts, 1u);
       *abort = 1;
@@ -76,6 +79,20 @@ __device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity, vol
     }
   }
   return true;
+}
+__device__ __forceinline__ bool wait_here(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  return wait_for<false>(bar, parity, abort);
+}
+__device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  return wait_for<true>(bar, parity, abort);
+}
+// One thread of a converged warp.  The MMA warp runs its loop whole and issues through this one, so
+// that the descriptors are computed once for the warp (in one thread's branch each MMA cost some
+// 100 cycles to issue, as much as it takes to run).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t chosen;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(chosen));
+  return chosen != 0;
 }
 
 // ------------------------------------------------------------------ tcgen05 on one CTA or a pair

@@ -226,7 +226,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(const __grid_const
       bool ok = true;
       for (int ks = ks0; ks < ks1; ++ks, ++it) {
         const int st = it % kStages;
-        ok = __all_sync(0xffffffffu, wait_or_abort(&empty[st], (uint32_t(it / kStages) & 1u) ^ 1u, abort));
+        ok = __all_sync(0xffffffffu, wait_here(&empty[st], (uint32_t(it / kStages) & 1u) ^ 1u, abort));
         if (!ok) break;
         const uint32_t a = smem_u32(ring + st * S::kStageBytes), b = a + kABytes;
         const uint32_t bar = kCtas == 2 ? mapa(&full[st], 0) : smem_u32(&full[st]);
@@ -277,13 +277,14 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(const __grid_const
     }
     // A pair's CTA stays until the commits that arrive here from the other CTA have.
     if (kCtas == 2)
-      for (int j = max(0, it - kStages); j < it; ++j) wait_or_abort(&empty[j % kStages], uint32_t(j / kStages) & 1u, abort);
+      for (int j = max(0, it - kStages); j < it; ++j) wait_here(&empty[j % kStages], uint32_t(j / kStages) & 1u, abort);
     // No load may still be landing when the CTA exits (only an expired wait leaves any).
     if (*abort && lane == 0 && rank * (kCtas - 1) == 0)
       for (int j = max(0, it - kStages); j < it; ++j) mbar_wait(&full[j % kStages], uint32_t(j / kStages) & 1u);
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA thread
-    if (lane == 0 && rank * (kCtas - 1) == 0) {
+    if (rank * (kCtas - 1) == 0) {
+      const bool elected = elect_one();
       int it = 0, count = 0;
       for (int t = first; t < tiles; t += stride) {
         const Tile x = walk.at(p, bounds, starts, t);
@@ -291,7 +292,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(const __grid_const
         my_steps(x, &ks0, &ks1);
         if (ks0 >= ks1) continue;
         const int ab = count & 1;
-        if (!wait_cluster(&acc_empty[ab], (uint32_t(count >> 1) & 1u) ^ 1u, abort)) break;
+        if (!__all_sync(0xffffffffu, wait_cluster(&acc_empty[ab], (uint32_t(count >> 1) & 1u) ^ 1u, abort))) break;
         ++count;
         tc_fence_after();
         const uint32_t d = tmem + uint32_t(ab * kNT);
@@ -299,7 +300,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(const __grid_const
         bool ok = true;
         for (int ks = ks0; ks < ks1; ++ks, ++it) {
           const int st = it % kStages;
-          ok = wait_or_abort(&full[st], uint32_t(it / kStages) & 1u, abort);
+          ok = __all_sync(0xffffffffu, wait_here(&full[st], uint32_t(it / kStages) & 1u, abort));
           if (!ok) break;
           tc_fence_after();
           const uint32_t sa = smem_u32(ring + st * S::kStageBytes);
@@ -307,16 +308,20 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(const __grid_const
           const uint64_t bd = kMode == kWeight ? mn_desc(sa + kABytes) : sw128_desc(sa + kABytes);
           constexpr int kAStep = kMode == kForward ? 2 : 128, kBStep = kMode == kWeight ? 128 : 2;
           const int subs = kMode == kWeight ? min(kStep, round_up(x.hi - x.lo - ks * kStep, 16)) / 16 : kStep / 16;
+          if (elected) {
 #pragma unroll
-          for (int k = 0; k < kStep / 16; ++k)
-            if (kMode != kWeight || k < subs)
-              mma_f16<kCtas>(d, ad + kAStep * k, bd + kBStep * k, idesc, (ks > ks0 || k > 0) ? 1u : 0u);
-          commit<kCtas>(&empty[st]);
+            for (int k = 0; k < kStep / 16; ++k)
+              if (kMode != kWeight || k < subs)
+                mma_f16<kCtas>(d, ad + kAStep * k, bd + kBStep * k, idesc, (ks > ks0 || k > 0) ? 1u : 0u);
+            commit<kCtas>(&empty[st]);
+          }
+          __syncwarp();
         }
         if (!ok) break;
-        commit<kCtas>(&acc_full[ab]);
+        if (elected) commit<kCtas>(&acc_full[ab]);
+        __syncwarp();
       }
-      if (*abort) {  // every MMA has retired before the TMEM columns are released
+      if (*abort && elected) {  // every MMA has retired before the TMEM columns are released
         commit<kCtas>(fin);
         mbar_wait(fin, 0);
       }
@@ -334,7 +339,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(const __grid_const
       const bool live = ks1 > ks0;
       const int ab = count & 1;
       if (live) {
-        if (!__all_sync(0xffffffffu, wait_or_abort(&acc_full[ab], uint32_t(count >> 1) & 1u, abort))) break;
+        if (!__all_sync(0xffffffffu, wait_here(&acc_full[ab], uint32_t(count >> 1) & 1u, abort))) break;
         ++count;
         tc_fence_after();
       }

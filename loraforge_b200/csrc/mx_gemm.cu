@@ -279,7 +279,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
           }
           for (int ks = ks0, j = it; ks < ks1; ++ks, ++j) {
             const int st = j % kStages;
-            ok = wait_or_abort(&empty[st], (uint32_t(j / kStages) & 1u) ^ 1u, abort);
+            ok = wait_here(&empty[st], (uint32_t(j / kStages) & 1u) ^ 1u, abort);
             if (!ok) break;
             uint8_t* stage = ring + st * S::kStageBytes;
             const uint32_t a = smem_u32(stage);
@@ -301,7 +301,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
       } else {
         for (int ks = ks0; ks < ks1; ++ks, ++it) {
           const int st = it % kStages;
-          ok = __all_sync(0xffffffffu, wait_or_abort(&empty[st], (uint32_t(it / kStages) & 1u) ^ 1u, abort));
+          ok = __all_sync(0xffffffffu, wait_here(&empty[st], (uint32_t(it / kStages) & 1u) ^ 1u, abort));
           if (!ok) break;
           const uint32_t a = smem_u32(ring + st * S::kStageBytes), bar = smem_u32(&full[st]);
           if (lane == 0) {
@@ -316,7 +316,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
     }
     // A pair's CTA stays until the commits that arrive here from the other CTA have.
     if (kCtas == 2)
-      for (int j = max(0, it - kStages); j < it; ++j) wait_or_abort(&empty[j % kStages], uint32_t(j / kStages) & 1u, abort);
+      for (int j = max(0, it - kStages); j < it; ++j) wait_here(&empty[j % kStages], uint32_t(j / kStages) & 1u, abort);
     // No load may still be landing when the CTA exits: after an expired wait, give them time.
     if (*abort && lane == 0)
       for (int j = max(0, it - kStages); j < it; ++j) {
@@ -325,35 +325,41 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
       }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA thread
-    if (lane == 0 && leader) {
+    if (leader) {
+      const bool elected = elect_one();
       int it = 0, count = 0;
       for (int t = first; t < tiles && live; t += stride) {
         const Tile x = walk.at(p, bounds, starts, t);
         const int ab = count & 1;
-        if (!wait_cluster(&acc_empty[ab], (uint32_t(count >> 1) & 1u) ^ 1u, abort)) break;
+        if (!__all_sync(0xffffffffu, wait_cluster(&acc_empty[ab], (uint32_t(count >> 1) & 1u) ^ 1u, abort))) break;
         ++count;
         const uint32_t d = tmem + uint32_t(ab * kNT);
         const uint32_t idesc0 = instruction(128 * kCtas, x.nt, 0), idesc1 = instruction(128 * kCtas, x.nt, 2);
         bool ok = true;
         for (int ks = ks0; ks < ks1; ++ks, ++it) {
           const int st = it % kStages, set = it % kSets;
-          ok = wait_or_abort(&full[st], uint32_t(it / kStages) & 1u, abort) &&
+          ok = wait_here(&full[st], uint32_t(it / kStages) & 1u, abort) &&
                wait_cluster(&set_full[set], uint32_t(it / kSets) & 1u, abort);
+          ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tc_fence_after();
           const uint32_t sa = smem_u32(ring + st * S::kStageBytes);
           const uint32_t ts = tmem + uint32_t(2 * kNT + set * S::kScaleColumns);  // W: 2 x 4 columns, then x
           const uint64_t ad = sw128_desc(sa), bd = sw128_desc(sa + kABytes);
+          if (elected) {
 #pragma unroll
-          for (int k = 0; k < kStep / 64; ++k)
-            mma_mxf4<kCtas>(d, ad + 2 * k, bd + 2 * k, k & 1 ? idesc1 : idesc0, ts + 4 * (k >> 1),
-                            ts + 8 + 4 * S::kHalves * (k >> 1), (ks > ks0 || k > 0) ? 1u : 0u);
-          commit<kCtas>(&empty[st]);
+            for (int k = 0; k < kStep / 64; ++k)
+              mma_mxf4<kCtas>(d, ad + 2 * k, bd + 2 * k, k & 1 ? idesc1 : idesc0, ts + 4 * (k >> 1),
+                              ts + 8 + 4 * S::kHalves * (k >> 1), (ks > ks0 || k > 0) ? 1u : 0u);
+            commit<kCtas>(&empty[st]);
+          }
+          __syncwarp();
         }
         if (!ok) break;
-        commit<kCtas>(&acc_full[ab]);
+        if (elected) commit<kCtas>(&acc_full[ab]);
+        __syncwarp();
       }
-      if (*abort) {  // every MMA has retired before the TMEM columns are released
+      if (*abort && elected) {  // every MMA has retired before the TMEM columns are released
         commit<kCtas>(fin);
         mbar_wait(fin, 0);
       }
@@ -368,7 +374,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
       const Tile x = walk.at(p, bounds, starts, t);
       const int ab = count & 1;
       if (live) {
-        if (!__all_sync(0xffffffffu, wait_or_abort(&acc_full[ab], uint32_t(count >> 1) & 1u, abort))) break;
+        if (!__all_sync(0xffffffffu, wait_here(&acc_full[ab], uint32_t(count >> 1) & 1u, abort))) break;
         tc_fence_after();
       }
       const uint32_t d = tmem + lanes + uint32_t(ab * kNT);
@@ -397,8 +403,8 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
       const int mine = first < tiles ? (tiles - first + stride - 1) / stride : 0;
       for (int it = 0; it < mine * steps; ++it) {
         const int before = it - kSets, st = it % kStages, set = it % kSets;
-        bool ready = wait_or_abort(&blocks_full[st], uint32_t(it / kStages) & 1u, abort);
-        if (before >= 0) ready = ready && wait_or_abort(&empty[before % kStages], uint32_t(before / kStages) & 1u, abort);
+        bool ready = wait_here(&blocks_full[st], uint32_t(it / kStages) & 1u, abort);
+        if (before >= 0) ready = ready && wait_here(&empty[before % kStages], uint32_t(before / kStages) & 1u, abort);
         if (!__all_sync(0xffffffffu, ready)) break;
         tc_fence_after();
         store_scales<2 * (1 + S::kHalves)>(quarter_set + uint32_t(set * S::kScaleColumns),
@@ -457,7 +463,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
         for (int j = 0; j < kSuper; ++j) {
           if (j >= todo || !ok) continue;
           const int set = it % kSets;  // free when the MMAs of its stage are done
-          ok = __all_sync(0xffffffffu, wait_or_abort(&empty[set], (uint32_t(it / kSets) & 1u) ^ 1u, abort));
+          ok = __all_sync(0xffffffffu, wait_here(&empty[set], (uint32_t(it / kSets) & 1u) ^ 1u, abort));
           if (!ok) continue;
           tc_fence_after();
           // Groups 2 j and 2 j + 1 of W, then of x; columns past the tile's rows are not read.
