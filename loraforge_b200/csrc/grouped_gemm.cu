@@ -192,6 +192,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(const __grid_const
 
   if (warp == 0) {
     // ------------------------------------------------------------ loads
+    const bool elected = elect_one();
     if (p.prepared) {
       if (kMode == kForward && lane == 0 && first < tiles) {
         const Tile x = walk.at(p, bounds, starts, first);
@@ -223,6 +224,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(const __grid_const
       const bool boxed = kMode != kWeight && !(kMode == kForward && kCtas == 1 && p.rows);
       const int loaded = kMode == kWeight ? share : boxed ? round_up(share, 16) : round_up(x.valid, 4);
       const uint32_t whole = kCtas * uint32_t(p.height + loaded) * 128u;
+      const CUtensorMap* b_rows = &p.b_rows[kMode == kWeight ? 0 : ceil_div(share, 16) - 1];
       bool ok = true;
       for (int ks = ks0; ks < ks1; ++ks, ++it) {
         const int st = it % kStages;
@@ -234,19 +236,35 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(const __grid_const
         // Weight: the rows of this step; the last one is loaded by 8 rows up to a multiple of 16.
         const int left = kMode == kWeight ? min(kStep, x.hi - x.lo - c) : kStep;
         const uint32_t bytes = left == kStep ? whole : whole / kStep * uint32_t(round_up(left, 16));
-        if (lane == 0 && rank * (kCtas - 1) == 0) mbar_arrive_expect_tx(&full[st], bytes);
+        const bool by_row = kMode == kForward && kCtas == 1 && p.rows;
+        if (elected) {
+          if (rank * (kCtas - 1) == 0) mbar_arrive_expect_tx(&full[st], bytes);
+          if (kMode == kForward) {
+            load_3d<kCtas>(a, &p.a_map, c, m_cta, x.e, bar);
+          } else if (kMode == kInput) {
+            load_3d<kCtas>(a, &p.a_map, m_cta, c, x.e, bar);
+            load_3d<kCtas>(a + 8192, &p.a_map, m_cta + 64, c, x.e, bar);
+          } else if (left == kStep) {
+            load_2d<kCtas>(a, &p.a_map, m_cta, x.lo + c, bar);
+            load_2d<kCtas>(a + 8192, &p.a_map, m_cta + 64, x.lo + c, bar);
+            load_2d<kCtas>(b, &p.b_map, n_cta, x.lo + c, bar);
+            if (share > 64) load_2d<kCtas>(b + 8192, &p.b_map, n_cta + 64, x.lo + c, bar);
+          }
+          // One box of the share's rows in steps of 16: small boxes cost the copy engine near 0.1 us
+          // each, whatever their size (rows past the share are loaded and not used).
+          if (kMode != kWeight && !by_row) load_2d<kCtas>(b, b_rows, c, n_cta, bar);
+        }
         __syncwarp();
-        if (kMode == kWeight) {
-          // Boxes of 64 features: two of x (lanes 0-15), one or two of dy (lanes 16-31).
+        if (by_row && 4 * lane < x.valid) gather4<kCtas>(b + lane * 512, &p.b_gather, c, row4, bar);
+        if (kMode == kWeight && left < kStep) {
+          // Boxes of 64 features x 8 rows: two of x (lanes 0-15), one or two of dy (lanes 16-31).
           const bool is_x = lane < 16;
           const int box = lane >> 3 & 1, unit = lane & 7;
           const int col = (is_x ? m_cta : n_cta) + 64 * box;
           const uint32_t dst = (is_x ? a : b) + box * 8192 + unit * 1024;
           const int r = x.lo + c + 8 * unit;
           if (is_x || box * 64 < share) {
-            if (left == kStep) {
-              if (unit == 0) load_2d<kCtas>(dst, is_x ? &p.a_map : &p.b_map, col, r, bar);
-            } else if (8 * unit + 8 <= left) {
+            if (8 * unit + 8 <= left) {
               load_2d<kCtas>(dst, is_x ? &p.a_small : &p.b_small, col, r, bar);
             } else if (8 * unit < round_up(left, 16)) {  // rows past the group's last read zeros
 #pragma unroll
@@ -258,19 +276,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(const __grid_const
               }
             }
           }
-        } else {
-          if (kMode == kForward) {
-            if (lane == 0) load_3d<kCtas>(a, &p.a_map, c, m_cta, x.e, bar);
-          } else if (lane < 2) {
-            load_3d<kCtas>(a + lane * 8192, &p.a_map, m_cta + 64 * lane, c, x.e, bar);
-          }
-          if (kMode == kForward && kCtas == 1 && p.rows) {
-            if (4 * lane < x.valid) gather4<kCtas>(b + lane * 512, &p.b_gather, c, row4, bar);
-          } else {
-            // One box of the share's rows in steps of 16: small boxes cost the copy engine near
-            // 0.1 us each, whatever their size (rows past the share are loaded and not used).
-            if (lane == 2) load_2d<kCtas>(b, &p.b_rows[ceil_div(share, 16) - 1], c, n_cta, bar);
-          }
+          __syncwarp();
         }
       }
       if (!ok) break;
@@ -279,7 +285,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(const __grid_const
     if (kCtas == 2)
       for (int j = max(0, it - kStages); j < it; ++j) wait_here(&empty[j % kStages], uint32_t(j / kStages) & 1u, abort);
     // No load may still be landing when the CTA exits (only an expired wait leaves any).
-    if (*abort && lane == 0 && rank * (kCtas - 1) == 0)
+    if (*abort && elected && rank * (kCtas - 1) == 0)
       for (int j = max(0, it - kStages); j < it; ++j) mbar_wait(&full[j % kStages], uint32_t(j / kStages) & 1u);
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA thread

@@ -237,6 +237,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
 
   if (warp == 0) {
     // ------------------------------------------------------------ codes
+    const bool elected = elect_one();
     if (p.prepared) {
       if (lane == 0 && first < tiles) {
         const Tile x = walk.at(p, bounds, starts, first);
@@ -266,24 +267,23 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
       const uint32_t bytes = kCtas * uint32_t(p.height + (by_row ? round_up(x.valid, 4) : round_up(share, 16))) * 128u;
       bool ok = true;
       if (!by_row) {
-        // One thread, its addresses kept from step to step (64 groups of 94 rows, 1416 x 2048: 38.2 us,
-        // 39.4 shared out over the warp).  One box of the share's rows in steps of 16, as small boxes
-        // cost the copy engine near 0.1 us each, whatever their size (rows past the share are loaded
-        // and not used).
-        if (lane == 0) {
-          const CUtensorMap* x_map = &p.x_map[ceil_div(share, 16) - 1];
-          const uint8_t *w_blocks = nullptr, *x_blocks = nullptr;
-          if (kCtas == 2) {
-            w_blocks = p.w_blocks + (int64_t(x.e * ceil_div(p.N, 256) * 2 + m_cta / 128) * p.groups + 2 * ks0) * 512;
-            x_blocks = p.x_blocks + (int64_t(x.row_tile) * p.groups + 2 * ks0) * 1024;
-          }
-          for (int ks = ks0, j = it; ks < ks1; ++ks, ++j) {
-            const int st = j % kStages;
-            ok = wait_here(&empty[st], (uint32_t(j / kStages) & 1u) ^ 1u, abort);
-            if (!ok) break;
-            uint8_t* stage = ring + st * S::kStageBytes;
-            const uint32_t a = smem_u32(stage);
-            const uint32_t bar = kCtas == 2 ? mapa(&full[st], 0) : smem_u32(&full[st]);
+        // Addresses kept from step to step (64 groups of 94 rows, 1416 x 2048: 38.2 us, 39.4 shared out
+        // over the lanes).  One box of the share's rows in steps of 16, as small boxes cost the copy
+        // engine near 0.1 us each, whatever their size (rows past the share are loaded and not used).
+        const CUtensorMap* x_map = &p.x_map[ceil_div(share, 16) - 1];
+        const uint8_t *w_blocks = nullptr, *x_blocks = nullptr;
+        if (kCtas == 2) {
+          w_blocks = p.w_blocks + (int64_t(x.e * ceil_div(p.N, 256) * 2 + m_cta / 128) * p.groups + 2 * ks0) * 512;
+          x_blocks = p.x_blocks + (int64_t(x.row_tile) * p.groups + 2 * ks0) * 1024;
+        }
+        for (int ks = ks0; ks < ks1; ++ks, ++it) {
+          const int st = it % kStages;
+          ok = __all_sync(0xffffffffu, wait_here(&empty[st], (uint32_t(it / kStages) & 1u) ^ 1u, abort));
+          if (!ok) break;
+          uint8_t* stage = ring + st * S::kStageBytes;
+          const uint32_t a = smem_u32(stage);
+          const uint32_t bar = kCtas == 2 ? mapa(&full[st], 0) : smem_u32(&full[st]);
+          if (elected) {
             if (leader) mbar_arrive_expect_tx(&full[st], bytes);
             load_3d<kCtas>(a, &p.w_map, ks * 128, m_cta, x.e, bar);
             load_2d<kCtas>(a + kABytes, x_map, ks * 128, n_cta, bar);
@@ -292,19 +292,18 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
               mbar_arrive_expect_tx(&blocks_full[st], S::kScaleBytes);
               bulk_g2s(sc, w_blocks, 1024, &blocks_full[st]);
               bulk_g2s(sc + 1024, x_blocks, 2048, &blocks_full[st]);
-              w_blocks += 1024, x_blocks += 2048;
             }
           }
+          __syncwarp();
+          if (kCtas == 2) w_blocks += 1024, x_blocks += 2048;
         }
-        it += ks1 - ks0;
-        ok = __all_sync(0xffffffffu, ok);
       } else {
         for (int ks = ks0; ks < ks1; ++ks, ++it) {
           const int st = it % kStages;
           ok = __all_sync(0xffffffffu, wait_here(&empty[st], (uint32_t(it / kStages) & 1u) ^ 1u, abort));
           if (!ok) break;
           const uint32_t a = smem_u32(ring + st * S::kStageBytes), bar = smem_u32(&full[st]);
-          if (lane == 0) {
+          if (elected) {
             mbar_arrive_expect_tx(&full[st], bytes);
             load_3d<1>(a, &p.w_map, ks * 128, m_cta, x.e, bar);
           }
@@ -318,7 +317,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
     if (kCtas == 2)
       for (int j = max(0, it - kStages); j < it; ++j) wait_here(&empty[j % kStages], uint32_t(j / kStages) & 1u, abort);
     // No load may still be landing when the CTA exits: after an expired wait, give them time.
-    if (*abort && lane == 0)
+    if (*abort && elected)
       for (int j = max(0, it - kStages); j < it; ++j) {
         if (leader) mbar_wait(&full[j % kStages], uint32_t(j / kStages) & 1u);
         if (kCtas == 2) mbar_wait(&blocks_full[j % kStages], uint32_t(j / kStages) & 1u);
