@@ -54,21 +54,17 @@ def cuda_tensor(value, name: str, ndim: int, dtypes, index: int | None = None) -
     return found
 
 
-def row_matrix(value, name: str, dtypes, index: int | None = None) -> int:
-    """A 2-D `cuda_tensor` of rows that do not overlap, with unit column stride."""
+def row_matrix(value, name: str, dtypes, index: int | None = None) -> tuple:
+    """A 2-D `cuda_tensor` of rows that do not overlap, with unit column stride: its device index,
+    rows, width and row stride (a single row's own stride says nothing: its width)."""
     index = cuda_tensor(value, name, 2, dtypes, index)
-    if not value.is_contiguous():
-        rows, width = value.shape
-        step, unit = value.stride()
-        if (rows > 1 and step < width) or (width > 1 and unit != 1):
-            raise ValueError(f"{name} must have unit column stride and rows that do not overlap")
-    return index
-
-
-def row_stride(t) -> int:
-    """Row stride of a `row_matrix` (a one-row tensor's own stride says nothing)."""
-    rows, width = t.shape
-    return t.stride(0) if rows > 1 else width
+    rows, width = value.shape
+    if value.is_contiguous():
+        return index, rows, width, width
+    step, unit = value.stride()
+    if (rows > 1 and step < width) or (width > 1 and unit != 1):
+        raise ValueError(f"{name} must have unit column stride and rows that do not overlap")
+    return index, rows, width, step if rows > 1 else width
 
 
 def packed_table(value, name: str, shape, index: int, dtype) -> None:
@@ -100,8 +96,7 @@ def route_experts(logits, top_k: int, *, renormalize: bool = True, scale: float 
     """
     import torch
 
-    index = row_matrix(logits, "logits", _kinds()[2])
-    T, E = logits.shape
+    index, T, E, stride = row_matrix(logits, "logits", _kinds()[2])
     if type(top_k) is not int or not 1 <= top_k <= min(E, MAX_TOP_K):
         raise ValueError(f"top_k must be in 1..min(experts, {MAX_TOP_K})")
     if E > MAX_EXPERTS:
@@ -125,7 +120,7 @@ def route_experts(logits, top_k: int, *, renormalize: bool = True, scale: float 
     room = _native.route_experts_workspace_ints(T, E)
     workspace = logits.new_empty(room, dtype=torch.int32) if room else None
     _native.launch(
-        "lf_route_experts", index, _native.dtype_code(logits.dtype), logits.data_ptr(), row_stride(logits), T, E, top_k,
+        "lf_route_experts", index, _native.dtype_code(logits.dtype), logits.data_ptr(), stride, T, E, top_k,
         renormalize, scale, out.weights.data_ptr(), out.experts.data_ptr(), out.offsets.data_ptr(),
         out.rows.data_ptr(), out.positions.data_ptr(), workspace.data_ptr() if room else None, room,
     )
@@ -141,8 +136,7 @@ def route_experts_backward(logits, routing: ExpertRouting, grad_weights, *, reno
     """
     import torch
 
-    index = row_matrix(logits, "logits", _kinds()[2])
-    T, E = logits.shape
+    index, T, E, stride = row_matrix(logits, "logits", _kinds()[2])
     if not isinstance(routing, ExpertRouting):
         raise TypeError("routing must be the ExpertRouting of the forward call")
     if getattr(routing.weights, "ndim", 0) != 2:
@@ -150,7 +144,7 @@ def route_experts_backward(logits, routing: ExpertRouting, grad_weights, *, reno
     k = routing.weights.shape[1]
     packed_table(routing.weights, "routing.weights", (T, k), index, torch.float32)
     packed_table(routing.experts, "routing.experts", (T, k), index, torch.int32)
-    row_matrix(grad_weights, "grad_weights", (torch.float32,), index)
+    grad_stride = row_matrix(grad_weights, "grad_weights", (torch.float32,), index)[3]
     if grad_weights.shape != (T, k):
         raise ValueError("grad_weights must have the weights' shape")
     if not 1 <= k <= min(E, MAX_TOP_K) or E > MAX_EXPERTS:
@@ -160,8 +154,8 @@ def route_experts_backward(logits, routing: ExpertRouting, grad_weights, *, reno
     scale = _scale(scale)
     grad = logits.new_empty((T, E))
     _native.launch(
-        "lf_route_experts_backward", index, _native.dtype_code(logits.dtype), logits.data_ptr(), row_stride(logits),
-        routing.weights.data_ptr(), routing.experts.data_ptr(), grad_weights.data_ptr(), row_stride(grad_weights),
+        "lf_route_experts_backward", index, _native.dtype_code(logits.dtype), logits.data_ptr(), stride,
+        routing.weights.data_ptr(), routing.experts.data_ptr(), grad_weights.data_ptr(), grad_stride,
         T, E, k, renormalize, scale, grad.data_ptr(), E,
     )
     return grad
@@ -188,21 +182,21 @@ def combine_experts(y, weights, positions, *, out=None):
     a gather), ``positions`` int32 [T, k]; a position outside [0, R) adds nothing, so a token
     without experts gets zeros.
     """
-    index = row_matrix(y, "y", _kinds()[2])
+    index, R, N, stride = row_matrix(y, "y", _kinds()[2])
     T, k = _combine_tables(positions, weights, index)
-    R, N = y.shape
     if N < 1:
         raise ValueError("y must have at least one column")
+    out_stride = N
     if out is None:
         out = y.new_empty((T, N))
     else:
-        row_matrix(out, "out", (y.dtype,), index)
+        out_stride = row_matrix(out, "out", (y.dtype,), index)[3]
         if out.shape != (T, N):
             raise ValueError("out must be [tokens, width]")
         output_is_distinct(out, (y, positions) if weights is None else (y, positions, weights))
     _native.launch(
-        "lf_combine_experts", index, _native.dtype_code(y.dtype), y.data_ptr(), row_stride(y), R,
-        None if weights is None else weights.data_ptr(), positions.data_ptr(), T, k, N, out.data_ptr(), row_stride(out),
+        "lf_combine_experts", index, _native.dtype_code(y.dtype), y.data_ptr(), stride, R,
+        None if weights is None else weights.data_ptr(), positions.data_ptr(), T, k, N, out.data_ptr(), out_stride,
     )
     return out
 
@@ -216,29 +210,28 @@ def combine_experts_backward(grad, y, weights, positions):
     """
     import torch
 
-    index = row_matrix(y, "y", _kinds()[2])
+    index, R, N, stride = row_matrix(y, "y", _kinds()[2])
     T, k = _combine_tables(positions, weights, index)
-    R, N = y.shape
-    row_matrix(grad, "grad", (y.dtype,), index)
+    grad_stride = row_matrix(grad, "grad", (y.dtype,), index)[3]
     if grad.shape != (T, N) or N < 1:
         raise ValueError("grad must be [tokens, width]")
     grad_y = y.new_empty((R, N))
     grad_weights = None if weights is None else y.new_empty((T, k), dtype=torch.float32)
     _native.launch(
-        "lf_combine_experts_backward", index, _native.dtype_code(y.dtype), grad.data_ptr(), row_stride(grad),
-        y.data_ptr(), row_stride(y), R, None if weights is None else weights.data_ptr(), positions.data_ptr(), T, k, N,
+        "lf_combine_experts_backward", index, _native.dtype_code(y.dtype), grad.data_ptr(), grad_stride,
+        y.data_ptr(), stride, R, None if weights is None else weights.data_ptr(), positions.data_ptr(), T, k, N,
         grad_y.data_ptr(), N, None if weights is None else grad_weights.data_ptr(),
     )
     return grad_y, grad_weights
 
 
-def _operand(value, name: str, dtypes, index: int | None = None) -> int:
-    """A row matrix that TMA can read: aligned, its row stride a multiple of 8."""
-    index = row_matrix(value, name, dtypes, index)
-    rows, width = value.shape
-    if width < 8 or width % 8 or (rows > 1 and value.stride(0) % 8) or value.data_ptr() % 16:
+def _operand(value, name: str, dtypes, index: int | None = None) -> tuple:
+    """A `row_matrix` that TMA can read: aligned, its row stride a multiple of 8."""
+    found = row_matrix(value, name, dtypes, index)
+    _, _, width, stride = found
+    if width < 8 or width % 8 or stride % 8 or value.data_ptr() % 16:
         raise ValueError(f"{name} must be 16-byte aligned with a width and row stride that are multiples of 8")
-    return index
+    return found
 
 
 def _expert_weight(weight, dtype, index: int) -> tuple:
@@ -279,24 +272,24 @@ def expert_linear(x, weight, offsets, *, rows=None, out=None):
     ``rows``, x's own rows are the sorted ones.  Sums are FP32, rounded once; rows of no group
     are zeros.  Returns y [R, N] (``out`` when given).
     """
-    index = _operand(x, "x", _kinds()[1])
+    index, T, width, stride = _operand(x, "x", _kinds()[1])
     E, N, K, by_expert, by_row = _expert_weight(weight, x.dtype, index)
-    T, width = x.shape
     if width != K:
         raise ValueError("x's width must be the weight's")
     R = group_tables(offsets, rows, E, T, index)
+    out_stride = N
     if out is None:
         out = x.new_empty((R, N))
     else:
-        row_matrix(out, "out", (x.dtype,), index)
+        out_stride = row_matrix(out, "out", (x.dtype,), index)[3]
         if out.shape != (R, N):
             raise ValueError("out must be [rows, out features]")
         output_is_distinct(out, (x, weight, offsets) if rows is None else (x, weight, offsets, rows))
     workspace, room = _gather_room(x, rows, E, R, K, False)
     _native.launch(
-        "lf_expert_linear", index, _native.dtype_code(x.dtype), x.data_ptr(), row_stride(x), T,
+        "lf_expert_linear", index, _native.dtype_code(x.dtype), x.data_ptr(), stride, T,
         None if rows is None else rows.data_ptr(), weight.data_ptr(), by_expert, by_row, offsets.data_ptr(), E, R, N, K,
-        out.data_ptr(), row_stride(out), workspace.data_ptr() if room else None, room,
+        out.data_ptr(), out_stride, workspace.data_ptr() if room else None, room,
     )
     return out
 
@@ -318,10 +311,9 @@ def expert_linear_backward(grad, x, weight, offsets, *, rows=None, weight_grad_d
     """
     import torch
 
-    index = _operand(x, "x", _kinds()[1])
+    index, T, width, x_stride = _operand(x, "x", _kinds()[1])
     E, N, K, by_expert, by_row = _expert_weight(weight, x.dtype, index)
-    _operand(grad, "grad", (x.dtype,), index)
-    T, width = x.shape
+    stride = _operand(grad, "grad", (x.dtype,), index)[3]
     if width != K:
         raise ValueError("x's width must be the weight's")
     R = group_tables(offsets, rows, E, T, index)
@@ -332,14 +324,14 @@ def expert_linear_backward(grad, x, weight, offsets, *, rows=None, weight_grad_d
         raise ValueError("weight_grad_dtype must be the operands' type or float32")
     grad_x = x.new_empty((R, K))
     grad_weight = x.new_empty((E, N, K), dtype=weight_grad_dtype)
-    dtype, stride = _native.dtype_code(x.dtype), row_stride(grad)
+    dtype = _native.dtype_code(x.dtype)
     _native.launch(
         "lf_expert_linear_input_grad", index, dtype, grad.data_ptr(), stride, weight.data_ptr(), by_expert, by_row,
         offsets.data_ptr(), E, R, N, K, grad_x.data_ptr(), K,
     )
     workspace, room = _gather_room(x, rows, E, R, K, True)
     _native.launch(
-        "lf_expert_linear_weight_grad", index, dtype, grad.data_ptr(), stride, x.data_ptr(), row_stride(x), T,
+        "lf_expert_linear_weight_grad", index, dtype, grad.data_ptr(), stride, x.data_ptr(), x_stride, T,
         None if rows is None else rows.data_ptr(), offsets.data_ptr(), E, R, N, K,
         _native.dtype_code(weight_grad_dtype), grad_weight.data_ptr(), workspace.data_ptr() if room else None, room,
     )

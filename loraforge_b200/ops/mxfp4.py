@@ -13,7 +13,7 @@ from typing import NamedTuple
 
 from loraforge_b200 import _native
 from loraforge_b200.ops._contract import output_is_distinct
-from loraforge_b200.ops.experts import MAX_EXPERTS, _kinds, cuda_tensor, group_tables, packed_table, row_matrix, row_stride
+from loraforge_b200.ops.experts import MAX_EXPERTS, _kinds, cuda_tensor, group_tables, packed_table, row_matrix
 
 BLOCK = 32
 
@@ -102,10 +102,11 @@ def expert_linear_mxfp4(x: MxTensor, weight: MxTensor, offsets, *, rows=None, dt
     R = group_tables(offsets, rows, E, T, index)
     if dtype is not None and dtype not in _kinds()[2]:
         raise ValueError("dtype must be float32, float16 or bfloat16")
+    out_stride = N
     if out is None:
         out = x.codes.new_empty((R, N), dtype=torch.bfloat16 if dtype is None else dtype)
     else:
-        row_matrix(out, "out", _kinds()[2] if dtype is None else (dtype,), index)
+        out_stride = row_matrix(out, "out", _kinds()[2] if dtype is None else (dtype,), index)[3]
         if out.shape != (R, N):
             raise ValueError("out must be [rows, out features]")
         output_is_distinct(out, (*x, *weight, offsets) if rows is None else (*x, *weight, offsets, rows))
@@ -114,6 +115,6 @@ def expert_linear_mxfp4(x: MxTensor, weight: MxTensor, offsets, *, rows=None, dt
     _native.launch(
         "lf_expert_linear_mxfp4", index, _native.dtype_code(out.dtype), x.codes.data_ptr(), x.scales.data_ptr(), T,
         None if rows is None else rows.data_ptr(), weight.codes.data_ptr(), weight.scales.data_ptr(),
-        offsets.data_ptr(), E, R, N, K, out.data_ptr(), row_stride(out), workspace.data_ptr() if room else None, room,
+        offsets.data_ptr(), E, R, N, K, out.data_ptr(), out_stride, workspace.data_ptr() if room else None, room,
     )
     return out
