@@ -214,6 +214,25 @@ __device__ __forceinline__ void ld_fragments(uint32_t taddr, uint32_t (&r)[32]) 
       : "r"(taddr), "r"(taddr + (16u << 16)));
 }
 
+// Rows of `words` 16-byte words to `out` in the order of `rows`, zeros for an index outside x: one
+// warp a row, eight words a lane in flight.
+__device__ __forceinline__ void copy_row(const uint4* x, int64_t stride, int x_rows, const int32_t* rows, int64_t r,
+                                         int words, uint4* out, int lane) {
+  const int src = rows[r];
+  const bool live = src >= 0 && src < x_rows;
+  const uint4* from = x + (live ? src * stride : 0);
+  uint4* to = out + r * words;
+  for (int c = lane; c < words; c += 256) {
+    uint4 v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (c + 32 * u < words) v[u] = live ? from[c + 32 * u] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (c + 32 * u < words) to[c + 32 * u] = v[u];
+  }
+}
+
 // ------------------------------------------------------------------ tiles of ragged groups
 __host__ __device__ constexpr int ceil_div(int a, int b) { return (a + b - 1) / b; }
 __host__ __device__ constexpr int round_up(int a, int b) { return (a + b - 1) / b * b; }

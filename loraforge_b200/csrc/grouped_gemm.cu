@@ -380,24 +380,14 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(const __grid_const
   }
 }
 
-// out[r] = x[rows[r]], zeros for an index outside x: 16 bytes a thread and step, four in flight.
+// out[r] = x[rows[r]], eight rows a block (a thread that divides its way to row and column for every
+// 16 bytes took 8 us for 6000 rows of 4 KB).
 __global__ void __launch_bounds__(256) gather_rows_kernel(const uint4* x, int64_t stride, int x_rows,
-                                                          const int32_t* rows, int chunks, int64_t total, uint4* out) {
+                                                          const int32_t* rows, int words, int64_t R, uint4* out) {
   pdl_wait();
   pdl_launch_dependents();
-  const int64_t first = int64_t(blockIdx.x) * 1024 + threadIdx.x;
-  uint4 v[4];
-#pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    const int64_t i = first + u * 256;
-    if (i >= total) continue;
-    const int64_t r = i / chunks;
-    const int src = rows[r];
-    v[u] = src >= 0 && src < x_rows ? x[src * stride + (i - r * chunks)] : make_uint4(0, 0, 0, 0);
-  }
-#pragma unroll
-  for (int u = 0; u < 4; ++u)
-    if (first + u * 256 < total) out[first + u * 256] = v[u];
+  const int64_t r = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (r < R) copy_row(x, stride, x_rows, rows, r, words, out, threadIdx.x & 31);
 }
 
 int gather_rows(const void* x, int64_t x_stride, int64_t x_rows, const int32_t* rows, int64_t R, int64_t width,
@@ -408,13 +398,12 @@ int gather_rows(const void* x, int64_t x_stride, int64_t x_rows, const int32_t* 
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   config.attrs = attr;
   config.numAttrs = 1;
-  const int64_t total = R * (width / 8);
-  config.gridDim = dim3(unsigned((total + 1023) / 1024));
+  config.gridDim = dim3(unsigned((R + 7) / 8));
   config.blockDim = dim3(256);
   config.stream = static_cast<cudaStream_t>(stream);
   const cudaError_t err =
       cudaLaunchKernelEx(&config, gather_rows_kernel, static_cast<const uint4*>(x), x_stride / 8, int(x_rows), rows,
-                         int(width / 8), total, static_cast<uint4*>(out));
+                         int(width / 8), R, static_cast<uint4*>(out));
   if (err != cudaSuccess) {
     last_error() = std::string(what) + ": " + cudaGetErrorString(err);
     return LF_E_CUDA;

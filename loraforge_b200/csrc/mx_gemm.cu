@@ -24,8 +24,6 @@
 //           were slower than the MMAs.
 //   narrow  every warp reads all rows itself (three of four times from a cache): 32 bytes, a
 //           whole sector, of each row for four stages, one such group ahead, also across tiles.
-// A narrow tile's MMAs have N = 32 at least: with 16 they were slower (eight 14336 x 4096 experts,
-// 16 rows: 60 us against 63).
 //
 // Per CTA: warp 0 loads (TMA), warp 1 MMA and TMEM, warps 2-5 store, warps 6-9 scales.
 // Every wait is bounded (tma.cuh): an expiry stops every role at its next wait.
@@ -140,7 +138,7 @@ struct Tiles {
     x.row_tile = row_tiles + walk.n;
     x.n0 = walk.lo + walk.n * each;
     x.valid = min(each, x.hi - x.n0);
-    x.nt = round_up(x.valid, kCtas == 1 ? 32 : 16);
+    x.nt = round_up(x.valid, 16);
     return x;
   }
 };
@@ -543,7 +541,7 @@ __device__ __forceinline__ void pack_groups(const uint8_t* const (&row)[4], int 
 constexpr int kPackThreads = 256;
 
 // One CUDA block writes the scale blocks of 128 features, or of a row tile (2 x 128 rows), a warp
-// those of four groups at a time.  Or it moves 1024 16-byte words of codes.
+// those of four groups at a time.  Or it moves eight rows of codes.
 template <int kNT>
 __global__ void __launch_bounds__(kPackThreads) pack_kernel(const __grid_constant__ PackParams p) {
   __shared__ int scan[kMaxWarps];
@@ -587,20 +585,8 @@ __global__ void __launch_bounds__(kPackThreads) pack_kernel(const __grid_constan
     return;
   }
   task -= p.x_tasks;
-  const int64_t total = int64_t(p.R) * p.words;
-  const int64_t at = int64_t(task) * (4 * kPackThreads) + tid;
-  uint4 v[4];
-#pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    const int64_t i = at + u * kPackThreads;
-    if (i >= total) continue;
-    const int64_t r = i / p.words;
-    const int src = p.rows[r];
-    v[u] = src >= 0 && src < p.x_rows ? p.x_codes[int64_t(src) * p.words + (i - r * p.words)] : make_uint4(0, 0, 0, 0);
-  }
-#pragma unroll
-  for (int u = 0; u < 4; ++u)
-    if (at + u * kPackThreads < total) p.codes[at + u * kPackThreads] = v[u];
+  const int64_t r = int64_t(task) * (kPackThreads / 32) + warp;
+  if (r < p.R) copy_row(p.x_codes, p.words, p.x_rows, p.rows, r, p.words, p.codes, lane);
 }
 
 template <int kCtas, int kNT>
@@ -722,7 +708,7 @@ extern "C" int lf_expert_linear_mxfp4(int32_t out_dtype, const uint8_t* x_codes,
     k.words = int(width / 32), k.w_tasks = w.groups ? int(w.w_blocks / w.groups) : 0, k.x_tasks = int(w.row_tiles);
     const uintptr_t bits = reinterpret_cast<uintptr_t>(x_scales) | reinterpret_cast<uintptr_t>(w_scales) | uintptr_t(p.blocks);
     k.align = bits & 3 ? 1 : bits & 15 ? 4 : 16;
-    const int64_t moves = move ? (num_rows * k.words + 4 * kPackThreads - 1) / (4 * kPackThreads) : 0;
+    const int64_t moves = move ? (num_rows + kPackThreads / 32 - 1) / (kPackThreads / 32) : 0;
     if (int rc = launch_clusters(pack_kernel<kWideRows>, int(k.w_tasks + k.x_tasks + moves), kPackThreads, 1,
                                  int(sizeof(int)) * 2 * (p.E + 1), stream, "expert_linear_mxfp4 (scales)", k))
       return rc;
