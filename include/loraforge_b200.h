@@ -498,9 +498,9 @@ int lf_mxfp4_dequantize(int32_t dtype, const uint8_t* codes, const uint8_t* scal
  * sums on the block-scaled tensor cores, one rounding to out_dtype:
  *   y[r, n] = sum_k x[i(r), k] w[e, n, k]  for rows r of group e, as in lf_expert_linear.
  * x [x_rows, width], w [num_experts, out_width, width], both contiguous; width a multiple of 32.
- * Groups of many rows lay out the scales, and with rows, those of more than a few x's codes in
- * order, in `workspace` first: lf_expert_linear_mxfp4_workspace_bytes bytes, 16-byte aligned,
- * not initialised (0: none needed; by_rows: whether rows is given).
+ * Groups of more than a few rows lay out the scales, and with rows x's codes in order, in
+ * `workspace` first: lf_expert_linear_mxfp4_workspace_bytes bytes, 16-byte aligned, not
+ * initialised (0: none needed; by_rows: whether rows is given).
  */
 int64_t lf_expert_linear_mxfp4_workspace_bytes(int32_t num_experts, int64_t num_rows,
                                                int64_t out_width, int64_t width,

@@ -504,12 +504,6 @@ __device__ __forceinline__ bool store_split(const Output& o, uint32_t d, bool li
   return true;
 }
 
-// Rows by index: with at most `most` a group on average the loads gather them, else they are put in
-// order first.  A gather4 fetches four rows of a stage and costs nothing beside the weights until
-// there are too many: two in the 16-bit products (64 experts of 2048 x 2048: 2 rows each 84 us
-// against 83 with rows in order, 16 rows 97 against 86), four in the MXFP4 ones.
-inline bool gather_in_loads(int64_t E, int64_t R, int most) { return R <= most * (E < R ? E : R); }
-
 // How the narrow kernels cut the work: `height` features a tile (the MMA always takes 128 lanes;
 // rows of A past the height are neither loaded nor stored) and the contraction over `split` CTAs.
 struct Cut {

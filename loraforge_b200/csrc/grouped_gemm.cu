@@ -440,11 +440,19 @@ int launch_grouped(GParams& p, int64_t tiles, void* stream, const char* what) {
                          smem_of<kCtas, kNT>(p.E), stream, what, p);
 }
 
-constexpr int kWideRows = 256, kNarrowRows = 64, kFewRows = 32, kGatherRows = 8;
+constexpr int kWideRows = 256, kNarrowRows = 64, kFewRows = 32;
 constexpr char kNoWorkspace[] = "expert_linear: workspace missing, too small or not 16-byte aligned (see lf_expert_linear_workspace_bytes)";
 
-// Groups of up to 64 rows on average take the narrow tiles.
-bool narrow(int64_t E, int64_t R) { return R <= kNarrowRows * (E < R ? E : R); }
+// Groups of up to 24 rows on average take the narrow tiles.  64 experts of 2048 x 2048: 20 rows each
+// 89 us against 91 in pairs, 40 rows 99 against 95, and 40 on average but unequal (the first expert
+// has 580) 116 against 99, as narrow tiles read the weights again for every 64 rows.
+bool narrow(int64_t E, int64_t R) { return R <= 24 * (E < R ? E : R); }
+
+// Rows by index: with up to eight a group on average the loads gather them, else they are put in
+// order first.  Two gather4 a stage, of four rows each, cost next to nothing beside the weights (64
+// experts of 2048 x 2048, 2 rows each: 84 us against 83 with rows in order), four do (16 rows: 97
+// against 86).
+bool gather_in_loads(int64_t E, int64_t R) { return R <= 8 * (E < R ? E : R); }
 
 int check_sizes(const char* what, int dtype, int E, int64_t R, int64_t N, int64_t K) {
   const int64_t limit = int64_t(1) << 31;
@@ -509,7 +517,9 @@ int launch_rows(GParams& p, CUtensorMapDataType type, const Weights& w, void* st
     if (kMode == kForward && !encode_weights(&p.a_map, type, w.data, w.K, w.N, p.E, w.row_stride, w.expert_stride, cut.height))
       return fail(LF_E_CUDA, (std::string(what) + ": cuTensorMapEncodeTiled failed").c_str());
     const int64_t mt = ceil_div(p.M, cut.height);  // tiles: at most
-    if (p.R <= kFewRows / 2 * groups) return launch_grouped<kMode, 1, kFewRows>(p, mt * (groups + p.R / kFewRows), stream, what);
+    // Tiles of 32 rows up to 16 on average: 20 rows each took 95 us in them against 89 in tiles of 64.
+    if (p.R <= kFewRows / 2 * groups)
+      return launch_grouped<kMode, 1, kFewRows>(p, mt * (groups + p.R / kFewRows), stream, what);
     return launch_grouped<kMode, 1, kNarrowRows>(p, mt * (groups + p.R / kNarrowRows), stream, what);
   }
   p.height = 128, p.split = 1;
@@ -539,7 +549,7 @@ using namespace lfb;
 extern "C" int64_t lf_expert_linear_workspace_bytes(int32_t num_experts, int64_t num_rows, int64_t width,
                                                     int32_t weight_grad) {
   if (num_experts < 1 || num_rows < 0 || width < 1) return -1;
-  return weight_grad || !gather_in_loads(num_experts, num_rows, kGatherRows) ? num_rows * width * 2 : 0;
+  return weight_grad || !gather_in_loads(num_experts, num_rows) ? num_rows * width * 2 : 0;
 }
 
 extern "C" int lf_expert_linear(int32_t dtype, const void* x, int64_t x_stride, int64_t x_rows, const int32_t* rows,

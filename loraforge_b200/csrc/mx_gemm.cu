@@ -9,7 +9,7 @@
 //
 // The tiles are those of the 16-bit products (grouped_gemm.cu): features on the TMEM lanes,
 // rows on the columns, CTA pairs with 256 features x up to 208 rows, or single CTAs with up to
-// 128 x 32 or 64 whose contraction may be split over a cluster.  208, not 256, rows: two
+// 128 x 32 whose contraction may be split over a cluster.  208, not 256, rows: two
 // accumulators of 208 columns leave 96 TMEM columns for four sets of scales.
 //
 // Scales.  The tensor core wants them in TMEM: for 128 operand rows and 128 codes a row, four
@@ -53,8 +53,6 @@ struct MxParams {
   const uint8_t* x_blocks;
   int groups;            // of 128 codes in them, an even number
   int height, split;
-  int gathered;  // x's codes (not its scales) are in the rows' order
-  int prepared;  // the grid before is pack_kernel: all but what it packs can be read before it ends
   Bands bands;
   CUtensorMap w_map;      // 128 bytes x 128 rows
   CUtensorMap x_map[7];   // 128 bytes x 16, 32, .. 112 rows
@@ -211,7 +209,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
     *abort = 0;
   }
   Tiles<kCtas, kNT> walk;
-  if (!p.prepared) pdl_wait();
+  if (kCtas == 1) pdl_wait();  // wide: the grid before is pack_kernel, and all but what it packs can be read before it ends
   if (warp == 1) alloc_tmem<kCtas>(tslot, S::kColumns);  // not while waiting for a grid that may want some too
   const int mtiles = p.bands.mt;
   list_tiles(p.offsets, p.E, p.R, bounds, starts, scan, [&](int rows) { return mtiles * ceil_div(rows, kNT); });
@@ -237,11 +235,10 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
   if (warp == 0) {
     // ------------------------------------------------------------ codes
     const bool elected = elect_one();
-    if (p.prepared) {
+    if (kCtas == 2) {
       if (lane == 0 && first < tiles) {
         const Tile x = walk.at(p, bounds, starts, first);
-        for (int ks = ks0; ks < min(ks1, ks0 + kAhead); ++ks)
-          prefetch_3d(&p.w_map, ks * 128, x.m0 + (kCtas == 2 ? rank * 128 : 0), x.e);
+        for (int ks = 0; ks < min(steps, kAhead); ++ks) prefetch_3d(&p.w_map, ks * 128, x.m0 + rank * 128, x.e);
       }
       __syncwarp();
       walk = {};
@@ -253,7 +250,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
       const int m_cta = x.m0 + (kCtas == 2 ? rank * 128 : 0);
       const int share = kCtas == 1 ? x.valid : x.nt / kCtas;
       const int n_cta = x.n0 + (kCtas == 2 ? rank * share : 0);
-      const bool by_row = kCtas == 1 && p.rows && !p.gathered;
+      const bool by_row = kCtas == 1 && p.rows;
       int row4[4];
       if (by_row) {
 #pragma unroll
@@ -490,9 +487,12 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
   }
 }
 
-constexpr int kWideRows = 208, kNarrowRows = 64, kFewRows = 32, kGatherRows = 16;
+constexpr int kWideRows = 208, kNarrowRows = 32;
 
-bool narrow(int64_t E, int64_t R) { return R <= kNarrowRows * (E < R ? E : R); }
+// Groups of up to 16 rows on average take the narrow tiles, whose loads gather rows by index; the
+// others' codes are put in order and the scales packed first.  64 experts of 2048 x 2048: 9 rows each
+// 34 us against 36, 17 rows 41 against 38, 40 unequal ones 51 against 43.
+bool narrow(int64_t E, int64_t R) { return R <= 16 * (E < R ? E : R); }
 
 // The wide tiles' workspace: W's scales as blocks [expert][128 features][group of 128 codes],
 // x's as [row tile][group][half], and x's codes in the rows' order.
@@ -622,20 +622,19 @@ bool encode_codes(CUtensorMap* map, const void* p, int64_t bytes, int64_t rows, 
   return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, p, dims, strides, box);
 }
 
-// Sizes of the workspace: 512-byte blocks of W's and of x's scales (wide tiles), then codes.
+// Sizes of the wide tiles' workspace: 512-byte blocks of W's and of x's scales, then codes.
 struct Workspace {
   int groups;
   int64_t row_tiles, w_blocks, x_blocks, bytes;
 };
 Workspace workspace_of(int64_t E, int64_t R, int64_t N, int64_t K, bool by_rows) {
   Workspace w{};
-  if (!narrow(E, R)) {
-    w.groups = 2 * int((K + kStep - 1) / kStep);
-    w.row_tiles = (E < R ? E : R) + R / kWideRows;  // at most
-    w.w_blocks = E * ((N + 255) / 256) * 2 * w.groups;
-    w.x_blocks = w.row_tiles * w.groups * 2;
-  }
-  w.bytes = (w.w_blocks + w.x_blocks) * 512 + (by_rows && !gather_in_loads(E, R, kGatherRows) ? R * (K / 2) : 0);
+  if (narrow(E, R)) return w;
+  w.groups = 2 * int((K + kStep - 1) / kStep);
+  w.row_tiles = (E < R ? E : R) + R / kWideRows;  // at most
+  w.w_blocks = E * ((N + 255) / 256) * 2 * w.groups;
+  w.x_blocks = w.row_tiles * w.groups * 2;
+  w.bytes = (w.w_blocks + w.x_blocks) * 512 + (by_rows ? R * (K / 2) : 0);
   return w;
 }
 
@@ -676,7 +675,7 @@ extern "C" int lf_expert_linear_mxfp4(int32_t out_dtype, const uint8_t* x_codes,
   if (out_dtype < LF_F32 || out_dtype > LF_BF16) return fail(LF_E_INVALID, "expert_linear_mxfp4: unknown output type");
   if (num_experts < 1 || num_experts > kMaxExperts || num_rows < 0 || num_rows >= limit - 256 || out_width < 1 ||
       out_width >= limit - 256 || width < 32 || width % 32 || width >= limit - 256 ||
-      (num_rows / kFewRows + num_experts + 1) * (out_width / 64 + 1) >= limit)
+      (num_rows / kNarrowRows + num_experts + 1) * (out_width / 64 + 1) >= limit)
     return fail(LF_E_INVALID, "expert_linear_mxfp4: needs 1..1024 experts, a width that is a multiple of 32, and rows and tiles that fit int32");
   if (num_rows == 0) return LF_OK;
   if (!x_codes || !x_scales || !w_codes || !w_scales || !offsets || !y || y_stride < out_width || !aligned16(x_codes) ||
@@ -692,30 +691,28 @@ extern "C" int lf_expert_linear_mxfp4(int32_t out_dtype, const uint8_t* x_codes,
   p.x_align = row_alignment(x_scales, p.blocks), p.w_align = row_alignment(w_scales, p.blocks);
   const bool few = narrow(num_experts, num_rows);
   int64_t code_rows = x_rows;
-  const Workspace w = workspace_of(num_experts, num_rows, out_width, width, rows != nullptr);
-  if (w.bytes) {
+  if (!few) {
+    const Workspace w = workspace_of(num_experts, num_rows, out_width, width, rows != nullptr);
     if (!workspace || workspace_bytes < w.bytes || !aligned16(workspace))
       return fail(LF_E_INVALID, "expert_linear_mxfp4: workspace missing, too small or not 16-byte aligned "
                                 "(see lf_expert_linear_mxfp4_workspace_bytes)");
     if (w.w_blocks >= limit || w.x_blocks >= limit)
       return fail(LF_E_INVALID, "expert_linear_mxfp4: too many scale blocks");
-    const bool move = rows && !gather_in_loads(num_experts, num_rows, kGatherRows);
     PackParams k{};
     k.offsets = offsets, k.rows = rows, k.x_scales = x_scales, k.w_scales = w_scales;
     k.w_blocks = static_cast<uint8_t*>(workspace), k.x_blocks = k.w_blocks + w.w_blocks * 512;
     k.codes = reinterpret_cast<uint4*>(k.x_blocks + w.x_blocks * 512);
     k.x_codes = reinterpret_cast<const uint4*>(x_codes);
     k.E = p.E, k.R = p.R, k.x_rows = p.x_rows, k.N = p.N, k.blocks = p.blocks, k.groups = w.groups;
-    k.words = int(width / 32), k.w_tasks = w.groups ? int(w.w_blocks / w.groups) : 0, k.x_tasks = int(w.row_tiles);
+    k.words = int(width / 32), k.w_tasks = int(w.w_blocks / w.groups), k.x_tasks = int(w.row_tiles);
     const uintptr_t bits = reinterpret_cast<uintptr_t>(x_scales) | reinterpret_cast<uintptr_t>(w_scales) | uintptr_t(p.blocks);
     k.align = bits & 3 ? 1 : bits & 15 ? 4 : 16;
-    const int64_t moves = move ? (num_rows + kPackThreads / 32 - 1) / (kPackThreads / 32) : 0;
+    const int64_t moves = rows ? (num_rows + kPackThreads / 32 - 1) / (kPackThreads / 32) : 0;
     if (int rc = launch_clusters(pack_kernel<kWideRows>, int(k.w_tasks + k.x_tasks + moves), kPackThreads, 1,
                                  int(sizeof(int)) * 2 * (p.E + 1), stream, "expert_linear_mxfp4 (scales)", k))
       return rc;
-    if (move) x_codes = reinterpret_cast<const uint8_t*>(k.codes), code_rows = num_rows, p.gathered = 1;
-    p.groups = w.groups, p.prepared = 1;
-    p.w_blocks = k.w_blocks, p.x_blocks = k.x_blocks;
+    if (rows) x_codes = reinterpret_cast<const uint8_t*>(k.codes), code_rows = num_rows;
+    p.groups = w.groups, p.w_blocks = k.w_blocks, p.x_blocks = k.x_blocks;
   }
   const cuuint64_t dims[3] = {cuuint64_t(width / 2), cuuint64_t(out_width), cuuint64_t(num_experts)};
   const cuuint64_t strides[2] = {cuuint64_t(width / 2), cuuint64_t(width / 2) * cuuint64_t(out_width)};
@@ -729,15 +726,11 @@ extern "C" int lf_expert_linear_mxfp4(int32_t out_dtype, const uint8_t* x_codes,
   p.height = cut.height, p.split = cut.split;
   const cuuint32_t box[3] = {128, cuuint32_t(cut.height), 1};
   bool ok = encode_map(&p.w_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, w_codes, dims, strides, box);
-  if (rows && few && !p.gathered) ok = ok && encode_codes(&p.x_gather, x_codes, width / 2, code_rows, 1);
+  if (rows && few) ok = ok && encode_codes(&p.x_gather, x_codes, width / 2, code_rows, 1);
   else
     for (int i = 0; i < (few ? kNarrowRows / 16 : 7) && ok; ++i)
       ok = encode_codes(&p.x_map[i], x_codes, width / 2, code_rows, 16 * (i + 1));
   if (!ok) return fail(LF_E_CUDA, "expert_linear_mxfp4: cuTensorMapEncodeTiled failed");
-  if (few) {
-    const int64_t mt = ceil_div(p.N, cut.height);  // tiles: at most
-    if (num_rows <= kFewRows / 2 * groups) return launch_mx<1, kFewRows>(p, mt * (groups + num_rows / kFewRows), stream);
-    return launch_mx<1, kNarrowRows>(p, mt * (groups + num_rows / kNarrowRows), stream);
-  }
+  if (few) return launch_mx<1, kNarrowRows>(p, ceil_div(p.N, cut.height) * (groups + num_rows / kNarrowRows), stream);
   return launch_mx<2, kWideRows>(p, int64_t(ceil_div(p.N, 256)) * (groups + num_rows / kWideRows), stream);
 }
