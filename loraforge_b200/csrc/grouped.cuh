@@ -435,16 +435,17 @@ __device__ __forceinline__ void store_chunk(uint32_t taddr, bool live, uint32_t 
 }
 
 // A tile's columns 0 .. valid - 1 of this warp's features f0 .. f0 + 31, those below `end` (TMEM
-// address `d`; zeros unless live), to rows row0 + column.
+// address `d`; zeros unless live), to rows row0 + column; of `parts` warps this one takes chunk `part`,
+// part + parts, ...
 __device__ __forceinline__ void store_whole(const Output& o, uint32_t d, bool live, int f0, int end, int64_t row0, int nt,
-                                            int valid, uint32_t staging, int lane) {
+                                            int valid, uint32_t staging, int lane, int part = 0, int parts = 1) {
   if (o.type != LF_F32 && (reinterpret_cast<uintptr_t>(o.data) & 15) == 0 && o.stride % 8 == 0 && o.features % 8 == 0) {
     uint8_t* dst = static_cast<uint8_t*>(o.data) + (row0 * o.stride + f0) * 2;
-    for (int c0 = 0; c0 < valid; c0 += 32)
+    for (int c0 = 32 * part; c0 < valid; c0 += 32 * parts)
       store_chunk(d + uint32_t(c0), live, staging, o.type == LF_BF16, dst + c0 * o.stride * 2, o.stride * 2, valid - c0,
                   end - f0, lane);
   } else {
-    for (int c0 = 0; c0 < nt; c0 += 16) {
+    for (int c0 = 16 * part; c0 < nt; c0 += 16 * parts) {
       uint32_t r[16];
       if (live) tc_ld16(d + uint32_t(c0), r);
 #pragma unroll

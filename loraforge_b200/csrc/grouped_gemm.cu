@@ -25,8 +25,8 @@
 // copies them into the caller's workspace first (2 x 134 MB there, 35 us).
 //
 // Per CTA: warp 0 loads 64-deep stages into a ring, warp 1 issues the MMAs and owns the TMEM
-// (two accumulators, so a tile's stores overlap the next tile's MMAs), warps 2-5 store.  The
-// grid is persistent and computes its tile list from `offsets` on the device.
+// (two accumulators, so a tile's stores overlap the next tile's MMAs), warps 2-5 store (2-9 for short
+// contractions).  The grid is persistent and computes its tile list from `offsets` on the device.
 //
 //   wide    CTA pairs (cta_group::2), 256 x 256 tiles: each CTA loads half of both operands.
 //   narrow  one CTA, up to 128 features x up to 32 or 64 rows, for groups of few rows, where the
@@ -36,7 +36,8 @@
 //
 // Measured: 8 x 2048 rows, 4096 -> 14336: 1262 us (1524 TFLOP/s; later calls 1345-1480 under the
 // power cap, as a dense library product of that size), input gradient 1455, weight gradient 1333;
-// 64 experts of 2048 x 2048, 2 rows each: 83 us (268 MB of weights at 6.4 TB/s).
+// 64 experts of 2048 x 2048, 2 rows each: 83 us (268 MB of weights at 6.4 TB/s); dW of 64 experts of
+// 1536 x 2048, 64 rows each: 136 us, bound by its writes (403 MB; a plain fill of them takes 131).
 //
 // Every wait is bounded (tma.cuh): an expiry stops every role at its next wait.
 #include "experts.cuh"
@@ -49,7 +50,6 @@ using namespace grouped;
 
 enum Mode { kForward = 0, kInput = 1, kWeight = 2 };
 
-constexpr int kThreads = 192;         // warp 0 loads, warp 1 MMA, warps 2-5 store (TMEM lane quarter = warp & 3)
 constexpr int kStep = 64;             // contraction per stage: 128 bytes
 constexpr int kABytes = 128 * 128;    // 128 features x 128 bytes (K-major), or two 64-feature boxes of 64 steps
 
@@ -60,7 +60,7 @@ struct GParams {
   int E, R, x_rows;
   int M, C;  // output features, contraction (forward K, input N; weight: the groups' rows)
   int N;     // weight: columns of D (dy's features)
-  int elem_bf16, height, split;
+  int elem_bf16, height, split, store_sets;
   int prepared;  // the grid before this one only put x's rows in order: all else can be read before it ends
   Bands bands;
   CUtensorMap a_map;     // forward: W boxes 64 k x 128 n; input: 64 k x 64 n; weight: x boxes 64 k x 64 rows
@@ -76,7 +76,9 @@ template <int kCtas, int kNT>
 struct Shape {
   static constexpr int kBRows = kNT / kCtas;  // a CTA's share of the columns
   static constexpr int kStageBytes = kABytes + kBRows * 128;
-  static constexpr int kPartBytes = kCtas == 1 ? kNT * 128 * 4 : 4 * kChunkBytes;  // sums, or the stores' staging
+  static constexpr int kStoreSets = kCtas == 1 ? 1 : 2;     // at most
+  static constexpr int kThreads = 64 + 128 * kStoreSets;  // warp 0 loads, warp 1 MMA, then sets of four that store
+  static constexpr int kPartBytes = kCtas == 1 ? kNT * 128 * 4 : kStoreSets * 4 * kChunkBytes;  // sums, or the stores' staging
   static constexpr int kStages = stages_of(kStageBytes, kPartBytes);  // what is in flight hides some 2 us a load
   static constexpr int kColumns = 2 * kNT;  // TMEM
 };
@@ -126,7 +128,7 @@ struct Tiles {
 };
 
 template <int kMode, int kCtas, int kNT>
-__global__ void __launch_bounds__(kThreads, 1) grouped_kernel(const __grid_constant__ GParams p) {
+__global__ void __launch_bounds__((Shape<kCtas, kNT>::kThreads), 1) grouped_kernel(const __grid_constant__ GParams p) {
   using S = Shape<kCtas, kNT>;
   constexpr int kStages = S::kStages;
   extern __shared__ uint8_t smem_raw[];
@@ -144,7 +146,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(const __grid_const
   uint32_t* tslot = reinterpret_cast<uint32_t*>(fin + 1);
   volatile int* abort = reinterpret_cast<volatile int*>(tslot + 1);
   int* scan = reinterpret_cast<int*>(tslot + 2);  // one int a warp
-  int* bounds = scan + 6;                         // [E + 1]
+  int* bounds = scan + kMaxWarps;                         // [E + 1]
   int* starts = bounds + p.E + 1;                 // [E + 1]
 
   // Pair: rank 0 issues the MMAs of both CTAs.  Split: the cluster's CTAs share the contraction.
@@ -157,7 +159,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(const __grid_const
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_empty[i], 4 * kCtas);
+      mbar_init(&acc_empty[i], 4 * p.store_sets * kCtas);
     }
     mbar_init(part_full, 4 * cluster);
     mbar_init(part_empty, 4 * cluster);
@@ -340,7 +342,7 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(const __grid_const
     // ------------------------------------------------------------ stores
     const int quarter = warp & 3;
     const uint32_t lanes = uint32_t(quarter * 32) << 16;
-    const uint32_t staging = smem_u32(part) + uint32_t(quarter * kChunkBytes);
+    const uint32_t staging = smem_u32(part) + uint32_t((warp - 2) * kChunkBytes);
     int count = 0, parts = 0;
     for (int t = first; t < tiles; t += stride) {
       const Tile x = walk.at(p, bounds, starts, t);
@@ -370,7 +372,8 @@ __global__ void __launch_bounds__(kThreads, 1) grouped_kernel(const __grid_const
           break;
         ++parts;
       } else {
-        store_whole(p.out, d, live, f0, x.end, row0, x.nt, x.valid, staging, lane);
+        store_whole(p.out, d, live, f0, x.end, row0, x.nt, x.valid, staging, lane, (warp - 2) >> 2,
+                    p.store_sets);
         release();
       }
     }
@@ -426,17 +429,24 @@ int clusters_at_once(Clusters* out) {
   const auto kernel = grouped_kernel<kMode, kCtas, kNT>;
   static int flags[64] = {};
   if (int rc = ensure_smem(kernel, smem_of<kCtas, kNT>(kMaxExperts), flags)) return rc;
-  return clusters_of(kernel, kThreads, smem_of<kCtas, kNT>(kMaxExperts), out);
+  return clusters_of(kernel, (Shape<kCtas, kNT>::kThreads), smem_of<kCtas, kNT>(kMaxExperts), out);
 }
+
+// Pairs with a contraction of up to kShort store with eight warps a CTA instead of four, which do not
+// keep up with the MMAs of so few steps.  16 experts, dW of 4096 x 2048: 128 rows each 94 us against
+// 107, 768 rows 175 against 190, but 1024 rows 234 against 224, as the stores then come in the way of
+// the loads; forward to 4096 features, 1024 rows each: 512 wide 94 against 98, 2048 wide 236 against 228.
+constexpr int kShort = 768;
 
 template <int kMode, int kCtas, int kNT>
 int launch_grouped(GParams& p, int64_t tiles, void* stream, const char* what) {
   p.bands = bands_of(ceil_div(p.M, p.height * kCtas));
   const int cluster = kCtas == 2 ? 2 : p.split;
+  p.store_sets = kCtas == 2 && (kMode == kWeight ? p.R / (p.E < p.R ? p.E : p.R) : p.C) <= kShort ? 2 : 1;
   Clusters clusters;
   if (int rc = clusters_at_once<kMode, kCtas, kNT>(&clusters)) return rc;
   const int64_t most = tiles < clusters.at_once[cluster] ? tiles : clusters.at_once[cluster];
-  return launch_clusters(grouped_kernel<kMode, kCtas, kNT>, int(most * cluster), kThreads, cluster,
+  return launch_clusters(grouped_kernel<kMode, kCtas, kNT>, int(most * cluster), 64 + 128 * p.store_sets, cluster,
                          smem_of<kCtas, kNT>(p.E), stream, what, p);
 }
 

@@ -106,6 +106,29 @@ def test_contractions_split_over_a_cluster(counts, N, K):
     assert _native.device_wait_timeouts(reset=True) == 0
 
 
+# Rows on average where the tiles change (16 and 24 rows a group), with groups of one row and of
+# more than a tile's, and contractions where the stores do (768).
+@pytest.mark.parametrize("counts", [[16] * 4, [1, 64, 0, 3], [20, 17, 15, 20], [1, 90, 4, 1], [24] * 4, [25, 24, 25, 24]])
+@pytest.mark.parametrize("N,K", [(136, 776), (776, 768), (520, 264)])
+def test_sizes_where_the_tiles_change(counts, N, K):
+    x, w, offsets, rows, grad = make(counts, N, K, torch.bfloat16, seed=sum(counts) + K, tail=0)
+    y = expert_linear(x, w, offsets, rows=rows)
+    check_forward(x, w, offsets, rows, y)
+    assert torch.equal(expert_linear(x[rows.long()].contiguous(), w, offsets), y)
+    check_backward(grad, x, w, offsets, rows, *expert_linear_backward(grad, x, w, offsets, rows=rows))
+    assert _native.device_wait_timeouts(reset=True) == 0
+
+
+@pytest.mark.parametrize("counts", [[768], [769], [1500, 36], [2, 1536]])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_weight_gradients_of_many_rows(counts, dtype):
+    x, w, offsets, rows, grad = make(counts, 328, 520, dtype, seed=sum(counts))
+    check_backward(grad, x, w, offsets, rows, *expert_linear_backward(grad, x, w, offsets, rows=rows))
+    dx, dw = expert_linear_backward(grad, x, w, offsets, rows=rows, weight_grad_dtype=torch.float32)
+    check_backward(grad, x, w, offsets, rows, dx, dw)
+    assert _native.device_wait_timeouts(reset=True) == 0
+
+
 def test_large_products():
     x, w, offsets, rows, grad = make([1500, 260, 2000, 3], 2048, 1024, torch.bfloat16, seed=1)
     check_forward(x, w, offsets, rows, expert_linear(x, w, offsets, rows=rows))

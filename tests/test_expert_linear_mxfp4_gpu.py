@@ -96,6 +96,18 @@ def test_contractions_split_over_a_cluster(counts, N, K):
     assert _native.device_wait_timeouts(reset=True) == 0
 
 
+# Rows on average where the tiles change (16 a group), with groups of more than a tile's rows.
+@pytest.mark.parametrize("counts", [[16] * 4, [17, 16, 16, 16], [1, 60, 0, 3], [1, 60, 2, 3], [31, 33, 0, 0]])
+@pytest.mark.parametrize("N,K", [(136, 800), (520, 2272)])
+def test_sizes_where_the_tiles_change(counts, N, K):
+    x, w, offsets, rows = make(counts, N, K, seed=sum(counts) + K)
+    y = expert_linear_mxfp4(x, w, offsets, rows=rows, dtype=torch.float32)
+    check(x, w, offsets, rows, y)
+    ordered = MxTensor(x.codes[rows.long()].contiguous(), x.scales[rows.long()].contiguous())
+    assert torch.equal(expert_linear_mxfp4(ordered, w, offsets, dtype=torch.float32), y)
+    assert _native.device_wait_timeouts(reset=True) == 0
+
+
 def test_large_products():
     x, w, offsets, rows = make([1500, 260, 2000, 3], 2048, 1024, seed=1)
     check(x, w, offsets, rows, expert_linear_mxfp4(x, w, offsets, rows=rows))
