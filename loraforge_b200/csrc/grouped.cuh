@@ -18,7 +18,7 @@ namespace grouped {
 using namespace tc;
 
 constexpr int kMaxExperts = 1024;
-constexpr int kMaxWarps = 10;
+constexpr int kMaxWarps = 14;
 
 // Stages that fit beside `other` bytes of shared memory (and the tables of kMaxExperts groups).
 constexpr int stages_of(int stage_bytes, int other) {

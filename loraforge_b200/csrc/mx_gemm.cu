@@ -24,9 +24,10 @@
 //   narrow  every warp reads all rows itself (three of four times from a cache): 32 bytes, a
 //           whole sector, of each row for four stages, one such group ahead, also across tiles.
 //
-// Per CTA: warp 0 loads (TMA), warp 1 MMA and TMEM, warps 2-5 store, warps 6-9 scales.  Measured on
-// eight experts of 14336 x 4096: 8 x 2048 rows 396-431 us (4.5-4.9 PFLOP/s, packing included; shared
-// memory moves some 113 bytes a cycle, and without the stores it is 338), 8 x 2 rows 50 us (5.0 TB/s).
+// Per CTA: warp 0 loads (TMA), warp 1 MMA and TMEM, warps 2-5 store (10-13 too for short
+// contractions), warps 6-9 scales.  Measured on eight experts of 14336 x 4096: 8 x 2048 rows
+// 396-478 us by the power cap (4.0-4.9 PFLOP/s, packing included; shared memory moves some 113 bytes a
+// cycle, and without the stores it is 338), 8 x 2 rows 50 us (5.0 TB/s).
 // Every wait is bounded (tma.cuh): an expiry stops every role at its next wait.
 #include "experts.cuh"
 #include "grouped.cuh"
@@ -36,7 +37,6 @@ namespace {
 
 using namespace grouped;
 
-constexpr int kThreads = 320;
 constexpr int kStep = 256;           // codes per stage: 128 bytes a row
 constexpr int kABytes = 128 * 128;
 constexpr int kSuper = 4;            // stages whose scales a thread loads at once (32 bytes a row)
@@ -52,7 +52,7 @@ struct MxParams {
   const uint8_t* w_blocks;  // wide: packed scales
   const uint8_t* x_blocks;
   int groups;            // of 128 codes in them, an even number
-  int height, split;
+  int height, split, store_sets;
   Bands bands;
   CUtensorMap w_map;      // 128 bytes x 128 rows
   CUtensorMap x_map[7];   // 128 bytes x 16, 32, .. 112 rows
@@ -65,7 +65,9 @@ struct Shape {
   static constexpr int kHalves = (kNT + 127) / 128;              // scale blocks of 128 rows of x
   static constexpr int kScaleBytes = kCtas == 2 ? 2 * 512 * (1 + kHalves) : 0;  // blocks of two groups of 128 codes
   static constexpr int kStageBytes = (kABytes + kBRows * 128 + kScaleBytes + 1023) / 1024 * 1024;
-  static constexpr int kPartBytes = kCtas == 1 ? kNT * 128 * 4 : 4 * kChunkBytes;
+  static constexpr int kStoreSets = kCtas == 1 ? 1 : 2;  // of four warps, at most
+  static constexpr int kThreads = 192 + 128 * kStoreSets;
+  static constexpr int kPartBytes = kCtas == 1 ? kNT * 128 * 4 : kStoreSets * 4 * kChunkBytes;
   static constexpr int kStages = stages_of(kStageBytes, kPartBytes);
   static constexpr int kScaleColumns = 2 * (4 + 4 * kHalves);  // a set of TMEM columns for a stage's scales
   static constexpr int kSets = kCtas == 2 ? 4 : kStages;       // that the stages use in turn
@@ -165,7 +167,7 @@ __device__ __forceinline__ void load_scales(const uint8_t* row, int k0, int bloc
 }
 
 template <int kCtas, int kNT>
-__global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__ MxParams p) {
+__global__ void __launch_bounds__((Shape<kCtas, kNT>::kThreads), 1) mx_kernel(const __grid_constant__ MxParams p) {
   using S = Shape<kCtas, kNT>;
   constexpr int kStages = S::kStages, kSets = S::kSets;
   extern __shared__ uint8_t smem_raw[];
@@ -199,7 +201,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_empty[i], 4 * kCtas);
+      mbar_init(&acc_empty[i], 4 * p.store_sets * kCtas);
     }
     for (int i = 0; i < kSets; ++i) mbar_init(&set_full[i], 4 * kCtas);
     mbar_init(part_full, 4 * cluster);
@@ -209,7 +211,8 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
     *abort = 0;
   }
   Tiles<kCtas, kNT> walk;
-  if (kCtas == 1) pdl_wait();  // wide: the grid before is pack_kernel, and all but what it packs can be read before it ends
+  // Wide: the grid before is pack_kernel, and all but what it packs can be read before it ends.
+  if (kCtas == 1) pdl_wait();
   if (warp == 1) alloc_tmem<kCtas>(tslot, S::kColumns);  // not while waiting for a grid that may want some too
   const int mtiles = p.bands.mt;
   list_tiles(p.offsets, p.E, p.R, bounds, starts, scan, [&](int rows) { return mtiles * ceil_div(rows, kNT); });
@@ -359,11 +362,12 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
         mbar_wait(fin, 0);
       }
     }
-  } else if (warp < 6) {
+  } else if (warp < 6 || warp >= 10) {
     // ------------------------------------------------------------ stores
     const int quarter = warp & 3;
     const uint32_t lanes = uint32_t(quarter * 32) << 16;
-    const uint32_t staging = smem_u32(part) + uint32_t(quarter * kChunkBytes);
+    const int set = warp >= 10 ? 1 : 0;
+    const uint32_t staging = smem_u32(part) + uint32_t((set * 4 + quarter) * kChunkBytes);
     int count = 0;
     for (int t = first; t < tiles; t += stride, ++count) {
       const Tile x = walk.at(p, bounds, starts, t);
@@ -387,7 +391,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_kernel(const __grid_constant__
                          quarter, lane, abort, release))
           break;
       } else {
-        store_whole(p.out, d, live, f0, x.end, x.n0, x.nt, x.valid, staging, lane);
+        store_whole(p.out, d, live, f0, x.end, x.n0, x.nt, x.valid, staging, lane, set, p.store_sets);
         release();
       }
     }
@@ -601,18 +605,25 @@ int clusters_at_once(Clusters* out) {
   const auto kernel = mx_kernel<kCtas, kNT>;
   static int flags[64] = {};
   if (int rc = ensure_smem(kernel, smem_of<kCtas, kNT>(kMaxExperts), flags)) return rc;
-  return clusters_of(kernel, kThreads, smem_of<kCtas, kNT>(kMaxExperts), out);
+  return clusters_of(kernel, (Shape<kCtas, kNT>::kThreads), smem_of<kCtas, kNT>(kMaxExperts), out);
 }
+
+// Pairs with a contraction of up to kShort store with eight warps a CTA instead of four, which do not
+// keep up with the MMAs of so few steps.  8 experts, 2048 rows each to 14336 features: 1024 wide 197 us
+// against 234, 2048 wide 272 against 308, but 4096 wide 485 against 477; 16 experts, 1024 rows each
+// to 4096 features: 2048 wide 83 against 92, 3040 wide 138 against 131.
+constexpr int kShort = 2048;
 
 template <int kCtas, int kNT>
 int launch_mx(MxParams& p, int64_t tiles, void* stream) {
   p.bands = bands_of(ceil_div(p.N, p.height * kCtas));
   const int cluster = kCtas == 2 ? 2 : p.split;
+  p.store_sets = kCtas == 2 && p.blocks * 32 <= kShort ? 2 : 1;
   Clusters clusters;
   if (int rc = clusters_at_once<kCtas, kNT>(&clusters)) return rc;
   const int64_t most = tiles < clusters.at_once[cluster] ? tiles : clusters.at_once[cluster];
-  return launch_clusters(mx_kernel<kCtas, kNT>, int(most * cluster), kThreads, cluster, smem_of<kCtas, kNT>(p.E), stream,
-                         "expert_linear_mxfp4", p);
+  return launch_clusters(mx_kernel<kCtas, kNT>, int(most * cluster), 192 + 128 * p.store_sets, cluster,
+                         smem_of<kCtas, kNT>(p.E), stream, "expert_linear_mxfp4", p);
 }
 
 bool encode_codes(CUtensorMap* map, const void* p, int64_t bytes, int64_t rows, int box_rows) {

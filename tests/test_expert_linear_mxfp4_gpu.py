@@ -108,6 +108,16 @@ def test_sizes_where_the_tiles_change(counts, N, K):
     assert _native.device_wait_timeouts(reset=True) == 0
 
 
+@pytest.mark.parametrize("counts", [[300, 0, 2, 209], [100, 417, 40]])
+@pytest.mark.parametrize("K", [64, 2048, 2080])
+def test_contractions_where_the_stores_change(counts, K):
+    x, w, offsets, rows = make(counts, 520, K, seed=K, tail=2)
+    rows[sum(counts):] = -1
+    for dtype in (torch.float32, torch.bfloat16):
+        check(x, w, offsets, rows, expert_linear_mxfp4(x, w, offsets, rows=rows, dtype=dtype))
+    assert _native.device_wait_timeouts(reset=True) == 0
+
+
 def test_large_products():
     x, w, offsets, rows = make([1500, 260, 2000, 3], 2048, 1024, seed=1)
     check(x, w, offsets, rows, expert_linear_mxfp4(x, w, offsets, rows=rows))
