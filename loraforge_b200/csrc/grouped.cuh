@@ -380,17 +380,20 @@ __device__ __forceinline__ void store_value(const Output& o, int64_t at, float v
   else static_cast<float*>(o.data)[at] = v;
 }
 
-// Zeros to rows [first, R), spread over the grid.
-__device__ __forceinline__ void zero_rows(const Output& o, int first, int R) {
+// Zeros to the rows of no group, [0, first) and [last, R), spread over the grid.  `first` is above 0
+// where the groups are part of a longer table, as on a rank that holds some of the experts.
+__device__ __forceinline__ void zero_rows(const Output& o, int first, int last, int R) {
   const int size = o.type == LF_F32 ? 4 : 2;
   const int64_t bytes = int64_t(o.features) * size;
-  for (int64_t r = first + int64_t(blockIdx.x); r < R; r += gridDim.x) {
+  const int64_t none = int64_t(first) + (R - last);
+  for (int64_t i = blockIdx.x; i < none; i += gridDim.x) {
+    const int64_t r = i < first ? i : i - first + last;
     uint8_t* row = static_cast<uint8_t*>(o.data) + r * o.stride * size;
     if (((reinterpret_cast<uintptr_t>(row) | uintptr_t(bytes)) & 15) == 0) {
-      for (int64_t i = threadIdx.x * 16; i < bytes; i += blockDim.x * 16)
-        *reinterpret_cast<uint4*>(row + i) = make_uint4(0, 0, 0, 0);
+      for (int64_t b = threadIdx.x * 16; b < bytes; b += blockDim.x * 16)
+        *reinterpret_cast<uint4*>(row + b) = make_uint4(0, 0, 0, 0);
     } else {
-      for (int64_t i = threadIdx.x * 2; i < bytes; i += blockDim.x * 2) *reinterpret_cast<uint16_t*>(row + i) = 0;
+      for (int64_t b = threadIdx.x * 2; b < bytes; b += blockDim.x * 2) *reinterpret_cast<uint16_t*>(row + b) = 0;
     }
   }
 }

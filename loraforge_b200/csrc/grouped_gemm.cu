@@ -182,7 +182,7 @@ __global__ void __launch_bounds__((Shape<kCtas, kNT>::kThreads), 1) grouped_kern
   const int tiles = starts[p.E];
   const int first = int(blockIdx.x) / cluster, stride = int(gridDim.x) / cluster;
 
-  if (kMode != kWeight) zero_rows(p.out, bounds[p.E], p.R);
+  if (kMode != kWeight) zero_rows(p.out, bounds[0], bounds[p.E], p.R);
 
   // The steps of a tile that this CTA takes.
   auto my_steps = [&](const Tile& x, int* ks0, int* ks1) {

@@ -223,7 +223,7 @@ __global__ void __launch_bounds__((Shape<kCtas, kNT>::kThreads), 1) mx_kernel(co
   const uint32_t tmem = *tslot;
   const int tiles = starts[p.E];
   const int first = int(blockIdx.x) / cluster, stride = int(gridDim.x) / cluster;
-  zero_rows(p.out, bounds[p.E], p.R);
+  zero_rows(p.out, bounds[0], bounds[p.E], p.R);
 
   // The steps this CTA takes of every tile, in whole groups of kSuper.
   const int steps = ceil_div(p.K, kStep);

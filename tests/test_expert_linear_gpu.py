@@ -300,3 +300,43 @@ def test_refusals():
         _native.call("lf_expert_linear", 2, 16, 64, 4, 16, 16, 4096, 64, 16, 1, 100, 64, 64, 16, 64, None, 0, None)
     with pytest.raises(RuntimeError, match="experts"):
         _native.call("lf_expert_linear", 2, 16, 64, 4, None, 16, 4096, 64, 16, 2000, 4, 64, 64, 16, 64, None, 0, None)
+
+
+# A rank that holds the experts lo .. hi - 1 passes its part of the offsets with all rows: those of
+# other experts, before the first bound and from the last one on, are rows of no group.
+SLICES = [
+    ([3, 0, 5, 2, 1, 4], 2, 5),          # few rows: gathered by the loads
+    ([9, 14, 17, 12, 11], 1, 3),         # the narrow tiles with rows put in order
+    ([40, 300, 90, 0, 260, 7], 1, 5),    # pairs
+    ([30, 70, 0, 0], 2, 4),              # no row of its own
+    ([600, 5], 1, 2),                    # all but the last few rows are others'
+]
+
+
+@pytest.mark.parametrize("counts,lo,hi", SLICES)
+@pytest.mark.parametrize("by_index", [True, False])
+@pytest.mark.parametrize("N,K,dtype", [(136, 200, torch.bfloat16), (264, 1024, torch.float16)])
+def test_a_slice_of_the_experts(counts, lo, hi, by_index, N, K, dtype):
+    x, w, offsets, rows, grad = make(counts, N, K, dtype, seed=sum(counts) + lo, tail=2)
+    rows[sum(counts):] = -1
+    if not by_index:
+        x, rows = x[rows.clamp(min=0).long()].contiguous(), None
+    R, mine, part = grad.shape[0], w[lo:hi], offsets[lo : hi + 1]
+    y = torch.full((R, N), math.nan, device="cuda", dtype=dtype)
+    expert_linear(x, mine, part, rows=rows, out=y)
+    check_forward(x, mine, part, rows, y)
+    dx = torch.full((R, K), math.nan, device="cuda", dtype=dtype)
+    _native.launch("lf_expert_linear_input_grad", 0, _native.dtype_code(dtype), grad.data_ptr(), N, mine.data_ptr(), N * K, K,
+                   part.data_ptr(), hi - lo, R, N, K, dx.data_ptr(), K)
+    check_backward(grad, x, mine, part, rows, dx, expert_linear_backward(grad, x, mine, part, rows=rows)[1])
+    first = int(part[0])
+    assert not y[:first].any() and not dx[:first].any()
+
+
+def test_rows_before_the_first_bound_of_a_strided_output():
+    x, w, offsets, rows, _ = make([70, 40, 33], 96, 128, torch.bfloat16, seed=21)
+    for width, left in ((104, 0), (101, 2)):  # 16-byte and element-wise stores
+        buffer = torch.full((143, width), 7.0, device="cuda").bfloat16()
+        y = expert_linear(x, w[1:], offsets[1:], rows=rows, out=buffer[:, left : left + 96])
+        check_forward(x, w[1:], offsets[1:], rows, y)
+        assert not y[:70].any() and (buffer[:, :left] == 7).all() and (buffer[:, left + 96 :] == 7).all()

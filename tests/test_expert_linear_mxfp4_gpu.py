@@ -243,3 +243,21 @@ def test_refusals():
         expert_linear_mxfp4(x, w, offsets, rows=rows, out=torch.empty(7, 64, device="cuda").bfloat16())
     with pytest.raises(RuntimeError, match="workspace"):
         _native.call("lf_expert_linear_mxfp4", 2, 16, 16, 4, 16, 16, 16, 16, 1, 100, 64, 64, 16, 64, None, 0, None)
+
+
+# A rank's part of the experts: rows before the first bound and from the last one on are of no group.
+@pytest.mark.parametrize("counts,lo,hi", [([3, 0, 5, 2, 1, 4], 2, 5), ([9, 14, 17, 12, 11], 1, 3), ([40, 300, 90, 0, 260, 7], 1, 5),
+                                          ([30, 70, 0, 0], 2, 4), ([600, 5], 1, 2)])
+@pytest.mark.parametrize("by_index", [True, False])
+@pytest.mark.parametrize("N,K,dtype", [(136, 192, torch.float32), (264, 1024, torch.bfloat16)])
+def test_a_slice_of_the_experts(counts, lo, hi, by_index, N, K, dtype):
+    x, w, offsets, rows = make(counts, N, K, seed=sum(counts) + lo, tail=2)
+    rows[sum(counts):] = -1
+    if not by_index:
+        inside = rows.clamp(min=0).long()
+        x, rows = MxTensor(x.codes[inside].contiguous(), x.scales[inside].contiguous()), None
+    mine, part = MxTensor(w.codes[lo:hi], w.scales[lo:hi]), offsets[lo : hi + 1]
+    y = torch.full((sum(counts) + 2, N), math.nan, device="cuda", dtype=dtype)
+    expert_linear_mxfp4(x, mine, part, rows=rows, out=y)
+    check(x, mine, part, rows, y)
+    assert not y[: int(part[0])].any()
