@@ -187,10 +187,11 @@ __global__ void __launch_bounds__(route_threads(V)) route_topk_kernel(
   for (int e = tid; e < E; e += blockDim.x) hist[e] = 0;
   pdl_wait();
   __syncthreads();
-  const int t0 = blockIdx.x * block_tokens, t1 = min(num_tokens, t0 + block_tokens);
-  for (int t = t0 + warp; t < t1; t += blockDim.x / 32) {
+  // 64 bits: the last block's end passes 2^31 with near as many tokens.
+  const int64_t t0 = int64_t(blockIdx.x) * block_tokens, t1 = min(int64_t(num_tokens), t0 + block_tokens);
+  for (int64_t t = t0 + warp; t < t1; t += blockDim.x / 32) {
     float v[V];
-    load_logits<T, V>(logits, int64_t(t) * stride, E, lane, v);
+    load_logits<T, V>(logits, t * stride, E, lane, v);
     uint32_t keys[V], best;
     int at;
 #pragma unroll
@@ -243,8 +244,8 @@ __global__ void __launch_bounds__(route_threads(V)) route_topk_kernel(
     }
     sum = warp_sum(sum);
     if (lane < k) {
-      weights[int64_t(t) * k + lane] = my_expert >= 0 ? scale * (mine / sum) : 0.f;
-      experts[int64_t(t) * k + lane] = my_expert;
+      weights[t * k + lane] = my_expert >= 0 ? scale * (mine / sum) : 0.f;
+      experts[t * k + lane] = my_expert;
       if (my_expert >= 0) atomicAdd(&hist[my_expert], 1);
     }
   }
@@ -263,9 +264,9 @@ __global__ void __launch_bounds__(kRouteThreads) route_scatter_kernel(const int3
                                                                       int32_t* positions) {
   extern __shared__ int smem[];
   pdl_wait();
-  const int t0 = blockIdx.x * block_tokens, t1 = min(num_tokens, t0 + block_tokens);
-  scatter_slots<false>(experts, counts, gridDim.x, blockIdx.x, int64_t(t0) * k, (t1 - t0) * k, int64_t(num_tokens) * k, E, k,
-                offsets, rows, positions, smem);
+  const int64_t t0 = int64_t(blockIdx.x) * block_tokens, t1 = min(int64_t(num_tokens), t0 + block_tokens);
+  scatter_slots<false>(experts, counts, gridDim.x, blockIdx.x, t0 * k, int(t1 - t0) * k, int64_t(num_tokens) * k, E, k,
+                       offsets, rows, positions, smem);
 }
 
 // dl_i = w_i (g_i - d) for the taken experts, with d = sum_j w_j g_j / scale, and for the
@@ -535,8 +536,9 @@ struct RouteBackwardCall {
   void* stream;
   template <typename D, int V>
   int operator()() const {
-    return launch_pdl(route_backward_kernel<D, V>, dim3((T + kBackThreads / 32 - 1) / (kBackThreads / 32)), kBackThreads, 0, stream,
-                      "route_experts_backward", logits, stride, weights, experts, grad, grad_stride, T, E, k,
+    constexpr int kWarps = kBackThreads / 32;
+    return launch_pdl(route_backward_kernel<D, V>, dim3(unsigned((int64_t(T) + kWarps - 1) / kWarps)), kBackThreads, 0,
+                      stream, "route_experts_backward", logits, stride, weights, experts, grad, grad_stride, T, E, k,
                       renormalize, scale, out, out_stride);
   }
 };
