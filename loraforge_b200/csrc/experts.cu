@@ -482,9 +482,14 @@ RoutePlan route_plan(int64_t tokens) {
   return {int(per), int((tokens + per - 1) / per)};
 }
 
+// tokens x k slots that int32 holds; the product is taken only where it fits 64 bits.
+bool slots_ok(int64_t tokens, int k) {
+  const int64_t limit = int64_t(1) << 31;
+  return k >= 1 && k <= kMaxTopK && tokens >= 0 && tokens < limit && tokens * k < limit;
+}
+
 bool route_sizes_ok(int64_t tokens, int E, int k) {
-  return tokens >= 0 && E >= 1 && E <= kMaxExperts && k >= 1 && k <= kMaxTopK && k <= E &&
-         tokens * k < (int64_t(1) << 31);
+  return E >= 1 && E <= kMaxExperts && k <= E && slots_ok(tokens, k);
 }
 
 // F<T, V> for the element type and the number of logits a lane holds.
@@ -613,8 +618,7 @@ namespace lfb {
 namespace {
 int combine_sizes(const char* what, int dtype, int64_t tokens, int k, int64_t rows, int N) {
   if (dtype < LF_F32 || dtype > LF_BF16) return fail(LF_E_INVALID, (std::string(what) + ": unknown element type").c_str());
-  if (tokens < 0 || k < 1 || k > kMaxTopK || tokens * k >= (int64_t(1) << 31) || rows < 0 ||
-      rows >= (int64_t(1) << 31) || N < 1)
+  if (!slots_ok(tokens, k) || rows < 0 || rows >= (int64_t(1) << 31) || N < 1)
     return fail(LF_E_INVALID, (std::string(what) + ": needs 1 <= top_k <= 32 and slots and rows that fit int32").c_str());
   return LF_OK;
 }

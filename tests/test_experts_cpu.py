@@ -43,6 +43,18 @@ def test_sizes_are_checked_on_the_host(entry, args, match):
         call(entry, args)
 
 
+@pytest.mark.parametrize("tokens", [2**58, 2**59, 2**62, 2**63 - 1])
+@pytest.mark.parametrize("entry,args", [
+    ("lf_route_experts", lambda t: (0, 16, 32, t, 32, 32, 1, 1.0, 16, 16, 16, 16, 16, 16, 2**62, None)),
+    ("lf_route_experts_backward", lambda t: (0, 16, 32, 16, 16, 16, 32, t, 32, 32, 1, 1.0, 16, 32, None)),
+    ("lf_combine_experts", lambda t: (0, 16, 8, 4, 16, 16, t, 32, 8, 16, 8, None)),
+    ("lf_combine_experts_backward", lambda t: (0, 16, 8, 16, 8, 4, 16, 16, t, 32, 8, 16, 8, 16, None)),
+])
+def test_slots_that_pass_64_bits(entry, args, tokens):
+    with pytest.raises(RuntimeError, match="fit int32"):
+        call(entry, args(tokens))
+
+
 def test_workspace_sizes():
     assert _native.route_experts_workspace_ints(64, 64) == 0 and _native.route_experts_workspace_ints(65, 64) == 128
     assert _native.expert_linear_workspace_bytes(8, 64, 512) == 0  # eight rows a group: gathered by the loads
