@@ -519,13 +519,8 @@ struct Cut {
 struct Clusters {
   int at_once[kMaxSplit + 1];
 };
-template <typename P>
-int clusters_of(void (*kernel)(P), int threads, int smem, Clusters* out) {
-  static Clusters known[64] = {};
-  int device = 0;
-  if (cudaGetDevice(&device) != cudaSuccess) return check_launch("cudaGetDevice");
-  Clusters& have = known[device & 63];
-  for (int s = 1; s <= kMaxSplit && !have.at_once[kMaxSplit]; ++s) {
+inline int count_clusters(const void* kernel, int threads, int smem, Clusters* out) {
+  for (int s = 1; s <= kMaxSplit; ++s) {
     cudaLaunchConfig_t config = {};
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -540,9 +535,33 @@ int clusters_of(void (*kernel)(P), int threads, int smem, Clusters* out) {
     int n = 0;
     if (cudaOccupancyMaxActiveClusters(&n, kernel, &config) != cudaSuccess)
       return check_launch("cudaOccupancyMaxActiveClusters");
-    have.at_once[s] = n > 0 ? n : 1;
+    out->at_once[s] = n > 0 ? n : 1;
   }
-  *out = have;
+  return LF_OK;
+}
+// The same, counted once for a kernel, its threads and shared memory, and a device; from any thread.
+template <typename P>
+int clusters_of(void (*kernel)(P), int threads, int smem, Clusters* out) {
+  struct Known {
+    const void* kernel;
+    int device, threads, smem;
+    Clusters clusters;
+  };
+  constexpr int kMostKnown = 256;  // past these, counted in every call
+  static std::mutex mutex;
+  static Known known[kMostKnown];
+  static int count = 0;
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return check_launch("cudaGetDevice");
+  const void* key = reinterpret_cast<const void*>(kernel);
+  std::lock_guard<std::mutex> lock(mutex);
+  for (int i = 0; i < count; ++i)
+    if (known[i].kernel == key && known[i].device == device && known[i].threads == threads && known[i].smem == smem) {
+      *out = known[i].clusters;
+      return LF_OK;
+    }
+  if (int rc = count_clusters(key, threads, smem, out)) return rc;
+  if (count < kMostKnown) known[count++] = {key, device, threads, smem, *out};
   return LF_OK;
 }
 
