@@ -515,7 +515,8 @@ struct Cut {
 };
 
 // How many clusters of 1, 2, .. kMaxSplit CTAs the device holds at a time (148 SMs, one CTA each: 33 of
-// 4, 15 of 8, as clusters stay inside a GPC).  More in a persistent grid would run in a second wave.
+// 4, 15 of 8, as clusters stay inside a GPC), 0 where it cannot place one.  More in a persistent grid
+// would run in a second wave.
 struct Clusters {
   int at_once[kMaxSplit + 1];
 };
@@ -535,7 +536,7 @@ inline int count_clusters(const void* kernel, int threads, int smem, Clusters* o
     int n = 0;
     if (cudaOccupancyMaxActiveClusters(&n, kernel, &config) != cudaSuccess)
       return check_launch("cudaOccupancyMaxActiveClusters");
-    out->at_once[s] = n > 0 ? n : 1;
+    out->at_once[s] = n > 0 ? n : 0;
   }
   return LF_OK;
 }
@@ -570,10 +571,12 @@ int clusters_of(void (*kernel)(P), int threads, int smem, Clusters* out) {
 // 2.9 ns each, the unit here.  Whole waves count (896 tiles of 128 over 148 CTAs are 7 waves for
 // 6.05 waves' work; 1024 tiles of 112 are 6.9).  A tile costs 0.5 us more, and where a cluster adds
 // up its parts 4 us that only other tiles' loads cover.  A CTA's steps are a multiple of `whole`.
+// Splits over clusters that the device cannot place are left out.
 inline Cut choose_cut(const Clusters& clusters, int64_t groups, int M, int steps, int whole, bool any_height) {
   Cut best{128, 1};
   double least = 1e30;
   for (int s = 1; s <= kMaxSplit && (s == 1 || steps >= 4 * s); ++s) {
+    if (clusters.at_once[s] < 1) continue;
     for (int h = 128; h >= (any_height ? 64 : 128); h -= 8) {
       const int64_t tiles = groups * ceil_div(M, h), wave = clusters.at_once[s];
       const double waves = double((tiles + wave - 1) / wave), joined = s > 1 ? 1400 : 0;
@@ -589,6 +592,17 @@ inline Cut choose_cut(const Clusters& clusters, int64_t groups, int M, int steps
 }
 
 // ------------------------------------------------------------------ launch
+// CTAs of a persistent grid over at most `tiles` tiles, one cluster each at a time; 0, with the error
+// set, where the device cannot place the cluster.
+inline int grid_of(const Clusters& clusters, int64_t tiles, int cluster, const char* what) {
+  const int at_once = clusters.at_once[cluster];
+  if (at_once < 1) {
+    last_error() = std::string(what) + ": the device cannot place a cluster of " + std::to_string(cluster) + " CTAs";
+    return 0;
+  }
+  return int(tiles < at_once ? tiles : at_once) * cluster;
+}
+
 template <typename P>
 int launch_clusters(void (*kernel)(P), int grid, int threads, int cluster, int smem, void* stream, const char* what,
                     const P& p) {

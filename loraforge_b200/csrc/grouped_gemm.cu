@@ -445,8 +445,9 @@ int launch_grouped(GParams& p, int64_t tiles, void* stream, const char* what) {
   p.store_sets = kCtas == 2 && (kMode == kWeight ? p.R / (p.E < p.R ? p.E : p.R) : p.C) <= kShort ? 2 : 1;
   Clusters clusters;
   if (int rc = clusters_at_once<kMode, kCtas, kNT>(&clusters)) return rc;
-  const int64_t most = tiles < clusters.at_once[cluster] ? tiles : clusters.at_once[cluster];
-  return launch_clusters(grouped_kernel<kMode, kCtas, kNT>, int(most * cluster), 64 + 128 * p.store_sets, cluster,
+  const int grid = grid_of(clusters, tiles, cluster, what);
+  if (!grid) return LF_E_CUDA;
+  return launch_clusters(grouped_kernel<kMode, kCtas, kNT>, grid, 64 + 128 * p.store_sets, cluster,
                          smem_of<kCtas, kNT>(p.E), stream, what, p);
 }
 

@@ -621,8 +621,9 @@ int launch_mx(MxParams& p, int64_t tiles, void* stream) {
   p.store_sets = kCtas == 2 && p.blocks * 32 <= kShort ? 2 : 1;
   Clusters clusters;
   if (int rc = clusters_at_once<kCtas, kNT>(&clusters)) return rc;
-  const int64_t most = tiles < clusters.at_once[cluster] ? tiles : clusters.at_once[cluster];
-  return launch_clusters(mx_kernel<kCtas, kNT>, int(most * cluster), 192 + 128 * p.store_sets, cluster,
+  const int grid = grid_of(clusters, tiles, cluster, "expert_linear_mxfp4");
+  if (!grid) return LF_E_CUDA;
+  return launch_clusters(mx_kernel<kCtas, kNT>, grid, 192 + 128 * p.store_sets, cluster,
                          smem_of<kCtas, kNT>(p.E), stream, "expert_linear_mxfp4", p);
 }
 

@@ -1,4 +1,7 @@
-"""How the expert products count the clusters a device holds, in small programs compiled with nvcc."""
+"""How the expert products count the clusters a device holds, and cut their work by it.
+
+The host code is compiled into small programs with nvcc; the first needs no GPU.
+"""
 
 import subprocess
 
@@ -16,6 +19,32 @@ def program(folder, body):
     subprocess.run([_build.nvcc(), *_build.ARCH, "-O1", "-std=c++17", "--expt-relaxed-constexpr", "-I", str(_build.INCLUDE),
                     "-I", str(_build.CSRC), str(source), "-o", str(out)], check=True, capture_output=True)
     return out
+
+
+CUTS = """
+int main() {
+  // Long contractions of few groups are split over many CTAs, here with nothing above `most` to hold them.
+  for (int most = 1; most <= kMaxSplit; ++most) {
+    Clusters c{};
+    for (int s = 1; s <= most; ++s) c.at_once[s] = 148 / s;
+    const Cut cut = choose_cut(c, 1, 256, 256, 1, true);
+    std::printf("%d\\n", cut.split);
+  }
+  // What the device cannot place is an error of the call, not a grid of none.
+  Clusters pairs{};
+  pairs.at_once[2] = 74;
+  return grid_of(pairs, 5, 2, "call") == 10 && grid_of(pairs, 500, 2, "call") == 148 && lfb::last_error().empty() &&
+                 grid_of(pairs, 5, 4, "call") == 0 && lfb::last_error() == "call: the device cannot place a cluster of 4 CTAs"
+             ? 0 : 3;
+}
+"""
+
+
+def test_no_cut_over_more_ctas_than_a_cluster_may_have(tmp_path):
+    out = subprocess.run([program(tmp_path, CUTS)], capture_output=True, text=True)
+    assert out.returncode == 0, out.returncode
+    splits = [int(v) for v in out.stdout.split()]
+    assert all(1 <= split <= most for most, split in enumerate(splits, 1)) and splits[-1] > 1
 
 
 COUNTS = """
