@@ -1,6 +1,8 @@
 // Launch helpers: per-device one-time kernel attributes and cluster launches.
 #pragma once
 
+#include <mutex>
+
 #include "common.cuh"
 
 namespace lfb {
@@ -10,19 +12,24 @@ namespace lfb {
 // carveout: otherwise the driver may size the SM's split for one CTA of a kernel that
 // is meant to run two per SM (a function attribute of this process, not a device
 // setting).  `configured` holds one entry per device (devices 0..63) for this kernel.
+// Host threads may call at once: the entry is read without a lock where it is high enough, and
+// limit and entry are raised under one, so that a lower limit never follows a higher one.
 template <typename Kernel>
 inline int ensure_smem(Kernel kernel, int bytes, int* configured) {
   if (bytes <= 48 * 1024) return LF_OK;
   int device = 0;
   if (cudaGetDevice(&device) != cudaSuccess) return check_launch("cudaGetDevice");
-  int& have = configured[device & 63];
-  if (have >= bytes) return LF_OK;
+  static std::mutex mutex;
+  int* have = &configured[device & 63];
+  if (__atomic_load_n(have, __ATOMIC_ACQUIRE) >= bytes) return LF_OK;
+  std::lock_guard<std::mutex> lock(mutex);
+  if (__atomic_load_n(have, __ATOMIC_RELAXED) >= bytes) return LF_OK;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) !=
           cudaSuccess ||
       cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
                            cudaSharedmemCarveoutMaxShared) != cudaSuccess)
     return check_launch("cudaFuncSetAttribute");
-  have = bytes;
+  __atomic_store_n(have, bytes, __ATOMIC_RELEASE);
   return LF_OK;
 }
 
