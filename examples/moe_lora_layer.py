@@ -23,7 +23,7 @@ if str(ROOT) not in sys.path:
     sys.path.insert(0, str(ROOT))
 
 from loraforge_b200.ops.experts import (  # noqa: E402
-    combine_experts, combine_experts_backward, expert_linear, expert_linear_backward, route_experts,
+    ExpertRouting, combine_experts, combine_experts_backward, expert_linear, expert_linear_backward, route_experts,
     route_experts_backward)
 from loraforge_b200.ops.fused import lora_shrink_expand  # noqa: E402
 from loraforge_b200.ops.grouping import group_tokens  # noqa: E402
@@ -70,14 +70,15 @@ class _Route(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, top_k):
         routing = route_experts(logits.detach(), top_k)
-        ctx.routing = routing
-        ctx.save_for_backward(logits)
+        # Saved, not kept on ctx: an output there would hold its own graph, and changes of it go unseen.
+        ctx.save_for_backward(logits, *routing)
         ctx.mark_non_differentiable(*routing[1:])
         return tuple(routing)
 
     @staticmethod
     def backward(ctx, grad_weights, *_):
-        return route_experts_backward(ctx.saved_tensors[0].detach(), ctx.routing, grad_weights.contiguous()), None
+        logits, *routing = (t.detach() for t in ctx.saved_tensors)
+        return route_experts_backward(logits, ExpertRouting(*routing), grad_weights.contiguous()), None
 
 
 class _ExpertLinear(torch.autograd.Function):

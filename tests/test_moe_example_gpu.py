@@ -1,5 +1,6 @@
 """The mixture-of-experts example on the B200: a served block and a trained one."""
 
+import gc
 import importlib.util
 import math
 from pathlib import Path
@@ -86,3 +87,33 @@ def test_main_trains(example, capsys):
     example.main()
     losses = [float(line.split()[-1]) for line in capsys.readouterr().out.splitlines() if line.startswith("training")]
     assert len(losses) == 5 and losses[-1] < losses[0] and all(math.isfinite(v) for v in losses)
+
+
+def test_training_steps_keep_no_memory(example):
+    # Without the cycle collector: what a step's graph holds goes with it.
+    device = torch.device("cuda", 0)
+    w = example.make_weights(5, 64, 96, 1, 16, device, seed=5)
+    leaves = [w[n].clone().requires_grad_() for n in ("router", "gate_up", "down")]
+    hidden = torch.randn(600, 64, device=device).bfloat16()
+    held = []
+    gc.collect()
+    gc.disable()
+    try:
+        for _ in range(6):
+            example.moe_block(hidden, *leaves, 2).float().square().mean().backward()
+            for leaf in leaves:
+                leaf.grad = None
+            held.append(torch.cuda.memory_allocated())
+    finally:
+        gc.enable()
+    assert len(set(held[1:])) == 1, held
+
+
+def test_changed_routing_weights_are_noticed(example):
+    logits = torch.randn(5, 4, device="cuda").requires_grad_()
+    weights = example._Route.apply(logits, 2)[0]
+    loss = weights.sum()
+    with torch.no_grad():
+        weights.mul_(2.0)  # the gradient's formula reads them
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
