@@ -254,3 +254,18 @@ def test_refusals():
     with pytest.raises(ValueError, match="grad"):
         combine_experts_backward(y[:3], y, r.weights, r.positions)
     assert isinstance(r, ExpertRouting)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_gradient_of_the_weights_adds_up_short_chains(dtype):
+    # The first value each lane of the warp reads is 1, all others half a unit in 1's last place,
+    # which an addition to it drops: a lane's chain over its N / 32 terms would lose 447 units of
+    # 2^-24 of the sum, chains of at most N / 128 terms and their joining stay below N / 128 + 12.
+    N, lane = 14336, 16 // torch.empty(0, dtype=dtype).element_size()
+    r = route_experts(torch.zeros(2, 3, device="cuda"), 2)
+    y = torch.full((4, N), 2.0**-24, device="cuda", dtype=dtype)
+    y[:, : 32 * lane : lane] = 1.0
+    grad = torch.ones(2, N, device="cuda", dtype=dtype)
+    got = combine_experts_backward(grad, y, r.weights, r.positions)[1].double()
+    want = y.double().sum(1)[r.positions.long()]
+    assert ((got - want).abs() <= (N / 128 + 12) * 2.0**-24 * want).all()
