@@ -5,7 +5,8 @@ gives by their experts' weights (``expert_linear``, which reads the tokens' rows
 tables), and adds each token's rows up with ``combine_experts``.
 Every operator reads its tables on the device, so a layer can be captured in a CUDA graph;
 the LoRA operators take the same batch beside it (the rows of a token keep its adapter).
-Each forward has an explicit gradient (``*_backward``).  The reference has no counterpart.
+Each forward has an explicit gradient (``*_backward``) and records none: where autograd is
+recording, tensors that require a gradient are refused.  The reference has no counterpart.
 """
 
 from __future__ import annotations
@@ -39,9 +40,18 @@ def _kinds():
     return torch.Tensor, halves, (torch.float32, *halves)
 
 
+def _refuse_gradient(name: str) -> None:
+    """For a tensor that requires a gradient: an error where autograd would record the call."""
+    import torch
+
+    if torch.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient, which the call does not record: detach it (gradients are "
+                         "the *_backward operators) or call under torch.no_grad()")
+
+
 def cuda_tensor(value, name: str, ndim: int, dtypes, index: int | None = None) -> int:
     """A CUDA tensor of rank `ndim` and one of `dtypes`, int32-indexable, on CUDA device `index`
-    if given; the index of its device."""
+    if given, that autograd does not follow; the index of its device."""
     if not isinstance(value, _kinds()[0]):
         raise TypeError(f"{name} must be a torch.Tensor")
     if value.ndim != ndim or value.dtype not in dtypes:
@@ -51,6 +61,8 @@ def cuda_tensor(value, name: str, ndim: int, dtypes, index: int | None = None) -
     found = value.get_device()  # -1: the host
     if found < 0 or not value.is_cuda or (index is not None and found != index):
         raise ValueError(f"{name} must be on the same CUDA GPU")
+    if value.requires_grad:
+        _refuse_gradient(name)
     return found
 
 
@@ -71,6 +83,8 @@ def packed_table(value, name: str, shape, index: int, dtype) -> None:
     """A contiguous table of exactly `shape` on CUDA device `index`."""
     if (isinstance(value, _kinds()[0]) and value.dtype is dtype and value.shape == shape and value.is_contiguous()
             and value.get_device() == index and value.is_cuda):
+        if value.requires_grad:
+            _refuse_gradient(name)
         return
     cuda_tensor(value, name, len(shape), (dtype,), index)
     raise ValueError(f"{name} must be contiguous with shape {tuple(shape)}")
