@@ -129,7 +129,7 @@ def route_experts(logits, top_k: int, *, renormalize: bool = True, scale: float 
         for name, shape, dtype in (("weights", (T, top_k), torch.float32), ("experts", (T, top_k), torch.int32),
                                    ("offsets", (E + 1,), torch.int32), ("rows", (T * top_k,), torch.int32),
                                    ("positions", (T, top_k), torch.int32)):
-            packed_table(getattr(out, name), f"out.{name}", shape, index, dtype)
+            packed_table(getattr(out, name, None), f"out.{name}", shape, index, dtype)
             output_is_distinct(getattr(out, name), (logits,))
     room = _native.route_experts_workspace_ints(T, E)
     workspace = logits.new_empty(room, dtype=torch.int32) if room else None
@@ -269,7 +269,7 @@ def group_tables(offsets, rows, num_experts: int, x_rows: int, index: int) -> in
     packed_table(offsets, "offsets", (num_experts + 1,), index, torch.int32)
     if rows is None:
         return x_rows
-    if getattr(rows, "ndim", 0) != 1:
+    if not isinstance(rows, torch.Tensor) or rows.ndim != 1:
         cuda_tensor(rows, "rows", 1, (torch.int32,), index)
     R = rows.numel()
     packed_table(rows, "rows", (R,), index, torch.int32)
