@@ -11,6 +11,8 @@ recording, tensors that require a gradient are refused.  The reference has no co
 
 from __future__ import annotations
 
+import ctypes
+import math
 from functools import lru_cache
 from typing import NamedTuple
 
@@ -91,8 +93,9 @@ def packed_table(value, name: str, shape, index: int, dtype) -> None:
 
 
 def _scale(value) -> float:
-    scale = float(value)
-    if not 0.0 < scale <= 3.4028234663852886e38:
+    """The factor as the kernels take it, in FP32."""
+    scale = ctypes.c_float(float(value)).value
+    if not 0.0 < scale < math.inf:
         raise ValueError("scale must be positive and finite")
     return scale
 

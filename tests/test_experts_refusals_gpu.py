@@ -9,7 +9,7 @@ pytestmark = [
 ]
 
 from loraforge_b200.ops.experts import (  # noqa: E402
-    combine_experts, expert_linear, expert_linear_backward, route_experts)
+    combine_experts, expert_linear, expert_linear_backward, route_experts, route_experts_backward)
 
 
 def test_tables_that_are_not_tensors():
@@ -28,3 +28,13 @@ def test_tables_that_are_not_tensors():
     for table in (r.positions.cpu().numpy(), r.positions.tolist()):
         with pytest.raises(TypeError, match="positions must be a torch.Tensor"):
             combine_experts(x, None, table)
+
+
+@pytest.mark.parametrize("scale", [1e-50, 1e-46, 3.5e38, -1.0, float("nan")])
+def test_scales_that_fp32_does_not_hold(scale):
+    logits = torch.randn(4, 8, device="cuda")
+    r = route_experts(logits, 2)
+    with pytest.raises(ValueError, match="scale must be positive and finite"):
+        route_experts(logits, 2, scale=scale)
+    with pytest.raises(ValueError, match="scale must be positive and finite"):
+        route_experts_backward(logits, r, r.weights, scale=scale)
