@@ -68,7 +68,11 @@ def mxfp4_quantize(x) -> MxTensor:
 
 
 def mxfp4_dequantize(x: MxTensor, dtype=None):
-    """The values ``x`` stands for in ``dtype`` (default BF16, which holds all of them exactly)."""
+    """The values ``x`` stands for in ``dtype`` (default BF16).
+
+    BF16 and FP32 hold exactly all that ``mxfp4_quantize`` gives (scale bytes up to 252).  Of the bytes
+    253 and 254, which other programs may write, values from 2^128 on become infinite; FP16 rounds.
+    """
     import torch
 
     dtype = torch.bfloat16 if dtype is None else dtype

@@ -111,3 +111,18 @@ def test_refusals():
         mxfp4_dequantize(MxTensor(q.codes, q.scales[:, :1]))
     with pytest.raises(ValueError, match="codes"):
         mxfp4_dequantize(MxTensor(q.codes[:, 1:], q.scales))
+
+
+def test_every_scale_byte_and_code():
+    # Scales of other programs' tensors: the quantiser itself ends at 252.  What passes a type's range is infinite in it.
+    codes = torch.arange(16, device="cuda", dtype=torch.uint8).repeat(256, 2)
+    packed = (codes[:, 0::2] | codes[:, 1::2] << 4).contiguous()
+    q = MxTensor(packed, torch.arange(256, device="cuda", dtype=torch.int32).to(torch.uint8)[:, None].contiguous())
+    levels = torch.tensor([*LEVELS, *(-LEVELS)], dtype=torch.float64, device="cuda").repeat(2)
+    powers = torch.tensor([math.ldexp(1.0, i - 127) for i in range(255)] + [math.nan], dtype=torch.float64, device="cuda")
+    want = levels * powers[:, None]
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        got = mxfp4_dequantize(q, dtype)
+        assert torch.equal(got.nan_to_num(7.5), want.to(dtype).nan_to_num(7.5)) and torch.equal(got.isnan(), want.isnan())
+    assert torch.equal(mxfp4_dequantize(q)[:253].double(), want[:253])  # BF16 holds these exactly
+    assert mxfp4_dequantize(q)[253:255].isinf().any(1).all()
