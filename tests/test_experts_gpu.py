@@ -269,3 +269,78 @@ def test_gradient_of_the_weights_adds_up_short_chains(dtype):
     got = combine_experts_backward(grad, y, r.weights, r.positions)[1].double()
     want = y.double().sum(1)[r.positions.long()]
     assert ((got - want).abs() <= (N / 128 + 12) * 2.0**-24 * want).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("renormalize,scale", [(True, 1.0), (False, 1.0), (False, 2.5), (True, 0.5)])
+def test_routing_gradient_with_fewer_experts_than_choices(renormalize, scale, dtype):
+    # Most experts masked: 0, 1, .. k + 1 of them left, by -inf and by NaN, some of the finite logits
+    # near the lowest value; the rows of the gradients are strided.
+    g = torch.Generator(device="cuda").manual_seed(7)
+    E, k = 12, 4
+    logits = (2 * torch.randn(36, E, generator=g, device="cuda")).to(dtype)
+    for t in range(36):
+        gone = torch.randperm(E, generator=g, device="cuda")[: E - t % 6]
+        logits[t, gone] = -math.inf if t % 2 else math.nan
+    logits[5, torch.isfinite(logits[5])] -= 1e30
+    wide = torch.randn(36, 9, generator=g, device="cuda")
+    grad = wide[:, 2 : 2 + k]
+    r = route_experts(logits, k, renormalize=renormalize, scale=scale)
+    check_routing(r, logits, k, renormalize, scale)
+    got = route_experts_backward(logits, r, grad, renormalize=renormalize, scale=scale).double()
+    # The formula in 64 bits over the experts left.
+    l = torch.where(torch.isfinite(logits), logits, -math.inf).double().cpu().requires_grad_()
+    experts = r.experts.cpu().long()
+    for t in range(36):
+        left = torch.isfinite(l[t].detach())
+        taken = experts[t][experts[t] >= 0]
+        assert len(taken) == min(k, int(left.sum())) == min(k, t % 6)
+        if not len(taken):
+            assert not got[t].any()
+            continue
+        p = torch.softmax(l[t][left], 0)
+        full = torch.zeros(E, dtype=torch.float64).masked_scatter(left, p)
+        w = full[taken] / (full[taken].sum() if renormalize else 1.0) * scale
+        gw = grad[t, : len(taken)].double().cpu()
+        (want,) = torch.autograd.grad((w * gw).sum(), l)
+        far = (got[t].cpu() - want[t].nan_to_num(0.0)).abs() - UNIT[dtype] * want[t].nan_to_num(0.0).abs()
+        assert (far <= 2e-5 * (w * gw).abs().max()).all(), t
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_combination_of_strided_gradients(dtype):
+    g = torch.Generator(device="cuda").manual_seed(10)
+    r = route_experts(torch.randn(30, 7, generator=g, device="cuda"), 3)
+    for N, pad in ((64, 16), (61, 3)):  # 16-byte and element-wise rows
+        y = torch.randn(90, N + pad, generator=g, device="cuda").to(dtype)[:, pad // 2 : pad // 2 + N]
+        grad = torch.randn(30, N + 2 * pad, generator=g, device="cuda").to(dtype)[:, pad : pad + N]
+        got = combine_experts_backward(grad, y, r.weights, r.positions)
+        want = combine_experts_backward(grad.contiguous(), y.contiguous(), r.weights, r.positions)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        rows = y.double()[r.positions.long()]
+        near = (r.weights.double()[..., None] * grad.double()[:, None]).reshape(90, N)
+        assert ((got[0].double()[r.positions.long().reshape(-1)] - near).abs() <= UNIT[dtype] * near.abs() + 6e-8).all()
+        size = (grad.double()[:, None] * rows).abs().sum(2)
+        assert ((got[1].double() - (grad.double()[:, None] * rows).sum(2)).abs() <= (N / 128 + 12) * 2.0**-24 * size).all()
+
+
+def test_combination_past_32_bits():
+    # 2.2e9 values of y and of its gradient, 1.1e9 of the output: the last tokens against 64 bits.
+    T, k, N = 67600, 2, 16384
+    g = torch.Generator(device="cuda").manual_seed(11)
+    r = route_experts(torch.randn(T, 4, generator=g, device="cuda"), k)
+    y = torch.empty(T * k, N, device="cuda", dtype=torch.bfloat16).normal_(generator=g)
+    grad = torch.empty(T, N, device="cuda", dtype=torch.bfloat16).normal_(generator=g)
+    assert T * k * N > 2**31
+    out = combine_experts(y, r.weights, r.positions)
+    grad_y, grad_w = combine_experts_backward(grad, y, r.weights, r.positions)
+    last = slice(T - 64, T)
+    at, w, gl = r.positions[last].long(), r.weights[last].double(), grad[last].double()
+    rows = y[at].double()
+    assert int(at.max()) * N > 2**31
+    far = (out[last].double() - (w[..., None] * rows).sum(1)).abs() - (w[..., None] * rows).abs().sum(1) * (k * 2.0**-24 + 2.0**-8)
+    assert (far <= 0).all()
+    near = w[..., None] * gl[:, None]
+    assert ((grad_y[at].double() - near).abs() <= 2.0**-8 * near.abs() + 1e-30).all()
+    terms = gl[:, None] * rows
+    assert ((grad_w[last].double() - terms.sum(2)).abs() <= (N / 128 + 12) * 2.0**-24 * terms.abs().sum(2)).all()
