@@ -11,8 +11,6 @@ recording, tensors that require a gradient are refused.  The reference has no co
 
 from __future__ import annotations
 
-import ctypes
-import math
 from functools import lru_cache
 from typing import NamedTuple
 
@@ -93,9 +91,8 @@ def packed_table(value, name: str, shape, index: int, dtype) -> None:
 
 
 def _scale(value) -> float:
-    """The factor as the kernels take it, in FP32."""
-    scale = ctypes.c_float(float(value)).value
-    if not 0.0 < scale < math.inf:
+    scale = float(value)
+    if not 2.0**-150 < scale <= 3.4028234663852886e38:  # what FP32 rounds to 0, and its largest value
         raise ValueError("scale must be positive and finite")
     return scale
 
