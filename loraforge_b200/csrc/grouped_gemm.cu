@@ -36,8 +36,8 @@
 //
 // Measured: 8 x 2048 rows, 4096 -> 14336: 1262 us (1524 TFLOP/s; later calls 1345-1480 under the
 // power cap, as a dense library product of that size), input gradient 1455, weight gradient 1333;
-// 64 experts of 2048 x 2048, 2 rows each: 83 us (268 MB of weights at 6.4 TB/s); dW of 64 experts of
-// 1536 x 2048, 64 rows each: 136 us, bound by its writes (403 MB; a plain fill of them takes 131).
+// 64 experts of 2048 x 2048, 2 rows each: 83 us (537 MB of weights at 6.4 TB/s); dW of 64 experts of
+// 1536 x 2048, 64 rows each: 136 us (403 MB written at 3.0 TB/s; a plain fill of them takes 105).
 //
 // Every wait is bounded (tma.cuh): an expiry stops every role at its next wait.
 #include "experts.cuh"

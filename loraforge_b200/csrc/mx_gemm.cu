@@ -26,8 +26,9 @@
 //
 // Per CTA: warp 0 loads (TMA), warp 1 MMA and TMEM, warps 2-5 store (10-13 too for short
 // contractions), warps 6-9 scales.  Measured on eight experts of 14336 x 4096: 8 x 2048 rows
-// 396-478 us by the power cap (4.0-4.9 PFLOP/s, packing included; shared memory moves some 113 bytes a
-// cycle, and without the stores it is 338), 8 x 2 rows 50 us (5.0 TB/s).
+// 396-478 us by the power cap (4.0-4.9 PFLOP/s, packing included; 338 without the stores; on 8 x 624
+// rows the tensor pipe is active in 66 % of the cycles and no other unit at its limit), 8 x 2 rows 50 us
+// (5.0 TB/s).
 // Every wait is bounded (tma.cuh): an expiry stops every role at its next wait.
 #include "experts.cuh"
 #include "grouped.cuh"
