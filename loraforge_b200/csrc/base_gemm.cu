@@ -431,12 +431,7 @@ int launch_pdl_ex(Kernel kernel, dim3 grid, dim3 block, int smem, cudaStream_t s
   config.blockDim = block;
   config.dynamicSmemBytes = smem;
   config.stream = stream;
-  const cudaError_t err = cudaLaunchKernelEx(&config, kernel, args...);
-  if (err != cudaSuccess) {
-    last_error() = std::string(what) + ": " + cudaGetErrorString(err);
-    return LF_E_CUDA;
-  }
-  return LF_OK;
+  return launch_status(cudaLaunchKernelEx(&config, kernel, args...), what);
 }
 
 struct GemmLayout {

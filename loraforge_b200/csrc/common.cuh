@@ -32,6 +32,15 @@ inline int check_launch(const char* what) {
   return LF_OK;
 }
 
+// The status of a launch that returned `err`.  The runtime keeps a failure until it is asked for, and
+// the next call's check would report it as its own.
+inline int launch_status(cudaError_t err, const char* what) {
+  if (err == cudaSuccess) return LF_OK;
+  cudaGetLastError();
+  last_error() = std::string(what) + ": " + cudaGetErrorString(err);
+  return LF_E_CUDA;
+}
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // ---------------------------------------------------------------- bf16 bits

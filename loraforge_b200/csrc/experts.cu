@@ -468,12 +468,7 @@ int launch_pdl(void (*kernel)(Params...), dim3 grid, int threads, int smem, void
   config.blockDim = dim3(threads);
   config.dynamicSmemBytes = smem;
   config.stream = static_cast<cudaStream_t>(stream);
-  const cudaError_t err = cudaLaunchKernelEx(&config, kernel, args...);
-  if (err != cudaSuccess) {
-    last_error() = std::string(what) + ": " + cudaGetErrorString(err);
-    return LF_E_CUDA;
-  }
-  return LF_OK;
+  return launch_status(cudaLaunchKernelEx(&config, kernel, args...), what);
 }
 
 struct RoutePlan {

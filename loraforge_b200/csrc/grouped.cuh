@@ -620,12 +620,7 @@ int launch_clusters(void (*kernel)(P), int grid, int threads, int cluster, int s
   config.blockDim = dim3(threads);
   config.dynamicSmemBytes = smem;
   config.stream = static_cast<cudaStream_t>(stream);
-  const cudaError_t err = cudaLaunchKernelEx(&config, kernel, p);
-  if (err != cudaSuccess) {
-    last_error() = std::string(what) + ": " + cudaGetErrorString(err);
-    return LF_E_CUDA;
-  }
-  return LF_OK;
+  return launch_status(cudaLaunchKernelEx(&config, kernel, p), what);
 }
 
 }  // namespace grouped

@@ -408,14 +408,9 @@ int gather_rows(const void* x, int64_t x_stride, int64_t x_rows, const int32_t* 
   config.gridDim = dim3(unsigned((R + 7) / 8));
   config.blockDim = dim3(256);
   config.stream = static_cast<cudaStream_t>(stream);
-  const cudaError_t err =
-      cudaLaunchKernelEx(&config, gather_rows_kernel, static_cast<const uint4*>(x), x_stride / 8, int(x_rows), rows,
-                         int(width / 8), R, static_cast<uint4*>(out));
-  if (err != cudaSuccess) {
-    last_error() = std::string(what) + ": " + cudaGetErrorString(err);
-    return LF_E_CUDA;
-  }
-  return LF_OK;
+  return launch_status(cudaLaunchKernelEx(&config, gather_rows_kernel, static_cast<const uint4*>(x), x_stride / 8,
+                                          int(x_rows), rows, int(width / 8), R, static_cast<uint4*>(out)),
+                       what);
 }
 
 template <int kCtas, int kNT>

@@ -171,12 +171,7 @@ int launch_flat(void (*kernel)(Params...), int64_t blocks, void* stream, const c
   config.gridDim = dim3(unsigned(blocks));
   config.blockDim = dim3(kThreads);
   config.stream = static_cast<cudaStream_t>(stream);
-  const cudaError_t err = cudaLaunchKernelEx(&config, kernel, args...);
-  if (err != cudaSuccess) {
-    last_error() = std::string(what) + ": " + cudaGetErrorString(err);
-    return LF_E_CUDA;
-  }
-  return LF_OK;
+  return launch_status(cudaLaunchKernelEx(&config, kernel, args...), what);
 }
 
 template <typename T>

@@ -1486,12 +1486,7 @@ int launch_pdl(Kernel kernel, int grid, int smem, cudaStream_t stream, const Par
   config.blockDim = dim3(kThreads);
   config.dynamicSmemBytes = smem;
   config.stream = stream;
-  const cudaError_t err = cudaLaunchKernelEx(&config, kernel, p);
-  if (err != cudaSuccess) {
-    last_error() = std::string(what) + ": " + cudaGetErrorString(err);
-    return LF_E_CUDA;
-  }
-  return LF_OK;
+  return launch_status(cudaLaunchKernelEx(&config, kernel, p), what);
 }
 
 }  // namespace
@@ -1697,12 +1692,7 @@ int fused_launch(const void* x, int64_t x_stride, const void* a, const void* b,
     config.blockDim = dim3(kThreads);
     config.dynamicSmemBytes = cc.smem;
     config.stream = s;
-    const cudaError_t err = cudaLaunchKernelEx(&config, kernel, p);
-    if (err != cudaSuccess) {
-      last_error() = std::string("fused_shrink_expand (one launch): ") + cudaGetErrorString(err);
-      return LF_E_CUDA;
-    }
-    return LF_OK;
+    return launch_status(cudaLaunchKernelEx(&config, kernel, p), "fused_shrink_expand (one launch)");
   }
   if (phases & kPhaseShrink) {
     // Up to 8 n tiles (S*r <= 64) the warps accumulate in registers.

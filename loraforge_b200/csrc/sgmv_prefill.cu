@@ -1069,12 +1069,7 @@ int launch_pdl(Kernel kernel, int grid, int block, int smem, cudaStream_t stream
   config.blockDim = dim3(block);
   config.dynamicSmemBytes = smem;
   config.stream = stream;
-  const cudaError_t err = cudaLaunchKernelEx(&config, kernel, p, extra...);
-  if (err != cudaSuccess) {
-    last_error() = std::string(what) + ": " + cudaGetErrorString(err);
-    return LF_E_CUDA;
-  }
-  return LF_OK;
+  return launch_status(cudaLaunchKernelEx(&config, kernel, p, extra...), what);
 }
 
 }  // namespace

@@ -387,11 +387,7 @@ int launch_token_shrink(const L& layout, const typename T::storage* x, int64_t x
   token_shrink_kernel<T, L><<<dim3(unsigned(T_tokens), unsigned(groups)), kTokThreads, 0, stream>>>(
       layout, x, x_stride, int(K));
   const cudaError_t err = cudaGetLastError();
-  if (err != cudaSuccess) {
-    last_error() = std::string(what) + ": " + cudaGetErrorString(err);
-    return LF_E_CUDA;
-  }
-  return LF_OK;
+  return launch_status(err, what);
 }
 
 template <typename T, int VEC, typename L>
@@ -413,11 +409,7 @@ int launch_shrink(const L& layout, const typename T::storage* x, int64_t x_strid
     err = launch_cluster_z(kernel, grid, dim3(kThreads), kShrinkSmem, stream, parts, layout, x,
                            x_stride, int(T_tokens), K);
   }
-  if (err != cudaSuccess) {
-    last_error() = std::string(what) + ": " + cudaGetErrorString(err);
-    return LF_E_CUDA;
-  }
-  return LF_OK;
+  return launch_status(err, what);
 }
 
 template <typename T, typename L>
