@@ -430,6 +430,7 @@ int lf_route_experts_backward(int32_t dtype, const void* logits, int64_t logits_
 /*
  * out[t] = sum_j weights[t, j] * y[positions[t, j]] in FP32, rounded once; positions outside
  * [0, num_rows) add nothing and weights = NULL stands for ones.  dtype is that of y and out.
+ * Sizes: slots and rows below 2^31, 1 <= top_k <= 32, width below 2^31 - 2048.
  */
 int lf_combine_experts(int32_t dtype, const void* y, int64_t y_stride, int64_t num_rows,
                        const float* weights, const int32_t* positions, int64_t num_tokens,

@@ -616,17 +616,26 @@ namespace lfb {
 namespace {
 int combine_sizes(const char* what, int dtype, int64_t tokens, int k, int64_t rows, int N) {
   if (dtype < LF_F32 || dtype > LF_BF16) return fail(LF_E_INVALID, (std::string(what) + ": unknown element type").c_str());
-  if (!slots_ok(tokens, k) || rows < 0 || rows >= (int64_t(1) << 31) || N < 1)
-    return fail(LF_E_INVALID, (std::string(what) + ": needs 1 <= top_k <= 32 and slots and rows that fit int32").c_str());
+  const int64_t limit = int64_t(1) << 31;  // the kernels' columns go up to 2048 past a row's last one
+  if (!slots_ok(tokens, k) || rows < 0 || rows >= limit || N < 1 || N >= limit - 2048)
+    return fail(LF_E_INVALID,
+                (std::string(what) + ": needs 1 <= top_k <= 32 and slots, rows and columns that fit int32").c_str());
   return LF_OK;
 }
 
 template <typename T, bool kVector>
 int launch_combine(const void* y, int64_t y_stride, int64_t rows, const float* weights, const int32_t* positions,
                    int64_t tokens, int k, int N, void* out, int64_t out_stride, void* stream) {
-  const int columns = 128 * Vec<T>::kWidth;
-  return launch_pdl(combine_kernel<T, kVector>, dim3(unsigned(tokens), (N + columns - 1) / columns), 128, 0, stream,
-                    "combine_experts", y, y_stride, rows, weights, positions, k, N, out, out_stride);
+  using S = typename T::storage;
+  constexpr int kColumns = 128 * Vec<T>::kWidth, kMost = 65535 * kColumns;  // of a block, and of a grid
+  for (int64_t c = 0; c < N; c += kMost) {
+    const int width = int(N - c < kMost ? N - c : kMost);
+    if (int rc = launch_pdl(combine_kernel<T, kVector>, dim3(unsigned(tokens), (width + kColumns - 1) / kColumns), 128, 0,
+                            stream, "combine_experts", static_cast<const void*>(static_cast<const S*>(y) + c), y_stride,
+                            rows, weights, positions, k, width, static_cast<void*>(static_cast<S*>(out) + c), out_stride))
+      return rc;
+  }
+  return LF_OK;
 }
 
 template <typename T, bool kVector>

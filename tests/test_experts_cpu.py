@@ -55,6 +55,16 @@ def test_slots_that_pass_64_bits(entry, args, tokens):
         call(entry, args(tokens))
 
 
+@pytest.mark.parametrize("entry,args", [
+    ("lf_combine_experts", lambda n: (2, 16, n, 4, 16, 16, 2, 2, n, 16, n, None)),
+    ("lf_combine_experts_backward", lambda n: (2, 16, n, 16, n, 4, 16, 16, 2, 2, n, 16, n, 16, None)),
+])
+@pytest.mark.parametrize("width", [2**31 - 1, 2**31 - 2048])
+def test_widths_whose_columns_int32_does_not_hold(entry, args, width):
+    with pytest.raises(RuntimeError, match="fit int32"):
+        call(entry, args(width))
+
+
 def test_workspace_sizes():
     assert _native.route_experts_workspace_ints(64, 64) == 0 and _native.route_experts_workspace_ints(65, 64) == 128
     assert _native.expert_linear_workspace_bytes(8, 64, 512) == 0  # eight rows a group: gathered by the loads

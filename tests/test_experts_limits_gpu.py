@@ -1,4 +1,4 @@
-"""Routing at the most slots it accepts, 2^31 - 1, on the B200 (some 60 GB)."""
+"""Routing and combination at the ends of the sizes they accept, on the B200 (routing: some 60 GB)."""
 
 import pytest
 
@@ -8,7 +8,8 @@ pytestmark = [
     pytest.mark.skipif(not torch.cuda.is_available(), reason="CUDA device required"),
 ]
 
-from loraforge_b200.ops.experts import route_experts, route_experts_backward  # noqa: E402
+from loraforge_b200.ops.experts import (  # noqa: E402
+    combine_experts, combine_experts_backward, route_experts, route_experts_backward)
 
 
 def test_routing_of_as_many_tokens_as_fit():
@@ -47,3 +48,22 @@ def test_routing_of_as_many_tokens_as_fit():
     assert at == [T - seconds, T]
     del logits, grad, r, dl
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dtype,width", [(torch.bfloat16, 65535 * 1024 + 1037), (torch.float32, 65535 * 512 + 8), (torch.float16, 2**27 + 64)])
+def test_combination_of_rows_wider_than_one_grid(dtype, width):
+    g = torch.Generator(device="cuda").manual_seed(3)
+    r = route_experts(torch.randn(2, 3, generator=g, device="cuda"), 2)
+    y = torch.empty(4, width, device="cuda", dtype=dtype).normal_(generator=g)
+    out = combine_experts(y, r.weights, r.positions)
+    unit = {torch.float32: 2.0**-24, torch.float16: 2.0**-11, torch.bfloat16: 2.0**-8}[dtype]
+    grad_y, _ = combine_experts_backward(out, y, r.weights, r.positions)
+    for a in range(0, width, 2**24):
+        part = slice(a, a + 2**24)
+        for t in range(2):
+            terms = [r.weights[t, j].double() * y[int(r.positions[t, j]), part].double() for j in range(2)]
+            far = (out[t, part].double() - terms[0] - terms[1]).abs()
+            assert (far <= (2 * 2.0**-24 + unit) * (terms[0].abs() + terms[1].abs()) + 2.0**-24).all()
+            for j in range(2):
+                want = r.weights[t, j].double() * out[t, part].double()
+                assert ((grad_y[int(r.positions[t, j]), part].double() - want).abs() <= unit * want.abs() + 2.0**-24).all()
